@@ -26,6 +26,15 @@ class ggq_tensor(ctypes.Structure):
                 ("blocks", ctypes.c_uint64)]
 
 
+class ggq_moe(ctypes.Structure):
+    _fields_ = [("router_type", ctypes.c_uint32), ("up_type", ctypes.c_uint32), ("down_type", ctypes.c_uint32),
+                ("reserved", ctypes.c_uint32), ("d_router", ctypes.c_void_p), ("d_gate", ctypes.c_void_p),
+                ("d_up", ctypes.c_void_p), ("d_down", ctypes.c_void_p), ("hidden", ctypes.c_uint64),
+                ("ff", ctypes.c_uint64), ("experts", ctypes.c_uint32), ("top_k", ctypes.c_uint32),
+                ("gating", ctypes.c_uint32), ("normalize", ctypes.c_uint32), ("activation", ctypes.c_uint32),
+                ("scale", ctypes.c_float)]
+
+
 class ggq_gguf_info(ctypes.Structure):
     _fields_ = [("version", ctypes.c_uint32), ("tensor_count", ctypes.c_uint64), ("kv_count", ctypes.c_uint64),
                 ("alignment", ctypes.c_uint64), ("data_offset", ctypes.c_uint64), ("data_len", ctypes.c_uint64),
@@ -47,7 +56,7 @@ class ggq_gguf_kv(ctypes.Structure):
 ggq_gguf_data_fn = ctypes.CFUNCTYPE(ctypes.c_void_p, ctypes.c_void_p, ctypes.c_uint64, ctypes.c_uint64)
 
 # every symbol include/ggq.h and include/ggq_gguf.h declare: name -> (restype, argtypes)
-_vp, _sz, _u32, _int = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32, ctypes.c_int
+_vp, _sz, _u32, _int, _u64 = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_uint32, ctypes.c_int, ctypes.c_uint64
 SYMBOLS = {
     "ggq_block_elems": (_sz, [_u32]),
     "ggq_block_bytes": (_sz, [_u32]),
@@ -77,6 +86,10 @@ SYMBOLS = {
     "ggq_ctx_fence": (_int, [_vp, _vp]),
     "ggq_ctx_wait_stream": (_int, [_vp, _vp]),
     "ggq_dequantize_noalloc": (_int, [_u32, _u32, _vp, _sz, _vp, _sz, _vp]),
+    "ggq_matvec_device": (_int, [_u32, _u64, _u64, _vp, _u32, _vp, _u64, _u64, _u32, _vp, _u64, _vp]),
+    "ggq_get_rows_device": (_int, [_u32, _u64, _u64, _vp, _u32, _vp, _u64, _u32, _vp, _u64, _vp]),
+    "ggq_moe_workspace_bytes": (_int, [ctypes.POINTER(ggq_moe), _u64, ctypes.POINTER(_sz)]),
+    "ggq_moe_device": (_int, [ctypes.POINTER(ggq_moe), _u32, _vp, _u64, _u64, _u32, _vp, _u64, _vp, _vp, _vp, _sz, _vp]),
     "ggq_selftest_fast_division": (_int, [ctypes.POINTER(ctypes.c_uint64), ctypes.POINTER(ctypes.c_uint64)]),
     "ggq_sync": (_int, [_vp]),
     "ggq_ctx_destroy": (None, [_vp]),

@@ -9,6 +9,7 @@
 #include "schedule.h"
 #include "rearrange.h"
 #include "scale.h"
+#include "internal.h"
 
 #include <algorithm>
 #include <cstdio>
@@ -67,6 +68,9 @@ bool hip_ok(hipError_t e, const char *what) {
     (void)hipGetLastError();
     return false;
 }
+}  // namespace
+bool ggq::report_hip(hipError_t e, const char *what) { return hip_ok(e, what); }
+namespace {
 #define HIP_TRY(call)                                  \
     do {                                               \
         if (!hip_ok((call), #call)) return GGQ_DEVICE; \

@@ -241,6 +241,18 @@ class _Block:
     def quantize_slice(cls, dst, src, stream=None):
         return quantize_slice(cls.TYPE, dst, src, stream)
 
+    @classmethod
+    def matvec(cls, dst, w, x, stream=None):
+        """gguf_amd.matvec for this block type."""
+        from .matmul import matvec
+        return matvec(cls.TYPE, dst, w, x, stream)
+
+    @classmethod
+    def get_rows(cls, dst, w, ids, stream=None):
+        """gguf_amd.get_rows for this block type."""
+        from .matmul import get_rows
+        return get_rows(cls.TYPE, dst, w, ids, stream)
+
 
 def _mk(name, ty):
     return type(name, (_Block,), {"TYPE": ty, "__doc__": f"Block type {name} (GGmlType {int(ty)})."})

@@ -270,6 +270,67 @@ ggq_status ggq_dequantize_noalloc(uint32_t ggml_type, uint32_t out_type,
                                   const void *h_src, size_t src_blocks,
                                   void *hip_stream);
 
+/* ---- products with packed weights -----------------------------------------
+ * No counterpart in the reference, which decodes a tensor before anything else can use it
+ * (ggml-quants/src/lib.rs:135-147).  These calls use a packed matrix as it lies in a GGUF file, without a
+ * decoded copy: W is `rows` rows of `cols` elements, cols contiguous (shape [cols, rows] of a GGUF tensor), of any
+ * block type that ggq_block_elems knows (F16 and BF16 among them); the values are exactly those that
+ * ggq_dequantize_device writes with F32 output.  Device pointers on the current device; enqueued on `hip_stream`,
+ * not synchronized, nothing allocated; all of them may be captured into a graph.  d_w may have any alignment;
+ * d_x and d_y are aligned to their element size (GGQ_MISALIGNED).  Outputs must not overlap inputs.
+ * Element types x_type and y_type: F32 (0), F16 (1) or BF16 (30); other types: GGQ_UNSUPPORTED.
+ * Strides are in elements, from one token's row to the next one's.
+ *
+ * ggq_matvec_device: y[t][r] = sum over c of W[r][c] * x[t][c], for t < tokens.  Products are exact, sums are held in
+ *   32 bits in an order that depends on the sizes alone, and one rounding to y_type ends each.  Made for the few
+ *   tokens of decoding; any number is computed.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
+ *   there are two tokens or more (GGQ_INVALID).  cols must be whole blocks (GGQ_INDIVISIBLE); cols == 0 gives zeros.
+ *   Intermediate sums are those of whole-number codes times x: |x| stays below 2^100, and non-finite x makes the
+ *   token's outputs non-finite where the row's codes reach it, of either kind.
+ * ggq_get_rows_device: y[i] = the decoded row ids[i] of W, i < n: the token embeddings of n ids.  id_type is the
+ *   GGmlType of the ids: I32 (26) or I64 (27); an id outside [0, rows) gives a row of zeros.  y_stride >= cols where
+ *   n > 1.  Values equal ggq_dequantize_device's bit for bit. */
+ggq_status ggq_matvec_device(uint32_t ggml_type, uint64_t rows, uint64_t cols, const void *d_w,
+                             uint32_t x_type, const void *d_x, uint64_t x_stride, uint64_t tokens,
+                             uint32_t y_type, void *d_y, uint64_t y_stride, void *hip_stream);
+ggq_status ggq_get_rows_device(uint32_t ggml_type, uint64_t rows, uint64_t cols, const void *d_w,
+                               uint32_t id_type, const void *d_ids, uint64_t n,
+                               uint32_t y_type, void *d_y, uint64_t y_stride, void *hip_stream);
+
+/* A mixture-of-experts layer whose experts are packed, as in the ffn_gate_exps / ffn_up_exps / ffn_down_exps tensors
+ * (shape [cols, rows, experts]) with the router of ffn_gate_inp.  Per token, with l = router * x (sums in 64 bits, one
+ * rounding to F32):
+ *   p = softmax(l) or sigmoid(l);  the top_k experts of the largest l, equal ones by the lowest index (a NaN counts as
+ *   lowest);  w = p of those, divided by their sum if `normalize`, times `scale`;
+ *   y = sum over the chosen e, in order, of w_e * down_e (act(gate_e x) * (up_e x)).
+ * The products between are held in 32 bits. */
+typedef struct ggq_moe {
+    uint32_t router_type;           /* F32, F16 or BF16: [experts][hidden], row-major      */
+    uint32_t up_type;               /* block type of gate and of up, [experts][ff][hidden] */
+    uint32_t down_type;             /* block type of down, [experts][hidden][ff]           */
+    uint32_t reserved;              /* must be 0                                           */
+    const void *d_router, *d_gate, *d_up, *d_down;
+    uint64_t hidden, ff;
+    uint32_t experts, top_k;        /* 1 <= top_k <= experts <= GGQ_MOE_MAX_EXPERTS, top_k <= GGQ_MOE_MAX_TOP_K */
+    uint32_t gating;                /* 0: softmax over all experts, 1: sigmoid             */
+    uint32_t normalize;             /* 0 or 1                                              */
+    uint32_t activation;            /* 0: SiLU, v / (1 + exp(-v)); 1: GELU, tanh form      */
+    float scale;                    /* factor on the weights, usually 1                    */
+} ggq_moe;
+#define GGQ_MOE_MAX_EXPERTS 512u
+#define GGQ_MOE_MAX_TOP_K 32u
+/* Most tokens of one ggq_moe_device call (GGQ_TOO_LARGE beyond; split the batch). */
+#define GGQ_MOE_MAX_TOKENS 64u
+/* Bytes of device memory that a call with this many tokens needs as workspace.  Its contents before the call do not
+ * matter and nothing is kept in it between calls; calls that can overlap need one each. */
+ggq_status ggq_moe_workspace_bytes(const ggq_moe *layer, uint64_t tokens, size_t *bytes_out);
+/* d_ids (int32 [tokens][top_k]) and d_weights (F32 [tokens][top_k]) receive the choice and the weights of each
+ * token; either may be NULL.  d_workspace: 256-byte aligned (GGQ_MISALIGNED), at least ggq_moe_workspace_bytes
+ * (GGQ_INVALID).  The layer description is read before the call returns and need not outlive it. */
+ggq_status ggq_moe_device(const ggq_moe *layer, uint32_t x_type, const void *d_x, uint64_t x_stride, uint64_t tokens,
+                          uint32_t y_type, void *d_y, uint64_t y_stride, int32_t *d_ids, float *d_weights,
+                          void *d_workspace, size_t workspace_bytes, void *hip_stream);
+
 /* Self-test, no counterpart in the reference.  The quantizers divide twice per block (delta = extreme / c and
  * 1 / delta, ggml-quants/src/structs/q8_0.rs:31-32 and the other formats alike); for blocks of ordinary magnitude
  * the kernels use shorter instruction sequences than the compiler's general IEEE division.  This call runs those
