@@ -4,15 +4,13 @@
 //
 // and what surrounds them in a decoding step: rows of a packed table by id, and a mixture-of-experts layer.
 #pragma once
-#include "formats.h"
+#include "slices.h"
 
 namespace ggq {
 
 // ---- packed bytes in global memory, at any alignment -----------------------------------------------------
 // The same interface as LdsBytes, reading exactly the bytes that are asked for: the last block of a tensor may end
 // at the end of an allocation.
-typedef uint32_t u32_any __attribute__((aligned(1), may_alias));
-typedef uint16_t u16_any __attribute__((aligned(1), may_alias));
 struct GlobalBytes {
     const uint8_t *p;
     __device__ __forceinline__ uint32_t u32(uint32_t off) const { return *(const u32_any *)(p + off); }
@@ -24,13 +22,6 @@ struct GlobalBytes {
         for (int g = 0; g < G; ++g) out[g] = u32(off + 4 * g);
     }
 };
-
-// The 16-bit floats as one-element block types
-struct WF16 { static constexpr uint32_t N = 1, BYTES = 2; };
-struct WBF16 { static constexpr uint32_t N = 1, BYTES = 2; };
-template <class F> constexpr bool is_float_type = false;
-template <> constexpr bool is_float_type<WF16> = true;
-template <> constexpr bool is_float_type<WBF16> = true;
 
 __device__ __forceinline__ float bf2f(uint32_t bits16) { return __builtin_bit_cast(float, bits16 << 16); }
 
@@ -69,33 +60,246 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
+// ---- the product ----------------------------------------------------------------------------------------
 struct MatvecArgs {
     const uint8_t *w;
     const void *x;
     void *y;
-    uint64_t rows, cols, tokens, x_stride, y_stride;
+    uint64_t rows, cols, x_stride, y_stride;
+    uint64_t first_tile;      // groups of four rows before this launch's
+    uint32_t tokens;          // of this launch's group: 1..4
     uint32_t x_kind, y_kind;
+    uint32_t pieces;          // bf16 pieces of an element of x: 1 (bf16), 2 (f16), 3 (f32)
+    uint32_t chunk;           // slices staged at a time, a multiple of 16 * ksplit
+    uint32_t ksplit;          // waves that share a row group's columns: 1, 2, 4 or 8
 };
 
-constexpr uint32_t MV_THREADS = 256;
+constexpr uint32_t MV_THREADS = 256;      // the other kernels here
+constexpr uint32_t QD_WAVES = 8, QD_THREADS = 64 * QD_WAVES;
 
-// one wave per row and token
-template <class F>
-__global__ __launch_bounds__(MV_THREADS) void matvec_rows(MatvecArgs a, uint64_t first_token) {
-    const uint64_t r = (uint64_t)blockIdx.x * (MV_THREADS / 64) + threadIdx.x / 64;
-    const uint64_t t = first_token + blockIdx.y;
-    if (r >= a.rows) return;
-    const uint8_t *row = a.w + r * (a.cols / F::N * F::BYTES);
-    float sum = 0.0f;
-    for (uint64_t c = 4 * (threadIdx.x % 64); c < a.cols; c += 256) {
-        float w[4];
-        row4<F>(row, c, a.cols, w);
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// x in shared memory, as the matrix unit takes it: fragments of eight bf16 (16 bytes), [piece][k][slice][column], k = the
+// fragment's place in its slice.  The 16 quads of a wave read the same k of 16 neighbouring slices, so their addresses are
+// consecutive; the pitch of a k is odd (in fragments), so that the staging threads, which run along k first, do not meet
+// in one bank either.  `cols`: columns kept, 1..4; behind the fragments lie the sums of x over each sub-block,
+// [sub-block][slice][column], for the formats with an offset.
+struct XLayout {
+    uint32_t cols, pitch, slices, chain, sums, sum_cols;
+    __device__ __forceinline__ XLayout(uint32_t slices_, uint32_t cols_, uint32_t chain_, uint32_t sum_cols_)
+        : cols(cols_), pitch(slices_ * cols_ | 1u), slices(slices_), chain(chain_), sums(chain_ * 8 * (slices_ * cols_ | 1u) * 16), sum_cols(sum_cols_) {}
+};
+__host__ __device__ __forceinline__ uint32_t x_bytes(uint32_t slices, uint32_t cols, uint32_t chain, uint32_t nsub, uint32_t sum_cols) {
+    return chain * 8 * (slices * cols | 1u) * 16 + nsub * slices * sum_cols * 4;
+}
+
+__device__ __forceinline__ float quad_xor1(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float quad_xor2(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
+}
+
+// eight elements of x from c on, 0 past the end
+__device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, uint64_t cols, uint32_t kind, float (&v)[8]) {
+    if (c + 8 <= cols) {
+        if (kind == EK_F32) {
+            const uint8_t *p = (const uint8_t *)x + 4 * (at + c);
+            const f32x4 a = __builtin_bit_cast(f32x4, ld16(p)), b = __builtin_bit_cast(f32x4, ld16(p + 16));
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < a.cols) sum = __builtin_fmaf(w[i], load_elem(a.x, t * a.x_stride + c + i, a.x_kind), sum);
+            for (int i = 0; i < 4; ++i) {
+                v[i] = a[i];
+                v[4 + i] = b[i];
+            }
+        } else {
+            const u32x4 a = ld16((const uint8_t *)x + 2 * (at + c));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                v[2 * i] = kind == EK_F16 ? h2f(a[i] & 0xFFFFu) : bf2f(a[i] & 0xFFFFu);
+                v[2 * i + 1] = kind == EK_F16 ? h2f(a[i] >> 16) : bf2f(a[i] >> 16);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? load_elem(x, at + c + i, kind) : 0.0f;
     }
-    sum = wave_sum(sum);
-    if (threadIdx.x % 64 == 0) store_elem(a.y, t * a.y_stride + r, a.y_kind, sum);
+}
+
+// Stages slices [first, first + l.slices) of `tokens` rows of x.  row(t): the element offset of token t's row.
+// one_token: the pieces of the only token are the columns; otherwise tokens are, and the pieces follow each other.
+template <class F, class Row>
+__device__ __forceinline__ void stage_x(uint8_t *lds, const XLayout &l, uint32_t first, const void *x, uint32_t kind, uint64_t cols,
+                                        uint32_t tokens, uint32_t pieces, bool one_token, Row row) {
+    typedef Slice<F> S;
+    const uint32_t frags = l.slices * 8;
+    for (uint32_t i = threadIdx.x; i < frags * tokens; i += blockDim.x) {
+        const uint32_t t = tokens == 1 ? 0 : i / frags, f = i - t * frags;
+        uint32_t sl, k;
+        if constexpr (S::PLANES) {
+            sl = ((f >> 5) << 2) | ((f >> 3) & 2u) | ((f >> 1) & 1u);
+            k = ((f >> 1) & 6u) | (f & 1u);
+        } else {
+            sl = f >> 3;
+            k = f & 7u;
+        }
+        float v[8];
+        load8(x, row(t), (uint64_t)first * 64 + f * 8, cols, kind, v);
+        float sum = 0.0f;
+        if constexpr (S::OFFSET) {
+            sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            sum += quad_xor1(sum);
+            if (S::SUB == 32) sum += quad_xor2(sum);
+            if (f % (S::SUB / 8) == 0) {
+                const uint32_t sub = k / (S::SUB / 8);
+                ((float *)(lds + l.sums))[(sub * l.slices + sl) * l.sum_cols + t] = sum;
+            }
+        }
+        for (uint32_t p = 0; p < pieces; ++p) {
+            uint32_t h[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) h[j] = take_bf16(v[j], v[j]);
+            const u32x4 w = {h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+            const uint32_t chain = one_token ? 0 : p, c = one_token ? p : t;
+            *(u32x4 *)(lds + 16 * ((chain * 8 + k) * l.pitch + sl * l.cols + c)) = w;
+        }
+    }
+}
+
+// acc[c] += the lane's slice of its row times column c of x
+template <class F, int NC>
+__device__ __forceinline__ void add_slice(const typename Slice<F>::Raw &raw, bool valid, const uint8_t *lds, const XLayout &l, uint32_t sl,
+                                          uint32_t lane_col, float (&acc)[NC]);
+
+template <class F, int NC, int S>
+__device__ __forceinline__ void add_sub(const typename Slice<F>::Raw &raw, bool valid, const uint8_t *lds, const XLayout &l, uint32_t sl,
+                                        uint32_t lane_col, float (&acc)[NC]) {
+    typedef Slice<F> T;
+    constexpr int WORDS = T::SUB / 2;
+    f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+    auto products = [&](const uint32_t (&b)[WORDS]) {
+        const uint8_t *at = lds + 16 * (S * (T::SUB / 8) * l.pitch + sl * l.cols + lane_col);
+        for (uint32_t p = 0; p < l.chain; ++p, at += 16 * 8 * l.pitch) {
+#pragma unroll
+            for (int k = 0; k < T::SUB / 8; ++k) {
+                const u32x4 a = *(const u32x4 *)(at + 16 * k * l.pitch);
+                const u32x2 a0 = {a[0], a[1]}, a1 = {a[2], a[3]}, b0 = {b[4 * k], b[4 * k + 1]}, b1 = {b[4 * k + 2], b[4 * k + 3]};
+                d = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, a0), __builtin_bit_cast(s16x4, b0), d, 0, 0, 0);
+                d = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, a1), __builtin_bit_cast(s16x4, b1), d, 0, 0, 0);
+            }
+        }
+    };
+    uint32_t b[WORDS];
+    if constexpr (is_float_type<F>) {
+#pragma unroll
+        for (int piece = 0; piece < T::WP; ++piece) {
+            T::template codes<S>(raw, b, piece);
+            products(b);
+        }
+    } else {
+        T::template codes<S>(raw, b);
+        products(b);
+    }
+    SubScale s = T::template scale<S>(raw);
+    if (!valid) s.a = s.c = 0.0f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = __builtin_fmaf(s.a, d[c], acc[c]);
+    if constexpr (T::OFFSET) {
+        const float *sums = (const float *)(lds + l.sums) + (S * l.slices + sl) * l.sum_cols;
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if ((uint32_t)c < l.sum_cols) acc[c] = __builtin_fmaf(-s.c, sums[c], acc[c]);
+    }
+}
+template <class F, int NC>
+__device__ __forceinline__ void add_slice(const typename Slice<F>::Raw &raw, bool valid, const uint8_t *lds, const XLayout &l, uint32_t sl,
+                                          uint32_t lane_col, float (&acc)[NC]) {
+    add_sub<F, NC, 0>(raw, valid, lds, l, sl, lane_col, acc);
+    add_sub<F, NC, 1>(raw, valid, lds, l, sl, lane_col, acc);
+    if constexpr (Slice<F>::NSUB == 4) {
+        add_sub<F, NC, 2>(raw, valid, lds, l, sl, lane_col, acc);
+        add_sub<F, NC, 3>(raw, valid, lds, l, sl, lane_col, acc);
+    }
+}
+
+// Sum over the 16 quads of a wave: afterwards every lane holds its row's total.
+__device__ __forceinline__ float quads_sum(float v) {
+#pragma unroll
+    for (int m = 4; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    return v;
+}
+
+// One to four tokens.  A wave owns four rows; its quads (four neighbouring lanes, one lane per row) take 16 neighbouring
+// slices at a time, each lane the packed bytes of its row's slice.  v_mfma_f32_4x4x4 with 16 blocks multiplies, in each
+// quad, the four rows' codes with up to four columns of x that the quad's lanes hold: every lane ends with its own row's
+// products, so that the sub-block's scale is applied in the lane that loaded it.  Columns are tokens, or the bf16 pieces
+// of the only token (f32 = three pieces, exactly; products with codes are exact, sums are f32).
+template <class F, int NC>
+__global__ __launch_bounds__(QD_THREADS) void matvec_quads(MatvecArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    typedef Slice<F> S;
+    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, quad = lane / 4;
+    const uint32_t kp = wave % a.ksplit, group = wave / a.ksplit, groups = QD_WAVES / a.ksplit;
+    const uint64_t tile = a.first_tile + (uint64_t)blockIdx.x * groups + group, row = tile * 4 + lane % 4;
+    const uint8_t *w = a.w + (row < a.rows ? row : a.rows - 1) * (a.cols / F::N * F::BYTES);
+    const uint32_t units = (uint32_t)(a.cols / S::UNIT), slices = (uint32_t)((a.cols + 63) / 64);
+    const bool one = a.tokens == 1;
+    const uint32_t xcols = one ? a.pieces : a.tokens, chain = one ? 1 : a.pieces;
+    const XLayout l(a.chunk, xcols, chain, a.tokens);
+    const uint32_t lane_col = lane % 4 < xcols ? lane % 4 : xcols - 1;
+    float acc[NC];
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = 0.0f;
+
+    typename S::Raw cur, nxt;
+    uint32_t s = kp * 16 + quad;                       // this lane's next slice
+    auto load = [&](typename S::Raw &r, uint32_t at) { r.load(w, at < slices ? at : slices - 1, units); };
+    load(cur, s);
+    for (uint32_t first = 0; first < slices; first += a.chunk) {
+        if (first) __syncthreads();
+        stage_x<F>(lds, l, first, a.x, a.x_kind, a.cols, a.tokens, a.pieces, one, [&](uint32_t t) { return t * a.x_stride; });
+        __syncthreads();
+        const uint32_t end = first + a.chunk < slices ? first + a.chunk : slices;
+        for (; s - quad < end; s += 16 * a.ksplit) {
+            if (s - quad + 16 * a.ksplit < slices) load(nxt, s + 16 * a.ksplit);
+            const bool valid = s < slices;
+            add_slice<F, NC>(cur, valid, lds, l, (valid ? s : slices - 1) - first, lane_col, acc);
+            cur = nxt;
+        }
+    }
+    if (NC > 1 && one) {
+        // the columns are pieces: only those that there are count
+        float sum = acc[0];
+#pragma unroll
+        for (int c = 1; c < NC; ++c) sum += (uint32_t)c < a.pieces ? acc[c] : 0.0f;
+        acc[0] = sum;
+    }
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = quads_sum(acc[c]);
+    if (a.ksplit > 1) {
+        __syncthreads();                               // the staged x is no longer needed
+        float *part = (float *)lds;                    // [wave][column][row]
+        if (lane < 4)
+#pragma unroll
+            for (int c = 0; c < NC; ++c) part[(wave * 4 + c) * 4 + lane] = acc[c];
+        __syncthreads();
+        if (kp == 0)
+#pragma unroll
+            for (int c = 0; c < NC; ++c)
+                for (uint32_t k = 1; k < a.ksplit; ++k) acc[c] += part[((wave + k) * 4 + c) * 4 + lane % 4];
+    }
+    if (kp == 0 && lane < 4 && row < a.rows) {
+#pragma unroll
+        for (int c = 0; c < NC; ++c)
+            if ((uint32_t)c < a.tokens) store_elem(a.y, c * a.y_stride + row, a.y_kind, acc[c]);
+    }
+}
+
+// a sum of nothing
+static __global__ __launch_bounds__(MV_THREADS) void fill_zero(MatvecArgs a) {
+    const uint64_t r = (uint64_t)blockIdx.x * MV_THREADS + threadIdx.x;
+    if (r >= a.rows) return;
+    for (uint32_t t = 0; t < a.tokens; ++t) store_elem(a.y, t * a.y_stride + r, a.y_kind, 0.0f);
 }
 
 // ---- rows by id -----------------------------------------------------------------------------------------

@@ -54,6 +54,34 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
     return stride < (1ull << 40) && (tokens <= 1 || stride >= width);
 }
 
+// Shared memory of one workgroup for x.
+constexpr uint32_t X_LDS = 60 << 10;
+
+template <class F>
+void launch_quads(MatvecArgs a, hipStream_t st) {
+    typedef Slice<F> S;
+    const uint32_t steps = (uint32_t)((a.cols + 1023) / 1024);
+    const uint64_t tiles = (a.rows + 3) / 4;
+    const bool one = a.tokens == 1;
+    const uint32_t xcols = one ? a.pieces : a.tokens, chain = one ? 1 : a.pieces;
+    const uint32_t sums = S::OFFSET ? S::NSUB : 0;
+    // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
+    a.ksplit = 1;
+    while (a.ksplit < QD_WAVES && a.ksplit < steps && tiles * a.ksplit < 2048 && x_bytes(32 * a.ksplit, xcols, chain, sums, a.tokens) <= X_LDS)
+        a.ksplit *= 2;
+    const uint32_t unit = 16 * a.ksplit;                             // a chunk is a whole number of these slices
+    const uint32_t per = x_bytes(unit, xcols, chain, sums, a.tokens);
+    const uint32_t most = std::max(1u, X_LDS / per), need = (steps + a.ksplit - 1) / a.ksplit, rounds = (need + most - 1) / most;
+    a.chunk = (need + rounds - 1) / rounds * unit;
+    const uint32_t bytes = std::max<uint32_t>(x_bytes(a.chunk, xcols, chain, sums, a.tokens), QD_WAVES * 16 * 4);
+    const uint32_t groups = QD_WAVES / a.ksplit;
+    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * groups) {
+        const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + groups - 1) / groups));
+        if (xcols == 1) matvec_quads<F, 1><<<grid, QD_THREADS, bytes, st>>>(a);
+        else matvec_quads<F, 4><<<grid, QD_THREADS, bytes, st>>>(a);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -72,18 +100,21 @@ ggq_status ggq_matvec_device(uint32_t ty, uint64_t rows, uint64_t cols, const vo
     if (!d_y || (cols && (!d_w || !d_x))) return GGQ_INVALID;
     if ((uintptr_t)d_y % yb != 0 || (uintptr_t)d_x % xb != 0) return GGQ_MISALIGNED;
     a.w = (const uint8_t *)d_w;
-    a.x = d_x;
-    a.y = d_y;
     a.rows = rows;
     a.cols = cols;
-    a.tokens = tokens;
     a.x_stride = x_stride;
     a.y_stride = y_stride;
-    const uint32_t gx = (uint32_t)((rows + 3) / 4);
-    const uint64_t per = std::max<uint64_t>(1, std::min<uint64_t>(65535, MAX_GRID / gx));
-    for (uint64_t t = 0; t < tokens; t += per) {
-        const dim3 grid(gx, (uint32_t)std::min(per, tokens - t));
-#define CASE(F) matvec_rows<F><<<grid, MV_THREADS, 0, (hipStream_t)hip_stream>>>(a, t)
+    a.pieces = x_type == GGQ_TYPE_F32 ? 3 : x_type == GGQ_TYPE_F16 ? 2 : 1;
+    hipStream_t st = (hipStream_t)hip_stream;
+    for (uint64_t t = 0; t < tokens; t += 4) {
+        a.tokens = (uint32_t)std::min<uint64_t>(4, tokens - t);
+        a.x = (const uint8_t *)d_x + t * x_stride * xb;
+        a.y = (uint8_t *)d_y + t * y_stride * yb;
+        if (cols == 0) {
+            fill_zero<<<(uint32_t)((rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
+            continue;
+        }
+#define CASE(F) launch_quads<F>(a, st)
         GGQ_FOR_TYPE(ty, CASE)
 #undef CASE
     }

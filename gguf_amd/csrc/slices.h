@@ -1,0 +1,469 @@
+// slices.h -- a lane's share of a packed row, for the products with packed weights (matmul.h).
+//
+// A row is cut into slices of 64 elements.  One lane loads the packed bytes of one slice and turns them into whole-number
+// codes in bf16, which holds every code exactly (at most 8 significant bits), so that products with bf16 pieces of x are
+// exact.  Elements that share a scale form a sub-block of SUB = 16, 32 or 64:
+//     w = a * q - c      q: code, a: scale of the sub-block, c: its offset
+// and the product needs a and c once per sub-block:  sum of w x = a * (sum of q x) - c * (sum of x).
+//
+// Per format:
+//     NSUB, SUB       sub-blocks of a slice and their elements (NSUB * SUB = 64)
+//     OFFSET          whether c can differ from zero
+//     PLANES          the sub-blocks of a slice are 16 elements each, 32 elements apart (two-level formats of 16-element
+//                     sub-blocks: the codes of elements l, l + 32, l + 64 and l + 96 share a byte); otherwise the slice is 64
+//                     consecutive elements
+//     Raw             the packed bytes in registers
+//     load(row, s, n) slice s of a row with n slices worth of data (s < n); never reads past the row's end
+//     codes<S>(r, b)  the codes of sub-block S as pairs of bf16, elements in order
+//     scale<S>(r)     {a, c} of sub-block S
+//
+// Codes below 16 become bf16 two at a time by v_cvt_scalef32_pk_bf16_fp8: an e4m3 byte of 0..15 is a subnormal or in the
+// first binade, both of which step by 2^-9, so with a scale of 2^9 its value is the byte itself (one full-rate instruction
+// for two codes; by way of f32 it is three).  Wider codes go through f32.
+#pragma once
+#include "formats.h"
+
+namespace ggq {
+
+typedef uint32_t u32_any __attribute__((aligned(1), may_alias));
+typedef uint16_t u16_any __attribute__((aligned(1), may_alias));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x4 u32x4_any __attribute__((aligned(1), may_alias));
+typedef u32x2 u32x2_any __attribute__((aligned(1), may_alias));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ u32x4 ld16(const uint8_t *p) { return *(const u32x4_any *)p; }
+__device__ __forceinline__ u32x2 ld8(const uint8_t *p) { return *(const u32x2_any *)p; }
+__device__ __forceinline__ uint32_t ld4(const uint8_t *p) { return *(const u32_any *)p; }
+__device__ __forceinline__ uint32_t ld2(const uint8_t *p) { return *(const u16_any *)p; }
+
+// four codes below 16 (bytes of w) -> two words of two bf16
+__device__ __forceinline__ void small_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, true));
+}
+// the upper halves of two f32 that bf16 holds exactly
+__device__ __forceinline__ uint32_t upper_halves(float lo, float hi) {
+    return __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo), 0x07060302u);
+}
+__device__ __forceinline__ void byte_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    w = opaque(w);
+    lo = upper_halves(ub<0>(w), ub<1>(w));
+    hi = upper_halves(ub<2>(w), ub<3>(w));
+}
+__device__ __forceinline__ void signed_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    w = opaque(w);
+    lo = upper_halves(sb<0>(w), sb<1>(w));
+    hi = upper_halves(sb<2>(w), sb<3>(w));
+}
+
+struct SubScale { float a, c; };
+
+// ---- 32-element formats: a slice is two blocks; the second may be missing at the end of a row --------------
+// `n`: blocks of the row.  A missing block is loaded as the last one and gets the scale 0.
+struct SliceOfTwo {
+    static constexpr bool PLANES = false;
+    static constexpr int NSUB = 2, SUB = 32;
+    static constexpr uint32_t UNIT = 32;
+};
+
+template <class F> struct Slice;
+
+// the 16-bit floats as one-element block types
+struct WF16 { static constexpr uint32_t N = 1, BYTES = 2; };
+struct WBF16 { static constexpr uint32_t N = 1, BYTES = 2; };
+template <class F> constexpr bool is_float_type = false;
+template <> constexpr bool is_float_type<WF16> = true;
+template <> constexpr bool is_float_type<WBF16> = true;
+
+template <uint32_t BYTES, uint32_t HEAD>       // HEAD bytes of scales in front of 16 bytes of nibbles
+struct NibbleRaw {
+    u32x4 q[2];
+    uint32_t h[2];
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t blocks) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t b = 2 * s + k;
+            const uint8_t *p = row + (b < blocks ? b : blocks - 1) * BYTES;
+            h[k] = HEAD == 2 ? ld2(p) : ld4(p);
+            if (b >= blocks) h[k] = 0;
+            q[k] = ld16(p + HEAD);
+        }
+    }
+    template <int S>
+    __device__ __forceinline__ void codes(uint32_t (&b)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            small_codes(q[S][i] & 0x0F0F0F0Fu, b[2 * i], b[2 * i + 1]);
+            small_codes((q[S][i] >> 4) & 0x0F0F0F0Fu, b[8 + 2 * i], b[9 + 2 * i]);
+        }
+    }
+};
+template <> struct Slice<Q4_0> : SliceOfTwo {
+    static constexpr bool OFFSET = true;
+    typedef NibbleRaw<18, 2> Raw;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const float d = h2f(r.h[S]);
+        return {d, 8.0f * d};
+    }
+};
+template <> struct Slice<Q4_1> : SliceOfTwo {
+    static constexpr bool OFFSET = true;
+    typedef NibbleRaw<20, 4> Raw;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        return {h2f(r.h[S] & 0xFFFFu), -h2f(r.h[S] >> 16)};
+    }
+};
+template <> struct Slice<IQ4NL> : SliceOfTwo {
+    static constexpr bool OFFSET = false;
+    typedef NibbleRaw<18, 2> Raw;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            signed_codes(iq4_lookup4(r.q[S][i] & 0x0F0F0F0Fu) ^ 0x80808080u, b[2 * i], b[2 * i + 1]);
+            signed_codes(iq4_lookup4((r.q[S][i] >> 4) & 0x0F0F0F0Fu) ^ 0x80808080u, b[8 + 2 * i], b[9 + 2 * i]);
+        }
+    }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.h[S]), 0.0f}; }
+};
+
+template <uint32_t BYTES, uint32_t HEAD>       // ... with 4 bytes of fifth bits between
+struct FiveRaw {
+    u32x4 q[2];
+    uint32_t h[2], hi[2];
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t blocks) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t b = 2 * s + k;
+            const uint8_t *p = row + (b < blocks ? b : blocks - 1) * BYTES;
+            h[k] = HEAD == 2 ? ld2(p) : ld4(p);
+            if (b >= blocks) h[k] = 0;
+            hi[k] = ld4(p + HEAD);
+            q[k] = ld16(p + HEAD + 4);
+        }
+    }
+    template <int S>
+    __device__ __forceinline__ void codes(uint32_t (&b)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            byte_codes((q[S][i] & 0x0F0F0F0Fu) | (spread4(hi[S] >> (4 * i)) << 4), b[2 * i], b[2 * i + 1]);
+            byte_codes(((q[S][i] >> 4) & 0x0F0F0F0Fu) | (spread4(hi[S] >> (16 + 4 * i)) << 4), b[8 + 2 * i], b[9 + 2 * i]);
+        }
+    }
+};
+template <> struct Slice<Q5_0> : SliceOfTwo {
+    static constexpr bool OFFSET = true;
+    typedef FiveRaw<22, 2> Raw;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const float d = h2f(r.h[S]);
+        return {d, 16.0f * d};
+    }
+};
+template <> struct Slice<Q5_1> : SliceOfTwo {
+    static constexpr bool OFFSET = true;
+    typedef FiveRaw<24, 4> Raw;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        return {h2f(r.h[S] & 0xFFFFu), -h2f(r.h[S] >> 16)};
+    }
+};
+
+template <uint32_t BYTES, uint32_t HEAD>       // 32 signed bytes
+struct ByteRaw {
+    u32x4 q[2][2];
+    uint32_t h[2];
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t blocks) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const uint32_t b = 2 * s + k;
+            const uint8_t *p = row + (b < blocks ? b : blocks - 1) * BYTES;
+            h[k] = b < blocks ? ld2(p) : 0u;
+            q[k][0] = ld16(p + HEAD);
+            q[k][1] = ld16(p + HEAD + 16);
+        }
+    }
+    template <int S>
+    __device__ __forceinline__ void codes(uint32_t (&b)[16]) const {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) signed_codes(q[S][i / 4][i % 4], b[2 * i], b[2 * i + 1]);
+    }
+};
+template <> struct Slice<Q8_0> : SliceOfTwo {
+    static constexpr bool OFFSET = false;
+    typedef ByteRaw<34, 2> Raw;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.h[S]), 0.0f}; }
+};
+template <> struct Slice<Q8_1> : SliceOfTwo {
+    static constexpr bool OFFSET = false;
+    typedef ByteRaw<36, 4> Raw;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.h[S]), 0.0f}; }
+};
+
+// ---- 256-element formats: four slices a block ------------------------------------------------------------
+struct SliceOfQuarter {
+    static constexpr uint32_t UNIT = 64;
+};
+
+// 6-bit scale and minimum of sub-blocks 2j and 2j + 1 (j = 0..3) from the twelve bytes in words s0, s1, s2: for j < 2 the
+// first two words' low six bits, for j >= 2 the third word's nibbles under the first two words' top two bits
+struct PairOfK4 { uint32_t sc[2], mn[2]; };
+__device__ __forceinline__ PairOfK4 scales_k4(uint32_t s0, uint32_t s1, uint32_t s2, uint32_t j) {
+    const uint32_t sh = 16 * (j & 1);            // two bytes of each word
+    const uint32_t a = s0 >> sh, b = s1 >> sh, c = s2 >> sh;
+    const bool low = j < 2;
+    const uint32_t sc = low ? a & 0x3F3Fu : (c & 0x0F0Fu) | ((a >> 2) & 0x3030u);
+    const uint32_t mn = low ? b & 0x3F3Fu : ((c >> 4) & 0x0F0Fu) | ((b >> 2) & 0x3030u);
+    return {{sc & 0xFFu, (sc >> 8) & 0xFFu}, {mn & 0xFFu, (mn >> 8) & 0xFFu}};
+}
+template <> struct Slice<Q4K> : SliceOfQuarter {
+    static constexpr bool PLANES = false, OFFSET = true;
+    static constexpr int NSUB = 2, SUB = 32;
+    struct Raw {
+        u32x4 h, q[2];
+        uint32_t j;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
+            const uint8_t *p = row + (s >> 2) * 144;
+            j = s & 3;
+            h = ld16(p);
+            q[0] = ld16(p + 16 + 32 * j);
+            q[1] = ld16(p + 32 + 32 * j);
+        }
+    };
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) small_codes((r.q[i / 4][i % 4] >> (4 * S)) & 0x0F0F0F0Fu, b[2 * i], b[2 * i + 1]);
+    }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], r.j);
+        return {h2f(r.h[0] & 0xFFFFu) * (float)k.sc[S], h2f(r.h[0] >> 16) * (float)k.mn[S]};
+    }
+};
+template <> struct Slice<Q5K> : SliceOfQuarter {
+    static constexpr bool PLANES = false, OFFSET = true;
+    static constexpr int NSUB = 2, SUB = 32;
+    struct Raw {
+        u32x4 h, q[2], f[2];
+        uint32_t j;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
+            const uint8_t *p = row + (s >> 2) * 176;
+            j = s & 3;
+            h = ld16(p);
+            f[0] = ld16(p + 16);
+            f[1] = ld16(p + 32);
+            q[0] = ld16(p + 48 + 32 * j);
+            q[1] = ld16(p + 64 + 32 * j);
+        }
+    };
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const uint32_t five = (r.f[i / 4][i % 4] >> (2 * r.j + S)) & 0x01010101u;
+            byte_codes(((r.q[i / 4][i % 4] >> (4 * S)) & 0x0F0F0F0Fu) | (five << 4), b[2 * i], b[2 * i + 1]);
+        }
+    }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], r.j);
+        return {h2f(r.h[0] & 0xFFFFu) * (float)k.sc[S], h2f(r.h[0] >> 16) * (float)k.mn[S]};
+    }
+};
+template <> struct Slice<IQ4XS> : SliceOfQuarter {
+    static constexpr bool PLANES = false, OFFSET = false;
+    static constexpr int NSUB = 2, SUB = 32;
+    struct Raw {
+        u32x2 h;
+        u32x4 q[2];
+        uint32_t j;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
+            const uint8_t *p = row + (s >> 2) * 136;
+            j = s & 3;
+            h = ld8(p);
+            q[0] = ld16(p + 8 + 32 * j);
+            q[1] = ld16(p + 24 + 32 * j);
+        }
+    };
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            signed_codes(iq4_lookup4(r.q[S][i] & 0x0F0F0F0Fu) ^ 0x80808080u, b[2 * i], b[2 * i + 1]);
+            signed_codes(iq4_lookup4((r.q[S][i] >> 4) & 0x0F0F0F0Fu) ^ 0x80808080u, b[8 + 2 * i], b[9 + 2 * i]);
+        }
+    }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const uint32_t ls = ((r.h[1] >> (8 * r.j + 4 * S)) & 0xFu) | (((r.h[0] >> (16 + 4 * r.j + 2 * S)) & 3u) << 4);
+        return {h2f(r.h[0] & 0xFFFFu) * (float)((int)ls - 32), 0.0f};
+    }
+};
+
+// Slice s = (block, half n, 16-element column h): sub-block p = elements 128 n + 32 p + 16 h + 0..15 of the block.
+struct SliceOfPlanes : SliceOfQuarter {
+    static constexpr bool PLANES = true;
+    static constexpr int NSUB = 4, SUB = 16;
+};
+template <> struct Slice<Q6K> : SliceOfPlanes {
+    static constexpr bool OFFSET = true;
+    struct Raw {
+        u32x4 l[2], f;
+        u32x2 sc;
+        uint32_t d, h;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
+            const uint8_t *p = row + (s >> 2) * 210;
+            const uint32_t n = (s >> 1) & 1;
+            h = s & 1;
+            l[0] = ld16(p + 64 * n + 16 * h);
+            l[1] = ld16(p + 64 * n + 32 + 16 * h);
+            f = ld16(p + 128 + 32 * n + 16 * h);
+            sc = ld8(p + 192 + 8 * n);
+            d = ld2(p + 208);
+        }
+    };
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t low = (r.l[S & 1][i] >> (4 * (S >> 1))) & 0x0F0F0F0Fu;
+            byte_codes(low | (((r.f[i] >> (2 * S)) & 0x03030303u) << 4), b[2 * i], b[2 * i + 1]);
+        }
+    }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const int sc = (int)(int8_t)(r.sc[S >> 1] >> (16 * (S & 1) + 8 * r.h));
+        const float a = h2f(r.d) * (float)sc;
+        return {a, 32.0f * a};
+    }
+};
+template <> struct Slice<Q2K> : SliceOfPlanes {
+    static constexpr bool OFFSET = true;
+    struct Raw {
+        u32x4 q;
+        u32x2 sc;
+        uint32_t dm, h;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
+            const uint8_t *p = row + (s >> 2) * 84;
+            const uint32_t n = (s >> 1) & 1;
+            h = s & 1;
+            sc = ld8(p + 8 * n);
+            q = ld16(p + 16 + 32 * n + 16 * h);
+            dm = ld4(p + 80);
+        }
+    };
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) small_codes((r.q[i] >> (2 * S)) & 0x03030303u, b[2 * i], b[2 * i + 1]);
+    }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const uint32_t sc = (r.sc[S >> 1] >> (16 * (S & 1) + 8 * r.h)) & 0xFFu;
+        return {h2f(r.dm & 0xFFFFu) * (float)(sc & 0xFu), h2f(r.dm >> 16) * (float)(sc >> 4)};
+    }
+};
+template <> struct Slice<Q3K> : SliceOfPlanes {
+    static constexpr bool OFFSET = true;
+    struct Raw {
+        u32x4 q, f;
+        uint32_t s0, s1, s2, d, n, h;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
+            const uint8_t *p = row + (s >> 2) * 110;
+            n = (s >> 1) & 1;
+            h = s & 1;
+            f = ld16(p + 16 * h);
+            q = ld16(p + 32 + 32 * n + 16 * h);
+            s0 = ld4(p + 96);
+            s1 = ld4(p + 100);
+            s2 = ld4(p + 104);
+            d = ld2(p + 108);
+        }
+    };
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t high = (r.f[i] >> (4 * r.n + S)) & 0x01010101u;
+            small_codes(((r.q[i] >> (2 * S)) & 0x03030303u) | (high << 2), b[2 * i], b[2 * i + 1]);
+        }
+    }
+    // sub-block g = 8 n + 2 S + h of 16: low nibble g % 8 of bytes 0..7 (high nibble for n = 1), top bits g / 4 of byte g % 4
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
+        const uint32_t w = S < 2 ? r.s0 : r.s1, sh = 16 * (S & 1) + 8 * r.h;
+        const uint32_t low = (w >> (sh + 4 * r.n)) & 0xFu, top = (r.s2 >> (sh + 4 * r.n + 2 * (S >> 1))) & 3u;
+        const float a = h2f(r.d) * (float)((int)(low | (top << 4)) - 32);
+        return {a, 4.0f * a};
+    }
+};
+template <> struct Slice<Q8K> : SliceOfQuarter {
+    static constexpr bool PLANES = false, OFFSET = false;
+    static constexpr int NSUB = 2, SUB = 32;
+    struct Raw {
+        u32x4 q[4];
+        uint32_t d;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
+            const uint8_t *p = row + (s >> 2) * 290;
+            d = ld2(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = ld16(p + 2 + 64 * (s & 3) + 16 * i);
+        }
+    };
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) signed_codes(r.q[2 * S + i / 4][i % 4], b[2 * i], b[2 * i + 1]);
+    }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.d), 0.0f}; }
+};
+
+// ---- 16-bit floats: rows of any length, 64 elements a slice ------------------------------------------------
+// The weights are their own codes; a half has eleven significant bits and becomes two bf16 (WP pieces).
+struct FloatRaw {
+    u32x4 q[8];
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t cols) {
+        const uint8_t *p = row + 128 * (uint64_t)s;
+        const uint32_t left = cols - 64 * s;
+        if (left >= 64) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = ld16(p + 16 * i);
+        } else {
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) {
+                uint32_t w = 2 * i < left ? ld2(p + 4 * i) : 0u;
+                if (2 * i + 1 < left) w |= ld2(p + 4 * i + 2) << 16;
+                q[i / 4][i % 4] = w;
+            }
+        }
+    }
+};
+struct SliceOfFloats {
+    static constexpr bool PLANES = false, OFFSET = false;
+    static constexpr int NSUB = 2, SUB = 32;
+    static constexpr uint32_t UNIT = 1;
+    typedef FloatRaw Raw;
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &) { return {1.0f, 0.0f}; }
+};
+// upper 16 bits of v, a NaN kept a NaN; `rest` = v minus that, exactly (0 where v is not finite)
+__device__ __forceinline__ uint32_t take_bf16(float v, float &rest) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const bool odd = (b & 0x7F800000u) == 0x7F800000u;
+    const uint32_t t = (v != v ? b | 0x00400000u : b) & 0xFFFF0000u;
+    rest = odd ? 0.0f : v - __builtin_bit_cast(float, t);
+    return t >> 16;
+}
+template <> struct Slice<WBF16> : SliceOfFloats {
+    static constexpr int WP = 1;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16], int) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) b[i] = r.q[4 * S + i / 4][i % 4];
+    }
+};
+template <> struct Slice<WF16> : SliceOfFloats {
+    static constexpr int WP = 2;
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16], int piece) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const uint32_t w = r.q[4 * S + i / 4][i % 4];
+            float l0, l1, none;
+            const uint32_t h0 = take_bf16(h2f(w & 0xFFFFu), l0), h1 = take_bf16(h2f(w >> 16), l1);
+            b[i] = piece == 0 ? h0 | (h1 << 16) : take_bf16(l0, none) | (take_bf16(l1, none) << 16);
+        }
+    }
+};
+
+}  // namespace ggq
