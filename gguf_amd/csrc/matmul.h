@@ -67,10 +67,10 @@ struct MatvecArgs {
     void *y;
     uint64_t rows, cols, x_stride, y_stride;
     uint64_t first_tile;      // groups of four rows before this launch's
-    uint32_t tokens;          // of this launch's group: 1..4
+    uint32_t tokens;          // of this launch's group: at most NC / parts
     uint32_t x_kind, y_kind;
-    uint32_t pieces;          // bf16 pieces of an element of x: 1 (bf16), 2 (f16), 3 (f32)
-    uint32_t chunk;           // slices staged at a time, a multiple of 16 * ksplit
+    uint32_t parts;           // columns that a token takes: its bf16 pieces, or 1 where they follow each other
+    uint32_t chunk;           // steps staged at a time, a multiple of ksplit
     uint32_t ksplit;          // waves that share a row group's columns: 1, 2, 4 or 8
 };
 
@@ -80,26 +80,26 @@ constexpr uint32_t QD_WAVES = 8, QD_THREADS = 64 * QD_WAVES;
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 
-// x in shared memory, as the matrix unit takes it: fragments of eight bf16 (16 bytes), [piece][k][slice][column], k = the
-// fragment's place in its slice.  The 16 quads of a wave read the same k of 16 neighbouring slices, so their addresses are
-// consecutive; the pitch of a k is odd (in fragments), so that the staging threads, which run along k first, do not meet
-// in one bank either.  `cols`: columns kept, 1..4; behind the fragments lie the sums of x over each sub-block,
-// [sub-block][slice][column], for the formats with an offset.
-struct XLayout {
-    uint32_t cols, pitch, slices, chain, sums, sum_cols;
-    __device__ __forceinline__ XLayout(uint32_t slices_, uint32_t cols_, uint32_t chain_, uint32_t sum_cols_)
-        : cols(cols_), pitch(slices_ * cols_ | 1u), slices(slices_), chain(chain_), sums(chain_ * 8 * (slices_ * cols_ | 1u) * 16), sum_cols(sum_cols_) {}
+// x in shared memory, as the matrix unit takes it: fragments of eight bf16 (16 bytes).  A step (16 slices, 1024 elements)
+// is [chain][k][slice][column], k = the fragment's place in its slice: the 16 quads of a wave read the same k of 16
+// neighbouring slices, so their addresses are consecutive and all other parts of the address are constants.  16 bytes
+// between one k and the next keep the staging threads, which run along k first, out of each other's banks.  Behind the
+// fragments, for formats with an offset, the sum of x over each sub-block: [sub-block][slice][column], f32, a token's whole
+// sum in the first of its columns and zero in the others.
+//   NC columns: tokens times their pieces side by side; CHAIN: pieces one after the other into the same columns.
+template <class F, int NC, int CHAIN>
+struct XStep {
+    typedef Slice<F> S;
+    static constexpr uint32_t K = 256 * NC + 16;
+    static constexpr uint32_t SUMS = CHAIN * 8 * K;
+    static constexpr uint32_t BYTES = SUMS + (S::OFFSET ? S::NSUB * 64 * NC : 0);
 };
-__host__ __device__ __forceinline__ uint32_t x_bytes(uint32_t slices, uint32_t cols, uint32_t chain, uint32_t nsub, uint32_t sum_cols) {
-    return chain * 8 * (slices * cols | 1u) * 16 + nsub * slices * sum_cols * 4;
-}
 
-__device__ __forceinline__ float quad_xor1(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0xB1, 0xF, 0xF, true));
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
-__device__ __forceinline__ float quad_xor2(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x4E, 0xF, 0xF, true));
-}
+constexpr int QUAD_XOR1 = 0xB1, QUAD_XOR2 = 0x4E, ROW_ROR4 = 0x124, ROW_ROR8 = 0x128;
 
 // eight elements of x from c on, 0 past the end
 __device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, uint64_t cols, uint32_t kind, float (&v)[8]) {
@@ -126,106 +126,100 @@ __device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, ui
     }
 }
 
-// Stages slices [first, first + l.slices) of `tokens` rows of x.  row(t): the element offset of token t's row.
-// one_token: the pieces of the only token are the columns; otherwise tokens are, and the pieces follow each other.
-template <class F, class Row>
-__device__ __forceinline__ void stage_x(uint8_t *lds, const XLayout &l, uint32_t first, const void *x, uint32_t kind, uint64_t cols,
-                                        uint32_t tokens, uint32_t pieces, bool one_token, Row row) {
+// Stages `steps` steps of x from step `first` on.  row(t): the element offset of token t's row.
+template <class F, int NC, int CHAIN, class Row>
+__device__ __forceinline__ void stage_x(uint8_t *lds, uint32_t first, uint32_t steps, const void *x, uint32_t kind, uint64_t cols,
+                                        uint32_t tokens, uint32_t parts, Row row) {
     typedef Slice<F> S;
-    const uint32_t frags = l.slices * 8;
-    for (uint32_t i = threadIdx.x; i < frags * tokens; i += blockDim.x) {
-        const uint32_t t = tokens == 1 ? 0 : i / frags, f = i - t * frags;
+    typedef XStep<F, NC, CHAIN> X;
+    const uint32_t frags = steps * 128;
+    for (uint32_t i = threadIdx.x; i < frags * tokens; i += blockDim.x) {       // whole waves: frags is a multiple of 64
+        const uint32_t t = NC == 1 || tokens == 1 ? 0 : i / frags, f = i - t * frags;
         uint32_t sl, k;
         if constexpr (S::PLANES) {
-            sl = ((f >> 5) << 2) | ((f >> 3) & 2u) | ((f >> 1) & 1u);
+            sl = ((f >> 3) & 12u) | ((f >> 3) & 2u) | ((f >> 1) & 1u);
             k = ((f >> 1) & 6u) | (f & 1u);
         } else {
-            sl = f >> 3;
+            sl = (f >> 3) & 15u;
             k = f & 7u;
         }
+        uint8_t *step = lds + (f >> 7) * X::BYTES;
         float v[8];
-        load8(x, row(t), (uint64_t)first * 64 + f * 8, cols, kind, v);
-        float sum = 0.0f;
+        load8(x, row(t), ((uint64_t)first * 128 + f) * 8, cols, kind, v);
+        const uint32_t col = t * parts;
         if constexpr (S::OFFSET) {
-            sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-            sum += quad_xor1(sum);
-            if (S::SUB == 32) sum += quad_xor2(sum);
+            float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            sum += dpp<QUAD_XOR1>(sum);
+            if (S::SUB == 32) sum += dpp<QUAD_XOR2>(sum);
             if (f % (S::SUB / 8) == 0) {
-                const uint32_t sub = k / (S::SUB / 8);
-                ((float *)(lds + l.sums))[(sub * l.slices + sl) * l.sum_cols + t] = sum;
+                float *to = (float *)(step + X::SUMS) + (k / (S::SUB / 8) * 16 + sl) * NC + col;
+                to[0] = sum;
+                for (uint32_t p = 1; p < parts; ++p) to[p] = 0.0f;
             }
         }
-        for (uint32_t p = 0; p < pieces; ++p) {
+        uint8_t *to = step + k * X::K + (sl * NC + col) * 16;
+        const uint32_t pieces = CHAIN > 1 ? CHAIN : parts, stride = CHAIN > 1 ? 8 * X::K : 16;
+        for (uint32_t p = 0; p < pieces; ++p, to += stride) {
             uint32_t h[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) h[j] = take_bf16(v[j], v[j]);
             const u32x4 w = {h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
-            const uint32_t chain = one_token ? 0 : p, c = one_token ? p : t;
-            *(u32x4 *)(lds + 16 * ((chain * 8 + k) * l.pitch + sl * l.cols + c)) = w;
+            *(u32x4 *)to = w;
         }
     }
 }
 
-// acc[c] += the lane's slice of its row times column c of x
-template <class F, int NC>
-__device__ __forceinline__ void add_slice(const typename Slice<F>::Raw &raw, bool valid, const uint8_t *lds, const XLayout &l, uint32_t sl,
-                                          uint32_t lane_col, float (&acc)[NC]);
-
-template <class F, int NC, int S>
-__device__ __forceinline__ void add_sub(const typename Slice<F>::Raw &raw, bool valid, const uint8_t *lds, const XLayout &l, uint32_t sl,
-                                        uint32_t lane_col, float (&acc)[NC]) {
+// acc[c] += sub-block S of the lane's slice times column c of x.  `x`: the step's fragments, from the lane's own on;
+// `sums`: the step's sums from the lane's slice on.
+template <class F, int NC, int CHAIN, int S>
+__device__ __forceinline__ void add_sub(const typename Slice<F>::Raw &raw, const typename Slice<F>::Lane &lane, const uint8_t *x,
+                                        const uint8_t *sums, float (&acc)[NC]) {
     typedef Slice<F> T;
-    constexpr int WORDS = T::SUB / 2;
+    typedef XStep<F, NC, CHAIN> X;
+    constexpr int FRAGS = T::SUB / 8, WORDS = T::SUB / 2;
+    constexpr int WP = [] { if constexpr (is_float_type<F>) return T::WP; else return 1; }();
     f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-    auto products = [&](const uint32_t (&b)[WORDS]) {
-        const uint8_t *at = lds + 16 * (S * (T::SUB / 8) * l.pitch + sl * l.cols + lane_col);
-        for (uint32_t p = 0; p < l.chain; ++p, at += 16 * 8 * l.pitch) {
 #pragma unroll
-            for (int k = 0; k < T::SUB / 8; ++k) {
-                const u32x4 a = *(const u32x4 *)(at + 16 * k * l.pitch);
+    for (int piece = 0; piece < WP; ++piece) {
+        uint32_t b[WORDS];
+        if constexpr (is_float_type<F>) T::template codes<S>(raw, lane, b, piece);
+        else T::template codes<S>(raw, lane, b);
+#pragma unroll
+        for (int p = 0; p < CHAIN; ++p)
+#pragma unroll
+            for (int k = 0; k < FRAGS; ++k) {
+                const u32x4 a = *(const u32x4 *)(x + (p * 8 + S * FRAGS + k) * X::K);
                 const u32x2 a0 = {a[0], a[1]}, a1 = {a[2], a[3]}, b0 = {b[4 * k], b[4 * k + 1]}, b1 = {b[4 * k + 2], b[4 * k + 3]};
                 d = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, a0), __builtin_bit_cast(s16x4, b0), d, 0, 0, 0);
                 d = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, a1), __builtin_bit_cast(s16x4, b1), d, 0, 0, 0);
             }
-        }
-    };
-    uint32_t b[WORDS];
-    if constexpr (is_float_type<F>) {
-#pragma unroll
-        for (int piece = 0; piece < T::WP; ++piece) {
-            T::template codes<S>(raw, b, piece);
-            products(b);
-        }
-    } else {
-        T::template codes<S>(raw, b);
-        products(b);
     }
-    SubScale s = T::template scale<S>(raw);
-    if (!valid) s.a = s.c = 0.0f;
+    const SubScale s = T::template scale<S>(raw, lane);
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = __builtin_fmaf(s.a, d[c], acc[c]);
     if constexpr (T::OFFSET) {
-        const float *sums = (const float *)(lds + l.sums) + (S * l.slices + sl) * l.sum_cols;
+        const float *sum = (const float *)(sums + S * 64 * NC);
 #pragma unroll
-        for (int c = 0; c < NC; ++c)
-            if ((uint32_t)c < l.sum_cols) acc[c] = __builtin_fmaf(-s.c, sums[c], acc[c]);
+        for (int c = 0; c < NC; ++c) acc[c] = __builtin_fmaf(-s.c, sum[c], acc[c]);
     }
 }
-template <class F, int NC>
-__device__ __forceinline__ void add_slice(const typename Slice<F>::Raw &raw, bool valid, const uint8_t *lds, const XLayout &l, uint32_t sl,
-                                          uint32_t lane_col, float (&acc)[NC]) {
-    add_sub<F, NC, 0>(raw, valid, lds, l, sl, lane_col, acc);
-    add_sub<F, NC, 1>(raw, valid, lds, l, sl, lane_col, acc);
+template <class F, int NC, int CHAIN>
+__device__ __forceinline__ void add_slice(const typename Slice<F>::Raw &raw, const typename Slice<F>::Lane &lane, const uint8_t *x,
+                                          const uint8_t *sums, float (&acc)[NC]) {
+    add_sub<F, NC, CHAIN, 0>(raw, lane, x, sums, acc);
+    add_sub<F, NC, CHAIN, 1>(raw, lane, x, sums, acc);
     if constexpr (Slice<F>::NSUB == 4) {
-        add_sub<F, NC, 2>(raw, valid, lds, l, sl, lane_col, acc);
-        add_sub<F, NC, 3>(raw, valid, lds, l, sl, lane_col, acc);
+        add_sub<F, NC, CHAIN, 2>(raw, lane, x, sums, acc);
+        add_sub<F, NC, CHAIN, 3>(raw, lane, x, sums, acc);
     }
 }
 
 // Sum over the 16 quads of a wave: afterwards every lane holds its row's total.
 __device__ __forceinline__ float quads_sum(float v) {
-#pragma unroll
-    for (int m = 4; m < 64; m <<= 1) v += __shfl_xor(v, m);
+    v += dpp<ROW_ROR8>(v);
+    v += dpp<ROW_ROR4>(v);
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
     return v;
 }
 
@@ -233,65 +227,56 @@ __device__ __forceinline__ float quads_sum(float v) {
 // slices at a time, each lane the packed bytes of its row's slice.  v_mfma_f32_4x4x4 with 16 blocks multiplies, in each
 // quad, the four rows' codes with up to four columns of x that the quad's lanes hold: every lane ends with its own row's
 // products, so that the sub-block's scale is applied in the lane that loaded it.  Columns are tokens, or the bf16 pieces
-// of the only token (f32 = three pieces, exactly; products with codes are exact, sums are f32).
-template <class F, int NC>
+// of a token (f32 = three pieces, exactly; products with codes are exact, sums are f32).
+template <class F, int NC, int CHAIN>
 __global__ __launch_bounds__(QD_THREADS) void matvec_quads(MatvecArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     typedef Slice<F> S;
-    const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64, quad = lane / 4;
+    typedef XStep<F, NC, CHAIN> X;
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), quad = lane / 4;
     const uint32_t kp = wave % a.ksplit, group = wave / a.ksplit, groups = QD_WAVES / a.ksplit;
-    const uint64_t tile = a.first_tile + (uint64_t)blockIdx.x * groups + group, row = tile * 4 + lane % 4;
-    const uint8_t *w = a.w + (row < a.rows ? row : a.rows - 1) * (a.cols / F::N * F::BYTES);
-    const uint32_t units = (uint32_t)(a.cols / S::UNIT), slices = (uint32_t)((a.cols + 63) / 64);
-    const bool one = a.tokens == 1;
-    const uint32_t xcols = one ? a.pieces : a.tokens, chain = one ? 1 : a.pieces;
-    const XLayout l(a.chunk, xcols, chain, a.tokens);
-    const uint32_t lane_col = lane % 4 < xcols ? lane % 4 : xcols - 1;
+    const uint64_t row = (a.first_tile + (uint64_t)blockIdx.x * groups + group) * 4 + lane % 4;
+    const uint32_t row_bytes = (uint32_t)(a.cols / F::N * F::BYTES), steps = (uint32_t)((a.cols + 1023) / 1024);
+    const uint8_t *w = a.w + (row < a.rows ? row : a.rows - 1) * row_bytes;
+    const typename S::Lane me(quad, row_bytes);
+    const uint8_t *x = lds + (quad * NC + (lane % 4 < NC ? lane % 4 : NC - 1)) * 16, *sums = lds + X::SUMS + quad * NC * 4;
     float acc[NC];
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = 0.0f;
 
-    typename S::Raw cur, nxt;
-    uint32_t s = kp * 16 + quad;                       // this lane's next slice
-    auto load = [&](typename S::Raw &r, uint32_t at) { r.load(w, at < slices ? at : slices - 1, units); };
-    load(cur, s);
-    for (uint32_t first = 0; first < slices; first += a.chunk) {
+    typename S::Raw r0, r1;
+    const uint32_t jump = S::STEP * a.ksplit;
+    uint32_t off = me.off + kp * S::STEP, step = kp;
+    r0.load(w, off, me);
+    for (uint32_t first = 0; first < steps; first += a.chunk) {
+        const uint32_t now = first + a.chunk < steps ? a.chunk : steps - first, end = first + now;
         if (first) __syncthreads();
-        stage_x<F>(lds, l, first, a.x, a.x_kind, a.cols, a.tokens, a.pieces, one, [&](uint32_t t) { return t * a.x_stride; });
+        stage_x<F, NC, CHAIN>(lds, first, now, a.x, a.x_kind, a.cols, a.tokens, a.parts, [&](uint32_t t) { return t * a.x_stride; });
         __syncthreads();
-        const uint32_t end = first + a.chunk < slices ? first + a.chunk : slices;
-        for (; s - quad < end; s += 16 * a.ksplit) {
-            if (s - quad + 16 * a.ksplit < slices) load(nxt, s + 16 * a.ksplit);
-            const bool valid = s < slices;
-            add_slice<F, NC>(cur, valid, lds, l, (valid ? s : slices - 1) - first, lane_col, acc);
-            cur = nxt;
+        uint32_t at = (step - first) * X::BYTES;
+        for (; step < end; step += a.ksplit, at += a.ksplit * X::BYTES) {
+            off += jump;
+            if (step + a.ksplit < steps) r1.load(w, off, me);
+            add_slice<F, NC, CHAIN>(r0, me, x + at, sums + at, acc);
+            r0 = r1;
         }
     }
-    if (NC > 1 && one) {
-        // the columns are pieces: only those that there are count
-        float sum = acc[0];
+    __syncthreads();                                   // the staged x is no longer needed
+    float *part = (float *)lds;                        // [wave][column][row]
 #pragma unroll
-        for (int c = 1; c < NC; ++c) sum += (uint32_t)c < a.pieces ? acc[c] : 0.0f;
-        acc[0] = sum;
+    for (int c = 0; c < NC; ++c) {
+        const float v = quads_sum(acc[c]);
+        if (lane < 4) part[(wave * NC + c) * 4 + lane] = v;
     }
-#pragma unroll
-    for (int c = 0; c < NC; ++c) acc[c] = quads_sum(acc[c]);
-    if (a.ksplit > 1) {
-        __syncthreads();                               // the staged x is no longer needed
-        float *part = (float *)lds;                    // [wave][column][row]
-        if (lane < 4)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) part[(wave * 4 + c) * 4 + lane] = acc[c];
-        __syncthreads();
-        if (kp == 0)
-#pragma unroll
-            for (int c = 0; c < NC; ++c)
-                for (uint32_t k = 1; k < a.ksplit; ++k) acc[c] += part[((wave + k) * 4 + c) * 4 + lane % 4];
-    }
-    if (kp == 0 && lane < 4 && row < a.rows) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c)
-            if ((uint32_t)c < a.tokens) store_elem(a.y, c * a.y_stride + row, a.y_kind, acc[c]);
+    __syncthreads();
+    // one thread per row and token: the waves' parts, and the token's pieces
+    if (threadIdx.x < groups * 4 * a.tokens) {
+        const uint32_t r = threadIdx.x % (groups * 4), t = threadIdx.x / (groups * 4), g = r / 4;
+        const uint64_t out = (a.first_tile + (uint64_t)blockIdx.x * groups) * 4 + r;
+        float v = 0.0f;
+        for (uint32_t k = 0; k < a.ksplit; ++k)
+            for (uint32_t p = 0; p < a.parts; ++p) v += part[((g * a.ksplit + k) * NC + t * a.parts + p) * 4 + r % 4];
+        if (out < a.rows) store_elem(a.y, t * a.y_stride + out, a.y_kind, v);
     }
 }
 

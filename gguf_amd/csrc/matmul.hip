@@ -46,7 +46,7 @@ bool elem_kind(uint32_t ty, uint32_t *kind, uint32_t *bytes) {
 }
 
 // Sizes beyond these have no use and would let products of sizes wrap.
-constexpr uint64_t MAX_DIM = 1ull << 31;
+constexpr uint64_t MAX_DIM = 1ull << 30;
 // Workgroups of one launch: the grid's threads are counted in 32 bits
 constexpr uint64_t MAX_GRID = 1ull << 22;
 
@@ -57,29 +57,43 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
 // Shared memory of one workgroup for x.
 constexpr uint32_t X_LDS = 60 << 10;
 
-template <class F>
+template <class F, int NC, int CHAIN>
 void launch_quads(MatvecArgs a, hipStream_t st) {
-    typedef Slice<F> S;
+    typedef XStep<F, NC, CHAIN> X;
     const uint32_t steps = (uint32_t)((a.cols + 1023) / 1024);
     const uint64_t tiles = (a.rows + 3) / 4;
-    const bool one = a.tokens == 1;
-    const uint32_t xcols = one ? a.pieces : a.tokens, chain = one ? 1 : a.pieces;
-    const uint32_t sums = S::OFFSET ? S::NSUB : 0;
     // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
     a.ksplit = 1;
-    while (a.ksplit < QD_WAVES && a.ksplit < steps && tiles * a.ksplit < 2048 && x_bytes(32 * a.ksplit, xcols, chain, sums, a.tokens) <= X_LDS)
-        a.ksplit *= 2;
-    const uint32_t unit = 16 * a.ksplit;                             // a chunk is a whole number of these slices
-    const uint32_t per = x_bytes(unit, xcols, chain, sums, a.tokens);
-    const uint32_t most = std::max(1u, X_LDS / per), need = (steps + a.ksplit - 1) / a.ksplit, rounds = (need + most - 1) / most;
-    a.chunk = (need + rounds - 1) / rounds * unit;
-    const uint32_t bytes = std::max<uint32_t>(x_bytes(a.chunk, xcols, chain, sums, a.tokens), QD_WAVES * 16 * 4);
-    const uint32_t groups = QD_WAVES / a.ksplit;
+    while (a.ksplit < QD_WAVES && a.ksplit < steps && tiles * a.ksplit < 2048 && 2 * a.ksplit * X::BYTES <= X_LDS) a.ksplit *= 2;
+    // equal chunks
+    const uint32_t turns = (steps + a.ksplit - 1) / a.ksplit, most = X_LDS / (X::BYTES * a.ksplit), chunks = (turns + most - 1) / most;
+    a.chunk = (turns + chunks - 1) / chunks * a.ksplit;
+    const uint32_t bytes = std::max<uint32_t>(std::min(a.chunk, steps) * X::BYTES, QD_WAVES * NC * 16), groups = QD_WAVES / a.ksplit;
     for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * groups) {
         const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + groups - 1) / groups));
-        if (xcols == 1) matvec_quads<F, 1><<<grid, QD_THREADS, bytes, st>>>(a);
-        else matvec_quads<F, 4><<<grid, QD_THREADS, bytes, st>>>(a);
+        matvec_quads<F, NC, CHAIN><<<grid, QD_THREADS, bytes, st>>>(a);
     }
+}
+
+// At most four tokens in one launch: columns of the matrix unit's four are tokens, or the pieces of one or two tokens
+// where all of them fit; otherwise a token is a column and its pieces follow each other.  Returns the tokens taken.
+template <class F>
+uint64_t launch_few(MatvecArgs a, uint64_t tokens, uint32_t pieces, hipStream_t st) {
+    a.tokens = (uint32_t)std::min<uint64_t>(tokens, 4);
+    a.parts = a.tokens * pieces <= 4 ? pieces : 1;
+    if (a.parts == pieces) {
+        switch (a.tokens * pieces) {
+        case 1: launch_quads<F, 1, 1>(a, st); break;
+        case 2: launch_quads<F, 2, 1>(a, st); break;
+        case 3: launch_quads<F, 3, 1>(a, st); break;
+        default: launch_quads<F, 4, 1>(a, st);
+        }
+    } else if (pieces == 2) {
+        launch_quads<F, 4, 2>(a, st);
+    } else {
+        launch_quads<F, 4, 3>(a, st);
+    }
+    return a.tokens;
 }
 
 }  // namespace
@@ -104,17 +118,17 @@ ggq_status ggq_matvec_device(uint32_t ty, uint64_t rows, uint64_t cols, const vo
     a.cols = cols;
     a.x_stride = x_stride;
     a.y_stride = y_stride;
-    a.pieces = x_type == GGQ_TYPE_F32 ? 3 : x_type == GGQ_TYPE_F16 ? 2 : 1;
+    const uint32_t pieces = x_type == GGQ_TYPE_F32 ? 3 : x_type == GGQ_TYPE_F16 ? 2 : 1;
     hipStream_t st = (hipStream_t)hip_stream;
-    for (uint64_t t = 0; t < tokens; t += 4) {
-        a.tokens = (uint32_t)std::min<uint64_t>(4, tokens - t);
+    for (uint64_t t = 0, done = 0; t < tokens; t += done) {
         a.x = (const uint8_t *)d_x + t * x_stride * xb;
         a.y = (uint8_t *)d_y + t * y_stride * yb;
         if (cols == 0) {
+            done = a.tokens = (uint32_t)std::min<uint64_t>(4, tokens - t);
             fill_zero<<<(uint32_t)((rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
             continue;
         }
-#define CASE(F) launch_quads<F>(a, st)
+#define CASE(F) done = launch_few<F>(a, tokens - t, pieces, st)
         GGQ_FOR_TYPE(ty, CASE)
 #undef CASE
     }

@@ -12,10 +12,13 @@
 //     PLANES          the sub-blocks of a slice are 16 elements each, 32 elements apart (two-level formats of 16-element
 //                     sub-blocks: the codes of elements l, l + 32, l + 64 and l + 96 share a byte); otherwise the slice is 64
 //                     consecutive elements
-//     Raw             the packed bytes in registers
-//     load(row, s, n) slice s of a row with n slices worth of data (s < n); never reads past the row's end
-//     codes<S>(r, b)  the codes of sub-block S as pairs of bf16, elements in order
-//     scale<S>(r)     {a, c} of sub-block S
+//     STEP            packed bytes of 16 slices, which the 16 quads of a wave take at a time
+//     Lane            what does not change from step to step: made of the lane's quad and the row's packed bytes; `off` is
+//                     the offset of the quad's first block.  A lane whose slice lies behind the row's end (the last step)
+//                     loads the last block again and gives it the scale 0, so nothing past the row is read.
+//     Raw             the packed bytes of a slice in registers; load(row, off, lane)
+//     codes<S>(r, l, b)  the codes of sub-block S as pairs of bf16, elements in order
+//     scale<S>(r, l)     {a, c} of sub-block S
 //
 // Codes below 16 become bf16 two at a time by v_cvt_scalef32_pk_bf16_fp8: an e4m3 byte of 0..15 is a subnormal or in the
 // first binade, both of which step by 2^-9, so with a scale of 2^9 its value is the byte itself (one full-rate instruction
@@ -60,13 +63,22 @@ __device__ __forceinline__ void signed_codes(uint32_t w, uint32_t &lo, uint32_t 
 
 struct SubScale { float a, c; };
 
+// ~0 where `off` is a block of the row, otherwise 0
+__device__ __forceinline__ uint32_t in_row(uint32_t off, uint32_t last) { return off <= last ? ~0u : 0u; }
+__device__ __forceinline__ uint32_t at_most(uint32_t off, uint32_t last) { return off < last ? off : last; }
+
 // ---- 32-element formats: a slice is two blocks; the second may be missing at the end of a row --------------
-// `n`: blocks of the row.  A missing block is loaded as the last one and gets the scale 0.
+template <uint32_t BYTES>
 struct SliceOfTwo {
     static constexpr bool PLANES = false;
     static constexpr int NSUB = 2, SUB = 32;
-    static constexpr uint32_t UNIT = 32;
+    static constexpr uint32_t STEP = 32 * BYTES;
+    struct Lane {
+        uint32_t off, last;
+        __device__ __forceinline__ Lane(uint32_t quad, uint32_t row_bytes) : off(2 * quad * BYTES), last(row_bytes - BYTES) {}
+    };
 };
+template <uint32_t BYTES> using LaneOfTwo = typename SliceOfTwo<BYTES>::Lane;
 
 template <class F> struct Slice;
 
@@ -80,14 +92,13 @@ template <> constexpr bool is_float_type<WBF16> = true;
 template <uint32_t BYTES, uint32_t HEAD>       // HEAD bytes of scales in front of 16 bytes of nibbles
 struct NibbleRaw {
     u32x4 q[2];
-    uint32_t h[2];
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t blocks) {
+    uint32_t h[2], live[2];
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const LaneOfTwo<BYTES> &l) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t b = 2 * s + k;
-            const uint8_t *p = row + (b < blocks ? b : blocks - 1) * BYTES;
+        for (int k = 0; k < 2; ++k, off += BYTES) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live[k] = in_row(off, l.last);
             h[k] = HEAD == 2 ? ld2(p) : ld4(p);
-            if (b >= blocks) h[k] = 0;
             q[k] = ld16(p + HEAD);
         }
     }
@@ -100,47 +111,46 @@ struct NibbleRaw {
         }
     }
 };
-template <> struct Slice<Q4_0> : SliceOfTwo {
+template <> struct Slice<Q4_0> : SliceOfTwo<18> {
     static constexpr bool OFFSET = true;
     typedef NibbleRaw<18, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const float d = h2f(r.h[S]);
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const float d = h2f(r.h[S] & r.live[S]);
         return {d, 8.0f * d};
     }
 };
-template <> struct Slice<Q4_1> : SliceOfTwo {
+template <> struct Slice<Q4_1> : SliceOfTwo<20> {
     static constexpr bool OFFSET = true;
     typedef NibbleRaw<20, 4> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        return {h2f(r.h[S] & 0xFFFFu), -h2f(r.h[S] >> 16)};
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        return {h2f(r.h[S] & r.live[S] & 0xFFFFu), -h2f((r.h[S] & r.live[S]) >> 16)};
     }
 };
-template <> struct Slice<IQ4NL> : SliceOfTwo {
+template <> struct Slice<IQ4NL> : SliceOfTwo<18> {
     static constexpr bool OFFSET = false;
     typedef NibbleRaw<18, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             signed_codes(iq4_lookup4(r.q[S][i] & 0x0F0F0F0Fu) ^ 0x80808080u, b[2 * i], b[2 * i + 1]);
             signed_codes(iq4_lookup4((r.q[S][i] >> 4) & 0x0F0F0F0Fu) ^ 0x80808080u, b[8 + 2 * i], b[9 + 2 * i]);
         }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.h[S]), 0.0f}; }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.h[S] & r.live[S]), 0.0f}; }
 };
 
 template <uint32_t BYTES, uint32_t HEAD>       // ... with 4 bytes of fifth bits between
 struct FiveRaw {
     u32x4 q[2];
-    uint32_t h[2], hi[2];
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t blocks) {
+    uint32_t h[2], hi[2], live[2];
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const LaneOfTwo<BYTES> &l) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t b = 2 * s + k;
-            const uint8_t *p = row + (b < blocks ? b : blocks - 1) * BYTES;
+        for (int k = 0; k < 2; ++k, off += BYTES) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live[k] = in_row(off, l.last);
             h[k] = HEAD == 2 ? ld2(p) : ld4(p);
-            if (b >= blocks) h[k] = 0;
             hi[k] = ld4(p + HEAD);
             q[k] = ld16(p + HEAD + 4);
         }
@@ -154,34 +164,34 @@ struct FiveRaw {
         }
     }
 };
-template <> struct Slice<Q5_0> : SliceOfTwo {
+template <> struct Slice<Q5_0> : SliceOfTwo<22> {
     static constexpr bool OFFSET = true;
     typedef FiveRaw<22, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const float d = h2f(r.h[S]);
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const float d = h2f(r.h[S] & r.live[S]);
         return {d, 16.0f * d};
     }
 };
-template <> struct Slice<Q5_1> : SliceOfTwo {
+template <> struct Slice<Q5_1> : SliceOfTwo<24> {
     static constexpr bool OFFSET = true;
     typedef FiveRaw<24, 4> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        return {h2f(r.h[S] & 0xFFFFu), -h2f(r.h[S] >> 16)};
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        return {h2f(r.h[S] & r.live[S] & 0xFFFFu), -h2f((r.h[S] & r.live[S]) >> 16)};
     }
 };
 
 template <uint32_t BYTES, uint32_t HEAD>       // 32 signed bytes
 struct ByteRaw {
     u32x4 q[2][2];
-    uint32_t h[2];
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t blocks) {
+    uint32_t h[2], live[2];
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const LaneOfTwo<BYTES> &l) {
 #pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const uint32_t b = 2 * s + k;
-            const uint8_t *p = row + (b < blocks ? b : blocks - 1) * BYTES;
-            h[k] = b < blocks ? ld2(p) : 0u;
+        for (int k = 0; k < 2; ++k, off += BYTES) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live[k] = in_row(off, l.last);
+            h[k] = ld2(p);
             q[k][0] = ld16(p + HEAD);
             q[k][1] = ld16(p + HEAD + 16);
         }
@@ -192,22 +202,27 @@ struct ByteRaw {
         for (int i = 0; i < 8; ++i) signed_codes(q[S][i / 4][i % 4], b[2 * i], b[2 * i + 1]);
     }
 };
-template <> struct Slice<Q8_0> : SliceOfTwo {
+template <> struct Slice<Q8_0> : SliceOfTwo<34> {
     static constexpr bool OFFSET = false;
     typedef ByteRaw<34, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.h[S]), 0.0f}; }
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.h[S] & r.live[S]), 0.0f}; }
 };
-template <> struct Slice<Q8_1> : SliceOfTwo {
+template <> struct Slice<Q8_1> : SliceOfTwo<36> {
     static constexpr bool OFFSET = false;
     typedef ByteRaw<36, 4> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.h[S]), 0.0f}; }
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.h[S] & r.live[S]), 0.0f}; }
 };
 
 // ---- 256-element formats: four slices a block ------------------------------------------------------------
+template <uint32_t BYTES>
 struct SliceOfQuarter {
-    static constexpr uint32_t UNIT = 64;
+    static constexpr uint32_t STEP = 4 * BYTES;
+    struct Lane {
+        uint32_t off, last, j;        // j: which quarter of its block
+        __device__ __forceinline__ Lane(uint32_t quad, uint32_t row_bytes) : off((quad >> 2) * BYTES), last(row_bytes - BYTES), j(quad & 3) {}
+    };
 };
 
 // 6-bit scale and minimum of sub-blocks 2j and 2j + 1 (j = 0..3) from the twelve bytes in words s0, s1, s2: for j < 2 the
@@ -216,208 +231,208 @@ struct PairOfK4 { uint32_t sc[2], mn[2]; };
 __device__ __forceinline__ PairOfK4 scales_k4(uint32_t s0, uint32_t s1, uint32_t s2, uint32_t j) {
     const uint32_t sh = 16 * (j & 1);            // two bytes of each word
     const uint32_t a = s0 >> sh, b = s1 >> sh, c = s2 >> sh;
-    const bool low = j < 2;
-    const uint32_t sc = low ? a & 0x3F3Fu : (c & 0x0F0Fu) | ((a >> 2) & 0x3030u);
-    const uint32_t mn = low ? b & 0x3F3Fu : ((c >> 4) & 0x0F0Fu) | ((b >> 2) & 0x3030u);
+    const uint32_t low = j < 2 ? 0x3F3Fu : 0u, high = 0x3F3Fu ^ low;        // a mask: lanes of one wave are in all quarters
+    const uint32_t sc = (a & low) | (((c & 0x0F0Fu) | ((a >> 2) & 0x3030u)) & high);
+    const uint32_t mn = (b & low) | ((((c >> 4) & 0x0F0Fu) | ((b >> 2) & 0x3030u)) & high);
     return {{sc & 0xFFu, (sc >> 8) & 0xFFu}, {mn & 0xFFu, (mn >> 8) & 0xFFu}};
 }
-template <> struct Slice<Q4K> : SliceOfQuarter {
+template <> struct Slice<Q4K> : SliceOfQuarter<144> {
     static constexpr bool PLANES = false, OFFSET = true;
     static constexpr int NSUB = 2, SUB = 32;
     struct Raw {
         u32x4 h, q[2];
-        uint32_t j;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
-            const uint8_t *p = row + (s >> 2) * 144;
-            j = s & 3;
+        uint32_t live;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live = in_row(off, l.last);
             h = ld16(p);
-            q[0] = ld16(p + 16 + 32 * j);
-            q[1] = ld16(p + 32 + 32 * j);
+            q[0] = ld16(p + 16 + 32 * l.j);
+            q[1] = ld16(p + 32 + 32 * l.j);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) small_codes((r.q[i / 4][i % 4] >> (4 * S)) & 0x0F0F0F0Fu, b[2 * i], b[2 * i + 1]);
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], r.j);
-        return {h2f(r.h[0] & 0xFFFFu) * (float)k.sc[S], h2f(r.h[0] >> 16) * (float)k.mn[S]};
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], l.j);
+        return {h2f(r.h[0] & r.live & 0xFFFFu) * (float)k.sc[S], h2f((r.h[0] & r.live) >> 16) * (float)k.mn[S]};
     }
 };
-template <> struct Slice<Q5K> : SliceOfQuarter {
+template <> struct Slice<Q5K> : SliceOfQuarter<176> {
     static constexpr bool PLANES = false, OFFSET = true;
     static constexpr int NSUB = 2, SUB = 32;
     struct Raw {
         u32x4 h, q[2], f[2];
-        uint32_t j;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
-            const uint8_t *p = row + (s >> 2) * 176;
-            j = s & 3;
+        uint32_t live;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live = in_row(off, l.last);
             h = ld16(p);
             f[0] = ld16(p + 16);
             f[1] = ld16(p + 32);
-            q[0] = ld16(p + 48 + 32 * j);
-            q[1] = ld16(p + 64 + 32 * j);
+            q[0] = ld16(p + 48 + 32 * l.j);
+            q[1] = ld16(p + 64 + 32 * l.j);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const uint32_t five = (r.f[i / 4][i % 4] >> (2 * r.j + S)) & 0x01010101u;
+            const uint32_t five = (r.f[i / 4][i % 4] >> (2 * l.j + S)) & 0x01010101u;
             byte_codes(((r.q[i / 4][i % 4] >> (4 * S)) & 0x0F0F0F0Fu) | (five << 4), b[2 * i], b[2 * i + 1]);
         }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], r.j);
-        return {h2f(r.h[0] & 0xFFFFu) * (float)k.sc[S], h2f(r.h[0] >> 16) * (float)k.mn[S]};
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], l.j);
+        return {h2f(r.h[0] & r.live & 0xFFFFu) * (float)k.sc[S], h2f((r.h[0] & r.live) >> 16) * (float)k.mn[S]};
     }
 };
-template <> struct Slice<IQ4XS> : SliceOfQuarter {
+template <> struct Slice<IQ4XS> : SliceOfQuarter<136> {
     static constexpr bool PLANES = false, OFFSET = false;
     static constexpr int NSUB = 2, SUB = 32;
     struct Raw {
         u32x2 h;
         u32x4 q[2];
-        uint32_t j;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
-            const uint8_t *p = row + (s >> 2) * 136;
-            j = s & 3;
+        uint32_t live;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live = in_row(off, l.last);
             h = ld8(p);
-            q[0] = ld16(p + 8 + 32 * j);
-            q[1] = ld16(p + 24 + 32 * j);
+            q[0] = ld16(p + 8 + 32 * l.j);
+            q[1] = ld16(p + 24 + 32 * l.j);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             signed_codes(iq4_lookup4(r.q[S][i] & 0x0F0F0F0Fu) ^ 0x80808080u, b[2 * i], b[2 * i + 1]);
             signed_codes(iq4_lookup4((r.q[S][i] >> 4) & 0x0F0F0F0Fu) ^ 0x80808080u, b[8 + 2 * i], b[9 + 2 * i]);
         }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const uint32_t ls = ((r.h[1] >> (8 * r.j + 4 * S)) & 0xFu) | (((r.h[0] >> (16 + 4 * r.j + 2 * S)) & 3u) << 4);
-        return {h2f(r.h[0] & 0xFFFFu) * (float)((int)ls - 32), 0.0f};
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const uint32_t ls = ((r.h[1] >> (8 * l.j + 4 * S)) & 0xFu) | (((r.h[0] >> (16 + 4 * l.j + 2 * S)) & 3u) << 4);
+        return {h2f(r.h[0] & r.live & 0xFFFFu) * (float)((int)ls - 32), 0.0f};
     }
 };
 
 // Slice s = (block, half n, 16-element column h): sub-block p = elements 128 n + 32 p + 16 h + 0..15 of the block.
-struct SliceOfPlanes : SliceOfQuarter {
+template <uint32_t BYTES>
+struct SliceOfPlanes : SliceOfQuarter<BYTES> {
     static constexpr bool PLANES = true;
     static constexpr int NSUB = 4, SUB = 16;
 };
-template <> struct Slice<Q6K> : SliceOfPlanes {
+template <> struct Slice<Q6K> : SliceOfPlanes<210> {
     static constexpr bool OFFSET = true;
     struct Raw {
-        u32x4 l[2], f;
+        u32x4 lo[2], f;
         u32x2 sc;
-        uint32_t d, h;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
-            const uint8_t *p = row + (s >> 2) * 210;
-            const uint32_t n = (s >> 1) & 1;
-            h = s & 1;
-            l[0] = ld16(p + 64 * n + 16 * h);
-            l[1] = ld16(p + 64 * n + 32 + 16 * h);
-            f = ld16(p + 128 + 32 * n + 16 * h);
-            sc = ld8(p + 192 + 8 * n);
+        uint32_t d, live;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live = in_row(off, l.last);
+            lo[0] = ld16(p + 64 * (l.j >> 1) + 16 * (l.j & 1));
+            lo[1] = ld16(p + 64 * (l.j >> 1) + 32 + 16 * (l.j & 1));
+            f = ld16(p + 128 + 16 * l.j);
+            sc = ld8(p + 192 + 8 * (l.j >> 1));
             d = ld2(p + 208);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[8]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t low = (r.l[S & 1][i] >> (4 * (S >> 1))) & 0x0F0F0F0Fu;
+            const uint32_t low = (r.lo[S & 1][i] >> (4 * (S >> 1))) & 0x0F0F0F0Fu;
             byte_codes(low | (((r.f[i] >> (2 * S)) & 0x03030303u) << 4), b[2 * i], b[2 * i + 1]);
         }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const int sc = (int)(int8_t)(r.sc[S >> 1] >> (16 * (S & 1) + 8 * r.h));
-        const float a = h2f(r.d) * (float)sc;
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const int sc = (int)(int8_t)(r.sc[S >> 1] >> (16 * (S & 1) + 8 * (l.j & 1)));
+        const float a = h2f(r.d & r.live) * (float)sc;
         return {a, 32.0f * a};
     }
 };
-template <> struct Slice<Q2K> : SliceOfPlanes {
+template <> struct Slice<Q2K> : SliceOfPlanes<84> {
     static constexpr bool OFFSET = true;
     struct Raw {
         u32x4 q;
         u32x2 sc;
-        uint32_t dm, h;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
-            const uint8_t *p = row + (s >> 2) * 84;
-            const uint32_t n = (s >> 1) & 1;
-            h = s & 1;
-            sc = ld8(p + 8 * n);
-            q = ld16(p + 16 + 32 * n + 16 * h);
+        uint32_t dm, live;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live = in_row(off, l.last);
+            sc = ld8(p + 8 * (l.j >> 1));
+            q = ld16(p + 16 + 16 * l.j);
             dm = ld4(p + 80);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[8]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) small_codes((r.q[i] >> (2 * S)) & 0x03030303u, b[2 * i], b[2 * i + 1]);
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const uint32_t sc = (r.sc[S >> 1] >> (16 * (S & 1) + 8 * r.h)) & 0xFFu;
-        return {h2f(r.dm & 0xFFFFu) * (float)(sc & 0xFu), h2f(r.dm >> 16) * (float)(sc >> 4)};
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const uint32_t sc = (r.sc[S >> 1] >> (16 * (S & 1) + 8 * (l.j & 1))) & 0xFFu;
+        return {h2f(r.dm & r.live & 0xFFFFu) * (float)(sc & 0xFu), h2f((r.dm & r.live) >> 16) * (float)(sc >> 4)};
     }
 };
-template <> struct Slice<Q3K> : SliceOfPlanes {
+template <> struct Slice<Q3K> : SliceOfPlanes<110> {
     static constexpr bool OFFSET = true;
     struct Raw {
         u32x4 q, f;
-        uint32_t s0, s1, s2, d, n, h;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
-            const uint8_t *p = row + (s >> 2) * 110;
-            n = (s >> 1) & 1;
-            h = s & 1;
-            f = ld16(p + 16 * h);
-            q = ld16(p + 32 + 32 * n + 16 * h);
+        uint32_t s0, s1, s2, d, live;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live = in_row(off, l.last);
+            f = ld16(p + 16 * (l.j & 1));
+            q = ld16(p + 32 + 16 * l.j);
             s0 = ld4(p + 96);
             s1 = ld4(p + 100);
             s2 = ld4(p + 104);
             d = ld2(p + 108);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[8]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[8]) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t high = (r.f[i] >> (4 * r.n + S)) & 0x01010101u;
+            const uint32_t high = (r.f[i] >> (4 * (l.j >> 1) + S)) & 0x01010101u;
             small_codes(((r.q[i] >> (2 * S)) & 0x03030303u) | (high << 2), b[2 * i], b[2 * i + 1]);
         }
     }
     // sub-block g = 8 n + 2 S + h of 16: low nibble g % 8 of bytes 0..7 (high nibble for n = 1), top bits g / 4 of byte g % 4
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) {
-        const uint32_t w = S < 2 ? r.s0 : r.s1, sh = 16 * (S & 1) + 8 * r.h;
-        const uint32_t low = (w >> (sh + 4 * r.n)) & 0xFu, top = (r.s2 >> (sh + 4 * r.n + 2 * (S >> 1))) & 3u;
-        const float a = h2f(r.d) * (float)((int)(low | (top << 4)) - 32);
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+        const uint32_t w = S < 2 ? r.s0 : r.s1, sh = 16 * (S & 1) + 8 * (l.j & 1);
+        const uint32_t low = (w >> (sh + 4 * (l.j >> 1))) & 0xFu, top = (r.s2 >> (sh + 4 * (l.j >> 1) + 2 * (S >> 1))) & 3u;
+        const float a = h2f(r.d & r.live) * (float)((int)(low | (top << 4)) - 32);
         return {a, 4.0f * a};
     }
 };
-template <> struct Slice<Q8K> : SliceOfQuarter {
+template <> struct Slice<Q8K> : SliceOfQuarter<290> {
     static constexpr bool PLANES = false, OFFSET = false;
     static constexpr int NSUB = 2, SUB = 32;
     struct Raw {
         u32x4 q[4];
-        uint32_t d;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t) {
-            const uint8_t *p = row + (s >> 2) * 290;
+        uint32_t d, live;
+        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
+            const uint8_t *p = row + at_most(off, l.last);
+            live = in_row(off, l.last);
             d = ld2(p);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = ld16(p + 2 + 64 * (s & 3) + 16 * i);
+            for (int i = 0; i < 4; ++i) q[i] = ld16(p + 2 + 64 * l.j + 16 * i);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16]) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) signed_codes(r.q[2 * S + i / 4][i % 4], b[2 * i], b[2 * i + 1]);
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r) { return {h2f(r.d), 0.0f}; }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.d & r.live), 0.0f}; }
 };
 
 // ---- 16-bit floats: rows of any length, 64 elements a slice ------------------------------------------------
 // The weights are their own codes; a half has eleven significant bits and becomes two bf16 (WP pieces).
 struct FloatRaw {
     u32x4 q[8];
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t s, uint32_t cols) {
-        const uint8_t *p = row + 128 * (uint64_t)s;
-        const uint32_t left = cols - 64 * s;
+    template <class L>
+    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const L &l) {
+        const uint8_t *p = row + off;
+        const uint32_t left = off < l.end ? (l.end - off) / 2 : 0;      // elements
         if (left >= 64) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = ld16(p + 16 * i);
@@ -434,9 +449,13 @@ struct FloatRaw {
 struct SliceOfFloats {
     static constexpr bool PLANES = false, OFFSET = false;
     static constexpr int NSUB = 2, SUB = 32;
-    static constexpr uint32_t UNIT = 1;
+    static constexpr uint32_t STEP = 2048;
+    struct Lane {
+        uint32_t off, end;
+        __device__ __forceinline__ Lane(uint32_t quad, uint32_t row_bytes) : off(128 * quad), end(row_bytes) {}
+    };
     typedef FloatRaw Raw;
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &) { return {1.0f, 0.0f}; }
+    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &, const Lane &) { return {1.0f, 0.0f}; }
 };
 // upper 16 bits of v, a NaN kept a NaN; `rest` = v minus that, exactly (0 where v is not finite)
 __device__ __forceinline__ uint32_t take_bf16(float v, float &rest) {
@@ -448,14 +467,14 @@ __device__ __forceinline__ uint32_t take_bf16(float v, float &rest) {
 }
 template <> struct Slice<WBF16> : SliceOfFloats {
     static constexpr int WP = 1;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16], int) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &, uint32_t (&b)[16], int) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) b[i] = r.q[4 * S + i / 4][i % 4];
     }
 };
 template <> struct Slice<WF16> : SliceOfFloats {
     static constexpr int WP = 2;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, uint32_t (&b)[16], int piece) {
+    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &, uint32_t (&b)[16], int piece) {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint32_t w = r.q[4 * S + i / 4][i % 4];
