@@ -169,50 +169,126 @@ __device__ __forceinline__ void stage_x(uint8_t *lds, uint32_t first, uint32_t s
     }
 }
 
-// acc[c] += sub-block S of the lane's slice times column c of x.  `x`: the step's fragments, from the lane's own on;
-// `sums`: the step's sums from the lane's slice on.
-template <class F, int NC, int CHAIN, int S>
-__device__ __forceinline__ void add_sub(const typename Slice<F>::Raw &raw, const typename Slice<F>::Lane &lane, const uint8_t *x,
-                                        const uint8_t *sums, float (&acc)[NC]) {
+// acc[t][c] += sub-block S of the lane's slice of its row in tile t, times column c of x, for RT tiles of four rows that
+// share the fragments.  `x`: the step's fragments, from the lane's own on; `sums`: the step's sums from the lane's slice on.
+template <class F, int NC, int CHAIN, int RT, int S>
+__device__ __forceinline__ void add_sub(const typename Slice<F>::Raw (&raw)[RT], const typename Slice<F>::Lane &lane, const uint8_t *x,
+                                        const uint8_t *sums, float (&acc)[RT][NC]) {
     typedef Slice<F> T;
     typedef XStep<F, NC, CHAIN> X;
     constexpr int FRAGS = T::SUB / 8, WORDS = T::SUB / 2;
     constexpr int WP = [] { if constexpr (is_float_type<F>) return T::WP; else return 1; }();
-    f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+    f32x4 d[RT];
+#pragma unroll
+    for (int t = 0; t < RT; ++t) d[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
     for (int piece = 0; piece < WP; ++piece) {
-        uint32_t b[WORDS];
-        if constexpr (is_float_type<F>) T::template codes<S>(raw, lane, b, piece);
-        else T::template codes<S>(raw, lane, b);
+        uint32_t b[RT][WORDS];
+#pragma unroll
+        for (int t = 0; t < RT; ++t) {
+            if constexpr (is_float_type<F>) T::template codes<S>(raw[t], lane, b[t], piece);
+            else T::template codes<S>(raw[t], lane, b[t]);
+        }
 #pragma unroll
         for (int p = 0; p < CHAIN; ++p)
 #pragma unroll
             for (int k = 0; k < FRAGS; ++k) {
-                const u32x4 a = *(const u32x4 *)(x + (p * 8 + S * FRAGS + k) * X::K);
-                const u32x2 a0 = {a[0], a[1]}, a1 = {a[2], a[3]}, b0 = {b[4 * k], b[4 * k + 1]}, b1 = {b[4 * k + 2], b[4 * k + 3]};
-                d = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, a0), __builtin_bit_cast(s16x4, b0), d, 0, 0, 0);
-                d = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, a1), __builtin_bit_cast(s16x4, b1), d, 0, 0, 0);
+                const u32x4 a = al16(x + (p * 8 + S * FRAGS + k) * X::K);
+#pragma unroll
+                for (int half = 0; half < 2; ++half)
+#pragma unroll
+                    for (int t = 0; t < RT; ++t) {
+                        const u32x2 av = {a[2 * half], a[2 * half + 1]}, bv = {b[t][4 * k + 2 * half], b[t][4 * k + 2 * half + 1]};
+                        d[t] = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, av), __builtin_bit_cast(s16x4, bv), d[t], 0, 0, 0);
+                    }
             }
     }
-    const SubScale s = T::template scale<S>(raw, lane);
-#pragma unroll
-    for (int c = 0; c < NC; ++c) acc[c] = __builtin_fmaf(s.a, d[c], acc[c]);
+    float sum[NC];
     if constexpr (T::OFFSET) {
-        const float *sum = (const float *)(sums + S * 64 * NC);
 #pragma unroll
-        for (int c = 0; c < NC; ++c) acc[c] = __builtin_fmaf(-s.c, sum[c], acc[c]);
+        for (int c = 0; c < NC; ++c) sum[c] = ((const float *)(sums + S * 64 * NC))[c];
+    }
+#pragma unroll
+    for (int t = 0; t < RT; ++t) {
+        const SubScale s = T::template scale<S>(raw[t], lane);
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            acc[t][c] = __builtin_fmaf(s.a, d[t][c], acc[t][c]);
+            if constexpr (T::OFFSET) acc[t][c] = __builtin_fmaf(-s.c, sum[c], acc[t][c]);
+        }
     }
 }
-template <class F, int NC, int CHAIN>
-__device__ __forceinline__ void add_slice(const typename Slice<F>::Raw &raw, const typename Slice<F>::Lane &lane, const uint8_t *x,
-                                          const uint8_t *sums, float (&acc)[NC]) {
-    add_sub<F, NC, CHAIN, 0>(raw, lane, x, sums, acc);
-    add_sub<F, NC, CHAIN, 1>(raw, lane, x, sums, acc);
+template <class F, int NC, int CHAIN, int RT>
+__device__ __forceinline__ void add_slices(const typename Slice<F>::Raw (&raw)[RT], const typename Slice<F>::Lane &lane, const uint8_t *x,
+                                           const uint8_t *sums, float (&acc)[RT][NC]) {
+    add_sub<F, NC, CHAIN, RT, 0>(raw, lane, x, sums, acc);
+    add_sub<F, NC, CHAIN, RT, 1>(raw, lane, x, sums, acc);
     if constexpr (Slice<F>::NSUB == 4) {
-        add_sub<F, NC, CHAIN, 2>(raw, lane, x, sums, acc);
-        add_sub<F, NC, CHAIN, 3>(raw, lane, x, sums, acc);
+        add_sub<F, NC, CHAIN, RT, 2>(raw, lane, x, sums, acc);
+        add_sub<F, NC, CHAIN, RT, 3>(raw, lane, x, sums, acc);
     }
 }
+
+// A wave's packed bytes of one step: 4 * RT rows.  Lanes that multiply together hold different rows, so loads straight
+// into their registers would touch a line per lane: the memory pipeline takes about two cycles for each, which held the
+// products at 4.1 TB/s whatever the format's arithmetic.  Instead neighbouring lanes load neighbouring 16-byte pieces into
+// registers, one step ahead, and hand them over through the wave's own part of shared memory.
+template <class F, int RT>
+struct Image {
+    typedef Slice<F> S;
+    static constexpr uint32_t ROWS = 4 * RT, PIECES = (S::UNIT + 15) / 16, PER_ROW = PIECES * S::UNITS, LOADS = (PER_ROW * ROWS + 63) / 64;
+    static constexpr uint32_t UNIT = PIECES * 16, ROW = UNIT * S::UNITS + (UNIT * S::UNITS % 64 == 32 ? 32 : 0) + 16 * (UNIT * S::UNITS % 32 / 16);
+    static constexpr uint32_t BYTES = ROW * ROWS;
+    uint32_t src[LOADS], dst[LOADS];          // from the tile's first row on; in the image
+    u32x4 v[LOADS];
+
+    // `rows` of the tile's rows exist; the others are the last one again
+    __device__ __forceinline__ Image(uint32_t lane, uint32_t rows, uint32_t row_bytes) {
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            uint32_t p = i * 64 + lane;
+            if (p >= PER_ROW * ROWS) p = PER_ROW * ROWS - 1;
+            const uint32_t r = p / PER_ROW, u = p % PER_ROW / PIECES, c = p % PIECES * 16;
+            src[i] = (r < rows ? r : rows - 1) * row_bytes + u * S::UNIT + c;
+            dst[i] = r * ROW + u * UNIT + c;
+        }
+    }
+    // The step that begins at `base` (in the tile's first row).  A unit's last piece and a row's last step may reach beyond
+    // them, into whatever follows in the tensor; `room` bytes of the tensor are left from base on, and where the furthest
+    // piece would end behind them (`reach`), pieces are moved back to end with it and shifted into place.
+    __device__ __forceinline__ void fetch(const uint8_t *base, uint64_t room, uint32_t reach) {
+        if (room >= reach) {
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) v[i] = ld16(base + src[i]);
+        } else {
+            const int32_t limit = (int32_t)room - 16;
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const int32_t from = (int32_t)src[i] < limit ? (int32_t)src[i] : limit;
+                const uint32_t back = src[i] - (uint32_t)from;
+                v[i] = shifted(ld16(base + from), back < 15 ? back : 15);
+            }
+        }
+    }
+    static __device__ __forceinline__ u32x4 shifted(u32x4 a, uint32_t bytes) {
+        const uint32_t b = (bytes & 3) * 8;
+        uint32_t w[8] = {a[0], a[1], a[2], a[3], 0, 0, 0, 0}, o[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t lo = bytes < 4 ? w[i] : bytes < 8 ? w[i + 1] : bytes < 12 ? w[i + 2] : w[i + 3];
+            const uint32_t hi = bytes < 4 ? w[i + 1] : bytes < 8 ? w[i + 2] : bytes < 12 ? w[i + 3] : w[i + 4];
+            o[i] = __builtin_amdgcn_alignbit(hi, lo, b);
+        }
+        return {o[0], o[1], o[2], o[3]};
+    }
+    __device__ __forceinline__ void put(uint8_t *image) const {
+#pragma unroll
+        for (uint32_t i = 0; i < LOADS; ++i) *(u32x4 *)(image + dst[i]) = v[i];
+    }
+};
+
+// Orders a wave's own accesses to shared memory (its lanes read what others of the wave wrote).
+__device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // Sum over the 16 quads of a wave: afterwards every lane holds its row's total.
 __device__ __forceinline__ float quads_sum(float v) {
@@ -228,55 +304,90 @@ __device__ __forceinline__ float quads_sum(float v) {
 // quad, the four rows' codes with up to four columns of x that the quad's lanes hold: every lane ends with its own row's
 // products, so that the sub-block's scale is applied in the lane that loaded it.  Columns are tokens, or the bf16 pieces
 // of a token (f32 = three pieces, exactly; products with codes are exact, sums are f32).
-template <class F, int NC, int CHAIN>
+template <class F, int NC, int CHAIN, int RT>
 __global__ __launch_bounds__(QD_THREADS) void matvec_quads(MatvecArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     typedef Slice<F> S;
     typedef XStep<F, NC, CHAIN> X;
+    typedef Image<F, RT> I;
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), quad = lane / 4;
     const uint32_t kp = wave % a.ksplit, group = wave / a.ksplit, groups = QD_WAVES / a.ksplit;
-    const uint64_t row = (a.first_tile + (uint64_t)blockIdx.x * groups + group) * 4 + lane % 4;
     const uint32_t row_bytes = (uint32_t)(a.cols / F::N * F::BYTES), steps = (uint32_t)((a.cols + 1023) / 1024);
-    const uint8_t *w = a.w + (row < a.rows ? row : a.rows - 1) * row_bytes;
-    const typename S::Lane me(quad, row_bytes);
-    const uint8_t *x = lds + (quad * NC + (lane % 4 < NC ? lane % 4 : NC - 1)) * 16, *sums = lds + X::SUMS + quad * NC * 4;
-    float acc[NC];
+    const uint64_t first_row = (a.first_tile + (uint64_t)blockIdx.x * groups) * I::ROWS;      // of the workgroup
+    const uint64_t row = first_row + group * I::ROWS;                                         // of the wave
+    const uint64_t own = row < a.rows ? row : a.rows - 1;
+    const uint32_t rows = a.rows - own < I::ROWS ? (uint32_t)(a.rows - own) : I::ROWS;
+    const uint8_t *w = a.w + own * row_bytes + (uint64_t)kp * S::STEP;
+    uint32_t left = row_bytes - (kp < steps ? kp : steps - 1) * S::STEP;       // of each row, from w on
+    const uint32_t reach = (rows - 1) * row_bytes + (S::UNITS - 1) * S::UNIT + I::UNIT;
+    const uint64_t behind = (a.rows - own - 1) * row_bytes;                    // of the tensor, behind the tile's first row
+    const typename S::Lane me(quad);
+    uint8_t *image = lds + wave * I::BYTES, *xs = lds + QD_WAVES * I::BYTES;
+    const uint8_t *x = xs + (quad * NC + (lane % 4 < NC ? lane % 4 : NC - 1)) * 16, *sums = xs + X::SUMS + quad * NC * 4;
+    float acc[RT][NC];
 #pragma unroll
-    for (int c = 0; c < NC; ++c) acc[c] = 0.0f;
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) acc[t][c] = 0.0f;
 
-    typename S::Raw r0, r1;
-    const uint32_t jump = S::STEP * a.ksplit;
-    uint32_t off = me.off + kp * S::STEP, step = kp;
-    r0.load(w, off, me);
+    I in(lane, rows, row_bytes);
+    if (kp < steps) in.fetch(w, behind + left, reach);
+    uint32_t step = kp;
     for (uint32_t first = 0; first < steps; first += a.chunk) {
         const uint32_t now = first + a.chunk < steps ? a.chunk : steps - first, end = first + now;
         if (first) __syncthreads();
-        stage_x<F, NC, CHAIN>(lds, first, now, a.x, a.x_kind, a.cols, a.tokens, a.parts, [&](uint32_t t) { return t * a.x_stride; });
+        stage_x<F, NC, CHAIN>(xs, first, now, a.x, a.x_kind, a.cols, a.tokens, a.parts, [&](uint32_t t) { return t * a.x_stride; });
         __syncthreads();
-        uint32_t at = (step - first) * X::BYTES;
-        for (; step < end; step += a.ksplit, at += a.ksplit * X::BYTES) {
-            off += jump;
-            if (step + a.ksplit < steps) r1.load(w, off, me);
-            add_slice<F, NC, CHAIN>(r0, me, x + at, sums + at, acc);
-            r0 = r1;
+        for (; step < end; step += a.ksplit) {
+            wave_order();
+            in.put(image);
+            wave_order();
+            const uint32_t here = left;
+            if (step + a.ksplit < steps) {
+                w += (uint64_t)a.ksplit * S::STEP;
+                left -= a.ksplit * S::STEP;
+                in.fetch(w, behind + left, reach);
+            }
+            typename S::Raw raw[RT];
+#pragma unroll
+            for (int t = 0; t < RT; ++t) raw[t].load(image + (t * 4 + lane % 4) * I::ROW, me, here);
+            const uint32_t at = (step - first) * X::BYTES;
+            add_slices<F, NC, CHAIN, RT>(raw, me, x + at, sums + at, acc);
         }
     }
     __syncthreads();                                   // the staged x is no longer needed
-    float *part = (float *)lds;                        // [wave][column][row]
+    float *part = (float *)xs;                         // [wave][column][row]
 #pragma unroll
-    for (int c = 0; c < NC; ++c) {
-        const float v = quads_sum(acc[c]);
-        if (lane < 4) part[(wave * NC + c) * 4 + lane] = v;
-    }
+    for (int t = 0; t < RT; ++t)
+#pragma unroll
+        for (int c = 0; c < NC; ++c) {
+            const float v = quads_sum(acc[t][c]);
+            if (lane < 4) part[(wave * NC + c) * I::ROWS + t * 4 + lane] = v;
+        }
     __syncthreads();
     // one thread per row and token: the waves' parts, and the token's pieces
-    if (threadIdx.x < groups * 4 * a.tokens) {
-        const uint32_t r = threadIdx.x % (groups * 4), t = threadIdx.x / (groups * 4), g = r / 4;
-        const uint64_t out = (a.first_tile + (uint64_t)blockIdx.x * groups) * 4 + r;
+    if (threadIdx.x < groups * I::ROWS * a.tokens) {
+        const uint32_t r = threadIdx.x % (groups * I::ROWS), t = threadIdx.x / (groups * I::ROWS), g = r / I::ROWS;
+        const uint64_t out = first_row + r;
         float v = 0.0f;
         for (uint32_t k = 0; k < a.ksplit; ++k)
-            for (uint32_t p = 0; p < a.parts; ++p) v += part[((g * a.ksplit + k) * NC + t * a.parts + p) * 4 + r % 4];
+            for (uint32_t p = 0; p < a.parts; ++p) v += part[((g * a.ksplit + k) * NC + t * a.parts + p) * I::ROWS + r % I::ROWS];
         if (out < a.rows) store_elem(a.y, t * a.y_stride + out, a.y_kind, v);
+    }
+}
+
+// Rows of 16-bit floats shorter than a piece of an image: a thread each.
+template <class F>
+__global__ __launch_bounds__(MV_THREADS) void matvec_short(MatvecArgs a) {
+    const uint64_t r = (uint64_t)blockIdx.x * MV_THREADS + threadIdx.x;
+    if (r >= a.rows) return;
+    for (uint32_t t = 0; t < a.tokens; ++t) {
+        float sum = 0.0f;
+        for (uint32_t c = 0; c < a.cols; ++c) {
+            const uint32_t b = ld2(a.w + 2 * (r * a.cols + c));
+            sum = __builtin_fmaf(__is_same(F, WF16) ? h2f(b) : bf2f(b), load_elem(a.x, t * a.x_stride + c, a.x_kind), sum);
+        }
+        store_elem(a.y, t * a.y_stride + r, a.y_kind, sum);
     }
 }
 

@@ -47,6 +47,8 @@ bool elem_kind(uint32_t ty, uint32_t *kind, uint32_t *bytes) {
 
 // Sizes beyond these have no use and would let products of sizes wrap.
 constexpr uint64_t MAX_DIM = 1ull << 30;
+// Columns: eight packed rows of any type are within 32-bit offsets.
+constexpr uint64_t MAX_COLS = 1ull << 26;
 // Workgroups of one launch: the grid's threads are counted in 32 bits
 constexpr uint64_t MAX_GRID = 1ull << 22;
 
@@ -55,23 +57,26 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
 }
 
 // Shared memory of one workgroup for x.
-constexpr uint32_t X_LDS = 60 << 10;
+constexpr uint32_t X_LDS = 40 << 10;
 
 template <class F, int NC, int CHAIN>
 void launch_quads(MatvecArgs a, hipStream_t st) {
+    constexpr int RT = Slice<F>::STEP <= 640 ? 2 : 1;
     typedef XStep<F, NC, CHAIN> X;
+    typedef Image<F, RT> I;
     const uint32_t steps = (uint32_t)((a.cols + 1023) / 1024);
-    const uint64_t tiles = (a.rows + 3) / 4;
+    const uint64_t tiles = (a.rows + I::ROWS - 1) / I::ROWS;
     // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
     a.ksplit = 1;
     while (a.ksplit < QD_WAVES && a.ksplit < steps && tiles * a.ksplit < 2048 && 2 * a.ksplit * X::BYTES <= X_LDS) a.ksplit *= 2;
     // equal chunks
     const uint32_t turns = (steps + a.ksplit - 1) / a.ksplit, most = X_LDS / (X::BYTES * a.ksplit), chunks = (turns + most - 1) / most;
     a.chunk = (turns + chunks - 1) / chunks * a.ksplit;
-    const uint32_t bytes = std::max<uint32_t>(std::min(a.chunk, steps) * X::BYTES, QD_WAVES * NC * 16), groups = QD_WAVES / a.ksplit;
+    const uint32_t x_bytes = std::max<uint32_t>(std::min(a.chunk, steps) * X::BYTES, QD_WAVES * NC * I::ROWS * 4);
+    const uint32_t bytes = QD_WAVES * I::BYTES + x_bytes, groups = QD_WAVES / a.ksplit;
     for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * groups) {
         const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + groups - 1) / groups));
-        matvec_quads<F, NC, CHAIN><<<grid, QD_THREADS, bytes, st>>>(a);
+        matvec_quads<F, NC, CHAIN, RT><<<grid, QD_THREADS, bytes, st>>>(a);
     }
 }
 
@@ -80,6 +85,12 @@ void launch_quads(MatvecArgs a, hipStream_t st) {
 template <class F>
 uint64_t launch_few(MatvecArgs a, uint64_t tokens, uint32_t pieces, hipStream_t st) {
     a.tokens = (uint32_t)std::min<uint64_t>(tokens, 4);
+    if constexpr (is_float_type<F>) {
+        if (a.cols < 8) {
+            matvec_short<F><<<(uint32_t)((a.rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
+            return a.tokens;
+        }
+    }
     a.parts = a.tokens * pieces <= 4 ? pieces : 1;
     if (a.parts == pieces) {
         switch (a.tokens * pieces) {
@@ -108,7 +119,7 @@ ggq_status ggq_matvec_device(uint32_t ty, uint64_t rows, uint64_t cols, const vo
     const uint64_t be = ggq_block_elems(ty);
     if (be == 0 || !elem_kind(x_type, &a.x_kind, &xb) || !elem_kind(y_type, &a.y_kind, &yb)) return GGQ_UNSUPPORTED;
     if (cols % be != 0) return GGQ_INDIVISIBLE;
-    if (rows >= MAX_DIM || cols >= MAX_DIM || tokens >= MAX_DIM) return GGQ_INVALID;
+    if (rows >= MAX_DIM || cols >= MAX_COLS || tokens >= MAX_DIM) return GGQ_INVALID;
     if (!strides_ok(y_stride, rows, tokens) || x_stride >= (1ull << 40)) return GGQ_INVALID;
     if (rows == 0 || tokens == 0) return GGQ_OK;
     if (!d_y || (cols && (!d_w || !d_x))) return GGQ_INVALID;
@@ -145,7 +156,7 @@ ggq_status ggq_get_rows_device(uint32_t ty, uint64_t rows, uint64_t cols, const 
     const uint32_t idb = id_type == 26 ? 4 : id_type == 27 ? 8 : 0;     // GGmlType I32, I64
     if (be == 0 || idb == 0 || !elem_kind(y_type, &a.y_kind, &yb)) return GGQ_UNSUPPORTED;
     if (cols % be != 0) return GGQ_INDIVISIBLE;
-    if (rows >= MAX_DIM || cols >= MAX_DIM || n >= MAX_DIM || !strides_ok(y_stride, cols, n)) return GGQ_INVALID;
+    if (rows >= MAX_DIM || cols >= MAX_COLS || n >= MAX_DIM || !strides_ok(y_stride, cols, n)) return GGQ_INVALID;
     if (cols == 0 || n == 0) return GGQ_OK;
     if (!d_y || !d_ids || (rows && !d_w)) return GGQ_INVALID;
     if ((uintptr_t)d_y % yb != 0 || (uintptr_t)d_ids % idb != 0) return GGQ_MISALIGNED;
@@ -179,7 +190,7 @@ ggq_status check_moe(const ggq_moe *m, uint64_t tokens) {
     uint32_t kind, bytes;
     const uint64_t ub = ggq_block_elems(m->up_type), db = ggq_block_elems(m->down_type);
     if (!ub || !db || !elem_kind(m->router_type, &kind, &bytes)) return GGQ_UNSUPPORTED;
-    if (m->hidden >= MAX_DIM || m->ff >= MAX_DIM || m->hidden == 0 || m->ff == 0) return GGQ_INVALID;
+    if (m->hidden >= MAX_COLS || m->ff >= MAX_COLS || m->hidden == 0 || m->ff == 0) return GGQ_INVALID;
     if (m->hidden % ub != 0 || m->ff % db != 0) return GGQ_INDIVISIBLE;
     if (m->experts == 0 || m->experts > GGQ_MOE_MAX_EXPERTS || m->top_k == 0 || m->top_k > m->experts || m->top_k > GGQ_MOE_MAX_TOP_K)
         return GGQ_INVALID;

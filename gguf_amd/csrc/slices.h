@@ -6,17 +6,22 @@
 //     w = a * q - c      q: code, a: scale of the sub-block, c: its offset
 // and the product needs a and c once per sub-block:  sum of w x = a * (sum of q x) - c * (sum of x).
 //
+// 16 neighbouring slices are a step: what the 16 quads of a wave take at a time.
+//
 // Per format:
 //     NSUB, SUB       sub-blocks of a slice and their elements (NSUB * SUB = 64)
 //     OFFSET          whether c can differ from zero
 //     PLANES          the sub-blocks of a slice are 16 elements each, 32 elements apart (two-level formats of 16-element
 //                     sub-blocks: the codes of elements l, l + 32, l + 64 and l + 96 share a byte); otherwise the slice is 64
 //                     consecutive elements
-//     STEP            packed bytes of 16 slices, which the 16 quads of a wave take at a time
-//     Lane            what does not change from step to step: made of the lane's quad and the row's packed bytes; `off` is
-//                     the offset of the quad's first block.  A lane whose slice lies behind the row's end (the last step)
-//                     loads the last block again and gives it the scale 0, so nothing past the row is read.
-//     Raw             the packed bytes of a slice in registers; load(row, off, lane)
+//     STEP            packed bytes of a step
+//     UNIT, UNITS     the bytes of a row's step come into shared memory as UNITS pieces of UNIT bytes, each at a 16-byte
+//                     aligned place: whole blocks of the 256-element formats, so that their parts can be read with wide
+//                     aligned loads; everything at once for the others, whose slices are whole words
+//     Lane            what a lane knows of its place: made of its quad (its slice within a step)
+//     Raw             the packed bytes of a slice in registers; load(row, lane, left): from the row's image in shared memory,
+//                     `left` bytes of the row from this step on.  Blocks behind the row's end hold anything there: they get
+//                     the scale 0
 //     codes<S>(r, l, b)  the codes of sub-block S as pairs of bf16, elements in order
 //     scale<S>(r, l)     {a, c} of sub-block S
 //
@@ -63,22 +68,47 @@ __device__ __forceinline__ void signed_codes(uint32_t w, uint32_t &lo, uint32_t 
 
 struct SubScale { float a, c; };
 
-// ~0 where `off` is a block of the row, otherwise 0
-__device__ __forceinline__ uint32_t in_row(uint32_t off, uint32_t last) { return off <= last ? ~0u : 0u; }
-__device__ __forceinline__ uint32_t at_most(uint32_t off, uint32_t last) { return off < last ? off : last; }
+// aligned loads, from shared memory
+__device__ __forceinline__ u32x4 al16(const uint8_t *p) { return *(const u32x4 *)p; }
+__device__ __forceinline__ u32x2 al8(const uint8_t *p) { return *(const u32x2 *)p; }
+__device__ __forceinline__ uint32_t al4(const uint8_t *p) { return *(const uint32_t *)p; }
+// ~0 where a block that ends at byte `end` is part of the row, otherwise 0
+__device__ __forceinline__ uint32_t in_row(uint32_t end, uint32_t left) { return end <= left ? ~0u : 0u; }
+__device__ __forceinline__ uint32_t funnel16(uint32_t hi, uint32_t lo) { return __builtin_amdgcn_alignbit(hi, lo, 16); }
 
 // ---- 32-element formats: a slice is two blocks; the second may be missing at the end of a row --------------
-template <uint32_t BYTES>
+// The two blocks are a whole number of words and lie at a whole word, so they are read as words.
+template <uint32_t B>
 struct SliceOfTwo {
     static constexpr bool PLANES = false;
     static constexpr int NSUB = 2, SUB = 32;
-    static constexpr uint32_t STEP = 32 * BYTES;
+    static constexpr uint32_t STEP = 32 * B, UNIT = STEP, UNITS = 1;
     struct Lane {
-        uint32_t off, last;
-        __device__ __forceinline__ Lane(uint32_t quad, uint32_t row_bytes) : off(2 * quad * BYTES), last(row_bytes - BYTES) {}
+        uint32_t at;
+        __device__ __forceinline__ explicit Lane(uint32_t quad) : at(2 * quad * B) {}
+    };
+    struct Raw {
+        uint32_t w[B / 2], live[2];
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+#pragma unroll
+            for (uint32_t i = 0; i < B / 2; ++i) w[i] = al4(row + l.at + 4 * i);
+            live[0] = in_row(l.at + B, left);
+            live[1] = in_row(l.at + 2 * B, left);
+        }
+        // the word at byte `off` of block S; both are whole words, or off + S * B is two bytes beyond one
+        template <int S, uint32_t OFF>
+        __device__ __forceinline__ uint32_t word() const {
+            constexpr uint32_t at = S * B + OFF;
+            if constexpr (at % 4 == 0) return w[at / 4];
+            else return funnel16(w[at / 4 + 1], w[at / 4]);
+        }
+        template <int S>
+        __device__ __forceinline__ uint32_t half() const {          // the first two bytes of block S, 0 behind the row
+            constexpr uint32_t at = S * B;
+            return (at % 4 ? w[at / 4] >> 16 : w[at / 4] & 0xFFFFu) & live[S];
+        }
     };
 };
-template <uint32_t BYTES> using LaneOfTwo = typename SliceOfTwo<BYTES>::Lane;
 
 template <class F> struct Slice;
 
@@ -89,139 +119,98 @@ template <class F> constexpr bool is_float_type = false;
 template <> constexpr bool is_float_type<WF16> = true;
 template <> constexpr bool is_float_type<WBF16> = true;
 
-template <uint32_t BYTES, uint32_t HEAD>       // HEAD bytes of scales in front of 16 bytes of nibbles
-struct NibbleRaw {
-    u32x4 q[2];
-    uint32_t h[2], live[2];
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const LaneOfTwo<BYTES> &l) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k, off += BYTES) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live[k] = in_row(off, l.last);
-            h[k] = HEAD == 2 ? ld2(p) : ld4(p);
-            q[k] = ld16(p + HEAD);
-        }
+// a template's loop over words whose places are constants: BODY(i) for i < N
+#define GGQ_WORDS4(BODY) BODY(0) BODY(1) BODY(2) BODY(3)
+#define GGQ_WORDS8(BODY) GGQ_WORDS4(BODY) BODY(4) BODY(5) BODY(6) BODY(7)
+
+// 16 bytes of nibbles behind HEAD bytes: word i holds elements 4 i.. in its low and 16 + 4 i.. in its high nibbles
+template <class Raw, int S, uint32_t HEAD>
+__device__ __forceinline__ void nibble_codes(const Raw &r, uint32_t (&b)[16]) {
+#define ONE(i)                                                                        \
+    {                                                                                 \
+        const uint32_t q = r.template word<S, HEAD + 4 * i>();                        \
+        small_codes(q & 0x0F0F0F0Fu, b[2 * i], b[2 * i + 1]);                         \
+        small_codes((q >> 4) & 0x0F0F0F0Fu, b[8 + 2 * i], b[9 + 2 * i]);              \
     }
-    template <int S>
-    __device__ __forceinline__ void codes(uint32_t (&b)[16]) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            small_codes(q[S][i] & 0x0F0F0F0Fu, b[2 * i], b[2 * i + 1]);
-            small_codes((q[S][i] >> 4) & 0x0F0F0F0Fu, b[8 + 2 * i], b[9 + 2 * i]);
-        }
+    GGQ_WORDS4(ONE)
+#undef ONE
+}
+template <class Raw, int S, uint32_t HEAD>
+__device__ __forceinline__ void iq4_codes(const Raw &r, uint32_t (&b)[16]) {
+#define ONE(i)                                                                                              \
+    {                                                                                                       \
+        const uint32_t q = r.template word<S, HEAD + 4 * i>();                                              \
+        signed_codes(iq4_lookup4(q & 0x0F0F0F0Fu) ^ 0x80808080u, b[2 * i], b[2 * i + 1]);                   \
+        signed_codes(iq4_lookup4((q >> 4) & 0x0F0F0F0Fu) ^ 0x80808080u, b[8 + 2 * i], b[9 + 2 * i]);        \
     }
-};
+    GGQ_WORDS4(ONE)
+#undef ONE
+}
+// ... with a word of fifth bits in front of the nibbles
+template <class Raw, int S, uint32_t HEAD>
+__device__ __forceinline__ void five_codes(const Raw &r, uint32_t (&b)[16]) {
+    const uint32_t hi = r.template word<S, HEAD>();
+#define ONE(i)                                                                                                              \
+    {                                                                                                                       \
+        const uint32_t q = r.template word<S, HEAD + 4 + 4 * i>();                                                          \
+        byte_codes((q & 0x0F0F0F0Fu) | (spread4(hi >> (4 * i)) << 4), b[2 * i], b[2 * i + 1]);                              \
+        byte_codes(((q >> 4) & 0x0F0F0F0Fu) | (spread4(hi >> (16 + 4 * i)) << 4), b[8 + 2 * i], b[9 + 2 * i]);              \
+    }
+    GGQ_WORDS4(ONE)
+#undef ONE
+}
+template <class Raw, int S, uint32_t HEAD>
+__device__ __forceinline__ void signed_byte_codes(const Raw &r, uint32_t (&b)[16]) {
+#define ONE(i) signed_codes(r.template word<S, HEAD + 4 * i>(), b[2 * i], b[2 * i + 1]);
+    GGQ_WORDS8(ONE)
+#undef ONE
+}
+
+#define GGQ_CODES(N) template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[N])
+#define GGQ_SCALE template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l)
 template <> struct Slice<Q4_0> : SliceOfTwo<18> {
     static constexpr bool OFFSET = true;
-    typedef NibbleRaw<18, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
-        const float d = h2f(r.h[S] & r.live[S]);
-        return {d, 8.0f * d};
-    }
-};
-template <> struct Slice<Q4_1> : SliceOfTwo<20> {
-    static constexpr bool OFFSET = true;
-    typedef NibbleRaw<20, 4> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
-        return {h2f(r.h[S] & r.live[S] & 0xFFFFu), -h2f((r.h[S] & r.live[S]) >> 16)};
-    }
+    GGQ_CODES(16) { nibble_codes<Raw, S, 2>(r, b); }
+    GGQ_SCALE { const float d = h2f(r.half<S>()); return {d, 8.0f * d}; }
 };
 template <> struct Slice<IQ4NL> : SliceOfTwo<18> {
     static constexpr bool OFFSET = false;
-    typedef NibbleRaw<18, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            signed_codes(iq4_lookup4(r.q[S][i] & 0x0F0F0F0Fu) ^ 0x80808080u, b[2 * i], b[2 * i + 1]);
-            signed_codes(iq4_lookup4((r.q[S][i] >> 4) & 0x0F0F0F0Fu) ^ 0x80808080u, b[8 + 2 * i], b[9 + 2 * i]);
-        }
-    }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.h[S] & r.live[S]), 0.0f}; }
+    GGQ_CODES(16) { iq4_codes<Raw, S, 2>(r, b); }
+    GGQ_SCALE { return {h2f(r.half<S>()), 0.0f}; }
 };
-
-template <uint32_t BYTES, uint32_t HEAD>       // ... with 4 bytes of fifth bits between
-struct FiveRaw {
-    u32x4 q[2];
-    uint32_t h[2], hi[2], live[2];
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const LaneOfTwo<BYTES> &l) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k, off += BYTES) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live[k] = in_row(off, l.last);
-            h[k] = HEAD == 2 ? ld2(p) : ld4(p);
-            hi[k] = ld4(p + HEAD);
-            q[k] = ld16(p + HEAD + 4);
-        }
-    }
-    template <int S>
-    __device__ __forceinline__ void codes(uint32_t (&b)[16]) const {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            byte_codes((q[S][i] & 0x0F0F0F0Fu) | (spread4(hi[S] >> (4 * i)) << 4), b[2 * i], b[2 * i + 1]);
-            byte_codes(((q[S][i] >> 4) & 0x0F0F0F0Fu) | (spread4(hi[S] >> (16 + 4 * i)) << 4), b[8 + 2 * i], b[9 + 2 * i]);
-        }
-    }
+template <> struct Slice<Q4_1> : SliceOfTwo<20> {
+    static constexpr bool OFFSET = true;
+    GGQ_CODES(16) { nibble_codes<Raw, S, 4>(r, b); }
+    GGQ_SCALE { return {h2f(r.half<S>()), -h2f((r.word<S, 0>() & r.live[S]) >> 16)}; }
 };
 template <> struct Slice<Q5_0> : SliceOfTwo<22> {
     static constexpr bool OFFSET = true;
-    typedef FiveRaw<22, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
-        const float d = h2f(r.h[S] & r.live[S]);
-        return {d, 16.0f * d};
-    }
+    GGQ_CODES(16) { five_codes<Raw, S, 2>(r, b); }
+    GGQ_SCALE { const float d = h2f(r.half<S>()); return {d, 16.0f * d}; }
 };
 template <> struct Slice<Q5_1> : SliceOfTwo<24> {
     static constexpr bool OFFSET = true;
-    typedef FiveRaw<24, 4> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
-        return {h2f(r.h[S] & r.live[S] & 0xFFFFu), -h2f((r.h[S] & r.live[S]) >> 16)};
-    }
-};
-
-template <uint32_t BYTES, uint32_t HEAD>       // 32 signed bytes
-struct ByteRaw {
-    u32x4 q[2][2];
-    uint32_t h[2], live[2];
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const LaneOfTwo<BYTES> &l) {
-#pragma unroll
-        for (int k = 0; k < 2; ++k, off += BYTES) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live[k] = in_row(off, l.last);
-            h[k] = ld2(p);
-            q[k][0] = ld16(p + HEAD);
-            q[k][1] = ld16(p + HEAD + 16);
-        }
-    }
-    template <int S>
-    __device__ __forceinline__ void codes(uint32_t (&b)[16]) const {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) signed_codes(q[S][i / 4][i % 4], b[2 * i], b[2 * i + 1]);
-    }
+    GGQ_CODES(16) { five_codes<Raw, S, 4>(r, b); }
+    GGQ_SCALE { return {h2f(r.half<S>()), -h2f((r.word<S, 0>() & r.live[S]) >> 16)}; }
 };
 template <> struct Slice<Q8_0> : SliceOfTwo<34> {
     static constexpr bool OFFSET = false;
-    typedef ByteRaw<34, 2> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.h[S] & r.live[S]), 0.0f}; }
+    GGQ_CODES(16) { signed_byte_codes<Raw, S, 2>(r, b); }
+    GGQ_SCALE { return {h2f(r.half<S>()), 0.0f}; }
 };
 template <> struct Slice<Q8_1> : SliceOfTwo<36> {
     static constexpr bool OFFSET = false;
-    typedef ByteRaw<36, 4> Raw;
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) { r.codes<S>(b); }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.h[S] & r.live[S]), 0.0f}; }
+    GGQ_CODES(16) { signed_byte_codes<Raw, S, 4>(r, b); }
+    GGQ_SCALE { return {h2f(r.half<S>()), 0.0f}; }
 };
 
 // ---- 256-element formats: four slices a block ------------------------------------------------------------
-template <uint32_t BYTES>
+template <uint32_t B>
 struct SliceOfQuarter {
-    static constexpr uint32_t STEP = 4 * BYTES;
+    static constexpr uint32_t STEP = 4 * B, UNIT = B, UNITS = 4;
     struct Lane {
-        uint32_t off, last, j;        // j: which quarter of its block
-        __device__ __forceinline__ Lane(uint32_t quad, uint32_t row_bytes) : off((quad >> 2) * BYTES), last(row_bytes - BYTES), j(quad & 3) {}
+        uint32_t at, end, j;          // its block's image, the block's end in the packed step, which quarter of the block
+        __device__ __forceinline__ explicit Lane(uint32_t quad) : at((quad >> 2) * ((B + 15) / 16 * 16)), end((quad >> 2) * B + B), j(quad & 3) {}
     };
 };
 
@@ -242,19 +231,19 @@ template <> struct Slice<Q4K> : SliceOfQuarter<144> {
     struct Raw {
         u32x4 h, q[2];
         uint32_t live;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live = in_row(off, l.last);
-            h = ld16(p);
-            q[0] = ld16(p + 16 + 32 * l.j);
-            q[1] = ld16(p + 32 + 32 * l.j);
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+            const uint8_t *p = row + l.at;
+            live = in_row(l.end, left);
+            h = al16(p);
+            q[0] = al16(p + 16 + 32 * l.j);
+            q[1] = al16(p + 32 + 32 * l.j);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
+    GGQ_CODES(16) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) small_codes((r.q[i / 4][i % 4] >> (4 * S)) & 0x0F0F0F0Fu, b[2 * i], b[2 * i + 1]);
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+    GGQ_SCALE {
         const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], l.j);
         return {h2f(r.h[0] & r.live & 0xFFFFu) * (float)k.sc[S], h2f((r.h[0] & r.live) >> 16) * (float)k.mn[S]};
     }
@@ -265,24 +254,24 @@ template <> struct Slice<Q5K> : SliceOfQuarter<176> {
     struct Raw {
         u32x4 h, q[2], f[2];
         uint32_t live;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live = in_row(off, l.last);
-            h = ld16(p);
-            f[0] = ld16(p + 16);
-            f[1] = ld16(p + 32);
-            q[0] = ld16(p + 48 + 32 * l.j);
-            q[1] = ld16(p + 64 + 32 * l.j);
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+            const uint8_t *p = row + l.at;
+            live = in_row(l.end, left);
+            h = al16(p);
+            f[0] = al16(p + 16);
+            f[1] = al16(p + 32);
+            q[0] = al16(p + 48 + 32 * l.j);
+            q[1] = al16(p + 64 + 32 * l.j);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
+    GGQ_CODES(16) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const uint32_t five = (r.f[i / 4][i % 4] >> (2 * l.j + S)) & 0x01010101u;
             byte_codes(((r.q[i / 4][i % 4] >> (4 * S)) & 0x0F0F0F0Fu) | (five << 4), b[2 * i], b[2 * i + 1]);
         }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+    GGQ_SCALE {
         const PairOfK4 k = scales_k4(r.h[1], r.h[2], r.h[3], l.j);
         return {h2f(r.h[0] & r.live & 0xFFFFu) * (float)k.sc[S], h2f((r.h[0] & r.live) >> 16) * (float)k.mn[S]};
     }
@@ -294,30 +283,34 @@ template <> struct Slice<IQ4XS> : SliceOfQuarter<136> {
         u32x2 h;
         u32x4 q[2];
         uint32_t live;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live = in_row(off, l.last);
-            h = ld8(p);
-            q[0] = ld16(p + 8 + 32 * l.j);
-            q[1] = ld16(p + 24 + 32 * l.j);
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+            const uint8_t *p = row + l.at;
+            live = in_row(l.end, left);
+            h = al8(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                    // 8-byte aligned
+                const u32x2 v = al8(p + 8 + 32 * l.j + 8 * i);
+                q[i / 2][2 * (i & 1)] = v[0];
+                q[i / 2][2 * (i & 1) + 1] = v[1];
+            }
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
+    GGQ_CODES(16) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             signed_codes(iq4_lookup4(r.q[S][i] & 0x0F0F0F0Fu) ^ 0x80808080u, b[2 * i], b[2 * i + 1]);
             signed_codes(iq4_lookup4((r.q[S][i] >> 4) & 0x0F0F0F0Fu) ^ 0x80808080u, b[8 + 2 * i], b[9 + 2 * i]);
         }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+    GGQ_SCALE {
         const uint32_t ls = ((r.h[1] >> (8 * l.j + 4 * S)) & 0xFu) | (((r.h[0] >> (16 + 4 * l.j + 2 * S)) & 3u) << 4);
         return {h2f(r.h[0] & r.live & 0xFFFFu) * (float)((int)ls - 32), 0.0f};
     }
 };
 
 // Slice s = (block, half n, 16-element column h): sub-block p = elements 128 n + 32 p + 16 h + 0..15 of the block.
-template <uint32_t BYTES>
-struct SliceOfPlanes : SliceOfQuarter<BYTES> {
+template <uint32_t B>
+struct SliceOfPlanes : SliceOfQuarter<B> {
     static constexpr bool PLANES = true;
     static constexpr int NSUB = 4, SUB = 16;
 };
@@ -327,24 +320,24 @@ template <> struct Slice<Q6K> : SliceOfPlanes<210> {
         u32x4 lo[2], f;
         u32x2 sc;
         uint32_t d, live;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live = in_row(off, l.last);
-            lo[0] = ld16(p + 64 * (l.j >> 1) + 16 * (l.j & 1));
-            lo[1] = ld16(p + 64 * (l.j >> 1) + 32 + 16 * (l.j & 1));
-            f = ld16(p + 128 + 16 * l.j);
-            sc = ld8(p + 192 + 8 * (l.j >> 1));
-            d = ld2(p + 208);
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+            const uint8_t *p = row + l.at;
+            live = in_row(l.end, left);
+            lo[0] = al16(p + 64 * (l.j >> 1) + 16 * (l.j & 1));
+            lo[1] = al16(p + 64 * (l.j >> 1) + 32 + 16 * (l.j & 1));
+            f = al16(p + 128 + 16 * l.j);
+            sc = al8(p + 192 + 8 * (l.j >> 1));
+            d = *(const uint16_t *)(p + 208);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[8]) {
+    GGQ_CODES(8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t low = (r.lo[S & 1][i] >> (4 * (S >> 1))) & 0x0F0F0F0Fu;
             byte_codes(low | (((r.f[i] >> (2 * S)) & 0x03030303u) << 4), b[2 * i], b[2 * i + 1]);
         }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+    GGQ_SCALE {
         const int sc = (int)(int8_t)(r.sc[S >> 1] >> (16 * (S & 1) + 8 * (l.j & 1)));
         const float a = h2f(r.d & r.live) * (float)sc;
         return {a, 32.0f * a};
@@ -356,19 +349,19 @@ template <> struct Slice<Q2K> : SliceOfPlanes<84> {
         u32x4 q;
         u32x2 sc;
         uint32_t dm, live;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live = in_row(off, l.last);
-            sc = ld8(p + 8 * (l.j >> 1));
-            q = ld16(p + 16 + 16 * l.j);
-            dm = ld4(p + 80);
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+            const uint8_t *p = row + l.at;
+            live = in_row(l.end, left);
+            sc = al8(p + 8 * (l.j >> 1));
+            q = al16(p + 16 + 16 * l.j);
+            dm = al4(p + 80);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[8]) {
+    GGQ_CODES(8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) small_codes((r.q[i] >> (2 * S)) & 0x03030303u, b[2 * i], b[2 * i + 1]);
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
+    GGQ_SCALE {
         const uint32_t sc = (r.sc[S >> 1] >> (16 * (S & 1) + 8 * (l.j & 1))) & 0xFFu;
         return {h2f(r.dm & r.live & 0xFFFFu) * (float)(sc & 0xFu), h2f((r.dm & r.live) >> 16) * (float)(sc >> 4)};
     }
@@ -376,20 +369,17 @@ template <> struct Slice<Q2K> : SliceOfPlanes<84> {
 template <> struct Slice<Q3K> : SliceOfPlanes<110> {
     static constexpr bool OFFSET = true;
     struct Raw {
-        u32x4 q, f;
-        uint32_t s0, s1, s2, d, live;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live = in_row(off, l.last);
-            f = ld16(p + 16 * (l.j & 1));
-            q = ld16(p + 32 + 16 * l.j);
-            s0 = ld4(p + 96);
-            s1 = ld4(p + 100);
-            s2 = ld4(p + 104);
-            d = ld2(p + 108);
+        u32x4 q, f, s;               // s: three words of scales, then the block's scale
+        uint32_t live;
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+            const uint8_t *p = row + l.at;
+            live = in_row(l.end, left);
+            f = al16(p + 16 * (l.j & 1));
+            q = al16(p + 32 + 16 * l.j);
+            s = al16(p + 96);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[8]) {
+    GGQ_CODES(8) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const uint32_t high = (r.f[i] >> (4 * (l.j >> 1) + S)) & 0x01010101u;
@@ -397,10 +387,10 @@ template <> struct Slice<Q3K> : SliceOfPlanes<110> {
         }
     }
     // sub-block g = 8 n + 2 S + h of 16: low nibble g % 8 of bytes 0..7 (high nibble for n = 1), top bits g / 4 of byte g % 4
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) {
-        const uint32_t w = S < 2 ? r.s0 : r.s1, sh = 16 * (S & 1) + 8 * (l.j & 1);
-        const uint32_t low = (w >> (sh + 4 * (l.j >> 1))) & 0xFu, top = (r.s2 >> (sh + 4 * (l.j >> 1) + 2 * (S >> 1))) & 3u;
-        const float a = h2f(r.d & r.live) * (float)((int)(low | (top << 4)) - 32);
+    GGQ_SCALE {
+        const uint32_t w = S < 2 ? r.s[0] : r.s[1], sh = 16 * (S & 1) + 8 * (l.j & 1);
+        const uint32_t low = (w >> (sh + 4 * (l.j >> 1))) & 0xFu, top = (r.s[2] >> (sh + 4 * (l.j >> 1) + 2 * (S >> 1))) & 3u;
+        const float a = h2f(r.s[3] & 0xFFFFu & r.live) * (float)((int)(low | (top << 4)) - 32);
         return {a, 4.0f * a};
     }
 };
@@ -408,54 +398,51 @@ template <> struct Slice<Q8K> : SliceOfQuarter<290> {
     static constexpr bool PLANES = false, OFFSET = false;
     static constexpr int NSUB = 2, SUB = 32;
     struct Raw {
-        u32x4 q[4];
-        uint32_t d, live;
-        __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const Lane &l) {
-            const uint8_t *p = row + at_most(off, l.last);
-            live = in_row(off, l.last);
-            d = ld2(p);
+        u32x4 q[4];                  // the codes begin two bytes behind a whole word
+        uint32_t over, d, live;
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+            const uint8_t *p = row + l.at;
+            live = in_row(l.end, left);
+            d = *(const uint16_t *)p;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) q[i] = ld16(p + 2 + 64 * l.j + 16 * i);
+            for (int i = 0; i < 4; ++i) q[i] = al16(p + 64 * l.j + 16 * i);
+            over = al4(p + 64 * l.j + 64);
         }
     };
-    template <int S> static __device__ __forceinline__ void codes(const Raw &r, const Lane &l, uint32_t (&b)[16]) {
+    GGQ_CODES(16) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) signed_codes(r.q[2 * S + i / 4][i % 4], b[2 * i], b[2 * i + 1]);
+        for (int i = 0; i < 8; ++i) {
+            constexpr int from = 8 * S;
+            const uint32_t lo = r.q[(from + i) / 4][(from + i) % 4], hi = from + i == 15 ? r.over : r.q[(from + i + 1) / 4 % 4][(from + i + 1) % 4];
+            signed_codes(funnel16(hi, lo), b[2 * i], b[2 * i + 1]);
+        }
     }
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &r, const Lane &l) { return {h2f(r.d & r.live), 0.0f}; }
+    GGQ_SCALE { return {h2f(r.d & r.live), 0.0f}; }
 };
 
 // ---- 16-bit floats: rows of any length, 64 elements a slice ------------------------------------------------
 // The weights are their own codes; a half has eleven significant bits and becomes two bf16 (WP pieces).
-struct FloatRaw {
-    u32x4 q[8];
-    template <class L>
-    __device__ __forceinline__ void load(const uint8_t *row, uint32_t off, const L &l) {
-        const uint8_t *p = row + off;
-        const uint32_t left = off < l.end ? (l.end - off) / 2 : 0;      // elements
-        if (left >= 64) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] = ld16(p + 16 * i);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) {
-                uint32_t w = 2 * i < left ? ld2(p + 4 * i) : 0u;
-                if (2 * i + 1 < left) w |= ld2(p + 4 * i + 2) << 16;
-                q[i / 4][i % 4] = w;
-            }
-        }
-    }
-};
 struct SliceOfFloats {
     static constexpr bool PLANES = false, OFFSET = false;
     static constexpr int NSUB = 2, SUB = 32;
-    static constexpr uint32_t STEP = 2048;
+    static constexpr uint32_t STEP = 2048, UNIT = STEP, UNITS = 1;
     struct Lane {
-        uint32_t off, end;
-        __device__ __forceinline__ Lane(uint32_t quad, uint32_t row_bytes) : off(128 * quad), end(row_bytes) {}
+        uint32_t at;
+        __device__ __forceinline__ explicit Lane(uint32_t quad) : at(128 * quad) {}
     };
-    typedef FloatRaw Raw;
-    template <int S> static __device__ __forceinline__ SubScale scale(const Raw &, const Lane &) { return {1.0f, 0.0f}; }
+    struct Raw {
+        u32x4 q[8];
+        __device__ __forceinline__ void load(const uint8_t *row, const Lane &l, uint32_t left) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] = al16(row + l.at + 16 * i);
+            if (left < STEP) {       // what lies behind the row may be anything, an infinity too
+                const uint32_t n = left > l.at ? (left - l.at) / 2 : 0;
+#pragma unroll
+                for (uint32_t i = 0; i < 32; ++i) q[i / 4][i % 4] &= 2 * i + 1 < n ? ~0u : 2 * i < n ? 0xFFFFu : 0u;
+            }
+        }
+    };
+    GGQ_SCALE { return {1.0f, 0.0f}; }
 };
 // upper 16 bits of v, a NaN kept a NaN; `rest` = v minus that, exactly (0 where v is not finite)
 __device__ __forceinline__ uint32_t take_bf16(float v, float &rest) {

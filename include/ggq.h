@@ -284,7 +284,8 @@ ggq_status ggq_dequantize_noalloc(uint32_t ggml_type, uint32_t out_type,
  * ggq_matvec_device: y[t][r] = sum over c of W[r][c] * x[t][c], for t < tokens.  Products are exact, sums are held in
  *   32 bits in an order that depends on the sizes alone, and one rounding to y_type ends each.  Made for the few
  *   tokens of decoding; any number is computed.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
- *   there are two tokens or more (GGQ_INVALID).  cols must be whole blocks (GGQ_INDIVISIBLE); cols == 0 gives zeros.
+ *   there are two tokens or more (GGQ_INVALID).  cols must be whole blocks (GGQ_INDIVISIBLE) and below 2^26, rows and tokens below
+ *   2^30 (GGQ_INVALID); cols == 0 gives zeros.
  *   Intermediate sums are those of whole-number codes times x: |x| stays below 2^100, and non-finite x makes the
  *   token's outputs non-finite where the row's codes reach it, of either kind.
  * ggq_get_rows_device: y[i] = the decoded row ids[i] of W, i < n: the token embeddings of n ids.  id_type is the
