@@ -126,26 +126,25 @@ __device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, ui
     }
 }
 
-// Stages `steps` steps of x from step `first` on.  row(t): the element offset of token t's row.
-template <class F, int NC, int CHAIN, class Row>
-__device__ __forceinline__ void stage_x(uint8_t *lds, uint32_t first, uint32_t steps, const void *x, uint32_t kind, uint64_t cols,
-                                        uint32_t tokens, uint32_t parts, Row row) {
+// Stages `steps` steps of x.  load(step, t, f, v): the eight elements of fragment f (of 128) of that step, for token t.
+template <class F, int NC, int CHAIN, class Load>
+__device__ __forceinline__ void stage_x(uint8_t *lds, uint32_t steps, uint32_t tokens, uint32_t parts, Load load) {
     typedef Slice<F> S;
     typedef XStep<F, NC, CHAIN> X;
     const uint32_t frags = steps * 128;
     for (uint32_t i = threadIdx.x; i < frags * tokens; i += blockDim.x) {       // whole waves: frags is a multiple of 64
-        const uint32_t t = NC == 1 || tokens == 1 ? 0 : i / frags, f = i - t * frags;
+        const uint32_t t = NC == 1 || tokens == 1 ? 0 : i / frags, f = (i - t * frags) & 127u, n = (i - t * frags) >> 7;
         uint32_t sl, k;
         if constexpr (S::PLANES) {
             sl = ((f >> 3) & 12u) | ((f >> 3) & 2u) | ((f >> 1) & 1u);
             k = ((f >> 1) & 6u) | (f & 1u);
         } else {
-            sl = (f >> 3) & 15u;
+            sl = f >> 3;
             k = f & 7u;
         }
-        uint8_t *step = lds + (f >> 7) * X::BYTES;
+        uint8_t *step = lds + n * X::BYTES;
         float v[8];
-        load8(x, row(t), ((uint64_t)first * 128 + f) * 8, cols, kind, v);
+        load(n, t, f, v);
         const uint32_t col = t * parts;
         if constexpr (S::OFFSET) {
             float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
@@ -239,33 +238,36 @@ struct Image {
     static constexpr uint32_t ROWS = 4 * RT, PIECES = (S::UNIT + 15) / 16, PER_ROW = PIECES * S::UNITS, LOADS = (PER_ROW * ROWS + 63) / 64;
     static constexpr uint32_t UNIT = PIECES * 16, ROW = UNIT * S::UNITS + (UNIT * S::UNITS % 64 == 32 ? 32 : 0) + 16 * (UNIT * S::UNITS % 32 / 16);
     static constexpr uint32_t BYTES = ROW * ROWS;
-    uint32_t src[LOADS], dst[LOADS];          // from the tile's first row on; in the image
+    // where this lane's pieces are
+    struct Places {
+        uint32_t src[LOADS], dst[LOADS];      // from the tile's first row on; in the image
+        // `rows` of the tile's rows exist; the others are the last one again
+        __device__ __forceinline__ Places(uint32_t lane, uint32_t rows, uint32_t row_bytes) {
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                uint32_t p = i * 64 + lane;
+                if (p >= PER_ROW * ROWS) p = PER_ROW * ROWS - 1;
+                const uint32_t r = p / PER_ROW, u = p % PER_ROW / PIECES, c = p % PIECES * 16;
+                src[i] = (r < rows ? r : rows - 1) * row_bytes + u * S::UNIT + c;
+                dst[i] = r * ROW + u * UNIT + c;
+            }
+        }
+    };
     u32x4 v[LOADS];
 
-    // `rows` of the tile's rows exist; the others are the last one again
-    __device__ __forceinline__ Image(uint32_t lane, uint32_t rows, uint32_t row_bytes) {
-#pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) {
-            uint32_t p = i * 64 + lane;
-            if (p >= PER_ROW * ROWS) p = PER_ROW * ROWS - 1;
-            const uint32_t r = p / PER_ROW, u = p % PER_ROW / PIECES, c = p % PIECES * 16;
-            src[i] = (r < rows ? r : rows - 1) * row_bytes + u * S::UNIT + c;
-            dst[i] = r * ROW + u * UNIT + c;
-        }
-    }
     // The step that begins at `base` (in the tile's first row).  A unit's last piece and a row's last step may reach beyond
     // them, into whatever follows in the tensor; `room` bytes of the tensor are left from base on, and where the furthest
     // piece would end behind them (`reach`), pieces are moved back to end with it and shifted into place.
-    __device__ __forceinline__ void fetch(const uint8_t *base, uint64_t room, uint32_t reach) {
+    __device__ __forceinline__ void fetch(const Places &at, const uint8_t *base, uint64_t room, uint32_t reach) {
         if (room >= reach) {
 #pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i) v[i] = ld16(base + src[i]);
+            for (uint32_t i = 0; i < LOADS; ++i) v[i] = ld16(base + at.src[i]);
         } else {
             const int32_t limit = (int32_t)room - 16;
 #pragma unroll
             for (uint32_t i = 0; i < LOADS; ++i) {
-                const int32_t from = (int32_t)src[i] < limit ? (int32_t)src[i] : limit;
-                const uint32_t back = src[i] - (uint32_t)from;
+                const int32_t from = (int32_t)at.src[i] < limit ? (int32_t)at.src[i] : limit;
+                const uint32_t back = at.src[i] - (uint32_t)from;
                 v[i] = shifted(ld16(base + from), back < 15 ? back : 15);
             }
         }
@@ -281,9 +283,9 @@ struct Image {
         }
         return {o[0], o[1], o[2], o[3]};
     }
-    __device__ __forceinline__ void put(uint8_t *image) const {
+    __device__ __forceinline__ void put(const Places &at, uint8_t *image) const {
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) *(u32x4 *)(image + dst[i]) = v[i];
+        for (uint32_t i = 0; i < LOADS; ++i) *(u32x4 *)(image + at.dst[i]) = v[i];
     }
 };
 
@@ -330,23 +332,26 @@ __global__ __launch_bounds__(QD_THREADS) void matvec_quads(MatvecArgs a) {
 #pragma unroll
         for (int c = 0; c < NC; ++c) acc[t][c] = 0.0f;
 
-    I in(lane, rows, row_bytes);
-    if (kp < steps) in.fetch(w, behind + left, reach);
+    const typename I::Places places(lane, rows, row_bytes);
+    I in;
+    if (kp < steps) in.fetch(places, w, behind + left, reach);
     uint32_t step = kp;
     for (uint32_t first = 0; first < steps; first += a.chunk) {
         const uint32_t now = first + a.chunk < steps ? a.chunk : steps - first, end = first + now;
         if (first) __syncthreads();
-        stage_x<F, NC, CHAIN>(xs, first, now, a.x, a.x_kind, a.cols, a.tokens, a.parts, [&](uint32_t t) { return t * a.x_stride; });
+        stage_x<F, NC, CHAIN>(xs, now, a.tokens, a.parts, [&](uint32_t n, uint32_t t, uint32_t f, float (&v)[8]) {
+            load8(a.x, t * a.x_stride, ((uint64_t)(first + n) * 128 + f) * 8, a.cols, a.x_kind, v);
+        });
         __syncthreads();
         for (; step < end; step += a.ksplit) {
             wave_order();
-            in.put(image);
+            in.put(places, image);
             wave_order();
             const uint32_t here = left;
             if (step + a.ksplit < steps) {
                 w += (uint64_t)a.ksplit * S::STEP;
                 left -= a.ksplit * S::STEP;
-                in.fetch(w, behind + left, reach);
+                in.fetch(places, w, behind + left, reach);
             }
             typename S::Raw raw[RT];
 #pragma unroll
@@ -423,141 +428,6 @@ __global__ __launch_bounds__(MV_THREADS) void get_rows(RowsArgs a, uint64_t firs
 #pragma unroll
     for (int j = 0; j < 4; ++j)
         if (c + j < a.cols) store_elem(a.y, i * a.y_stride + c + j, a.y_kind, w[j]);
-}
-
-// ---- mixture of experts ---------------------------------------------------------------------------------
-struct MoeArgs {
-    const uint8_t *gate, *up, *down;
-    const void *router, *x;
-    void *y;
-    float *logits;        // [tokens][experts]
-    int32_t *ids;         // [tokens][top_k]
-    float *weights;       // [tokens][top_k]
-    float *h;             // [tokens * top_k][ff]
-    int32_t *out_ids;     // the caller's, or null
-    float *out_weights;
-    uint64_t hidden, ff, x_stride, y_stride;
-    uint32_t tokens, experts, top_k, router_kind, x_kind, y_kind;
-    uint32_t sigmoid, normalize, gelu;
-    float scale;
-};
-
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-    return v;
-}
-
-// one workgroup per expert; a product of two f32 values is exact in 64 bits
-__global__ __launch_bounds__(MV_THREADS) static void moe_logits(MoeArgs a) {
-    __shared__ double part[MV_THREADS / 64];
-    const uint32_t e = blockIdx.x;
-    for (uint32_t t = 0; t < a.tokens; ++t) {
-        double s = 0.0;
-        for (uint64_t c = threadIdx.x; c < a.hidden; c += MV_THREADS)
-            s = __builtin_fma((double)load_elem(a.router, e * a.hidden + c, a.router_kind), (double)load_elem(a.x, t * a.x_stride + c, a.x_kind), s);
-        s = wave_sum(s);
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (uint32_t w = 1; w < MV_THREADS / 64; ++w) s += part[w];
-            a.logits[(uint64_t)t * a.experts + e] = (float)s;
-        }
-        __syncthreads();
-    }
-}
-
-// an order-preserving key of a logit: larger logit, larger key; NaN below everything; -0 equals +0
-__device__ __forceinline__ uint32_t logit_key(float v) {
-    if (v != v) return 0u;
-    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-
-// one wave per token
-__global__ __launch_bounds__(64) static void moe_route(MoeArgs a) {
-    const uint32_t t = blockIdx.x, lane = threadIdx.x;
-    const float *l = a.logits + (uint64_t)t * a.experts;
-    float top = -__builtin_inff();
-    for (uint32_t e = lane; e < a.experts; e += 64) top = __builtin_fmaxf(top, l[e]);
-    for (int m = 32; m; m >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, m));
-    float total = 0.0f;
-    if (!a.sigmoid) {
-        for (uint32_t e = lane; e < a.experts; e += 64) total += expf(l[e] - top);
-        total = wave_sum(total);
-    }
-    uint64_t last = ~0ull;
-    float sum = 0.0f, mine = 0.0f;
-    for (uint32_t j = 0; j < a.top_k; ++j) {
-        uint64_t best = 0;
-        for (uint32_t e = lane; e < a.experts; e += 64) {
-            const uint64_t key = ((uint64_t)logit_key(l[e]) << 32) | (0xFFFFFFFFu - e);
-            if (key < last && key > best) best = key;
-        }
-        for (int m = 32; m; m >>= 1) {
-            const uint64_t other = __shfl_xor(best, m);
-            if (other > best) best = other;
-        }
-        last = best;
-        const uint32_t e = 0xFFFFFFFFu - (uint32_t)best;
-        const float v = l[e], p = a.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) / total;
-        sum += p;
-        if (lane == j) mine = p;
-        if (lane == 0) {
-            a.ids[t * a.top_k + j] = (int32_t)e;
-            if (a.out_ids) a.out_ids[t * a.top_k + j] = (int32_t)e;
-        }
-    }
-    if (lane < a.top_k) {
-        const float w = (a.normalize ? mine / sum : mine) * a.scale;
-        a.weights[t * a.top_k + lane] = w;
-        if (a.out_weights) a.out_weights[t * a.top_k + lane] = w;
-    }
-}
-
-__device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
-    if (!gelu) return g / (1.0f + expf(-g));
-    const float z = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-    return 0.5f * g * (1.0f + tanhf(z));
-}
-
-template <class F>
-__device__ __forceinline__ float row_dot(const uint8_t *row, uint64_t cols, const void *x, uint64_t at, uint32_t kind) {
-    float sum = 0.0f;
-    for (uint64_t c = 4 * (threadIdx.x % 64); c < cols; c += 256) {
-        float w[4];
-        row4<F>(row, c, cols, w);
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (c + i < cols) sum = __builtin_fmaf(w[i], load_elem(x, at + c + i, kind), sum);
-    }
-    return wave_sum(sum);
-}
-
-template <class F>
-__global__ __launch_bounds__(MV_THREADS) void moe_up(MoeArgs a) {
-    const uint64_t r = (uint64_t)blockIdx.x * (MV_THREADS / 64) + threadIdx.x / 64;
-    if (r >= a.ff) return;
-    const uint32_t pair = blockIdx.y, t = pair / a.top_k;
-    const uint64_t e = (uint64_t)a.ids[pair];
-    const float g = row_dot<F>(a.gate + (e * a.ff + r) * (a.hidden / F::N * F::BYTES), a.hidden, a.x, t * a.x_stride, a.x_kind);
-    const float u = row_dot<F>(a.up + (e * a.ff + r) * (a.hidden / F::N * F::BYTES), a.hidden, a.x, t * a.x_stride, a.x_kind);
-    if (threadIdx.x % 64 == 0) a.h[pair * a.ff + r] = moe_act(g, a.gelu) * u;
-}
-
-template <class FD>
-__global__ __launch_bounds__(MV_THREADS) void moe_down(MoeArgs a) {
-    const uint64_t r = (uint64_t)blockIdx.x * (MV_THREADS / 64) + threadIdx.x / 64;
-    if (r >= a.hidden) return;
-    const uint32_t t = blockIdx.y;
-    float y = 0.0f;
-    for (uint32_t j = 0; j < a.top_k; ++j) {
-        const uint32_t pair = t * a.top_k + j;
-        const uint64_t e = (uint64_t)a.ids[pair];
-        const float d = row_dot<FD>(a.down + (e * a.hidden + r) * (a.ff / FD::N * FD::BYTES), a.ff, a.h, pair * a.ff, EK_F32);
-        y = __builtin_fmaf(a.weights[pair], d, y);
-    }
-    if (threadIdx.x % 64 == 0) store_elem(a.y, t * a.y_stride + r, a.y_kind, y);
 }
 
 }  // namespace ggq

@@ -2,6 +2,7 @@
 #include "../../include/ggq.h"
 #include "internal.h"
 #include "matmul.h"
+#include "moe.h"
 
 #include <algorithm>
 
@@ -59,24 +60,36 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
 // Shared memory of one workgroup for x.
 constexpr uint32_t X_LDS = 40 << 10;
 
+// Tiles of a wave: with a few hundred packed bytes a row and step, two share the fragments of x.
+template <class F> constexpr int row_tiles() { return Slice<F>::STEP <= 640 ? 2 : 1; }
+
+// The shape of a launch over `tiles` wave tiles, each of which takes `steps` steps: how many waves share a tile's steps,
+// the steps staged at a time (equal chunks, whole turns of the waves), the shared memory.
+struct Shape {
+    uint32_t ksplit, chunk, groups, bytes;
+    Shape(uint64_t tiles, uint32_t steps, uint32_t step_bytes, uint32_t image_bytes, uint32_t part_bytes) {
+        // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
+        ksplit = 1;
+        while (ksplit < QD_WAVES && ksplit < steps && tiles * ksplit < 2048 && 2 * ksplit * step_bytes <= X_LDS) ksplit *= 2;
+        const uint32_t turns = (steps + ksplit - 1) / ksplit, most = X_LDS / (step_bytes * ksplit), chunks = (turns + most - 1) / most;
+        chunk = (turns + chunks - 1) / chunks * ksplit;
+        groups = QD_WAVES / ksplit;
+        bytes = QD_WAVES * image_bytes + std::max(std::min(chunk, steps) * step_bytes, QD_WAVES * part_bytes);
+    }
+};
+
 template <class F, int NC, int CHAIN>
 void launch_quads(MatvecArgs a, hipStream_t st) {
-    constexpr int RT = Slice<F>::STEP <= 640 ? 2 : 1;
+    constexpr int RT = row_tiles<F>();
     typedef XStep<F, NC, CHAIN> X;
     typedef Image<F, RT> I;
-    const uint32_t steps = (uint32_t)((a.cols + 1023) / 1024);
     const uint64_t tiles = (a.rows + I::ROWS - 1) / I::ROWS;
-    // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
-    a.ksplit = 1;
-    while (a.ksplit < QD_WAVES && a.ksplit < steps && tiles * a.ksplit < 2048 && 2 * a.ksplit * X::BYTES <= X_LDS) a.ksplit *= 2;
-    // equal chunks
-    const uint32_t turns = (steps + a.ksplit - 1) / a.ksplit, most = X_LDS / (X::BYTES * a.ksplit), chunks = (turns + most - 1) / most;
-    a.chunk = (turns + chunks - 1) / chunks * a.ksplit;
-    const uint32_t x_bytes = std::max<uint32_t>(std::min(a.chunk, steps) * X::BYTES, QD_WAVES * NC * I::ROWS * 4);
-    const uint32_t bytes = QD_WAVES * I::BYTES + x_bytes, groups = QD_WAVES / a.ksplit;
-    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * groups) {
-        const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + groups - 1) / groups));
-        matvec_quads<F, NC, CHAIN, RT><<<grid, QD_THREADS, bytes, st>>>(a);
+    const Shape sh(tiles, (uint32_t)((a.cols + 1023) / 1024), X::BYTES, I::BYTES, NC * I::ROWS * 4);
+    a.ksplit = sh.ksplit;
+    a.chunk = sh.chunk;
+    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * sh.groups) {
+        const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + sh.groups - 1) / sh.groups));
+        matvec_quads<F, NC, CHAIN, RT><<<grid, QD_THREADS, sh.bytes, st>>>(a);
     }
 }
 
@@ -105,6 +118,106 @@ uint64_t launch_few(MatvecArgs a, uint64_t tokens, uint32_t pieces, hipStream_t 
         launch_quads<F, 4, 3>(a, st);
     }
     return a.tokens;
+}
+
+}  // namespace
+
+// ---- mixture of experts ---------------------------------------------------------------------------------
+namespace {
+
+uint64_t up256(uint64_t v) { return (v + 255) & ~255ull; }
+
+ggq_status check_moe(const ggq_moe *m, uint64_t tokens) {
+    if (!m) return GGQ_INVALID;
+    uint32_t kind, bytes;
+    const uint64_t ub = ggq_block_elems(m->up_type), db = ggq_block_elems(m->down_type);
+    if (!ub || !db || !elem_kind(m->router_type, &kind, &bytes)) return GGQ_UNSUPPORTED;
+    if (m->hidden >= MAX_COLS || m->ff >= MAX_COLS || m->hidden == 0 || m->ff == 0) return GGQ_INVALID;
+    if (m->hidden % ub != 0 || m->ff % db != 0) return GGQ_INDIVISIBLE;
+    if (m->experts == 0 || m->experts > GGQ_MOE_MAX_EXPERTS || m->top_k == 0 || m->top_k > m->experts || m->top_k > GGQ_MOE_MAX_TOP_K)
+        return GGQ_INVALID;
+    if (m->reserved || m->gating > 1 || m->normalize > 1 || m->activation > 1) return GGQ_INVALID;
+    if (tokens > GGQ_MOE_MAX_TOKENS) return GGQ_TOO_LARGE;
+    return GGQ_OK;
+}
+
+// byte offsets of the workspace's parts
+struct MoeSpace {
+    uint64_t ids, weights, h, o, end;
+    MoeSpace(const ggq_moe &m, uint64_t tokens) {
+        ids = up256(4 * tokens * m.experts);
+        weights = ids + up256(4 * tokens * m.top_k);
+        h = weights + up256(4 * tokens * m.top_k);
+        o = h + up256(4 * tokens * m.top_k * m.ff);
+        end = o + (tokens > 4 ? up256(4 * tokens * m.top_k * m.hidden) : 0);
+    }
+};
+
+template <class F, int NC, int CHAIN>
+void launch_up(MoeArgs a, hipStream_t st) {
+    typedef Image<F, 1> I;
+    const uint32_t tiles = (uint32_t)((a.ff + 3) / 4);
+    const Shape sh((uint64_t)tiles * a.slots, (uint32_t)((a.hidden + 1023) / 1024), XStep<F, NC, CHAIN>::BYTES, 2 * I::BYTES, 2 * NC * 16);
+    a.ksplit = sh.ksplit;
+    a.chunk = sh.chunk;
+    moe_up<F, NC, CHAIN><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), QD_THREADS, sh.bytes, st>>>(a);
+}
+
+template <class F>
+void launch_up_of(MoeArgs a, hipStream_t st) {
+    if constexpr (is_float_type<F>) {
+        if (a.hidden < 8) {
+            moe_up_short<F><<<dim3((uint32_t)((a.ff + MV_THREADS - 1) / MV_THREADS), a.tokens * a.top_k), MV_THREADS, 0, st>>>(a);
+            return;
+        }
+    }
+    const uint32_t pieces = a.x_kind == EK_F32 ? 3 : a.x_kind == EK_F16 ? 2 : 1;
+    a.parts = a.tokens == 1 ? pieces : 1;
+    if (a.tokens == 1) {
+        if (pieces == 1) launch_up<F, 1, 1>(a, st);
+        else if (pieces == 2) launch_up<F, 2, 1>(a, st);
+        else launch_up<F, 3, 1>(a, st);
+    } else {
+        if (pieces == 1) launch_up<F, 4, 1>(a, st);
+        else if (pieces == 2) launch_up<F, 4, 2>(a, st);
+        else launch_up<F, 4, 3>(a, st);
+    }
+}
+
+template <class F, int NC, int CHAIN>
+void launch_down_few(MoeArgs a, hipStream_t st) {
+    constexpr int RT = row_tiles<F>();
+    typedef Image<F, RT> I;
+    const uint32_t tiles = (uint32_t)((a.hidden + I::ROWS - 1) / I::ROWS);
+    const Shape sh(tiles, (uint32_t)((a.ff + 1023) / 1024) * a.tokens * a.top_k, XStep<F, NC, CHAIN>::BYTES, I::BYTES, NC * I::ROWS * 4);
+    a.ksplit = sh.ksplit;
+    a.chunk = sh.chunk;
+    moe_down_few<F, NC, CHAIN, RT><<<(tiles + sh.groups - 1) / sh.groups, QD_THREADS, sh.bytes, st>>>(a);
+}
+
+template <class F>
+void launch_down_of(MoeArgs a, hipStream_t st) {
+    if constexpr (is_float_type<F>) {
+        if (a.ff < 8) {
+            moe_down_short<F><<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
+            return;
+        }
+    }
+    a.parts = a.tokens == 1 ? 3 : 1;
+    if (a.tokens == 1) {
+        launch_down_few<F, 3, 1>(a, st);
+    } else if (a.tokens <= 4) {
+        launch_down_few<F, 4, 3>(a, st);
+    } else {
+        constexpr int RT = row_tiles<F>();
+        typedef Image<F, RT> I;
+        const uint32_t tiles = (uint32_t)((a.hidden + I::ROWS - 1) / I::ROWS);
+        const Shape sh((uint64_t)tiles * a.slots, (uint32_t)((a.ff + 1023) / 1024), XStep<F, 4, 3>::BYTES, I::BYTES, 4 * I::ROWS * 4);
+        a.ksplit = sh.ksplit;
+        a.chunk = sh.chunk;
+        moe_down_many<F, RT><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), QD_THREADS, sh.bytes, st>>>(a);
+        moe_sum<<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
+    }
 }
 
 }  // namespace
@@ -181,37 +294,6 @@ ggq_status ggq_get_rows_device(uint32_t ty, uint64_t rows, uint64_t cols, const 
 }
 
 // ---- mixture of experts ---------------------------------------------------------------------------------
-namespace {
-
-uint64_t up256(uint64_t v) { return (v + 255) & ~255ull; }
-
-ggq_status check_moe(const ggq_moe *m, uint64_t tokens) {
-    if (!m) return GGQ_INVALID;
-    uint32_t kind, bytes;
-    const uint64_t ub = ggq_block_elems(m->up_type), db = ggq_block_elems(m->down_type);
-    if (!ub || !db || !elem_kind(m->router_type, &kind, &bytes)) return GGQ_UNSUPPORTED;
-    if (m->hidden >= MAX_COLS || m->ff >= MAX_COLS || m->hidden == 0 || m->ff == 0) return GGQ_INVALID;
-    if (m->hidden % ub != 0 || m->ff % db != 0) return GGQ_INDIVISIBLE;
-    if (m->experts == 0 || m->experts > GGQ_MOE_MAX_EXPERTS || m->top_k == 0 || m->top_k > m->experts || m->top_k > GGQ_MOE_MAX_TOP_K)
-        return GGQ_INVALID;
-    if (m->reserved || m->gating > 1 || m->normalize > 1 || m->activation > 1) return GGQ_INVALID;
-    if (tokens > GGQ_MOE_MAX_TOKENS) return GGQ_TOO_LARGE;
-    return GGQ_OK;
-}
-
-// byte offsets of the workspace's parts
-struct MoeSpace {
-    uint64_t ids, weights, h, end;
-    MoeSpace(const ggq_moe &m, uint64_t tokens) {
-        ids = up256(4 * tokens * m.experts);
-        weights = ids + up256(4 * tokens * m.top_k);
-        h = weights + up256(4 * tokens * m.top_k);
-        end = h + up256(4 * tokens * m.top_k * m.ff);
-    }
-};
-
-}  // namespace
-
 ggq_status ggq_moe_workspace_bytes(const ggq_moe *m, uint64_t tokens, size_t *bytes_out) {
     const ggq_status st = check_moe(m, tokens);
     if (st != GGQ_OK) return st;
@@ -247,6 +329,7 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     a.ids = (int32_t *)(space + ws.ids);
     a.weights = (float *)(space + ws.weights);
     a.h = (float *)(space + ws.h);
+    a.o = (float *)(space + ws.o);
     a.out_ids = d_ids;
     a.out_weights = d_weights;
     a.hidden = m->hidden;
@@ -263,11 +346,11 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     hipStream_t st = (hipStream_t)hip_stream;
     moe_logits<<<m->experts, MV_THREADS, 0, st>>>(a);
     moe_route<<<(uint32_t)tokens, 64, 0, st>>>(a);
-    const dim3 up_grid((uint32_t)((m->ff + 3) / 4), (uint32_t)tokens * m->top_k), down_grid((uint32_t)((m->hidden + 3) / 4), (uint32_t)tokens);
-#define CASE(F) moe_up<F><<<up_grid, MV_THREADS, 0, st>>>(a)
+    a.slots = std::min(m->experts, (uint32_t)tokens * m->top_k);
+#define CASE(F) launch_up_of<F>(a, st)
     GGQ_FOR_TYPE(m->up_type, CASE)
 #undef CASE
-#define CASE(F) moe_down<F><<<down_grid, MV_THREADS, 0, st>>>(a)
+#define CASE(F) launch_down_of<F>(a, st)
     GGQ_FOR_TYPE(m->down_type, CASE)
 #undef CASE
     HIP_TRY(hipGetLastError());
