@@ -159,11 +159,11 @@ __device__ __forceinline__ void stage_x(uint8_t *lds, uint32_t steps, uint32_t t
         uint8_t *to = step + k * X::K + (sl * NC + col) * 16;
         const uint32_t pieces = CHAIN > 1 ? CHAIN : parts, stride = CHAIN > 1 ? 8 * X::K : 16;
         for (uint32_t p = 0; p < pieces; ++p, to += stride) {
-            uint32_t h[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) h[j] = take_bf16(v[j], v[j]);
-            const u32x4 w = {h[0] | (h[1] << 16), h[2] | (h[3] << 16), h[4] | (h[5] << 16), h[6] | (h[7] << 16)};
+            const u32x4 w = {upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7])};
             *(u32x4 *)to = w;
+            if (p + 1 < pieces)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = below_bf16(v[j]);
         }
     }
 }

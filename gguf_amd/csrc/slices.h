@@ -444,13 +444,9 @@ struct SliceOfFloats {
     };
     GGQ_SCALE { return {1.0f, 0.0f}; }
 };
-// upper 16 bits of v, a NaN kept a NaN; `rest` = v minus that, exactly (0 where v is not finite)
-__device__ __forceinline__ uint32_t take_bf16(float v, float &rest) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const bool odd = (b & 0x7F800000u) == 0x7F800000u;
-    const uint32_t t = (v != v ? b | 0x00400000u : b) & 0xFFFF0000u;
-    rest = odd ? 0.0f : v - __builtin_bit_cast(float, t);
-    return t >> 16;
+// v minus its upper 16 bits as a bf16, exactly; a NaN where v is not finite
+__device__ __forceinline__ float below_bf16(float v) {
+    return v - __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & 0xFFFF0000u);
 }
 template <> struct Slice<WBF16> : SliceOfFloats {
     static constexpr int WP = 1;
@@ -465,9 +461,8 @@ template <> struct Slice<WF16> : SliceOfFloats {
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const uint32_t w = r.q[4 * S + i / 4][i % 4];
-            float l0, l1, none;
-            const uint32_t h0 = take_bf16(h2f(w & 0xFFFFu), l0), h1 = take_bf16(h2f(w >> 16), l1);
-            b[i] = piece == 0 ? h0 | (h1 << 16) : take_bf16(l0, none) | (take_bf16(l1, none) << 16);
+            const float v0 = h2f(w & 0xFFFFu), v1 = h2f(w >> 16);
+            b[i] = piece == 0 ? upper_halves(v0, v1) : upper_halves(below_bf16(v0), below_bf16(v1));
         }
     }
 };
