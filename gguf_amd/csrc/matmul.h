@@ -5,6 +5,7 @@
 // and what surrounds them in a decoding step: rows of a packed table by id, and a mixture-of-experts layer.
 #pragma once
 #include "slices.h"
+#include <type_traits>
 
 namespace ggq {
 
@@ -60,46 +61,36 @@ __device__ __forceinline__ float wave_sum(float v) {
     return v;
 }
 
-// ---- the product ----------------------------------------------------------------------------------------
+// ---- shared by the products -------------------------------------------------------------------------------
 struct MatvecArgs {
     const uint8_t *w;
     const void *x;
     void *y;
     uint64_t rows, cols, x_stride, y_stride;
-    uint64_t first_tile;      // groups of four rows before this launch's
-    uint32_t tokens;          // of this launch's group: at most NC / parts
+    uint64_t first_tile;      // wave tiles before this launch's
+    uint32_t tokens;          // of this launch's group
     uint32_t x_kind, y_kind;
-    uint32_t parts;           // columns that a token takes: its bf16 pieces, or 1 where they follow each other
-    uint32_t chunk;           // steps staged at a time, a multiple of ksplit
-    uint32_t ksplit;          // waves that share a row group's columns: 1, 2, 4 or 8
+    uint32_t chunk;           // turns staged at a time, a multiple of ksplit
+    uint32_t ksplit;          // waves that share a tile's columns: 1, 2, 4 or 8
 };
 
-constexpr uint32_t MV_THREADS = 256;      // the other kernels here
-constexpr uint32_t QD_WAVES = 8, QD_THREADS = 64 * QD_WAVES;
+constexpr uint32_t MV_THREADS = 256;      // the small kernels here
+constexpr uint32_t TILE_WAVES = 8, TILE_THREADS = 64 * TILE_WAVES;
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
 
-// x in shared memory, as the matrix unit takes it: fragments of eight bf16 (16 bytes).  A step (16 slices, 1024 elements)
-// is [chain][k][slice][column], k = the fragment's place in its slice: the 16 quads of a wave read the same k of 16
-// neighbouring slices, so their addresses are consecutive and all other parts of the address are constants.  16 bytes
-// between one k and the next keep the staging threads, which run along k first, out of each other's banks.  Behind the
-// fragments, for formats with an offset, the sum of x over each sub-block: [sub-block][slice][column], f32, a token's whole
-// sum in the first of its columns and zero in the others.
-//   NC columns: tokens times their pieces side by side; CHAIN: pieces one after the other into the same columns.
-template <class F, int NC, int CHAIN>
-struct XStep {
-    typedef Slice<F> S;
-    static constexpr uint32_t K = 256 * NC + 16;
-    static constexpr uint32_t SUMS = CHAIN * 8 * K;
-    static constexpr uint32_t BYTES = SUMS + (S::OFFSET ? S::NSUB * 64 * NC : 0);
-};
-
-template <int CTRL>
-__device__ __forceinline__ float dpp(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
-}
 constexpr int QUAD_XOR1 = 0xB1, QUAD_XOR2 = 0x4E, ROW_ROR4 = 0x124, ROW_ROR8 = 0x128;
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) { return __builtin_bit_cast(float, dpp<CTRL>(__builtin_bit_cast(uint32_t, v))); }
+
+// Orders a wave's own accesses to shared memory (its lanes read what others of the wave wrote).
+__device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
 
 // eight elements of x from c on, 0 past the end
 __device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, uint64_t cols, uint32_t kind, float (&v)[8]) {
@@ -126,117 +117,17 @@ __device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, ui
     }
 }
 
-// Stages `steps` steps of x.  load(step, t, f, v): the eight elements of fragment f (of 128) of that step, for token t.
-template <class F, int NC, int CHAIN, class Load>
-__device__ __forceinline__ void stage_x(uint8_t *lds, uint32_t steps, uint32_t tokens, uint32_t parts, Load load) {
-    typedef Slice<F> S;
-    typedef XStep<F, NC, CHAIN> X;
-    const uint32_t frags = steps * 128;
-    for (uint32_t i = threadIdx.x; i < frags * tokens; i += blockDim.x) {       // whole waves: frags is a multiple of 64
-        const uint32_t t = NC == 1 || tokens == 1 ? 0 : i / frags, f = (i - t * frags) & 127u, n = (i - t * frags) >> 7;
-        uint32_t sl, k;
-        if constexpr (S::PLANES) {
-            sl = ((f >> 3) & 12u) | ((f >> 3) & 2u) | ((f >> 1) & 1u);
-            k = ((f >> 1) & 6u) | (f & 1u);
-        } else {
-            sl = f >> 3;
-            k = f & 7u;
-        }
-        uint8_t *step = lds + n * X::BYTES;
-        float v[8];
-        load(n, t, f, v);
-        const uint32_t col = t * parts;
-        if constexpr (S::OFFSET) {
-            float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-            sum += dpp<QUAD_XOR1>(sum);
-            if (S::SUB == 32) sum += dpp<QUAD_XOR2>(sum);
-            if (f % (S::SUB / 8) == 0) {
-                float *to = (float *)(step + X::SUMS) + (k / (S::SUB / 8) * 16 + sl) * NC + col;
-                to[0] = sum;
-                for (uint32_t p = 1; p < parts; ++p) to[p] = 0.0f;
-            }
-        }
-        uint8_t *to = step + k * X::K + (sl * NC + col) * 16;
-        const uint32_t pieces = CHAIN > 1 ? CHAIN : parts, stride = CHAIN > 1 ? 8 * X::K : 16;
-        for (uint32_t p = 0; p < pieces; ++p, to += stride) {
-            const u32x4 w = {upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7])};
-            *(u32x4 *)to = w;
-            if (p + 1 < pieces)
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = below_bf16(v[j]);
-        }
-    }
-}
-
-// acc[t][c] += sub-block S of the lane's slice of its row in tile t, times column c of x, for RT tiles of four rows that
-// share the fragments.  `x`: the step's fragments, from the lane's own on; `sums`: the step's sums from the lane's slice on.
-template <class F, int NC, int CHAIN, int RT, int S>
-__device__ __forceinline__ void add_sub(const typename Slice<F>::Raw (&raw)[RT], const typename Slice<F>::Lane &lane, const uint8_t *x,
-                                        const uint8_t *sums, float (&acc)[RT][NC]) {
-    typedef Slice<F> T;
-    typedef XStep<F, NC, CHAIN> X;
-    constexpr int FRAGS = T::SUB / 8, WORDS = T::SUB / 2;
-    constexpr int WP = [] { if constexpr (is_float_type<F>) return T::WP; else return 1; }();
-    f32x4 d[RT];
-#pragma unroll
-    for (int t = 0; t < RT; ++t) d[t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-    for (int piece = 0; piece < WP; ++piece) {
-        uint32_t b[RT][WORDS];
-#pragma unroll
-        for (int t = 0; t < RT; ++t) {
-            if constexpr (is_float_type<F>) T::template codes<S>(raw[t], lane, b[t], piece);
-            else T::template codes<S>(raw[t], lane, b[t]);
-        }
-#pragma unroll
-        for (int p = 0; p < CHAIN; ++p)
-#pragma unroll
-            for (int k = 0; k < FRAGS; ++k) {
-                const u32x4 a = al16(x + (p * 8 + S * FRAGS + k) * X::K);
-#pragma unroll
-                for (int half = 0; half < 2; ++half)
-#pragma unroll
-                    for (int t = 0; t < RT; ++t) {
-                        const u32x2 av = {a[2 * half], a[2 * half + 1]}, bv = {b[t][4 * k + 2 * half], b[t][4 * k + 2 * half + 1]};
-                        d[t] = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, av), __builtin_bit_cast(s16x4, bv), d[t], 0, 0, 0);
-                    }
-            }
-    }
-    float sum[NC];
-    if constexpr (T::OFFSET) {
-#pragma unroll
-        for (int c = 0; c < NC; ++c) sum[c] = ((const float *)(sums + S * 64 * NC))[c];
-    }
-#pragma unroll
-    for (int t = 0; t < RT; ++t) {
-        const SubScale s = T::template scale<S>(raw[t], lane);
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            acc[t][c] = __builtin_fmaf(s.a, d[t][c], acc[t][c]);
-            if constexpr (T::OFFSET) acc[t][c] = __builtin_fmaf(-s.c, sum[c], acc[t][c]);
-        }
-    }
-}
-template <class F, int NC, int CHAIN, int RT>
-__device__ __forceinline__ void add_slices(const typename Slice<F>::Raw (&raw)[RT], const typename Slice<F>::Lane &lane, const uint8_t *x,
-                                           const uint8_t *sums, float (&acc)[RT][NC]) {
-    add_sub<F, NC, CHAIN, RT, 0>(raw, lane, x, sums, acc);
-    add_sub<F, NC, CHAIN, RT, 1>(raw, lane, x, sums, acc);
-    if constexpr (Slice<F>::NSUB == 4) {
-        add_sub<F, NC, CHAIN, RT, 2>(raw, lane, x, sums, acc);
-        add_sub<F, NC, CHAIN, RT, 3>(raw, lane, x, sums, acc);
-    }
-}
-
-// A wave's packed bytes of one step: 4 * RT rows.  Lanes that multiply together hold different rows, so loads straight
-// into their registers would touch a line per lane: the memory pipeline takes about two cycles for each, which held the
-// products at 4.1 TB/s whatever the format's arithmetic.  Instead neighbouring lanes load neighbouring 16-byte pieces into
-// registers, one step ahead, and hand them over through the wave's own part of shared memory.
-template <class F, int RT>
+// A wave's packed bytes of one turn.  Lanes that multiply together hold different rows, so loads straight into their
+// registers would touch a line per lane: the memory pipeline takes about two cycles for each, which held the products at
+// 4.1 TB/s whatever the format's arithmetic.  Instead neighbouring lanes load neighbouring 16-byte pieces into registers,
+// one turn ahead, and hand them over through the wave's own part of shared memory.
+template <class F, uint32_t ROWS>
 struct Image {
     typedef Slice<F> S;
-    static constexpr uint32_t ROWS = 4 * RT, PIECES = (S::UNIT + 15) / 16, PER_ROW = PIECES * S::UNITS, LOADS = (PER_ROW * ROWS + 63) / 64;
-    static constexpr uint32_t UNIT = PIECES * 16, ROW = UNIT * S::UNITS + (UNIT * S::UNITS % 64 == 32 ? 32 : 0) + 16 * (UNIT * S::UNITS % 32 / 16);
+    static constexpr uint32_t TURN_BYTES = S::STEP * S::TURN;          // packed, of a row
+    static constexpr uint32_t PIECES = (S::UNIT + 15) / 16, PER_ROW = PIECES * S::UNITS, LOADS = (PER_ROW * ROWS + 63) / 64;
+    // an odd number of 16-byte places from row to row: the rows' parts of one column lie in different banks
+    static constexpr uint32_t UNIT = PIECES * 16, ROW = 16 * (PER_ROW | 1);
     static constexpr uint32_t BYTES = ROW * ROWS;
     // where this lane's pieces are
     struct Places {
@@ -253,15 +144,21 @@ struct Image {
             }
         }
     };
+    // bytes from a turn's begin in the tile's first row to the end of its furthest piece
+    static __device__ __forceinline__ uint32_t reach(uint32_t rows, uint32_t row_bytes) { return (rows - 1) * row_bytes + (S::UNITS - 1) * S::UNIT + UNIT; }
     u32x4 v[LOADS];
 
-    // The step that begins at `base` (in the tile's first row).  A unit's last piece and a row's last step may reach beyond
+    // The turn that begins at `base` (in the tile's first row).  A unit's last piece and a row's last turn may reach beyond
     // them, into whatever follows in the tensor; `room` bytes of the tensor are left from base on, and where the furthest
-    // piece would end behind them (`reach`), pieces are moved back to end with it and shifted into place.
+    // piece would end behind them, pieces are moved back to end with it and shifted into place.
     __device__ __forceinline__ void fetch(const Places &at, const uint8_t *base, uint64_t room, uint32_t reach) {
         if (room >= reach) {
 #pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i) v[i] = ld16(base + at.src[i]);
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                uint32_t o = at.src[i];
+                asm("" : "+v"(o));            // keeps the offset 32 bits wide, for a load with a scalar base
+                v[i] = ld16(base + o);
+            }
         } else {
             const int32_t limit = (int32_t)room - 16;
 #pragma unroll
@@ -289,95 +186,371 @@ struct Image {
     }
 };
 
-// Orders a wave's own accesses to shared memory (its lanes read what others of the wave wrote).
-__device__ __forceinline__ void wave_order() { __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront"); }
+// What a wave does with a tile of rows, for up to T tokens.  Two kinds, with the same members:
+//     ROWS, ELEMS       rows of the tile, elements of a turn
+//     X_BYTES           shared memory of a turn of x
+//     CLEAR             bytes of zeros in front of the staged x
+//     stage             puts turns of x into shared memory
+//     Me                what a lane knows of its place
+//     add               the products of one turn
+//     total             a lane's sum over the lanes that share its row; lane r < ROWS has row r's
 
-// Sum over the 16 quads of a wave: afterwards every lane holds its row's total.
-__device__ __forceinline__ float quads_sum(float v) {
-    v += dpp<ROW_ROR8>(v);
-    v += dpp<ROW_ROR4>(v);
-    v += __shfl_xor(v, 16);
-    v += __shfl_xor(v, 32);
-    return v;
-}
-
-// One to four tokens.  A wave owns four rows; its quads (four neighbouring lanes, one lane per row) take 16 neighbouring
-// slices at a time, each lane the packed bytes of its row's slice.  v_mfma_f32_4x4x4 with 16 blocks multiplies, in each
-// quad, the four rows' codes with up to four columns of x that the quad's lanes hold: every lane ends with its own row's
-// products, so that the sub-block's scale is applied in the lane that loaded it.  Columns are tokens, or the bf16 pieces
-// of a token (f32 = three pieces, exactly; products with codes are exact, sums are f32).
-template <class F, int NC, int CHAIN, int RT>
-__global__ __launch_bounds__(QD_THREADS) void matvec_quads(MatvecArgs a) {
-    extern __shared__ __align__(16) uint8_t lds[];
+// ---- packed whole-number codes: x in digits ---------------------------------------------------------------
+// The matrix unit multiplies e4m3 bytes with a block scale for each 32 of them.  Codes are such bytes already (slices.h),
+// and so are the digits of x: 32 neighbouring elements share an exponent e, the largest one's; each becomes a whole number
+// of 16 CH bits (truncated, 2^-32 of the largest element, for CH = 2; rounded, 2^-17 of it, for CH = 1, which is taken where
+// the result is rounded to 16 bits anyway) and that CH * 4 hexadecimal digits, each a byte 0..15 with x's sign.  All
+// products and their sums over a sub-block are whole numbers below 2^13, so nothing is rounded before a sub-block's scale.
+//
+// v_mfma_scale_f32_16x16x128: A is x, B the codes of 16 rows.  Lane (n, g), n = lane % 16, g = lane / 16, brings 32 codes of
+// row n, slice g.  Row m of A is digit m % 4 of the slices g = m / 4 and zero for the other slices, so that D's rows
+// 4 g .. 4 g + 3, which lane (n, g) receives, are the four digits' sums of the lane's own codes: slices are kept apart, and
+// the scale that a lane has unpacked is applied where it is.  The lanes of A whose slice is not m / 4's read zeros.  Digits
+// carry their weight 16^-d in A's block scale, so a sub-block's sum is the sum of the four.
+//
+// Against codes in bf16 (x as three pieces, v_mfma_f32_4x4x4, what 16-bit float weights take below): a third of the vector
+// instructions, which bound those.
+//
+// Staged x, per turn and token: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e - 2 as a byte, then
+// the sums of x, f32: [step][slice][sub-block].
+template <class F, int T, int CH>
+struct CodeTile {
     typedef Slice<F> S;
-    typedef XStep<F, NC, CHAIN> X;
-    typedef Image<F, RT> I;
-    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), quad = lane / 4;
-    const uint32_t kp = wave % a.ksplit, group = wave / a.ksplit, groups = QD_WAVES / a.ksplit;
-    const uint32_t row_bytes = (uint32_t)(a.cols / F::N * F::BYTES), steps = (uint32_t)((a.cols + 1023) / 1024);
-    const uint64_t first_row = (a.first_tile + (uint64_t)blockIdx.x * groups) * I::ROWS;      // of the workgroup
-    const uint64_t row = first_row + group * I::ROWS;                                         // of the wave
-    const uint64_t own = row < a.rows ? row : a.rows - 1;
-    const uint32_t rows = a.rows - own < I::ROWS ? (uint32_t)(a.rows - own) : I::ROWS;
-    const uint8_t *w = a.w + own * row_bytes + (uint64_t)kp * S::STEP;
-    uint32_t left = row_bytes - (kp < steps ? kp : steps - 1) * S::STEP;       // of each row, from w on
-    const uint32_t reach = (rows - 1) * row_bytes + (S::UNITS - 1) * S::UNIT + I::UNIT;
-    const uint64_t behind = (a.rows - own - 1) * row_bytes;                    // of the tensor, behind the tile's first row
-    const typename S::Lane me(quad);
-    uint8_t *image = lds + wave * I::BYTES, *xs = lds + QD_WAVES * I::BYTES;
-    const uint8_t *x = xs + (quad * NC + (lane % 4 < NC ? lane % 4 : NC - 1)) * 16, *sums = xs + X::SUMS + quad * NC * 4;
-    float acc[RT][NC];
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) acc[t][c] = 0.0f;
+    static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN;
+    typedef Image<F, ROWS> I;
+    static constexpr uint32_t DIGITS = CH * 1024, EXPS = DIGITS * S::TURN, SUMS = EXPS + 8 * S::TURN + 8 * (S::TURN & 1);
+    static constexpr uint32_t PER_TOKEN = SUMS + 16 * S::NSUB * S::TURN, X_BYTES = T * PER_TOKEN, CLEAR = DIGITS;
 
-    const typename I::Places places(lane, rows, row_bytes);
-    I in;
-    if (kp < steps) in.fetch(places, w, behind + left, reach);
-    uint32_t step = kp;
-    for (uint32_t first = 0; first < steps; first += a.chunk) {
-        const uint32_t now = first + a.chunk < steps ? a.chunk : steps - first, end = first + now;
+    // load(turn, t, c, v): elements [c, c + 8) of token t in that turn
+    template <class Load>
+    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t tokens, Load load) {
+        constexpr uint32_t FRAGS = 32 * S::TURN;               // of eight elements; four lanes side by side have a block
+        for (uint32_t i = threadIdx.x; i < FRAGS * turns * tokens; i += TILE_THREADS) {
+            const uint32_t t = T == 1 ? 0 : i / (FRAGS * turns), j = i - t * FRAGS * turns, turn = j / FRAGS, f = j % FRAGS;
+            const uint32_t step = f / 32, block = f / 4 % 8, half = f / 2 % 2;
+            uint8_t *to = lds + (turn * T + t) * PER_TOKEN;
+            float v[8];
+            load(turn, t, f * 8, v);
+            float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            sum += dpp<QUAD_XOR1>(sum);
+            float *sums = (float *)(to + SUMS) + step * 4 * S::NSUB;
+            if constexpr (S::PLANES) {                         // 16 elements: column `half` of sub-block block % 4
+                if (f % 2 == 0) sums[(block / 4 * 2 + half) * 4 + block % 4] = sum;
+            } else {
+                sum += dpp<QUAD_XOR2>(sum);
+                if (f % 4 == 0) sums[block] = sum;
+            }
+            uint32_t top = 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t b = __builtin_bit_cast(uint32_t, v[k]) & 0x7FFFFFFFu;
+                top = b > top ? b : top;
+            }
+            const uint32_t o1 = dpp<QUAD_XOR1>(top);
+            top = o1 > top ? o1 : top;
+            const uint32_t o2 = dpp<QUAD_XOR2>(top);
+            top = o2 > top ? o2 : top;
+            uint32_t e = top >> 23;                            // biased; smaller ones than 2^-95 are multiples of 2^-127
+            e = e < 32 ? 32 : e;
+            const uint32_t bad = e == 255 ? 0x7F7F7F7Fu : 0u;  // an infinity or NaN among them: e4m3's NaN
+            e = e > 254 ? 254 : e;
+            if (f % 4 == 0) to[EXPS + step * 8 + block] = (uint8_t)(e - 2);
+            // x = whole * 2^(e - 126 - 16 CH)
+            const float unit = __builtin_bit_cast(float, (253u + 16 * CH - e) << 23);
+            uint32_t whole[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float m = __builtin_fabsf(v[k]) * unit;
+                whole[k] = CH == 2 ? (uint32_t)m : (uint32_t)(m + 0.5f);
+                if (CH == 1) whole[k] = whole[k] < 65535u ? whole[k] : 65535u;
+            }
+            uint8_t *digits = to + step * DIGITS + block * 128 + half * 64 + f % 2 * 8;
+            uint32_t sign[2], plane[2][2 * CH];                // four elements a word; byte p of the whole numbers
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t *n = whole + 4 * q;
+                const float *x = v + 4 * q;
+                const uint32_t s0 = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[1]), __builtin_bit_cast(uint32_t, x[0]), 0x0C0C0703u);
+                const uint32_t s1 = __builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[3]), __builtin_bit_cast(uint32_t, x[2]), 0x07030C0Cu);
+                sign[q] = ((s0 | s1) & 0x80808080u) | bad;
+                const uint32_t a = __builtin_amdgcn_perm(n[1], n[0], 0x05010400u), b = __builtin_amdgcn_perm(n[3], n[2], 0x05010400u);
+                plane[q][0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
+                plane[q][1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                if constexpr (CH == 2) {
+                    const uint32_t c = __builtin_amdgcn_perm(n[1], n[0], 0x07030602u), d = __builtin_amdgcn_perm(n[3], n[2], 0x07030602u);
+                    plane[q][2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+                    plane[q][3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
+                }
+            }
+#pragma unroll
+            for (int p = 0; p < 2 * CH; ++p) {                 // the highest byte first: digits 2 p and 2 p + 1
+                uint8_t *d = digits + p / 2 * 1024 + p % 2 * 32;
+                const uint32_t w0 = plane[0][2 * CH - 1 - p], w1 = plane[1][2 * CH - 1 - p];
+                *(u32x2 *)d = u32x2{((w0 >> 4) & LOW4) | sign[0], ((w1 >> 4) & LOW4) | sign[1]};
+                *(u32x2 *)(d + 16) = u32x2{(w0 & LOW4) | sign[0], (w1 & LOW4) | sign[1]};
+            }
+        }
+    }
+    struct Me {
+        uint32_t g, row;              // the lane's slice, its row's image
+        uint32_t own, digits, exps;   // ~0 where the lane's part of A is not zero; its place in a step's digits; of its row's exponents
+        uint32_t weight;              // its digit's weight, in each byte
+        // zeros: in shared memory, in front of the staged x
+        __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) {
+            const uint32_t m = lane % 16, p = m % 4, gm = m / 4;
+            g = lane / 16;
+            row = m * I::ROW;
+            own = gm == g ? ~0u : 0u;
+            digits = S::PLANES ? (g / 2 * 4) * 128 + g % 2 * 64 + p * 16 : g * 256 + p * 16;
+            exps = S::PLANES ? gm / 2 * 4 : gm * 2;
+            weight = p * 0x04040404u;
+        }
+    };
+    struct Sums { float v[T]; };
+
+    static __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
+        return {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+    }
+    template <int SB>
+    static __device__ __forceinline__ f32x4 multiply(const i32x8 &x, uint32_t x_exp, const i32x8 &w, int w_exp, f32x4 d) {
+        // 8 of A's exponent stand in B's, which keeps A's in range for every x
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, d, 0, 0, SB, (int)x_exp, 0, w_exp + 127 + 8);
+    }
+    // `x`: the step's digits of the token, or the zeros; `weights`: the step's exponents less the digits' weights
+    template <int SB>
+    static __device__ __forceinline__ f32x4 sub_block(const i32x8 &lo, const i32x8 &hi, const uint8_t *x, uint32_t exps) {
+        f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const uint8_t *at = x + c * 1024 + SB * 128;
+            const u32x4 none = {0, 0, 0, 0};
+            const i32x8 a = join(al16(at), S::PLANES ? none : al16(at + 64));
+            d = multiply<SB>(a, exps - c * 0x10101010u, lo, S::template LOW_EXP<SB>, d);
+            if constexpr (S::HIGH) d = multiply<SB>(a, exps - c * 0x10101010u, hi, S::template HIGH_EXP<SB>, d);
+        }
+        return d;
+    }
+    template <int SB>
+    static __device__ __forceinline__ void add_sub(const typename S::Raw &raw, const Me &me, const uint8_t *clear, const uint8_t *x, uint32_t step,
+                                                   uint32_t tokens, Sums &acc) {
+        constexpr int WORDS = S::SUB / 4;
+        uint32_t b[WORDS], h[WORDS];
+        S::template low<SB>(raw, b);
+        if constexpr (S::HIGH) S::template high<SB>(raw, h);
+        i32x8 lo, hi;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                          // 16 codes: the second half meets zeros
+            lo[i] = (int)b[i % WORDS];
+            hi[i] = S::HIGH ? (int)h[i % WORDS] : 0;
+        }
+        const SubScale s = S::template scale<SB>(raw);
+#pragma unroll
+        for (uint32_t t = 0; t < T; ++t) {
+            if (T > 1 && t >= tokens) break;
+            const uint8_t *xt = x + t * PER_TOKEN;
+            const uint32_t exps = (S::PLANES ? al4(xt + EXPS + step * 8 + me.exps) : al2(xt + EXPS + step * 8 + me.exps)) - me.weight;
+            const uint8_t *digits = clear + ((uint32_t)(xt + step * DIGITS + me.digits - clear) & me.own);
+            const f32x4 d = sub_block<SB>(lo, hi, digits, exps);
+            const float sum = ((const float *)(xt + SUMS))[(step * 4 + me.g) * S::NSUB + SB];
+            acc.v[t] = __builtin_fmaf(s.a, (d[0] + d[1]) + (d[2] + d[3]), acc.v[t]);
+            acc.v[t] = __builtin_fmaf(-s.c, sum, acc.v[t]);
+        }
+    }
+    // one turn: `image` the wave's bytes, `x` the turn's staged x, `clear` the zeros, `left` bytes of the row from the turn on
+    static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *clear, const uint8_t *x, uint32_t left,
+                                               uint32_t tokens, Sums &acc) {
+#pragma unroll
+        for (uint32_t step = 0; step < S::TURN; ++step) {
+            typename S::Raw raw;
+            raw.load(image + me.row, step, me.g, left);
+            // one sub-block after the other: scheduled into each other they take the registers of more waves
+            add_sub<0>(raw, me, clear, x, step, tokens, acc);
+            __builtin_amdgcn_sched_barrier(0);
+            add_sub<1>(raw, me, clear, x, step, tokens, acc);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (S::NSUB == 4) {
+                add_sub<2>(raw, me, clear, x, step, tokens, acc);
+                __builtin_amdgcn_sched_barrier(0);
+                add_sub<3>(raw, me, clear, x, step, tokens, acc);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+    static __device__ __forceinline__ float total(float v) {
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+        return v;
+    }
+};
+
+// ---- 16-bit float weights: bf16 pieces -----------------------------------------------------------------------
+// x in CH bf16 pieces (bf16 one, f16 two, f32 three, exactly), the weights in one or two: products are exact, sums f32.
+// A wave takes four rows; its quads (four neighbouring lanes, one lane per row) take 16 neighbouring slices at a time, and
+// v_mfma_f32_4x4x4 with 16 blocks multiplies, in each quad, the four rows with the tokens that the quad's lanes hold.
+// Staged x, per turn: [piece][k][slice][token] fragments of eight bf16, k = the fragment's place in its slice; the quads
+// read the same k of neighbouring slices, so their addresses are consecutive; 16 bytes between one k and the next keep the
+// staging threads, which run along k first, out of each other's banks.
+template <class F, int T, int CH>
+struct FloatTile {
+    typedef Slice<F> S;
+    static constexpr uint32_t ROWS = 4, ELEMS = 1024;
+    typedef Image<F, ROWS> I;
+    static constexpr uint32_t K = 256 * T + 16, X_BYTES = CH * 8 * K, CLEAR = 0;
+
+    template <class Load>
+    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t tokens, Load load) {
+        for (uint32_t i = threadIdx.x; i < 128 * turns * tokens; i += TILE_THREADS) {
+            const uint32_t t = T == 1 ? 0 : i / (128 * turns), j = i - t * 128 * turns, turn = j / 128, f = j % 128;
+            float v[8];
+            load(turn, t, f * 8, v);
+            uint8_t *to = lds + turn * X_BYTES + f % 8 * K + (f / 8 * T + t) * 16;
+#pragma unroll
+            for (int p = 0; p < CH; ++p) {
+                *(u32x4 *)(to + p * 8 * K) = u32x4{upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7])};
+                if (p + 1 < CH)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = below_bf16(v[k]);
+            }
+        }
+    }
+    struct Me {
+        uint32_t quad, row, x;
+        __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) : quad(lane / 4), row(lane % 4 * I::ROW), x((lane / 4 * T + (lane % 4 < T ? lane % 4 : T - 1)) * 16) {}
+    };
+    struct Sums { float v[T]; };
+    static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *, const uint8_t *x, uint32_t left, uint32_t, Sums &acc) {
+        typename S::Raw raw;
+        raw.load(image + me.row, me.quad, left);
+        f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int piece = 0; piece < S::WP; ++piece) {
+                uint32_t b[16];
+                S::codes(raw, s, piece, b);
+#pragma unroll
+                for (int p = 0; p < CH; ++p)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const u32x4 a = al16(x + me.x + (p * 8 + 4 * s + k) * K);
+#pragma unroll
+                        for (int half = 0; half < 2; ++half) {
+                            const u32x2 av = {a[2 * half], a[2 * half + 1]}, bv = {b[4 * k + 2 * half], b[4 * k + 2 * half + 1]};
+                            d = __builtin_amdgcn_mfma_f32_4x4x4bf16_1k(__builtin_bit_cast(s16x4, av), __builtin_bit_cast(s16x4, bv), d, 0, 0, 0);
+                        }
+                    }
+            }
+#pragma unroll
+        for (int t = 0; t < T; ++t) acc.v[t] += d[t];
+    }
+    static __device__ __forceinline__ float total(float v) {
+        v += dpp<ROW_ROR8>(v);
+        v += dpp<ROW_ROR4>(v);
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+        return v;
+    }
+};
+
+template <class F, int T, int CH>
+using Tile = std::conditional_t<is_float_type<F>, FloatTile<F, T, CH>, CodeTile<F, T, CH>>;
+
+// ---- the loop over a row ----------------------------------------------------------------------------------------
+// The wave's part of a tile: turns kp, kp + ksplit, ... of `turns`, the next one's bytes on the way while one is multiplied.
+// All waves of the workgroup call this together, since they stage x for each other, `chunk` turns at a time.
+//     at(turn)           {where the turn begins in the tile's first row, bytes of the row and of the tensor from there on}
+//     load(turn, t, c, v)   elements [c, c + 8) of token t in that turn
+struct Turn {
+    const uint8_t *base;
+    uint32_t left;
+    uint64_t room;
+};
+struct Share { uint32_t kp, ksplit, chunk, turns, tokens; };
+template <class M, class At, class Load>
+__device__ __forceinline__ void run_turns(uint8_t *image, uint8_t *clear, const typename M::I::Places &places, uint32_t reach, const Share &sh, At at, Load load,
+                                          typename M::Sums &acc) {
+    const uint32_t lane = threadIdx.x % 64;
+    uint8_t *xs = clear + M::CLEAR;
+    const typename M::Me me(lane, clear);
+    typename M::I in;
+    uint32_t left = 0, turn = sh.kp;
+    auto fetch = [&](uint32_t n) {
+        const Turn t = at(n);
+        in.fetch(places, t.base, t.room, reach);
+        return t.left;
+    };
+    if (turn < sh.turns) left = fetch(turn);
+    for (uint32_t i = threadIdx.x * 16; i < M::CLEAR; i += TILE_THREADS * 16) *(u32x4 *)(clear + i) = u32x4{0, 0, 0, 0};
+    for (uint32_t first = 0; first < sh.turns; first += sh.chunk) {
+        const uint32_t now = first + sh.chunk < sh.turns ? sh.chunk : sh.turns - first, end = first + now;
         if (first) __syncthreads();
-        stage_x<F, NC, CHAIN>(xs, now, a.tokens, a.parts, [&](uint32_t n, uint32_t t, uint32_t f, float (&v)[8]) {
-            load8(a.x, t * a.x_stride, ((uint64_t)(first + n) * 128 + f) * 8, a.cols, a.x_kind, v);
-        });
+        M::stage(xs, now, sh.tokens, [&](uint32_t n, uint32_t t, uint32_t c, float (&v)[8]) { load(first + n, t, c, v); });
         __syncthreads();
-        for (; step < end; step += a.ksplit) {
+        for (; turn < end; turn += sh.ksplit) {
             wave_order();
             in.put(places, image);
             wave_order();
             const uint32_t here = left;
-            if (step + a.ksplit < steps) {
-                w += (uint64_t)a.ksplit * S::STEP;
-                left -= a.ksplit * S::STEP;
-                in.fetch(places, w, behind + left, reach);
-            }
-            typename S::Raw raw[RT];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) raw[t].load(image + (t * 4 + lane % 4) * I::ROW, me, here);
-            const uint32_t at = (step - first) * X::BYTES;
-            add_slices<F, NC, CHAIN, RT>(raw, me, x + at, sums + at, acc);
+            if (turn + sh.ksplit < sh.turns) left = fetch(turn + sh.ksplit);
+            M::add(image, me, clear, xs + (turn - first) * M::X_BYTES, here, sh.tokens, acc);
         }
     }
+}
+// The waves' sums to part[wave][token][row].
+template <class M, int T>
+__device__ __forceinline__ void put_parts(float *part, uint32_t wave, const typename M::Sums &acc) {
+    const uint32_t lane = threadIdx.x % 64;
     __syncthreads();                                   // the staged x is no longer needed
-    float *part = (float *)xs;                         // [wave][column][row]
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const float v = quads_sum(acc[t][c]);
-            if (lane < 4) part[(wave * NC + c) * I::ROWS + t * 4 + lane] = v;
-        }
+    for (int t = 0; t < T; ++t) {
+        const float v = M::total(acc.v[t]);
+        if (lane < M::ROWS) part[(wave * T + t) * M::ROWS + lane] = v;
+    }
     __syncthreads();
-    // one thread per row and token: the waves' parts, and the token's pieces
-    if (threadIdx.x < groups * I::ROWS * a.tokens) {
-        const uint32_t r = threadIdx.x % (groups * I::ROWS), t = threadIdx.x / (groups * I::ROWS), g = r / I::ROWS;
-        const uint64_t out = first_row + r;
+}
+template <class M>
+__device__ __forceinline__ typename M::Sums no_sums() {
+    typename M::Sums s;
+#pragma unroll
+    for (uint32_t t = 0; t < sizeof(s.v) / 4; ++t) s.v[t] = 0.0f;
+    return s;
+}
+
+// ---- one matrix -----------------------------------------------------------------------------------------------
+// Up to T tokens.  A wave owns a tile of rows, or shares it with others that take other turns of its columns.
+template <class F, int T, int CH>
+__global__ __launch_bounds__(TILE_THREADS) void matvec_tiles(MatvecArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    typedef Tile<F, T, CH> M;
+    typedef typename M::I I;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t group = wave / a.ksplit, groups = TILE_WAVES / a.ksplit;
+    const uint32_t row_bytes = (uint32_t)(a.cols / F::N * F::BYTES), turns = (uint32_t)((a.cols + M::ELEMS - 1) / M::ELEMS);
+    const uint64_t first_row = (a.first_tile + (uint64_t)blockIdx.x * groups) * M::ROWS;      // of the workgroup
+    const uint64_t row = first_row + group * M::ROWS;                                         // of the wave
+    const uint64_t own = row < a.rows ? row : a.rows - 1;
+    const uint32_t rows = a.rows - own < M::ROWS ? (uint32_t)(a.rows - own) : M::ROWS;
+    const uint8_t *w = a.w + own * row_bytes;
+    const uint64_t behind = (a.rows - own - 1) * row_bytes;                                   // of the tensor, behind the row
+    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    typename M::Sums acc = no_sums<M>();
+    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
+                 Share{wave % a.ksplit, a.ksplit, a.chunk, turns, a.tokens},
+                 [&](uint32_t turn) {
+                     const uint32_t off = turn * I::TURN_BYTES;
+                     return Turn{w + off, row_bytes - off, behind + row_bytes - off};
+                 },
+                 [&](uint32_t turn, uint32_t t, uint32_t c, float (&v)[8]) {
+                     load8(a.x, t * a.x_stride, (uint64_t)turn * M::ELEMS + c, a.cols, a.x_kind, v);
+                 },
+                 acc);
+    float *part = (float *)(clear + M::CLEAR);
+    put_parts<M, T>(part, wave, acc);
+    for (uint32_t i = threadIdx.x; i < groups * M::ROWS * a.tokens; i += TILE_THREADS) {
+        const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.ksplit; ++k)
-            for (uint32_t p = 0; p < a.parts; ++p) v += part[((g * a.ksplit + k) * NC + t * a.parts + p) * I::ROWS + r % I::ROWS];
-        if (out < a.rows) store_elem(a.y, t * a.y_stride + out, a.y_kind, v);
+        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
+        if (first_row + r < a.rows) store_elem(a.y, t * a.y_stride + first_row + r, a.y_kind, v);
     }
 }
 

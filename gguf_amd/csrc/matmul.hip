@@ -57,65 +57,65 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
     return stride < (1ull << 40) && (tokens <= 1 || stride >= width);
 }
 
-// Shared memory of one workgroup for x.
+// Shared memory of one workgroup for x, beside its waves' images.
 constexpr uint32_t X_LDS = 40 << 10;
 
-// Tiles of a wave: with a few hundred packed bytes a row and step, two share the fragments of x.
-template <class F> constexpr int row_tiles() { return Slice<F>::STEP <= 640 ? 2 : 1; }
-
-// The shape of a launch over `tiles` wave tiles, each of which takes `steps` steps: how many waves share a tile's steps,
-// the steps staged at a time (equal chunks, whole turns of the waves), the shared memory.
+// The shape of a launch over `tiles` wave tiles, each of which takes `turns` turns: how many waves share a tile's turns,
+// the turns staged at a time (equal chunks, whole rounds of the waves), the shared memory.
+template <class M>
 struct Shape {
-    uint32_t ksplit, chunk, groups, bytes;
-    Shape(uint64_t tiles, uint32_t steps, uint32_t step_bytes, uint32_t image_bytes, uint32_t part_bytes) {
+    uint32_t ksplit = 1, chunk, groups, bytes;
+    // `waves`: of a workgroup that may share a tile's turns
+    Shape(uint64_t tiles, uint32_t turns, uint32_t waves, uint32_t tokens) {
         // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
-        ksplit = 1;
-        while (ksplit < QD_WAVES && ksplit < steps && tiles * ksplit < 2048 && 2 * ksplit * step_bytes <= X_LDS) ksplit *= 2;
-        const uint32_t turns = (steps + ksplit - 1) / ksplit, most = X_LDS / (step_bytes * ksplit), chunks = (turns + most - 1) / most;
-        chunk = (turns + chunks - 1) / chunks * ksplit;
-        groups = QD_WAVES / ksplit;
-        bytes = QD_WAVES * image_bytes + std::max(std::min(chunk, steps) * step_bytes, QD_WAVES * part_bytes);
+        while (ksplit < waves && ksplit < turns && tiles * ksplit < 2048 && 2 * ksplit * M::X_BYTES <= X_LDS) ksplit *= 2;
+        const uint32_t rounds = (turns + ksplit - 1) / ksplit, most = std::max(1u, X_LDS / (M::X_BYTES * ksplit)), chunks = (rounds + most - 1) / most;
+        chunk = (rounds + chunks - 1) / chunks * ksplit;
+        groups = waves / ksplit;
+        bytes = TILE_WAVES * M::I::BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk, turns) * M::X_BYTES, TILE_WAVES * tokens * M::ROWS * 4);
     }
 };
+template <class M> constexpr uint32_t turns_of(uint64_t cols) { return (uint32_t)((cols + M::ELEMS - 1) / M::ELEMS); }
 
-template <class F, int NC, int CHAIN>
-void launch_quads(MatvecArgs a, hipStream_t st) {
-    constexpr int RT = row_tiles<F>();
-    typedef XStep<F, NC, CHAIN> X;
-    typedef Image<F, RT> I;
-    const uint64_t tiles = (a.rows + I::ROWS - 1) / I::ROWS;
-    const Shape sh(tiles, (uint32_t)((a.cols + 1023) / 1024), X::BYTES, I::BYTES, NC * I::ROWS * 4);
+template <class F, int T, int CH>
+void launch_tiles(MatvecArgs a, hipStream_t st) {
+    typedef Tile<F, T, CH> M;
+    const uint64_t tiles = (a.rows + M::ROWS - 1) / M::ROWS;
+    const Shape<M> sh(tiles, turns_of<M>(a.cols), TILE_WAVES, T);
     a.ksplit = sh.ksplit;
     a.chunk = sh.chunk;
     for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * sh.groups) {
         const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + sh.groups - 1) / sh.groups));
-        matvec_quads<F, NC, CHAIN, RT><<<grid, QD_THREADS, sh.bytes, st>>>(a);
+        matvec_tiles<F, T, CH><<<grid, TILE_THREADS, sh.bytes, st>>>(a);
     }
 }
 
-// At most four tokens in one launch: columns of the matrix unit's four are tokens, or the pieces of one or two tokens
-// where all of them fit; otherwise a token is a column and its pieces follow each other.  Returns the tokens taken.
+// Digits of x for codes: 32 bits, or 16 where both x and y are 16-bit floats.
+bool short_digits(uint32_t x_kind, uint32_t y_kind) { return x_kind != EK_F32 && y_kind != EK_F32; }
+
+// At most four tokens in one launch.  Returns the tokens taken.
 template <class F>
-uint64_t launch_few(MatvecArgs a, uint64_t tokens, uint32_t pieces, hipStream_t st) {
+uint64_t launch_few(MatvecArgs a, uint64_t tokens, hipStream_t st) {
     a.tokens = (uint32_t)std::min<uint64_t>(tokens, 4);
     if constexpr (is_float_type<F>) {
         if (a.cols < 8) {
             matvec_short<F><<<(uint32_t)((a.rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
-            return a.tokens;
+        } else if (a.x_kind == EK_BF16) {
+            if (a.tokens == 1) launch_tiles<F, 1, 1>(a, st);
+            else launch_tiles<F, 4, 1>(a, st);
+        } else if (a.x_kind == EK_F16) {
+            if (a.tokens == 1) launch_tiles<F, 1, 2>(a, st);
+            else launch_tiles<F, 4, 2>(a, st);
+        } else {
+            if (a.tokens == 1) launch_tiles<F, 1, 3>(a, st);
+            else launch_tiles<F, 4, 3>(a, st);
         }
-    }
-    a.parts = a.tokens * pieces <= 4 ? pieces : 1;
-    if (a.parts == pieces) {
-        switch (a.tokens * pieces) {
-        case 1: launch_quads<F, 1, 1>(a, st); break;
-        case 2: launch_quads<F, 2, 1>(a, st); break;
-        case 3: launch_quads<F, 3, 1>(a, st); break;
-        default: launch_quads<F, 4, 1>(a, st);
-        }
-    } else if (pieces == 2) {
-        launch_quads<F, 4, 2>(a, st);
+    } else if (short_digits(a.x_kind, a.y_kind)) {
+        if (a.tokens == 1) launch_tiles<F, 1, 1>(a, st);
+        else launch_tiles<F, 4, 1>(a, st);
     } else {
-        launch_quads<F, 4, 3>(a, st);
+        if (a.tokens == 1) launch_tiles<F, 1, 2>(a, st);
+        else launch_tiles<F, 4, 2>(a, st);
     }
     return a.tokens;
 }
@@ -153,14 +153,14 @@ struct MoeSpace {
     }
 };
 
-template <class F, int NC, int CHAIN>
+template <class F, int T, int CH>
 void launch_up(MoeArgs a, hipStream_t st) {
-    typedef Image<F, 1> I;
-    const uint32_t tiles = (uint32_t)((a.ff + 3) / 4);
-    const Shape sh((uint64_t)tiles * a.slots, (uint32_t)((a.hidden + 1023) / 1024), XStep<F, NC, CHAIN>::BYTES, 2 * I::BYTES, 2 * NC * 16);
+    typedef Tile<F, T, CH> M;
+    const uint32_t tiles = (uint32_t)((a.ff + M::ROWS - 1) / M::ROWS);
+    const Shape<M> sh(2 * (uint64_t)tiles * a.slots, turns_of<M>(a.hidden), TILE_WAVES / 2, T);
     a.ksplit = sh.ksplit;
     a.chunk = sh.chunk;
-    moe_up<F, NC, CHAIN><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), QD_THREADS, sh.bytes, st>>>(a);
+    moe_up<F, T, CH><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, sh.bytes, st>>>(a);
 }
 
 template <class F>
@@ -168,31 +168,41 @@ void launch_up_of(MoeArgs a, hipStream_t st) {
     if constexpr (is_float_type<F>) {
         if (a.hidden < 8) {
             moe_up_short<F><<<dim3((uint32_t)((a.ff + MV_THREADS - 1) / MV_THREADS), a.tokens * a.top_k), MV_THREADS, 0, st>>>(a);
-            return;
+        } else if (a.x_kind == EK_BF16) {
+            launch_up<F, 4, 1>(a, st);
+        } else if (a.x_kind == EK_F16) {
+            launch_up<F, 4, 2>(a, st);
+        } else {
+            launch_up<F, 4, 3>(a, st);
         }
-    }
-    const uint32_t pieces = a.x_kind == EK_F32 ? 3 : a.x_kind == EK_F16 ? 2 : 1;
-    a.parts = a.tokens == 1 ? pieces : 1;
-    if (a.tokens == 1) {
-        if (pieces == 1) launch_up<F, 1, 1>(a, st);
-        else if (pieces == 2) launch_up<F, 2, 1>(a, st);
-        else launch_up<F, 3, 1>(a, st);
+    } else if (short_digits(a.x_kind, a.y_kind)) {
+        if (a.tokens == 1) launch_up<F, 1, 1>(a, st);
+        else launch_up<F, 4, 1>(a, st);
     } else {
-        if (pieces == 1) launch_up<F, 4, 1>(a, st);
-        else if (pieces == 2) launch_up<F, 4, 2>(a, st);
-        else launch_up<F, 4, 3>(a, st);
+        if (a.tokens == 1) launch_up<F, 1, 2>(a, st);
+        else launch_up<F, 4, 2>(a, st);
     }
 }
 
-template <class F, int NC, int CHAIN>
+template <class F, int T, int CH>
 void launch_down_few(MoeArgs a, hipStream_t st) {
-    constexpr int RT = row_tiles<F>();
-    typedef Image<F, RT> I;
-    const uint32_t tiles = (uint32_t)((a.hidden + I::ROWS - 1) / I::ROWS);
-    const Shape sh(tiles, (uint32_t)((a.ff + 1023) / 1024) * a.tokens * a.top_k, XStep<F, NC, CHAIN>::BYTES, I::BYTES, NC * I::ROWS * 4);
+    typedef Tile<F, T, CH> M;
+    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS);
+    const Shape<M> sh(tiles, turns_of<M>(a.ff) * a.tokens * a.top_k, TILE_WAVES, T);
     a.ksplit = sh.ksplit;
     a.chunk = sh.chunk;
-    moe_down_few<F, NC, CHAIN, RT><<<(tiles + sh.groups - 1) / sh.groups, QD_THREADS, sh.bytes, st>>>(a);
+    moe_down_few<F, T, CH><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes, st>>>(a);
+}
+
+template <class F, int T, int CH>
+void launch_down_many(MoeArgs a, hipStream_t st) {
+    typedef Tile<F, T, CH> M;
+    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS);
+    const Shape<M> sh((uint64_t)tiles * a.slots, turns_of<M>(a.ff), TILE_WAVES, T);
+    a.ksplit = sh.ksplit;
+    a.chunk = sh.chunk;
+    moe_down_many<F, T, CH><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, sh.bytes, st>>>(a);
+    moe_sum<<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
 }
 
 template <class F>
@@ -200,23 +210,19 @@ void launch_down_of(MoeArgs a, hipStream_t st) {
     if constexpr (is_float_type<F>) {
         if (a.ff < 8) {
             moe_down_short<F><<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
-            return;
+        } else if (a.tokens <= 4) {
+            launch_down_few<F, 4, 3>(a, st);
+        } else {
+            launch_down_many<F, 4, 3>(a, st);
         }
-    }
-    a.parts = a.tokens == 1 ? 3 : 1;
-    if (a.tokens == 1) {
-        launch_down_few<F, 3, 1>(a, st);
-    } else if (a.tokens <= 4) {
-        launch_down_few<F, 4, 3>(a, st);
+    } else if (short_digits(a.x_kind, a.y_kind)) {
+        if (a.tokens == 1) launch_down_few<F, 1, 1>(a, st);
+        else if (a.tokens <= 4) launch_down_few<F, 4, 1>(a, st);
+        else launch_down_many<F, 4, 1>(a, st);
     } else {
-        constexpr int RT = row_tiles<F>();
-        typedef Image<F, RT> I;
-        const uint32_t tiles = (uint32_t)((a.hidden + I::ROWS - 1) / I::ROWS);
-        const Shape sh((uint64_t)tiles * a.slots, (uint32_t)((a.ff + 1023) / 1024), XStep<F, 4, 3>::BYTES, I::BYTES, 4 * I::ROWS * 4);
-        a.ksplit = sh.ksplit;
-        a.chunk = sh.chunk;
-        moe_down_many<F, RT><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), QD_THREADS, sh.bytes, st>>>(a);
-        moe_sum<<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
+        if (a.tokens == 1) launch_down_few<F, 1, 2>(a, st);
+        else if (a.tokens <= 4) launch_down_few<F, 4, 2>(a, st);
+        else launch_down_many<F, 4, 2>(a, st);
     }
 }
 
@@ -242,7 +248,6 @@ ggq_status ggq_matvec_device(uint32_t ty, uint64_t rows, uint64_t cols, const vo
     a.cols = cols;
     a.x_stride = x_stride;
     a.y_stride = y_stride;
-    const uint32_t pieces = x_type == GGQ_TYPE_F32 ? 3 : x_type == GGQ_TYPE_F16 ? 2 : 1;
     hipStream_t st = (hipStream_t)hip_stream;
     for (uint64_t t = 0, done = 0; t < tokens; t += done) {
         a.x = (const uint8_t *)d_x + t * x_stride * xb;
@@ -252,7 +257,7 @@ ggq_status ggq_matvec_device(uint32_t ty, uint64_t rows, uint64_t cols, const vo
             fill_zero<<<(uint32_t)((rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
             continue;
         }
-#define CASE(F) done = launch_few<F>(a, tokens - t, pieces, st)
+#define CASE(F) done = launch_few<F>(a, tokens - t, st)
         GGQ_FOR_TYPE(ty, CASE)
 #undef CASE
     }
@@ -346,7 +351,9 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     hipStream_t st = (hipStream_t)hip_stream;
     moe_logits<<<m->experts, MV_THREADS, 0, st>>>(a);
     moe_route<<<(uint32_t)tokens, 64, 0, st>>>(a);
-    a.slots = std::min(m->experts, (uint32_t)tokens * m->top_k);
+    // groups of up to four pairs with the same expert: one for each pair, or one for each expert and one more for each four pairs
+    const uint32_t pairs = (uint32_t)tokens * m->top_k, in_use = std::min(m->experts, pairs);
+    a.slots = std::min(pairs, in_use + (pairs - in_use) / 4);
 #define CASE(F) launch_up_of<F>(a, st)
     GGQ_FOR_TYPE(m->up_type, CASE)
 #undef CASE

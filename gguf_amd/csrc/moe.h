@@ -24,8 +24,8 @@ struct MoeArgs {
     uint64_t hidden, ff, x_stride, y_stride;
     uint32_t tokens, experts, top_k, router_kind, x_kind, y_kind;
     uint32_t sigmoid, normalize, gelu;
-    uint32_t parts, chunk, ksplit;            // as in MatvecArgs, of the launch
-    uint32_t slots;                           // experts that may be in use: workgroups along y
+    uint32_t chunk, ksplit;                   // as in MatvecArgs, of the launch
+    uint32_t slots;                           // most slots there may be: workgroups along y
     float scale;
 };
 
@@ -128,173 +128,120 @@ __device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
 
 
 // ---- which expert, and which tokens ----------------------------------------------------------------------
-// The tokens that chose the slot-th expert in use (experts in use in order of their index).
+// Experts in use, in the order of their index, each with its tokens four at a time: a slot is one such group.
 struct Slot {
-    uint32_t expert, count;
-    uint64_t mask;                // bit t: token t
+    uint32_t expert, count;       // of tokens; 0: no such slot
 };
 struct SlotSpace {
     uint32_t low[MOE_MAX_EXPERTS], high[MOE_MAX_EXPERTS];         // masks of tokens, by expert
+    uint32_t pair[4];             // of the slot's tokens: token * top_k + place
 };
 __device__ __forceinline__ uint32_t nth_bit(uint64_t m, uint32_t n) {
     for (; n; --n) m &= m - 1;
     return (uint32_t)__builtin_ctzll(m);
 }
-// All threads of the workgroup; ids: the choices of all tokens.
-__device__ __forceinline__ Slot find_slot(SlotSpace &s, const int32_t *ids, const MoeArgs &a, uint32_t slot) {
+// All threads of the workgroup, of 64 lanes or more; ids: the choices of all tokens.  The same answer in all of them.
+__device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, uint32_t slot) {
+    const uint32_t lane = threadIdx.x % 64;
     for (uint32_t e = threadIdx.x; e < a.experts; e += blockDim.x) s.low[e] = s.high[e] = 0;
     __syncthreads();
     for (uint32_t p = threadIdx.x; p < a.tokens * a.top_k; p += blockDim.x) {
         const uint32_t t = p / a.top_k;
-        atomicOr(t < 32 ? &s.low[ids[p]] : &s.high[ids[p]], 1u << (t & 31));
+        atomicOr(t < 32 ? &s.low[a.ids[p]] : &s.high[a.ids[p]], 1u << (t & 31));
     }
     __syncthreads();
-    const uint32_t lane = threadIdx.x % 64;
-    Slot r{0, 0, 0};
-    uint32_t seen = 0;
+    uint32_t seen = 0, expert = 0, count = 0;
     for (uint32_t base = 0; base < a.experts; base += 64) {
         const uint32_t e = base + lane;
-        const uint64_t used = __ballot(e < a.experts && (s.low[e < a.experts ? e : 0] | s.high[e < a.experts ? e : 0]));
-        const uint32_t n = (uint32_t)__popcll(used);
-        if (slot < seen + n) {
-            r.expert = base + nth_bit(used, slot - seen);
-            r.mask = s.low[r.expert] | ((uint64_t)s.high[r.expert] << 32);
-            r.expert = __builtin_amdgcn_readfirstlane(r.expert);
-            r.count = (uint32_t)__popcll(r.mask);
-            return r;
+        const uint32_t tokens = e < a.experts ? (uint32_t)__popc(s.low[e]) + (uint32_t)__popc(s.high[e]) : 0u, mine = (tokens + 3) / 4;
+        uint32_t upto = mine;                                     // slots of the lanes up to this one
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const uint32_t o = __shfl_up(upto, d);
+            upto += lane >= (uint32_t)d ? o : 0u;
         }
-        seen += n;
+        const uint64_t here = __ballot(slot < seen + upto);
+        if (here) {
+            const uint32_t l = (uint32_t)__builtin_ctzll(here);
+            const uint32_t group = __builtin_amdgcn_readfirstlane(slot - seen - __shfl(upto - mine, l));
+            expert = base + l;
+            const uint32_t low = __builtin_amdgcn_readfirstlane(s.low[expert]), high = __builtin_amdgcn_readfirstlane(s.high[expert]);
+            const uint64_t mask = low | ((uint64_t)high << 32);
+            const uint32_t n = (uint32_t)__popcll(mask) - group * 4;
+            count = n < 4 ? n : 4;
+            if (threadIdx.x < count) {
+                const uint32_t first = nth_bit(mask, group * 4 + threadIdx.x) * a.top_k;
+                uint32_t pair = first;
+                for (uint32_t j = 0; j < a.top_k; ++j) pair = (uint32_t)a.ids[first + j] == expert ? first + j : pair;
+                s.pair[threadIdx.x] = pair;
+            }
+            break;
+        }
+        seen += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
     }
-    return r;
-}
-
-// the pair of a token and an expert that it chose
-__device__ __forceinline__ uint32_t pair_with(const MoeArgs &a, uint32_t token, uint32_t expert) {
-    uint32_t pair = token * a.top_k;
-    for (uint32_t j = 0; j < a.top_k; ++j) pair = (uint32_t)a.ids[token * a.top_k + j] == expert ? token * a.top_k + j : pair;
-    return pair;
+    __syncthreads();
+    return {(uint32_t)__builtin_amdgcn_readfirstlane(expert), (uint32_t)__builtin_amdgcn_readfirstlane(count)};
 }
 
 // ---- gate and up ----------------------------------------------------------------------------------------
-// As matvec_quads, with a tile of gate's rows and the same rows of up in each wave; grid: (row groups, slots).
-template <class F, int NC, int CHAIN>
-__global__ __launch_bounds__(QD_THREADS) void moe_up(MoeArgs a) {
+// As matvec_tiles; half of a workgroup's waves take gate's rows, the others the same rows of up.  Grid: (row groups, slots).
+template <class F, int T, int CH>
+__global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ SlotSpace space;
-    __shared__ uint32_t pairs[MOE_MAX_TOKENS];
-    typedef Slice<F> S;
-    typedef XStep<F, NC, CHAIN> X;
-    typedef Image<F, 1> I;
-    const Slot slot = find_slot(space, a.ids, a, blockIdx.y);
+    typedef Tile<F, T, CH> M;
+    typedef typename M::I I;
+    const Slot slot = find_slot(space, a, blockIdx.y);
     if (slot.count == 0) return;
-    if (threadIdx.x < slot.count) pairs[threadIdx.x] = pair_with(a, nth_bit(slot.mask, threadIdx.x), slot.expert);
-    __syncthreads();
-    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), quad = lane / 4;
-    const uint32_t kp = wave % a.ksplit, group = wave / a.ksplit, groups = QD_WAVES / a.ksplit;
-    const uint32_t row_bytes = (uint32_t)(a.hidden / F::N * F::BYTES), steps = (uint32_t)((a.hidden + 1023) / 1024);
-    const uint32_t ff = (uint32_t)a.ff, first_row = blockIdx.x * groups * 4, row = first_row + group * 4, own = row < ff ? row : ff - 1;
-    const uint32_t rows = ff - own < 4 ? ff - own : 4;
-    const uint64_t at_row = ((uint64_t)slot.expert * ff + own) * row_bytes;
-    const uint32_t reach = (rows - 1) * row_bytes + (S::UNITS - 1) * S::UNIT + I::UNIT;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t second = wave / (TILE_WAVES / 2), group = wave % (TILE_WAVES / 2) / a.ksplit, groups = TILE_WAVES / 2 / a.ksplit;
+    const uint32_t row_bytes = (uint32_t)(a.hidden / F::N * F::BYTES), turns = (uint32_t)((a.hidden + M::ELEMS - 1) / M::ELEMS);
+    const uint32_t ff = (uint32_t)a.ff, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS, own = row < ff ? row : ff - 1;
+    const uint32_t rows = ff - own < M::ROWS ? ff - own : M::ROWS;
+    const uint8_t *w = (second ? a.up : a.gate) + ((uint64_t)slot.expert * ff + own) * row_bytes;
     const uint64_t behind = ((uint64_t)(a.experts - slot.expert) * ff - own - 1) * row_bytes;
-    const typename S::Lane me(quad);
-    uint8_t *image = lds + wave * 2 * I::BYTES, *xs = lds + QD_WAVES * 2 * I::BYTES;
-    const uint8_t *x = xs + (quad * NC + (lane % 4 < NC ? lane % 4 : NC - 1)) * 16, *sums = xs + X::SUMS + quad * NC * 4;
-    const typename I::Places places(lane, rows, row_bytes);
-    I gate, up;
-    const uint32_t most = NC / a.parts;
-
-    for (uint32_t done = 0; done < slot.count; done += most) {
-        const uint32_t tokens = slot.count - done < most ? slot.count - done : most;
-        float acc[2][NC];
+    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    typename M::Sums acc = no_sums<M>();
+    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
+                 Share{wave % a.ksplit, a.ksplit, a.chunk, turns, slot.count},
+                 [&](uint32_t turn) {
+                     const uint32_t off = turn * I::TURN_BYTES;
+                     return Turn{w + off, row_bytes - off, behind + row_bytes - off};
+                 },
+                 [&](uint32_t turn, uint32_t t, uint32_t c, float (&v)[8]) {
+                     load8(a.x, space.pair[t] / a.top_k * a.x_stride, (uint64_t)turn * M::ELEMS + c, a.hidden, a.x_kind, v);
+                 },
+                 acc);
+    float *part = (float *)(clear + M::CLEAR);
+    put_parts<M, T>(part, wave, acc);
+    for (uint32_t i = threadIdx.x; i < groups * M::ROWS * slot.count; i += TILE_THREADS) {
+        const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
+        float v[2] = {0.0f, 0.0f};
+        for (uint32_t k = 0; k < a.ksplit; ++k)
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) acc[t][c] = 0.0f;
-        uint64_t off = at_row + (uint64_t)kp * S::STEP;
-        uint32_t left = row_bytes - (kp < steps ? kp : steps - 1) * S::STEP, step = kp;
-        if (kp < steps) {
-            gate.fetch(places, a.gate + off, behind + left, reach);
-            up.fetch(places, a.up + off, behind + left, reach);
-        }
-        for (uint32_t first = 0; first < steps; first += a.chunk) {
-            const uint32_t now = first + a.chunk < steps ? a.chunk : steps - first, end = first + now;
-            if (first || done) __syncthreads();
-            stage_x<F, NC, CHAIN>(xs, now, tokens, a.parts, [&](uint32_t n, uint32_t t, uint32_t f, float (&v)[8]) {
-                load8(a.x, pairs[done + t] / a.top_k * a.x_stride, ((uint64_t)(first + n) * 128 + f) * 8, a.hidden, a.x_kind, v);
-            });
-            __syncthreads();
-            for (; step < end; step += a.ksplit) {
-                wave_order();
-                gate.put(places, image);
-                up.put(places, image + I::BYTES);
-                wave_order();
-                const uint32_t here = left;
-                if (step + a.ksplit < steps) {
-                    off += (uint64_t)a.ksplit * S::STEP;
-                    left -= a.ksplit * S::STEP;
-                    gate.fetch(places, a.gate + off, behind + left, reach);
-                    up.fetch(places, a.up + off, behind + left, reach);
-                }
-                const uint32_t at = (step - first) * X::BYTES;
-                if constexpr (S::STEP <= 640) {
-                    typename S::Raw raw[2];
-                    raw[0].load(image + lane % 4 * I::ROW, me, here);
-                    raw[1].load(image + I::BYTES + lane % 4 * I::ROW, me, here);
-                    add_slices<F, NC, CHAIN, 2>(raw, me, x + at, sums + at, acc);
-                } else {
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) {          // one after the other: their bytes would not fit in registers
-                        typename S::Raw raw[1];
-                        raw[0].load(image + m * I::BYTES + lane % 4 * I::ROW, me, here);
-                        add_slices<F, NC, CHAIN, 1>(raw, me, x + at, sums + at, *(float (*)[1][NC])&acc[m]);
-                        wave_order();
-                    }
-                }
-            }
-        }
-        __syncthreads();
-        float *part = (float *)xs;                         // [wave][gate, up][column][row]
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float v = quads_sum(acc[t][c]);
-                if (lane < 4) part[((wave * 2 + t) * NC + c) * 4 + lane] = v;
-            }
-        __syncthreads();
-        if (threadIdx.x < groups * 4 * tokens) {
-            const uint32_t r = threadIdx.x % (groups * 4), t = threadIdx.x / (groups * 4), g = r / 4;
-            float v[2] = {0.0f, 0.0f};
-            for (uint32_t k = 0; k < a.ksplit; ++k)
-                for (uint32_t p = 0; p < a.parts; ++p)
-#pragma unroll
-                    for (int m = 0; m < 2; ++m) v[m] += part[(((g * a.ksplit + k) * 2 + m) * NC + t * a.parts + p) * 4 + r % 4];
-            if (first_row + r < ff) a.h[(uint64_t)pairs[done + t] * ff + first_row + r] = moe_act(v[0], a.gelu) * v[1];
-        }
+            for (uint32_t m = 0; m < 2; ++m) v[m] += part[((m * TILE_WAVES / 2 + g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
+        if (first_row + r < ff) a.h[(uint64_t)space.pair[t] * ff + first_row + r] = moe_act(v[0], a.gelu) * v[1];
     }
 }
 
 // ---- down -----------------------------------------------------------------------------------------------
-// Up to four tokens: the rows of all experts in use, one behind the other, are one long row times the tokens' h, each
-// times its weight (0 for a token that did not choose the expert); the sum over a token's experts is the sum over the
-// row.  NC columns are the three pieces of the only token's h, or the tokens, whose pieces follow each other.
-template <class F, int NC, int CHAIN, int RT>
-__global__ __launch_bounds__(QD_THREADS) void moe_down_few(MoeArgs a) {
+// Up to T tokens: the rows of all experts in use, one behind the other, are one long row times the tokens' h, each times
+// its weight (0 for a token that did not choose the expert); the sum over a token's experts is the sum over the row.
+template <class F, int T, int CH>
+__global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ uint32_t items[4 * MOE_MAX_TOP_K];          // experts in use, in the order of their first pair
-    __shared__ int32_t pair_of[4 * MOE_MAX_TOP_K][4];      // the pair of item and token, or -1
+    __shared__ int32_t pair_at[4 * MOE_MAX_TOP_K][4];      // the pair of item and token, or -1
     __shared__ int32_t ids[4 * MOE_MAX_TOP_K];
     __shared__ uint64_t fresh_of[2];
-    typedef Slice<F> S;
-    typedef XStep<F, NC, CHAIN> X;
-    typedef Image<F, RT> I;
-    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), quad = lane / 4;
+    typedef Tile<F, T, CH> M;
+    typedef typename M::I I;
+    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t pairs = a.tokens * a.top_k, me_pair = threadIdx.x;      // at most 128: the first two waves
     if (me_pair < 4 * MOE_MAX_TOP_K) {
         ids[me_pair] = me_pair < pairs ? a.ids[me_pair] : -1;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) pair_of[me_pair][t] = -1;
+        for (int t = 0; t < 4; ++t) pair_at[me_pair][t] = -1;
     }
     __syncthreads();
     uint32_t front = me_pair;                              // the first pair with the same expert
@@ -307,160 +254,78 @@ __global__ __launch_bounds__(QD_THREADS) void moe_down_few(MoeArgs a) {
         const uint32_t below = (uint32_t)__popcll(fresh_of[front / 64] & ((1ull << (front % 64)) - 1));
         const uint32_t place = below + (front >= 64 ? (uint32_t)__popcll(fresh_of[0]) : 0u);
         if (front == me_pair) items[place] = (uint32_t)ids[me_pair];
-        pair_of[place][me_pair / a.top_k] = (int32_t)me_pair;
+        pair_at[place][me_pair / a.top_k] = (int32_t)me_pair;
     }
     __syncthreads();
     const uint32_t count = __builtin_amdgcn_readfirstlane((uint32_t)(__popcll(fresh_of[0]) + __popcll(fresh_of[1])));
-    const uint32_t kp = wave % a.ksplit, group = wave / a.ksplit, groups = QD_WAVES / a.ksplit;
-    const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), each = (uint32_t)((a.ff + 1023) / 1024), steps = each * count;
-    const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * groups * I::ROWS, row = first_row + group * I::ROWS, own = row < hidden ? row : hidden - 1;
-    const uint32_t rows = hidden - own < I::ROWS ? hidden - own : I::ROWS;
-    const uint32_t reach = (rows - 1) * row_bytes + (S::UNITS - 1) * S::UNIT + I::UNIT;
-    const typename S::Lane me(quad);
-    uint8_t *image = lds + wave * I::BYTES, *xs = lds + QD_WAVES * I::BYTES;
-    const uint8_t *x = xs + (quad * NC + (lane % 4 < NC ? lane % 4 : NC - 1)) * 16, *sums = xs + X::SUMS + quad * NC * 4;
-    float acc[RT][NC];
+    const uint32_t group = wave / a.ksplit, groups = TILE_WAVES / a.ksplit;
+    const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), each = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
+    const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS, own = row < hidden ? row : hidden - 1;
+    const uint32_t rows = hidden - own < M::ROWS ? hidden - own : M::ROWS;
+    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    typename M::Sums acc = no_sums<M>();
+    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes),
+                 Share{wave % a.ksplit, a.ksplit, a.chunk, each * count, a.tokens},
+                 [&](uint32_t turn) {
+                     const uint32_t item = turn / each, off = (turn - item * each) * I::TURN_BYTES;
+                     const uint64_t e = __builtin_amdgcn_readfirstlane(items[item]);
+                     return Turn{a.down + (e * hidden + own) * row_bytes + off, row_bytes - off, ((a.experts - e) * hidden - own) * row_bytes - off};
+                 },
+                 [&](uint32_t turn, uint32_t t, uint32_t c, float (&v)[8]) {
+                     const uint32_t item = turn / each;
+                     const int32_t pair = pair_at[item][t];
+                     const uint32_t from = pair < 0 ? 0u : (uint32_t)pair;
+                     const float weight = pair < 0 ? 0.0f : a.weights[from];
+                     load8(a.h, from * a.ff, (uint64_t)(turn - item * each) * M::ELEMS + c, a.ff, EK_F32, v);
 #pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) acc[t][c] = 0.0f;
-
-    const typename I::Places places(lane, rows, row_bytes);
-    I in;
-    uint32_t item = kp / each, local = kp % each;          // of the step that is fetched
-    auto fetch = [&]() {
-        const uint64_t e = __builtin_amdgcn_readfirstlane(items[item]);
-        const uint32_t left = row_bytes - local * S::STEP;
-        in.fetch(places, a.down + (e * hidden + own) * row_bytes + (uint64_t)local * S::STEP, ((a.experts - e) * hidden - own - 1) * row_bytes + left, reach);
-        return left;
-    };
-    uint32_t left = 0, step = kp;
-    if (kp < steps) left = fetch();
-    for (uint32_t first = 0; first < steps; first += a.chunk) {
-        const uint32_t now = first + a.chunk < steps ? a.chunk : steps - first, end = first + now;
-        if (first) __syncthreads();
-        stage_x<F, NC, CHAIN>(xs, now, a.tokens, a.parts, [&](uint32_t n, uint32_t t, uint32_t f, float (&v)[8]) {
-            const uint32_t i = (first + n) / each, s = (first + n) % each;
-            const int32_t pair = pair_of[i][t];
-            const uint32_t from = pair < 0 ? 0u : (uint32_t)pair;
-            const float w = pair < 0 ? 0.0f : a.weights[from];
-            load8(a.h, from * a.ff, ((uint64_t)s * 128 + f) * 8, a.ff, EK_F32, v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = pair < 0 ? 0.0f : v[j] * w;
-        });
-        __syncthreads();
-        for (; step < end; step += a.ksplit) {
-            wave_order();
-            in.put(places, image);
-            wave_order();
-            const uint32_t here = left;
-            if (step + a.ksplit < steps) {
-                for (local += a.ksplit; local >= each; local -= each) ++item;
-                left = fetch();
-            }
-            typename S::Raw raw[RT];
-#pragma unroll
-            for (int t = 0; t < RT; ++t) raw[t].load(image + (t * 4 + lane % 4) * I::ROW, me, here);
-            const uint32_t at = (step - first) * X::BYTES;
-            add_slices<F, NC, CHAIN, RT>(raw, me, x + at, sums + at, acc);
-        }
-    }
-    __syncthreads();
-    float *part = (float *)xs;                             // [wave][column][row]
-#pragma unroll
-    for (int t = 0; t < RT; ++t)
-#pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const float v = quads_sum(acc[t][c]);
-            if (lane < 4) part[(wave * NC + c) * I::ROWS + t * 4 + lane] = v;
-        }
-    __syncthreads();
-    if (threadIdx.x < groups * I::ROWS * a.tokens) {
-        const uint32_t r = threadIdx.x % (groups * I::ROWS), t = threadIdx.x / (groups * I::ROWS), g = r / I::ROWS;
+                     for (int j = 0; j < 8; ++j) v[j] = pair < 0 ? 0.0f : v[j] * weight;
+                 },
+                 acc);
+    float *part = (float *)(clear + M::CLEAR);
+    put_parts<M, T>(part, wave, acc);
+    for (uint32_t i = threadIdx.x; i < groups * M::ROWS * a.tokens; i += TILE_THREADS) {
+        const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.ksplit; ++k)
-            for (uint32_t p = 0; p < a.parts; ++p) v += part[((g * a.ksplit + k) * NC + t * a.parts + p) * I::ROWS + r % I::ROWS];
+        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
         if (first_row + r < hidden) store_elem(a.y, t * a.y_stride + first_row + r, a.y_kind, v);
     }
 }
 
-// More tokens: expert by expert, four of its tokens at a time, into o[pair]; grid: (row groups, slots).
-template <class F, int RT>
-__global__ __launch_bounds__(QD_THREADS) void moe_down_many(MoeArgs a) {
+// More tokens: expert by expert, up to T of its tokens at a time, into o[pair]; grid: (row groups, slots).
+template <class F, int T, int CH>
+__global__ __launch_bounds__(TILE_THREADS) void moe_down_many(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ SlotSpace space;
-    __shared__ uint32_t pairs[MOE_MAX_TOKENS];
-    constexpr int NC = 4, CHAIN = 3;
-    typedef Slice<F> S;
-    typedef XStep<F, NC, CHAIN> X;
-    typedef Image<F, RT> I;
-    const Slot slot = find_slot(space, a.ids, a, blockIdx.y);
+    typedef Tile<F, T, CH> M;
+    typedef typename M::I I;
+    const Slot slot = find_slot(space, a, blockIdx.y);
     if (slot.count == 0) return;
-    if (threadIdx.x < slot.count) pairs[threadIdx.x] = pair_with(a, nth_bit(slot.mask, threadIdx.x), slot.expert);
-    __syncthreads();
-    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), quad = lane / 4;
-    const uint32_t kp = wave % a.ksplit, group = wave / a.ksplit, groups = QD_WAVES / a.ksplit;
-    const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), steps = (uint32_t)((a.ff + 1023) / 1024);
-    const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * groups * I::ROWS, row = first_row + group * I::ROWS, own = row < hidden ? row : hidden - 1;
-    const uint32_t rows = hidden - own < I::ROWS ? hidden - own : I::ROWS;
-    const uint64_t at_row = ((uint64_t)slot.expert * hidden + own) * row_bytes;
-    const uint32_t reach = (rows - 1) * row_bytes + (S::UNITS - 1) * S::UNIT + I::UNIT;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+    const uint32_t group = wave / a.ksplit, groups = TILE_WAVES / a.ksplit;
+    const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), turns = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
+    const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS, own = row < hidden ? row : hidden - 1;
+    const uint32_t rows = hidden - own < M::ROWS ? hidden - own : M::ROWS;
+    const uint8_t *w = a.down + ((uint64_t)slot.expert * hidden + own) * row_bytes;
     const uint64_t behind = ((uint64_t)(a.experts - slot.expert) * hidden - own - 1) * row_bytes;
-    const typename S::Lane me(quad);
-    uint8_t *image = lds + wave * I::BYTES, *xs = lds + QD_WAVES * I::BYTES;
-    const uint8_t *x = xs + (quad * NC + lane % 4) * 16, *sums = xs + X::SUMS + quad * NC * 4;
-    const typename I::Places places(lane, rows, row_bytes);
-    I in;
-    for (uint32_t done = 0; done < slot.count; done += NC) {
-        const uint32_t tokens = slot.count - done < NC ? slot.count - done : NC;
-        float acc[RT][NC];
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) acc[t][c] = 0.0f;
-        uint64_t off = at_row + (uint64_t)kp * S::STEP;
-        uint32_t left = row_bytes - (kp < steps ? kp : steps - 1) * S::STEP, step = kp;
-        if (kp < steps) in.fetch(places, a.down + off, behind + left, reach);
-        for (uint32_t first = 0; first < steps; first += a.chunk) {
-            const uint32_t now = first + a.chunk < steps ? a.chunk : steps - first, end = first + now;
-            if (first || done) __syncthreads();
-            stage_x<F, NC, CHAIN>(xs, now, tokens, 1, [&](uint32_t n, uint32_t t, uint32_t f, float (&v)[8]) {
-                load8(a.h, pairs[done + t] * a.ff, ((uint64_t)(first + n) * 128 + f) * 8, a.ff, EK_F32, v);
-            });
-            __syncthreads();
-            for (; step < end; step += a.ksplit) {
-                wave_order();
-                in.put(places, image);
-                wave_order();
-                const uint32_t here = left;
-                if (step + a.ksplit < steps) {
-                    off += (uint64_t)a.ksplit * S::STEP;
-                    left -= a.ksplit * S::STEP;
-                    in.fetch(places, a.down + off, behind + left, reach);
-                }
-                typename S::Raw raw[RT];
-#pragma unroll
-                for (int t = 0; t < RT; ++t) raw[t].load(image + (t * 4 + lane % 4) * I::ROW, me, here);
-                const uint32_t at = (step - first) * X::BYTES;
-                add_slices<F, NC, CHAIN, RT>(raw, me, x + at, sums + at, acc);
-            }
-        }
-        __syncthreads();
-        float *part = (float *)xs;
-#pragma unroll
-        for (int t = 0; t < RT; ++t)
-#pragma unroll
-            for (int c = 0; c < NC; ++c) {
-                const float v = quads_sum(acc[t][c]);
-                if (lane < 4) part[(wave * NC + c) * I::ROWS + t * 4 + lane] = v;
-            }
-        __syncthreads();
-        if (threadIdx.x < groups * I::ROWS * tokens) {
-            const uint32_t r = threadIdx.x % (groups * I::ROWS), t = threadIdx.x / (groups * I::ROWS), g = r / I::ROWS;
-            float v = 0.0f;
-            for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * NC + t) * I::ROWS + r % I::ROWS];
-            if (first_row + r < hidden) a.o[(uint64_t)pairs[done + t] * hidden + first_row + r] = v;
-        }
+    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    typename M::Sums acc = no_sums<M>();
+    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
+                 Share{wave % a.ksplit, a.ksplit, a.chunk, turns, slot.count},
+                 [&](uint32_t turn) {
+                     const uint32_t off = turn * I::TURN_BYTES;
+                     return Turn{w + off, row_bytes - off, behind + row_bytes - off};
+                 },
+                 [&](uint32_t turn, uint32_t t, uint32_t c, float (&v)[8]) {
+                     load8(a.h, space.pair[t] * a.ff, (uint64_t)turn * M::ELEMS + c, a.ff, EK_F32, v);
+                 },
+                 acc);
+    float *part = (float *)(clear + M::CLEAR);
+    put_parts<M, T>(part, wave, acc);
+    for (uint32_t i = threadIdx.x; i < groups * M::ROWS * slot.count; i += TILE_THREADS) {
+        const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
+        float v = 0.0f;
+        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
+        if (first_row + r < hidden) a.o[(uint64_t)space.pair[t] * hidden + first_row + r] = v;
     }
 }
 // ... and the sum over a token's experts, in order
