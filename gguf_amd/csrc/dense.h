@@ -1,0 +1,420 @@
+// dense.h -- two to sixteen tokens at once: the tile of a wave for the products with packed weights (matmul.h).
+//
+// With several tokens the matrix unit's rows are tokens, all of them in use: v_mfma_f32_16x16x32_bf16 multiplies 32 codes of
+// 16 rows, one sub-block, with 16 tokens (16x16x16 for sub-blocks of 16).  Codes are turned into bf16, which holds every code
+// exactly (two at a time by v_cvt_scalef32_pk_bf16_fp8 where they are below 16: an e4m3 byte of 0..15 times 2^9 is itself);
+// x is in bf16 pieces, P of them: one for bf16, two for f16 and three for f32, exactly, and two for f32 where the result is
+// rounded to 16 bits anyway (2^-17 of an element).  Lane (n, g), n = lane % 16, g = lane / 16, brings the codes k = 8 g ..
+// 8 g + 7 (4 g .. 4 g + 3) of row n and receives the sums of tokens 4 g .. 4 g + 3, which it scales: two multiply-adds for
+// each eight codes and token, whatever the format, are most of the vector work.  The scales of a step are unpacked once,
+// each lane a quarter of its row's, and handed round through shared memory.
+//
+// Against the digits of one token (matmul.h), whose work grows with the tokens: q4_k 11008 x 4096, two tokens 9.6 against
+// 11.1 us.
+#pragma once
+#include "matmul.h"
+
+namespace ggq {
+
+// A format's step (256 elements of a row, its image in shared memory) as this tile takes it:
+//     SUB, OFFSET       elements of a sub-block, whether c can differ from zero
+//     scale(row, g, left, out)   {a, c} of the sub-blocks g * N .. g * N + N - 1, N = 64 / SUB; 0 behind the row's end
+//     codes(row, s, g, b)        sub-block s: the lane's 8 codes (SUB 32) or 4 (SUB 16) as bf16
+template <class F> struct Step;
+
+// four codes below 16 (bytes of w) -> two words of two bf16
+__device__ __forceinline__ void small_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, false));
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, true));
+}
+__device__ __forceinline__ void byte_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    w = opaque(w);
+    lo = upper_halves(ub<0>(w), ub<1>(w));
+    hi = upper_halves(ub<2>(w), ub<3>(w));
+}
+__device__ __forceinline__ void signed_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    w = opaque(w);
+    lo = upper_halves(sb<0>(w), sb<1>(w));
+    hi = upper_halves(sb<2>(w), sb<3>(w));
+}
+__device__ __forceinline__ void iq4_codes(uint32_t nibbles, uint32_t &lo, uint32_t &hi) { signed_codes(iq4_lookup4(nibbles) ^ 0x80808080u, lo, hi); }
+
+// ---- 32-element formats: sub-block s is block s of the step, at byte s * B -----------------------------------
+template <uint32_t B>
+struct StepOfBlocks {
+    static constexpr int SUB = 32;
+    static __device__ __forceinline__ uint32_t live(uint32_t s, uint32_t left) { return in_row((s + 1) * B, left); }
+    // the words at bytes AT and AT + 4 of block s; s is a constant once the loop over it is unrolled
+    static __device__ __forceinline__ void two_words(const uint8_t *row, uint32_t at, bool odd, uint32_t (&w)[2]) {
+        if (!odd) {
+            w[0] = al4(row + at);
+            w[1] = al4(row + at + 4);
+        } else {                                   // two bytes beyond a whole word
+            const uint32_t a = al4(row + at - 2), b = al4(row + at + 2), c = al4(row + at + 6);
+            w[0] = funnel16(b, a);
+            w[1] = funnel16(c, b);
+        }
+    }
+    // bytes 8 (g % 2) .. of the nibbles at byte HEAD of the block, the half of each that lane g's codes are in
+    template <uint32_t HEAD>
+    static __device__ __forceinline__ void nibbles(const uint8_t *row, uint32_t s, uint32_t g, uint32_t (&w)[2]) {
+        two_words(row, s * B + HEAD + 8 * (g & 1), (s * B + HEAD) % 4 != 0, w);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i] = (w[i] >> (4 * (g >> 1))) & LOW4;
+    }
+    // the fifth bits of lane g's codes
+    template <uint32_t HEAD>
+    static __device__ __forceinline__ void with_fifth(const uint8_t *row, uint32_t s, uint32_t g, uint32_t (&w)[2]) {
+        nibbles<HEAD + 4>(row, s, g, w);
+        const uint32_t bits = row[s * B + HEAD + g];
+        w[0] |= spread4(bits) << 4;
+        w[1] |= spread4(bits >> 4) << 4;
+    }
+};
+#define GGQ_STEP_SCALES(N) static __device__ __forceinline__ void scale(const uint8_t *row, uint32_t g, uint32_t left, SubScale (&out)[N])
+#define GGQ_STEP_CODES(N) static __device__ __forceinline__ void codes(const uint8_t *row, uint32_t s, uint32_t g, uint32_t (&b)[N])
+// {d, c(d)} of blocks 2 g and 2 g + 1 with a half at their begin; {d, m} with two
+#define GGQ_BLOCK_SCALES(EXPR_C)                                                        \
+    GGQ_STEP_SCALES(2) {                                                                \
+        _Pragma("unroll") for (uint32_t k = 0; k < 2; ++k) {                            \
+            const uint32_t s = 2 * g + k, on = live(s, left);                           \
+            const uint8_t *p = row + s * BYTES;                                         \
+            const float d = h2f(al2(p) & on);                                           \
+            out[k] = {d, EXPR_C};                                                       \
+        }                                                                               \
+    }
+template <> struct Step<Q4_0> : StepOfBlocks<18> {
+    static constexpr bool OFFSET = true;
+    static constexpr uint32_t BYTES = 18;
+    GGQ_BLOCK_SCALES(8.0f * d)
+    GGQ_STEP_CODES(4) {
+        uint32_t w[2];
+        nibbles<2>(row, s, g, w);
+        small_codes(w[0], b[0], b[1]);
+        small_codes(w[1], b[2], b[3]);
+    }
+};
+template <> struct Step<Q4_1> : StepOfBlocks<20> {
+    static constexpr bool OFFSET = true;
+    static constexpr uint32_t BYTES = 20;
+    GGQ_BLOCK_SCALES(-h2f(al2(p + 2) & on))
+    GGQ_STEP_CODES(4) {
+        uint32_t w[2];
+        nibbles<4>(row, s, g, w);
+        small_codes(w[0], b[0], b[1]);
+        small_codes(w[1], b[2], b[3]);
+    }
+};
+template <> struct Step<Q5_0> : StepOfBlocks<22> {
+    static constexpr bool OFFSET = true;
+    static constexpr uint32_t BYTES = 22;
+    GGQ_BLOCK_SCALES(16.0f * d)
+    GGQ_STEP_CODES(4) {
+        uint32_t w[2];
+        with_fifth<2>(row, s, g, w);
+        byte_codes(w[0], b[0], b[1]);
+        byte_codes(w[1], b[2], b[3]);
+    }
+};
+template <> struct Step<Q5_1> : StepOfBlocks<24> {
+    static constexpr bool OFFSET = true;
+    static constexpr uint32_t BYTES = 24;
+    GGQ_BLOCK_SCALES(-h2f(al2(p + 2) & on))
+    GGQ_STEP_CODES(4) {
+        uint32_t w[2];
+        with_fifth<4>(row, s, g, w);
+        byte_codes(w[0], b[0], b[1]);
+        byte_codes(w[1], b[2], b[3]);
+    }
+};
+template <uint32_t B, uint32_t HEAD>
+struct StepOfBytes : StepOfBlocks<B> {
+    static constexpr uint32_t BYTES = B;
+    static __device__ __forceinline__ void codes(const uint8_t *row, uint32_t s, uint32_t g, uint32_t (&b)[4]) {
+        uint32_t w[2];
+        StepOfBlocks<B>::two_words(row, s * B + HEAD + 8 * g, (s * B + HEAD) % 4 != 0, w);
+        signed_codes(w[0], b[0], b[1]);
+        signed_codes(w[1], b[2], b[3]);
+    }
+};
+template <> struct Step<Q8_0> : StepOfBytes<34, 2> {
+    static constexpr bool OFFSET = false;
+    GGQ_BLOCK_SCALES(0.0f)
+};
+template <> struct Step<Q8_1> : StepOfBytes<36, 4> {
+    static constexpr bool OFFSET = false;
+    GGQ_BLOCK_SCALES(0.0f)
+};
+template <> struct Step<IQ4NL> : StepOfBlocks<18> {
+    static constexpr bool OFFSET = false;
+    static constexpr uint32_t BYTES = 18;
+    GGQ_BLOCK_SCALES(0.0f)
+    GGQ_STEP_CODES(4) {
+        uint32_t w[2];
+        nibbles<2>(row, s, g, w);
+        iq4_codes(w[0], b[0], b[1]);
+        iq4_codes(w[1], b[2], b[3]);
+    }
+};
+
+// ---- 256-element formats: the step is a block ----------------------------------------------------------------
+template <> struct Step<Q4K> {
+    static constexpr bool OFFSET = true;
+    static constexpr int SUB = 32;
+    GGQ_STEP_SCALES(2) {
+        const u32x4 h = al16(row);
+        const uint32_t dm = h[0] & in_row(144, left);
+        const PairOfK4 k = scales_k4(h[1], h[2], h[3], g);
+        const float d = h2f(dm & 0xFFFFu), m = h2f(dm >> 16);
+        out[0] = {d * ub<0>(k.sc), m * ub<0>(k.mn)};
+        out[1] = {d * ub<1>(k.sc), m * ub<1>(k.mn)};
+    }
+    GGQ_STEP_CODES(4) {
+        const u32x2 q = al8(row + 16 + 32 * (s >> 1) + 8 * g);
+        small_codes((q[0] >> (4 * (s & 1))) & LOW4, b[0], b[1]);
+        small_codes((q[1] >> (4 * (s & 1))) & LOW4, b[2], b[3]);
+    }
+};
+template <> struct Step<Q5K> {
+    static constexpr bool OFFSET = true;
+    static constexpr int SUB = 32;
+    GGQ_STEP_SCALES(2) {
+        const u32x4 h = al16(row);
+        const uint32_t dm = h[0] & in_row(176, left);
+        const PairOfK4 k = scales_k4(h[1], h[2], h[3], g);
+        const float d = h2f(dm & 0xFFFFu), m = h2f(dm >> 16);
+        out[0] = {d * ub<0>(k.sc), m * ub<0>(k.mn)};
+        out[1] = {d * ub<1>(k.sc), m * ub<1>(k.mn)};
+    }
+    GGQ_STEP_CODES(4) {
+        const u32x2 q = al8(row + 48 + 32 * (s >> 1) + 8 * g), f = al8(row + 16 + 8 * g);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            byte_codes(((q[i] >> (4 * (s & 1))) & LOW4) | (((f[i] >> s) & 0x01010101u) << 4), b[2 * i], b[2 * i + 1]);
+    }
+};
+template <> struct Step<IQ4XS> {
+    static constexpr bool OFFSET = false;
+    static constexpr int SUB = 32;
+    GGQ_STEP_SCALES(2) {
+        const u32x2 h = al8(row);
+        const float d = h2f(h[0] & 0xFFFFu & in_row(136, left));
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+            const uint32_t ls = ((h[1] >> (8 * g + 4 * k)) & 0xFu) | (((h[0] >> (16 + 4 * g + 2 * k)) & 3u) << 4);
+            out[k] = {d * (float)((int)ls - 32), 0.0f};
+        }
+    }
+    GGQ_STEP_CODES(4) {
+        const u32x2 q = al8(row + 8 + 16 * s + 8 * (g & 1));
+        iq4_codes((q[0] >> (4 * (g >> 1))) & LOW4, b[0], b[1]);
+        iq4_codes((q[1] >> (4 * (g >> 1))) & LOW4, b[2], b[3]);
+    }
+};
+template <> struct Step<Q8K> {
+    static constexpr bool OFFSET = false;
+    static constexpr int SUB = 32;
+    GGQ_STEP_SCALES(2) {
+        const float d = h2f(al2(row) & in_row(290, left));
+        out[0] = out[1] = {d, 0.0f};
+    }
+    GGQ_STEP_CODES(4) {
+        const uint8_t *p = row + 32 * s + 8 * g;             // the codes begin two bytes behind
+        const u32x2 q = al8(p);
+        const uint32_t over = al4(p + 8);
+        signed_codes(funnel16(q[1], q[0]), b[0], b[1]);
+        signed_codes(funnel16(over, q[1]), b[2], b[3]);
+    }
+};
+// sub-blocks of 16: s = 8 n + 2 p + h, elements 128 n + 32 p + 16 h + 0..15; lane g the elements 4 g .. of them
+template <> struct Step<Q6K> {
+    static constexpr bool OFFSET = true;
+    static constexpr int SUB = 16;
+    GGQ_STEP_SCALES(4) {
+        const float d = h2f(al2(row + 208) & in_row(210, left));
+        const uint32_t sc = al4(row + 192 + 4 * g);
+        const float a[4] = {d * sb<0>(sc), d * sb<1>(sc), d * sb<2>(sc), d * sb<3>(sc)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[k] = {a[k], 32.0f * a[k]};
+    }
+    GGQ_STEP_CODES(2) {
+        const uint32_t n = s >> 3, p = (s >> 1) & 3, h = s & 1;
+        const uint32_t low = (al4(row + 64 * n + 32 * (p & 1) + 16 * h + 4 * g) >> (4 * (p >> 1))) & LOW4;
+        const uint32_t high = (al4(row + 128 + 32 * n + 16 * h + 4 * g) >> (2 * p)) & 0x03030303u;
+        byte_codes(low | (high << 4), b[0], b[1]);
+    }
+};
+template <> struct Step<Q2K> {
+    static constexpr bool OFFSET = true;
+    static constexpr int SUB = 16;
+    GGQ_STEP_SCALES(4) {
+        const uint32_t dm = al4(row + 80) & in_row(84, left), sc = al4(row + 4 * g);
+        const float d = h2f(dm & 0xFFFFu), m = h2f(dm >> 16);
+        const uint32_t lo = sc & LOW4, hi = (sc >> 4) & LOW4;
+        out[0] = {d * ub<0>(lo), m * ub<0>(hi)};
+        out[1] = {d * ub<1>(lo), m * ub<1>(hi)};
+        out[2] = {d * ub<2>(lo), m * ub<2>(hi)};
+        out[3] = {d * ub<3>(lo), m * ub<3>(hi)};
+    }
+    GGQ_STEP_CODES(2) {
+        const uint32_t n = s >> 3, p = (s >> 1) & 3, h = s & 1;
+        small_codes((al4(row + 16 + 32 * n + 16 * h + 4 * g) >> (2 * p)) & 0x03030303u, b[0], b[1]);
+    }
+};
+template <> struct Step<Q3K> {
+    static constexpr bool OFFSET = true;
+    static constexpr int SUB = 16;
+    GGQ_STEP_SCALES(4) {
+        const float d = h2f(al2(row + 108) & in_row(110, left));
+        // scales 4 g .. 4 g + 3: nibbles of word g % 2 (high ones for g >= 2), top bits 2 g.. of the third word's bytes
+        const uint32_t lo = (al4(row + 96 + 4 * (g & 1)) >> (4 * (g >> 1))) & LOW4, hi = (al4(row + 104) >> (2 * g)) & 0x03030303u;
+        const uint32_t sc = lo | (hi << 4);
+        const float a[4] = {d * (ub<0>(sc) - 32.0f), d * (ub<1>(sc) - 32.0f), d * (ub<2>(sc) - 32.0f), d * (ub<3>(sc) - 32.0f)};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) out[k] = {a[k], 4.0f * a[k]};
+    }
+    GGQ_STEP_CODES(2) {
+        const uint32_t n = s >> 3, p = (s >> 1) & 3, h = s & 1;
+        const uint32_t low = (al4(row + 32 + 32 * n + 16 * h + 4 * g) >> (2 * p)) & 0x03030303u;
+        const uint32_t high = (al4(row + 16 * h + 4 * g) >> (4 * n + p)) & 0x01010101u;
+        small_codes(low | (high << 2), b[0], b[1]);
+    }
+};
+
+// ---- 16-bit floats: no scales; a half in two pieces ----------------------------------------------------------
+template <class F>
+struct StepOfFloats {
+    static constexpr int SUB = 32;
+    static constexpr bool OFFSET = false;
+    // elements 32 s + 8 g .. + 7; what lies behind the row may be anything, an infinity too
+    static __device__ __forceinline__ u32x4 load(const uint8_t *row, uint32_t s, uint32_t g, uint32_t left) {
+        const uint32_t at = 64 * s + 16 * g;
+        u32x4 v = al16(row + at);
+        if (left < 512) {
+            const uint32_t n = left > at ? (left - at) / 2 : 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) v[i] &= 2 * i + 1 < n ? ~0u : 2 * i < n ? 0xFFFFu : 0u;
+        }
+        return v;
+    }
+};
+template <> struct Step<WF16> : StepOfFloats<WF16> {};
+template <> struct Step<WBF16> : StepOfFloats<WBF16> {};
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+
+// The members of Tile (matmul.h), for up to 16 tokens.
+// Staged x, per turn: [piece][fragment of 8 elements][token] 16 bytes, 32 bytes between one fragment and the next for the
+// staging threads' banks; then the sums of x over each sub-block, [sub-block][token], f32.
+template <class F, int P>
+struct DenseTile {
+    typedef Step<F> S;
+    static constexpr uint32_t ROWS = 16, ELEMS = 256, TOKENS = 16;
+    typedef Image<F, ROWS, 1> I;
+    static constexpr uint32_t FRAG = TOKENS * 16 + 32, PIECE = 32 * FRAG, SUBS = 256 / S::SUB;
+    static constexpr uint32_t SUMS = P * PIECE, X_BYTES = SUMS + (S::OFFSET ? SUBS * TOKENS * 4 : 0), CLEAR = 0;
+    static constexpr uint32_t WAVE_BYTES = I::BYTES + (is_float_type<F> ? 0 : SUBS * ROWS * 8);       // the image, then {a, c} [sub-block][row]
+
+    template <class Load>
+    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t tokens, Load load) {
+        // four lanes side by side take 32 neighbouring elements of a token
+        const uint32_t quads = turns * 8 * tokens;
+        for (uint32_t i = threadIdx.x; i < quads * 4; i += TILE_THREADS) {
+            const uint32_t q = i / 4, t = q % tokens, n = q / tokens, turn = n / 8, f = n % 8 * 4 + i % 4;
+            uint8_t *to = lds + turn * X_BYTES;
+            float v[8];
+            load(turn, t, f * 8, v);
+            if constexpr (S::OFFSET) {
+                float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+                sum += dpp<QUAD_XOR1>(sum);
+                if (S::SUB == 32) sum += dpp<QUAD_XOR2>(sum);
+                if (f % (S::SUB / 8) == 0) ((float *)(to + SUMS))[f / (S::SUB / 8) * TOKENS + t] = sum;
+            }
+            to += f * FRAG + t * 16;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                *(u32x4 *)(to + p * PIECE) = u32x4{upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7])};
+                if (p + 1 < P)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v[k] = below_bf16(v[k]);
+            }
+        }
+    }
+    struct Me {
+        uint32_t n, g;
+        __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) : n(lane % 16), g(lane / 16) {}
+    };
+    struct Sums { float v[4]; };                 // of tokens 4 g .. 4 g + 3
+    static __device__ __forceinline__ void add(uint8_t *image, const Me &me, const uint8_t *, const uint8_t *x, uint32_t left, uint32_t, Sums &acc) {
+        const uint8_t *row = image + me.n * I::ROW;
+        if constexpr (is_float_type<F>) {
+            f32x4 d = {acc.v[0], acc.v[1], acc.v[2], acc.v[3]};
+#pragma unroll
+            for (uint32_t s = 0; s < SUBS; ++s) {
+                u32x4 b = S::load(row, s, me.g, left), low = {0, 0, 0, 0};
+                if constexpr (__is_same(F, WF16)) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t w = b[i];
+                        const float v0 = h2f(w & 0xFFFFu), v1 = h2f(w >> 16);
+                        b[i] = upper_halves(v0, v1);
+                        low[i] = upper_halves(below_bf16(v0), below_bf16(v1));
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+                    const bf16x8 a = __builtin_bit_cast(bf16x8, al16(x + p * PIECE + (4 * s + me.g) * FRAG + me.n * 16));
+                    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, b), d, 0, 0, 0);
+                    if constexpr (__is_same(F, WF16)) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, low), d, 0, 0, 0);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) acc.v[r] = d[r];
+        } else {
+            float *scales = (float *)(image + I::BYTES);
+            constexpr uint32_t EACH = SUBS / 4;
+            SubScale mine[EACH];
+            S::scale(row, me.g, left, mine);
+#pragma unroll
+            for (uint32_t k = 0; k < EACH; ++k) *(f32x2 *)(scales + ((me.g * EACH + k) * ROWS + me.n) * 2) = f32x2{mine[k].a, mine[k].c};
+            wave_order();
+#pragma unroll
+            for (uint32_t s = 0; s < SUBS; ++s) {
+                f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+                if constexpr (S::SUB == 32) {
+                    uint32_t b[4];
+                    S::codes(row, s, me.g, b);
+                    const bf16x8 w = __builtin_bit_cast(bf16x8, u32x4{b[0], b[1], b[2], b[3]});
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const u32x4 a = al16(x + p * PIECE + (4 * s + me.g) * FRAG + me.n * 16);
+                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), w, d, 0, 0, 0);
+                    }
+                } else {
+                    uint32_t b[2];
+                    S::codes(row, s, me.g, b);
+                    const s16x4 w = __builtin_bit_cast(s16x4, u32x2{b[0], b[1]});
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        const u32x2 a = al8(x + p * PIECE + (2 * s + (me.g >> 1)) * FRAG + me.n * 16 + 8 * (me.g & 1));
+                        d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), w, d, 0, 0, 0);
+                    }
+                }
+                const f32x2 k = *(const f32x2 *)(scales + (s * ROWS + me.n) * 2);
+                const f32x4 sum = *(const f32x4 *)(x + SUMS + (s * TOKENS + 4 * me.g) * 4);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    acc.v[r] = __builtin_fmaf(k[0], d[r], acc.v[r]);
+                    if constexpr (S::OFFSET) acc.v[r] = __builtin_fmaf(-k[1], sum[r], acc.v[r]);
+                }
+            }
+        }
+    }
+    static __device__ __forceinline__ void put(float *part, uint32_t lane, const Sums &acc) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) part[(4 * (lane / 16) + r) * ROWS + lane % 16] = acc.v[r];
+    }
+};
+
+}  // namespace ggq

@@ -5,7 +5,6 @@
 // and what surrounds them in a decoding step: rows of a packed table by id, and a mixture-of-experts layer.
 #pragma once
 #include "slices.h"
-#include <type_traits>
 
 namespace ggq {
 
@@ -121,11 +120,12 @@ __device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, ui
 // registers would touch a line per lane: the memory pipeline takes about two cycles for each, which held the products at
 // 4.1 TB/s whatever the format's arithmetic.  Instead neighbouring lanes load neighbouring 16-byte pieces into registers,
 // one turn ahead, and hand them over through the wave's own part of shared memory.
-template <class F, uint32_t ROWS>
+template <class F, uint32_t ROWS, uint32_t TURN>
 struct Image {
     typedef Slice<F> S;
-    static constexpr uint32_t TURN_BYTES = S::STEP * S::TURN;          // packed, of a row
-    static constexpr uint32_t PIECES = (S::UNIT + 15) / 16, PER_ROW = PIECES * S::UNITS, LOADS = (PER_ROW * ROWS + 63) / 64;
+    static constexpr uint32_t TURN_BYTES = S::STEP * TURN;             // packed, of a row
+    static constexpr uint32_t UNITS = S::BLOCKS ? TURN : 1, UNIT_BYTES = TURN_BYTES / UNITS;
+    static constexpr uint32_t PIECES = (UNIT_BYTES + 15) / 16, PER_ROW = PIECES * UNITS, LOADS = (PER_ROW * ROWS + 63) / 64;
     // an odd number of 16-byte places from row to row: the rows' parts of one column lie in different banks
     static constexpr uint32_t UNIT = PIECES * 16, ROW = 16 * (PER_ROW | 1);
     static constexpr uint32_t BYTES = ROW * ROWS;
@@ -139,13 +139,13 @@ struct Image {
                 uint32_t p = i * 64 + lane;
                 if (p >= PER_ROW * ROWS) p = PER_ROW * ROWS - 1;
                 const uint32_t r = p / PER_ROW, u = p % PER_ROW / PIECES, c = p % PIECES * 16;
-                src[i] = (r < rows ? r : rows - 1) * row_bytes + u * S::UNIT + c;
+                src[i] = (r < rows ? r : rows - 1) * row_bytes + u * UNIT_BYTES + c;
                 dst[i] = r * ROW + u * UNIT + c;
             }
         }
     };
     // bytes from a turn's begin in the tile's first row to the end of its furthest piece
-    static __device__ __forceinline__ uint32_t reach(uint32_t rows, uint32_t row_bytes) { return (rows - 1) * row_bytes + (S::UNITS - 1) * S::UNIT + UNIT; }
+    static __device__ __forceinline__ uint32_t reach(uint32_t rows, uint32_t row_bytes) { return (rows - 1) * row_bytes + (UNITS - 1) * UNIT_BYTES + UNIT; }
     u32x4 v[LOADS];
 
     // The turn that begins at `base` (in the tile's first row).  A unit's last piece and a row's last turn may reach beyond
@@ -186,16 +186,17 @@ struct Image {
     }
 };
 
-// What a wave does with a tile of rows, for up to T tokens.  Two kinds, with the same members:
+// What a wave does with a tile of rows, for up to TOKENS tokens.  Three kinds, with the same members (the third: dense.h):
 //     ROWS, ELEMS       rows of the tile, elements of a turn
 //     X_BYTES           shared memory of a turn of x
 //     CLEAR             bytes of zeros in front of the staged x
 //     stage             puts turns of x into shared memory
 //     Me                what a lane knows of its place
 //     add               the products of one turn
-//     total             a lane's sum over the lanes that share its row; lane r < ROWS has row r's
+//     put               the wave's sums to part[token][row]
+//     TOKENS            rows of part; WAVE_BYTES: shared memory of a wave, its image first
 
-// ---- packed whole-number codes: x in digits ---------------------------------------------------------------
+// ---- packed whole-number codes, one token: x in digits ------------------------------------------------------
 // The matrix unit multiplies e4m3 bytes with a block scale for each 32 of them.  Codes are such bytes already (slices.h),
 // and so are the digits of x: 32 neighbouring elements share an exponent e, the largest one's; each becomes a whole number
 // of 16 CH bits (truncated, 2^-32 of the largest element, for CH = 2; rounded, 2^-17 of it, for CH = 1, which is taken where
@@ -208,29 +209,28 @@ struct Image {
 // the scale that a lane has unpacked is applied where it is.  The lanes of A whose slice is not m / 4's read zeros.  Digits
 // carry their weight 16^-d in A's block scale, so a sub-block's sum is the sum of the four.
 //
-// Against codes in bf16 (x as three pieces, v_mfma_f32_4x4x4, what 16-bit float weights take below): a third of the vector
-// instructions, which bound those.
+// Against codes in bf16 (x as three pieces, v_mfma_f32_4x4x4, what 16-bit float weights take below) it needs a third of the
+// vector instructions, which bound those: q6_k 4096 x 11008 11.2 against 12.6 us, q5_k 11008 x 4096 8.8 against 11.4.
 //
 // Staged x, per turn and token: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e - 2 as a byte, then
 // the sums of x, f32: [step][slice][sub-block].
-template <class F, int T, int CH>
+template <class F, int CH>
 struct CodeTile {
     typedef Slice<F> S;
-    static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN;
-    typedef Image<F, ROWS> I;
+    static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN, TOKENS = 1;
+    typedef Image<F, ROWS, S::TURN> I;
     static constexpr uint32_t DIGITS = CH * 1024, EXPS = DIGITS * S::TURN, SUMS = EXPS + 8 * S::TURN + 8 * (S::TURN & 1);
-    static constexpr uint32_t PER_TOKEN = SUMS + 16 * S::NSUB * S::TURN, X_BYTES = T * PER_TOKEN, CLEAR = DIGITS;
+    static constexpr uint32_t X_BYTES = SUMS + 16 * S::NSUB * S::TURN, CLEAR = DIGITS, WAVE_BYTES = I::BYTES;
 
-    // load(turn, t, c, v): elements [c, c + 8) of token t in that turn
     template <class Load>
-    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t tokens, Load load) {
+    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t, Load load) {
         constexpr uint32_t FRAGS = 32 * S::TURN;               // of eight elements; four lanes side by side have a block
-        for (uint32_t i = threadIdx.x; i < FRAGS * turns * tokens; i += TILE_THREADS) {
-            const uint32_t t = T == 1 ? 0 : i / (FRAGS * turns), j = i - t * FRAGS * turns, turn = j / FRAGS, f = j % FRAGS;
+        for (uint32_t i = threadIdx.x; i < FRAGS * turns; i += TILE_THREADS) {
+            const uint32_t turn = i / FRAGS, f = i % FRAGS;
             const uint32_t step = f / 32, block = f / 4 % 8, half = f / 2 % 2;
-            uint8_t *to = lds + (turn * T + t) * PER_TOKEN;
+            uint8_t *to = lds + turn * X_BYTES;
             float v[8];
-            load(turn, t, f * 8, v);
+            load(turn, 0, f * 8, v);
             float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
             sum += dpp<QUAD_XOR1>(sum);
             float *sums = (float *)(to + SUMS) + step * 4 * S::NSUB;
@@ -306,7 +306,7 @@ struct CodeTile {
             weight = p * 0x04040404u;
         }
     };
-    struct Sums { float v[T]; };
+    struct Sums { float v[1]; };
 
     static __device__ __forceinline__ i32x8 join(u32x4 a, u32x4 b) {
         return {(int)a[0], (int)a[1], (int)a[2], (int)a[3], (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
@@ -332,7 +332,7 @@ struct CodeTile {
     }
     template <int SB>
     static __device__ __forceinline__ void add_sub(const typename S::Raw &raw, const Me &me, const uint8_t *clear, const uint8_t *x, uint32_t step,
-                                                   uint32_t tokens, Sums &acc) {
+                                                   Sums &acc) {
         constexpr int WORDS = S::SUB / 4;
         uint32_t b[WORDS], h[WORDS];
         S::template low<SB>(raw, b);
@@ -344,66 +344,63 @@ struct CodeTile {
             hi[i] = S::HIGH ? (int)h[i % WORDS] : 0;
         }
         const SubScale s = S::template scale<SB>(raw);
-#pragma unroll
-        for (uint32_t t = 0; t < T; ++t) {
-            if (T > 1 && t >= tokens) break;
-            const uint8_t *xt = x + t * PER_TOKEN;
-            const uint32_t exps = (S::PLANES ? al4(xt + EXPS + step * 8 + me.exps) : al2(xt + EXPS + step * 8 + me.exps)) - me.weight;
-            const uint8_t *digits = clear + ((uint32_t)(xt + step * DIGITS + me.digits - clear) & me.own);
-            const f32x4 d = sub_block<SB>(lo, hi, digits, exps);
-            const float sum = ((const float *)(xt + SUMS))[(step * 4 + me.g) * S::NSUB + SB];
-            acc.v[t] = __builtin_fmaf(s.a, (d[0] + d[1]) + (d[2] + d[3]), acc.v[t]);
-            acc.v[t] = __builtin_fmaf(-s.c, sum, acc.v[t]);
-        }
+        const uint32_t exps = (S::PLANES ? al4(x + EXPS + step * 8 + me.exps) : al2(x + EXPS + step * 8 + me.exps)) - me.weight;
+        const uint8_t *digits = clear + ((uint32_t)(x + step * DIGITS + me.digits - clear) & me.own);
+        const f32x4 d = sub_block<SB>(lo, hi, digits, exps);
+        const float sum = ((const float *)(x + SUMS))[(step * 4 + me.g) * S::NSUB + SB];
+        acc.v[0] = __builtin_fmaf(s.a, (d[0] + d[1]) + (d[2] + d[3]), acc.v[0]);
+        acc.v[0] = __builtin_fmaf(-s.c, sum, acc.v[0]);
     }
     // one turn: `image` the wave's bytes, `x` the turn's staged x, `clear` the zeros, `left` bytes of the row from the turn on
     static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *clear, const uint8_t *x, uint32_t left,
-                                               uint32_t tokens, Sums &acc) {
+                                               uint32_t, Sums &acc) {
 #pragma unroll
         for (uint32_t step = 0; step < S::TURN; ++step) {
             typename S::Raw raw;
             raw.load(image + me.row, step, me.g, left);
             // one sub-block after the other: scheduled into each other they take the registers of more waves
-            add_sub<0>(raw, me, clear, x, step, tokens, acc);
+            add_sub<0>(raw, me, clear, x, step, acc);
             __builtin_amdgcn_sched_barrier(0);
-            add_sub<1>(raw, me, clear, x, step, tokens, acc);
+            add_sub<1>(raw, me, clear, x, step, acc);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (S::NSUB == 4) {
-                add_sub<2>(raw, me, clear, x, step, tokens, acc);
+                add_sub<2>(raw, me, clear, x, step, acc);
                 __builtin_amdgcn_sched_barrier(0);
-                add_sub<3>(raw, me, clear, x, step, tokens, acc);
+                add_sub<3>(raw, me, clear, x, step, acc);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
-    static __device__ __forceinline__ float total(float v) {
+    static __device__ __forceinline__ void put(float *part, uint32_t lane, const Sums &acc) {
+        float v = acc.v[0];
         v += __shfl_xor(v, 16);
         v += __shfl_xor(v, 32);
-        return v;
+        if (lane < ROWS) part[lane] = v;
     }
 };
 
-// ---- 16-bit float weights: bf16 pieces -----------------------------------------------------------------------
+// ---- 16-bit float weights, one token: bf16 pieces ------------------------------------------------------------
 // x in CH bf16 pieces (bf16 one, f16 two, f32 three, exactly), the weights in one or two: products are exact, sums f32.
 // A wave takes four rows; its quads (four neighbouring lanes, one lane per row) take 16 neighbouring slices at a time, and
-// v_mfma_f32_4x4x4 with 16 blocks multiplies, in each quad, the four rows with the tokens that the quad's lanes hold.
-// Staged x, per turn: [piece][k][slice][token] fragments of eight bf16, k = the fragment's place in its slice; the quads
+// v_mfma_f32_4x4x4 with 16 blocks multiplies, in each quad, the four rows with the x that the quad's lanes hold, the same in
+// all four: a lane's result is its row's.
+// Staged x, per turn: [piece][k][slice] fragments of eight bf16, k = the fragment's place in its slice; the quads
 // read the same k of neighbouring slices, so their addresses are consecutive; 16 bytes between one k and the next keep the
 // staging threads, which run along k first, out of each other's banks.
-template <class F, int T, int CH>
+template <class F, int CH>
 struct FloatTile {
     typedef Slice<F> S;
-    static constexpr uint32_t ROWS = 4, ELEMS = 1024;
-    typedef Image<F, ROWS> I;
-    static constexpr uint32_t K = 256 * T + 16, X_BYTES = CH * 8 * K, CLEAR = 0;
+    static constexpr uint32_t ROWS = 4, ELEMS = 1024, TOKENS = 1;
+    typedef Image<F, ROWS, S::TURN> I;
+    static constexpr uint32_t K = 256 + 16, X_BYTES = CH * 8 * K, CLEAR = 0, WAVE_BYTES = I::BYTES;
 
     template <class Load>
-    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t tokens, Load load) {
-        for (uint32_t i = threadIdx.x; i < 128 * turns * tokens; i += TILE_THREADS) {
-            const uint32_t t = T == 1 ? 0 : i / (128 * turns), j = i - t * 128 * turns, turn = j / 128, f = j % 128;
+    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t, Load load) {
+        for (uint32_t i = threadIdx.x; i < 128 * turns; i += TILE_THREADS) {
+            const uint32_t turn = i / 128, f = i % 128;
             float v[8];
-            load(turn, t, f * 8, v);
-            uint8_t *to = lds + turn * X_BYTES + f % 8 * K + (f / 8 * T + t) * 16;
+            load(turn, 0, f * 8, v);
+            uint8_t *to = lds + turn * X_BYTES + f % 8 * K + f / 8 * 16;
 #pragma unroll
             for (int p = 0; p < CH; ++p) {
                 *(u32x4 *)(to + p * 8 * K) = u32x4{upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7])};
@@ -415,9 +412,9 @@ struct FloatTile {
     }
     struct Me {
         uint32_t quad, row, x;
-        __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) : quad(lane / 4), row(lane % 4 * I::ROW), x((lane / 4 * T + (lane % 4 < T ? lane % 4 : T - 1)) * 16) {}
+        __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) : quad(lane / 4), row(lane % 4 * I::ROW), x(lane / 4 * 16) {}
     };
-    struct Sums { float v[T]; };
+    struct Sums { float v[1]; };
     static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *, const uint8_t *x, uint32_t left, uint32_t, Sums &acc) {
         typename S::Raw raw;
         raw.load(image + me.row, me.quad, left);
@@ -440,20 +437,17 @@ struct FloatTile {
                         }
                     }
             }
-#pragma unroll
-        for (int t = 0; t < T; ++t) acc.v[t] += d[t];
+        acc.v[0] += d[0];
     }
-    static __device__ __forceinline__ float total(float v) {
+    static __device__ __forceinline__ void put(float *part, uint32_t lane, const Sums &acc) {
+        float v = acc.v[0];
         v += dpp<ROW_ROR8>(v);
         v += dpp<ROW_ROR4>(v);
         v += __shfl_xor(v, 16);
         v += __shfl_xor(v, 32);
-        return v;
+        if (lane < ROWS) part[lane] = v;
     }
 };
-
-template <class F, int T, int CH>
-using Tile = std::conditional_t<is_float_type<F>, FloatTile<F, T, CH>, CodeTile<F, T, CH>>;
 
 // ---- the loop over a row ----------------------------------------------------------------------------------------
 // The wave's part of a tile: turns kp, kp + ksplit, ... of `turns`, the next one's bytes on the way while one is multiplied.
@@ -497,15 +491,10 @@ __device__ __forceinline__ void run_turns(uint8_t *image, uint8_t *clear, const 
     }
 }
 // The waves' sums to part[wave][token][row].
-template <class M, int T>
+template <class M>
 __device__ __forceinline__ void put_parts(float *part, uint32_t wave, const typename M::Sums &acc) {
-    const uint32_t lane = threadIdx.x % 64;
     __syncthreads();                                   // the staged x is no longer needed
-#pragma unroll
-    for (int t = 0; t < T; ++t) {
-        const float v = M::total(acc.v[t]);
-        if (lane < M::ROWS) part[(wave * T + t) * M::ROWS + lane] = v;
-    }
+    M::put(part + wave * M::TOKENS * M::ROWS, threadIdx.x % 64, acc);
     __syncthreads();
 }
 template <class M>
@@ -517,11 +506,10 @@ __device__ __forceinline__ typename M::Sums no_sums() {
 }
 
 // ---- one matrix -----------------------------------------------------------------------------------------------
-// Up to T tokens.  A wave owns a tile of rows, or shares it with others that take other turns of its columns.
-template <class F, int T, int CH>
+// Up to M::TOKENS tokens.  A wave owns a tile of rows, or shares it with others that take other turns of its columns.
+template <class F, class M>
 __global__ __launch_bounds__(TILE_THREADS) void matvec_tiles(MatvecArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    typedef Tile<F, T, CH> M;
     typedef typename M::I I;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t group = wave / a.ksplit, groups = TILE_WAVES / a.ksplit;
@@ -532,9 +520,9 @@ __global__ __launch_bounds__(TILE_THREADS) void matvec_tiles(MatvecArgs a) {
     const uint32_t rows = a.rows - own < M::ROWS ? (uint32_t)(a.rows - own) : M::ROWS;
     const uint8_t *w = a.w + own * row_bytes;
     const uint64_t behind = (a.rows - own - 1) * row_bytes;                                   // of the tensor, behind the row
-    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;
     typename M::Sums acc = no_sums<M>();
-    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
+    run_turns<M>(lds + wave * M::WAVE_BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
                  Share{wave % a.ksplit, a.ksplit, a.chunk, turns, a.tokens},
                  [&](uint32_t turn) {
                      const uint32_t off = turn * I::TURN_BYTES;
@@ -545,11 +533,11 @@ __global__ __launch_bounds__(TILE_THREADS) void matvec_tiles(MatvecArgs a) {
                  },
                  acc);
     float *part = (float *)(clear + M::CLEAR);
-    put_parts<M, T>(part, wave, acc);
+    put_parts<M>(part, wave, acc);
     for (uint32_t i = threadIdx.x; i < groups * M::ROWS * a.tokens; i += TILE_THREADS) {
         const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
+        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * M::TOKENS + t) * M::ROWS + r % M::ROWS];
         if (first_row + r < a.rows) store_elem(a.y, t * a.y_stride + first_row + r, a.y_kind, v);
     }
 }

@@ -1,6 +1,7 @@
 // matmul.hip -- entry points of the products with packed weights (include/ggq.h): argument checks and launches.
 #include "../../include/ggq.h"
 #include "internal.h"
+#include "dense.h"
 #include "matmul.h"
 #include "moe.h"
 
@@ -62,62 +63,62 @@ constexpr uint32_t X_LDS = 40 << 10;
 
 // The shape of a launch over `tiles` wave tiles, each of which takes `turns` turns: how many waves share a tile's turns,
 // the turns staged at a time (equal chunks, whole rounds of the waves), the shared memory.
-template <class M>
 struct Shape {
-    uint32_t ksplit = 1, chunk, groups, bytes;
-    // `waves`: of a workgroup that may share a tile's turns
-    Shape(uint64_t tiles, uint32_t turns, uint32_t waves, uint32_t tokens) {
+    uint32_t ksplit = 1, groups;
+    // `waves`: of a workgroup that may share a tile's turns; x_bytes: shared memory of a turn of x
+    Shape(uint64_t tiles, uint32_t turns, uint32_t waves, uint32_t x_bytes) {
         // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
-        while (ksplit < waves && ksplit < turns && tiles * ksplit < 2048 && 2 * ksplit * M::X_BYTES <= X_LDS) ksplit *= 2;
-        const uint32_t rounds = (turns + ksplit - 1) / ksplit, most = std::max(1u, X_LDS / (M::X_BYTES * ksplit)), chunks = (rounds + most - 1) / most;
-        chunk = (rounds + chunks - 1) / chunks * ksplit;
+        while (ksplit < waves && ksplit < turns && tiles * ksplit < 2048 && 2 * ksplit * x_bytes <= X_LDS) ksplit *= 2;
         groups = waves / ksplit;
-        bytes = TILE_WAVES * M::I::BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk, turns) * M::X_BYTES, TILE_WAVES * tokens * M::ROWS * 4);
+    }
+    template <class M> uint32_t chunk(uint32_t turns) const {
+        const uint32_t rounds = (turns + ksplit - 1) / ksplit, most = std::max(1u, X_LDS / (M::X_BYTES * ksplit)), chunks = (rounds + most - 1) / most;
+        return (rounds + chunks - 1) / chunks * ksplit;
+    }
+    template <class M> uint32_t bytes(uint32_t turns) const {
+        return TILE_WAVES * M::WAVE_BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk<M>(turns), turns) * M::X_BYTES, TILE_WAVES * M::TOKENS * M::ROWS * 4);
     }
 };
 template <class M> constexpr uint32_t turns_of(uint64_t cols) { return (uint32_t)((cols + M::ELEMS - 1) / M::ELEMS); }
 
-template <class F, int T, int CH>
-void launch_tiles(MatvecArgs a, hipStream_t st) {
-    typedef Tile<F, T, CH> M;
+template <class F, class M>
+uint64_t launch_tiles(MatvecArgs a, uint64_t tokens, hipStream_t st) {
+    a.tokens = (uint32_t)std::min<uint64_t>(tokens, M::TOKENS);
     const uint64_t tiles = (a.rows + M::ROWS - 1) / M::ROWS;
-    const Shape<M> sh(tiles, turns_of<M>(a.cols), TILE_WAVES, T);
+    const uint32_t turns = turns_of<M>(a.cols);
+    const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
     a.ksplit = sh.ksplit;
-    a.chunk = sh.chunk;
+    a.chunk = sh.chunk<M>(turns);
     for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * sh.groups) {
         const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + sh.groups - 1) / sh.groups));
-        matvec_tiles<F, T, CH><<<grid, TILE_THREADS, sh.bytes, st>>>(a);
-    }
-}
-
-// Digits of x for codes: 32 bits, or 16 where both x and y are 16-bit floats.
-bool short_digits(uint32_t x_kind, uint32_t y_kind) { return x_kind != EK_F32 && y_kind != EK_F32; }
-
-// At most four tokens in one launch.  Returns the tokens taken.
-template <class F>
-uint64_t launch_few(MatvecArgs a, uint64_t tokens, hipStream_t st) {
-    a.tokens = (uint32_t)std::min<uint64_t>(tokens, 4);
-    if constexpr (is_float_type<F>) {
-        if (a.cols < 8) {
-            matvec_short<F><<<(uint32_t)((a.rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
-        } else if (a.x_kind == EK_BF16) {
-            if (a.tokens == 1) launch_tiles<F, 1, 1>(a, st);
-            else launch_tiles<F, 4, 1>(a, st);
-        } else if (a.x_kind == EK_F16) {
-            if (a.tokens == 1) launch_tiles<F, 1, 2>(a, st);
-            else launch_tiles<F, 4, 2>(a, st);
-        } else {
-            if (a.tokens == 1) launch_tiles<F, 1, 3>(a, st);
-            else launch_tiles<F, 4, 3>(a, st);
-        }
-    } else if (short_digits(a.x_kind, a.y_kind)) {
-        if (a.tokens == 1) launch_tiles<F, 1, 1>(a, st);
-        else launch_tiles<F, 4, 1>(a, st);
-    } else {
-        if (a.tokens == 1) launch_tiles<F, 1, 2>(a, st);
-        else launch_tiles<F, 4, 2>(a, st);
+        matvec_tiles<F, M><<<grid, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
     }
     return a.tokens;
+}
+
+// x is taken to 16 bits below an element, or the largest of 32, where the result is rounded to a 16-bit float anyway.
+bool to_16_bits(uint32_t x_kind, uint32_t y_kind) { return x_kind != EK_F32 && y_kind != EK_F32; }
+
+// One launch over the first of the tokens.  Returns how many it takes.
+template <class F>
+uint64_t launch_some(MatvecArgs a, uint64_t tokens, hipStream_t st) {
+    if constexpr (is_float_type<F>) {
+        if (a.cols < 8) {
+            a.tokens = (uint32_t)std::min<uint64_t>(tokens, 64);
+            matvec_short<F><<<(uint32_t)((a.rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
+            return a.tokens;
+        }
+        if (tokens == 1) {
+            if (a.x_kind == EK_BF16) return launch_tiles<F, FloatTile<F, 1>>(a, 1, st);
+            if (a.x_kind == EK_F16) return launch_tiles<F, FloatTile<F, 2>>(a, 1, st);
+            return launch_tiles<F, FloatTile<F, 3>>(a, 1, st);
+        }
+    } else if (tokens == 1) {
+        return to_16_bits(a.x_kind, a.y_kind) ? launch_tiles<F, CodeTile<F, 1>>(a, 1, st) : launch_tiles<F, CodeTile<F, 2>>(a, 1, st);
+    }
+    if (a.x_kind == EK_BF16) return launch_tiles<F, DenseTile<F, 1>>(a, tokens, st);
+    if (a.x_kind == EK_F16) return launch_tiles<F, DenseTile<F, 2>>(a, tokens, st);
+    return launch_tiles<F, DenseTile<F, 3>>(a, tokens, st);
 }
 
 }  // namespace
@@ -153,14 +154,17 @@ struct MoeSpace {
     }
 };
 
-template <class F, int T, int CH>
+// One: the tile of experts with one token, Many: of the others
+template <class F, class One, class Many>
 void launch_up(MoeArgs a, hipStream_t st) {
-    typedef Tile<F, T, CH> M;
-    const uint32_t tiles = (uint32_t)((a.ff + M::ROWS - 1) / M::ROWS);
-    const Shape<M> sh(2 * (uint64_t)tiles * a.slots, turns_of<M>(a.hidden), TILE_WAVES / 2, T);
+    const uint32_t tiles = (uint32_t)((a.ff + Many::ROWS - 1) / Many::ROWS);
+    static_assert(One::ROWS == Many::ROWS, "one grid for both");
+    const uint32_t one = turns_of<One>(a.hidden), many = turns_of<Many>(a.hidden);
+    const Shape sh(2 * (uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES / 2, std::max(One::X_BYTES, Many::X_BYTES));
     a.ksplit = sh.ksplit;
-    a.chunk = sh.chunk;
-    moe_up<F, T, CH><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, sh.bytes, st>>>(a);
+    a.chunk_one = sh.chunk<One>(one);
+    a.chunk = sh.chunk<Many>(many);
+    moe_up<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
 }
 
 template <class F>
@@ -169,39 +173,39 @@ void launch_up_of(MoeArgs a, hipStream_t st) {
         if (a.hidden < 8) {
             moe_up_short<F><<<dim3((uint32_t)((a.ff + MV_THREADS - 1) / MV_THREADS), a.tokens * a.top_k), MV_THREADS, 0, st>>>(a);
         } else if (a.x_kind == EK_BF16) {
-            launch_up<F, 4, 1>(a, st);
+            launch_up<F, DenseTile<F, 1>, DenseTile<F, 1>>(a, st);
         } else if (a.x_kind == EK_F16) {
-            launch_up<F, 4, 2>(a, st);
+            launch_up<F, DenseTile<F, 2>, DenseTile<F, 2>>(a, st);
         } else {
-            launch_up<F, 4, 3>(a, st);
+            launch_up<F, DenseTile<F, 3>, DenseTile<F, 3>>(a, st);
         }
-    } else if (short_digits(a.x_kind, a.y_kind)) {
-        if (a.tokens == 1) launch_up<F, 1, 1>(a, st);
-        else launch_up<F, 4, 1>(a, st);
+    } else if (a.tokens == 1) {
+        if (to_16_bits(a.x_kind, a.y_kind)) launch_up<F, CodeTile<F, 1>, CodeTile<F, 1>>(a, st);
+        else launch_up<F, CodeTile<F, 2>, CodeTile<F, 2>>(a, st);
     } else {
-        if (a.tokens == 1) launch_up<F, 1, 2>(a, st);
-        else launch_up<F, 4, 2>(a, st);
+        if (a.x_kind == EK_BF16) launch_up<F, CodeTile<F, 2>, DenseTile<F, 1>>(a, st);
+        else if (a.x_kind == EK_F16) launch_up<F, CodeTile<F, 2>, DenseTile<F, 2>>(a, st);
+        else launch_up<F, CodeTile<F, 2>, DenseTile<F, 3>>(a, st);
     }
 }
 
-template <class F, int T, int CH>
+template <class F, class M>
 void launch_down_few(MoeArgs a, hipStream_t st) {
-    typedef Tile<F, T, CH> M;
-    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS);
-    const Shape<M> sh(tiles, turns_of<M>(a.ff) * a.tokens * a.top_k, TILE_WAVES, T);
+    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.ff) * a.tokens * a.top_k;
+    const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
     a.ksplit = sh.ksplit;
-    a.chunk = sh.chunk;
-    moe_down_few<F, T, CH><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes, st>>>(a);
+    a.chunk = sh.chunk<M>(turns);
+    moe_down_few<F, M><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
 }
 
-template <class F, int T, int CH>
+template <class F, class One, class Many>
 void launch_down_many(MoeArgs a, hipStream_t st) {
-    typedef Tile<F, T, CH> M;
-    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS);
-    const Shape<M> sh((uint64_t)tiles * a.slots, turns_of<M>(a.ff), TILE_WAVES, T);
+    const uint32_t tiles = (uint32_t)((a.hidden + Many::ROWS - 1) / Many::ROWS), one = turns_of<One>(a.ff), many = turns_of<Many>(a.ff);
+    const Shape sh((uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES, std::max(One::X_BYTES, Many::X_BYTES));
     a.ksplit = sh.ksplit;
-    a.chunk = sh.chunk;
-    moe_down_many<F, T, CH><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, sh.bytes, st>>>(a);
+    a.chunk_one = sh.chunk<One>(one);
+    a.chunk = sh.chunk<Many>(many);
+    moe_down_many<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
     moe_sum<<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
 }
 
@@ -211,18 +215,18 @@ void launch_down_of(MoeArgs a, hipStream_t st) {
         if (a.ff < 8) {
             moe_down_short<F><<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
         } else if (a.tokens <= 4) {
-            launch_down_few<F, 4, 3>(a, st);
+            launch_down_few<F, DenseTile<F, 3>>(a, st);
         } else {
-            launch_down_many<F, 4, 3>(a, st);
+            launch_down_many<F, DenseTile<F, 3>, DenseTile<F, 3>>(a, st);
         }
-    } else if (short_digits(a.x_kind, a.y_kind)) {
-        if (a.tokens == 1) launch_down_few<F, 1, 1>(a, st);
-        else if (a.tokens <= 4) launch_down_few<F, 4, 1>(a, st);
-        else launch_down_many<F, 4, 1>(a, st);
+    } else if (to_16_bits(a.x_kind, a.y_kind)) {
+        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 1>>(a, st);
+        else if (a.tokens <= 4) launch_down_few<F, DenseTile<F, 2>>(a, st);
+        else launch_down_many<F, CodeTile<F, 1>, DenseTile<F, 2>>(a, st);
     } else {
-        if (a.tokens == 1) launch_down_few<F, 1, 2>(a, st);
-        else if (a.tokens <= 4) launch_down_few<F, 4, 2>(a, st);
-        else launch_down_many<F, 4, 2>(a, st);
+        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 2>>(a, st);
+        else if (a.tokens <= 4) launch_down_few<F, DenseTile<F, 3>>(a, st);
+        else launch_down_many<F, CodeTile<F, 2>, DenseTile<F, 3>>(a, st);
     }
 }
 
@@ -257,7 +261,7 @@ ggq_status ggq_matvec_device(uint32_t ty, uint64_t rows, uint64_t cols, const vo
             fill_zero<<<(uint32_t)((rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
             continue;
         }
-#define CASE(F) done = launch_few<F>(a, tokens - t, st)
+#define CASE(F) done = launch_some<F>(a, tokens - t, st)
         GGQ_FOR_TYPE(ty, CASE)
 #undef CASE
     }
@@ -351,9 +355,9 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     hipStream_t st = (hipStream_t)hip_stream;
     moe_logits<<<m->experts, MV_THREADS, 0, st>>>(a);
     moe_route<<<(uint32_t)tokens, 64, 0, st>>>(a);
-    // groups of up to four pairs with the same expert: one for each pair, or one for each expert and one more for each four pairs
+    // groups of up to 16 pairs with the same expert: one for each pair, or one for each expert and one more for each 16 pairs
     const uint32_t pairs = (uint32_t)tokens * m->top_k, in_use = std::min(m->experts, pairs);
-    a.slots = std::min(pairs, in_use + (pairs - in_use) / 4);
+    a.slots = std::min(pairs, in_use + (pairs - in_use) / SLOT_TOKENS);
 #define CASE(F) launch_up_of<F>(a, st)
     GGQ_FOR_TYPE(m->up_type, CASE)
 #undef CASE

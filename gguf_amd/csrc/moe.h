@@ -3,10 +3,10 @@
 //     l = router x;  the top_k experts of each token;  h_e = act(gate_e x) * (up_e x);  y = sum of w_e down_e h_e
 //
 // The launches: logits, choice, gate and up of the experts in use, down with the sum over a token's experts (for more than
-// four tokens down and the sum apart).  Bound by the bytes of the experts in use: each is read once for up to four of its
-// tokens, and once more for each further four.
+// four tokens down and the sum apart).  Bound by the bytes of the experts in use: each is read once for up to 16 of its
+// tokens, and once more for each further 16.
 #pragma once
-#include "matmul.h"
+#include "dense.h"
 
 namespace ggq {
 
@@ -24,7 +24,7 @@ struct MoeArgs {
     uint64_t hidden, ff, x_stride, y_stride;
     uint32_t tokens, experts, top_k, router_kind, x_kind, y_kind;
     uint32_t sigmoid, normalize, gelu;
-    uint32_t chunk, ksplit;                   // as in MatvecArgs, of the launch
+    uint32_t ksplit, chunk, chunk_one;        // as in MatvecArgs, of the launch; chunk_one: of experts with one token
     uint32_t slots;                           // most slots there may be: workgroups along y
     float scale;
 };
@@ -128,13 +128,14 @@ __device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
 
 
 // ---- which expert, and which tokens ----------------------------------------------------------------------
-// Experts in use, in the order of their index, each with its tokens four at a time: a slot is one such group.
+// Experts in use, in the order of their index, each with its tokens 16 at a time: a slot is one such group.
+constexpr uint32_t SLOT_TOKENS = 16;
 struct Slot {
     uint32_t expert, count;       // of tokens; 0: no such slot
 };
 struct SlotSpace {
     uint32_t low[MOE_MAX_EXPERTS], high[MOE_MAX_EXPERTS];         // masks of tokens, by expert
-    uint32_t pair[4];             // of the slot's tokens: token * top_k + place
+    uint32_t pair[SLOT_TOKENS];             // of the slot's tokens: token * top_k + place
 };
 __device__ __forceinline__ uint32_t nth_bit(uint64_t m, uint32_t n) {
     for (; n; --n) m &= m - 1;
@@ -153,7 +154,7 @@ __device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, uint32
     uint32_t seen = 0, expert = 0, count = 0;
     for (uint32_t base = 0; base < a.experts; base += 64) {
         const uint32_t e = base + lane;
-        const uint32_t tokens = e < a.experts ? (uint32_t)__popc(s.low[e]) + (uint32_t)__popc(s.high[e]) : 0u, mine = (tokens + 3) / 4;
+        const uint32_t tokens = e < a.experts ? (uint32_t)__popc(s.low[e]) + (uint32_t)__popc(s.high[e]) : 0u, mine = (tokens + SLOT_TOKENS - 1) / SLOT_TOKENS;
         uint32_t upto = mine;                                     // slots of the lanes up to this one
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -167,10 +168,10 @@ __device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, uint32
             expert = base + l;
             const uint32_t low = __builtin_amdgcn_readfirstlane(s.low[expert]), high = __builtin_amdgcn_readfirstlane(s.high[expert]);
             const uint64_t mask = low | ((uint64_t)high << 32);
-            const uint32_t n = (uint32_t)__popcll(mask) - group * 4;
-            count = n < 4 ? n : 4;
+            const uint32_t n = (uint32_t)__popcll(mask) - group * SLOT_TOKENS;
+            count = n < SLOT_TOKENS ? n : SLOT_TOKENS;
             if (threadIdx.x < count) {
-                const uint32_t first = nth_bit(mask, group * 4 + threadIdx.x) * a.top_k;
+                const uint32_t first = nth_bit(mask, group * SLOT_TOKENS + threadIdx.x) * a.top_k;
                 uint32_t pair = first;
                 for (uint32_t j = 0; j < a.top_k; ++j) pair = (uint32_t)a.ids[first + j] == expert ? first + j : pair;
                 s.pair[threadIdx.x] = pair;
@@ -184,15 +185,10 @@ __device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, uint32
 }
 
 // ---- gate and up ----------------------------------------------------------------------------------------
-// As matvec_tiles; half of a workgroup's waves take gate's rows, the others the same rows of up.  Grid: (row groups, slots).
-template <class F, int T, int CH>
-__global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ SlotSpace space;
-    typedef Tile<F, T, CH> M;
+// As matvec_tiles; half of a workgroup's waves take gate's rows, the others the same rows of up.
+template <class F, class M>
+__device__ __forceinline__ void up_rows(const MoeArgs &a, uint8_t *lds, const Slot &slot, const uint32_t *pair, uint32_t chunk) {
     typedef typename M::I I;
-    const Slot slot = find_slot(space, a, blockIdx.y);
-    if (slot.count == 0) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t second = wave / (TILE_WAVES / 2), group = wave % (TILE_WAVES / 2) / a.ksplit, groups = TILE_WAVES / 2 / a.ksplit;
     const uint32_t row_bytes = (uint32_t)(a.hidden / F::N * F::BYTES), turns = (uint32_t)((a.hidden + M::ELEMS - 1) / M::ELEMS);
@@ -200,41 +196,55 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
     const uint32_t rows = ff - own < M::ROWS ? ff - own : M::ROWS;
     const uint8_t *w = (second ? a.up : a.gate) + ((uint64_t)slot.expert * ff + own) * row_bytes;
     const uint64_t behind = ((uint64_t)(a.experts - slot.expert) * ff - own - 1) * row_bytes;
-    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;
     typename M::Sums acc = no_sums<M>();
-    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
-                 Share{wave % a.ksplit, a.ksplit, a.chunk, turns, slot.count},
+    run_turns<M>(lds + wave * M::WAVE_BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
+                 Share{wave % a.ksplit, a.ksplit, chunk, turns, slot.count},
                  [&](uint32_t turn) {
                      const uint32_t off = turn * I::TURN_BYTES;
                      return Turn{w + off, row_bytes - off, behind + row_bytes - off};
                  },
                  [&](uint32_t turn, uint32_t t, uint32_t c, float (&v)[8]) {
-                     load8(a.x, space.pair[t] / a.top_k * a.x_stride, (uint64_t)turn * M::ELEMS + c, a.hidden, a.x_kind, v);
+                     load8(a.x, pair[t] / a.top_k * a.x_stride, (uint64_t)turn * M::ELEMS + c, a.hidden, a.x_kind, v);
                  },
                  acc);
     float *part = (float *)(clear + M::CLEAR);
-    put_parts<M, T>(part, wave, acc);
+    put_parts<M>(part, wave, acc);
     for (uint32_t i = threadIdx.x; i < groups * M::ROWS * slot.count; i += TILE_THREADS) {
         const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
         float v[2] = {0.0f, 0.0f};
         for (uint32_t k = 0; k < a.ksplit; ++k)
 #pragma unroll
-            for (uint32_t m = 0; m < 2; ++m) v[m] += part[((m * TILE_WAVES / 2 + g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
-        if (first_row + r < ff) a.h[(uint64_t)space.pair[t] * ff + first_row + r] = moe_act(v[0], a.gelu) * v[1];
+            for (uint32_t m = 0; m < 2; ++m) v[m] += part[((m * TILE_WAVES / 2 + g * a.ksplit + k) * M::TOKENS + t) * M::ROWS + r % M::ROWS];
+        if (first_row + r < ff) a.h[(uint64_t)pair[t] * ff + first_row + r] = moe_act(v[0], a.gelu) * v[1];
     }
+}
+// Grid: (row groups, slots).  One: the tile of experts with one token, Many: of the others.
+template <class F, class One, class Many>
+__global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ SlotSpace space;
+    const Slot slot = find_slot(space, a, blockIdx.y);
+    if (slot.count == 0) return;
+    if constexpr (!__is_same(One, Many)) {
+        if (slot.count == 1) {
+            up_rows<F, One>(a, lds, slot, space.pair, a.chunk_one);
+            return;
+        }
+    }
+    up_rows<F, Many>(a, lds, slot, space.pair, a.chunk);
 }
 
 // ---- down -----------------------------------------------------------------------------------------------
-// Up to T tokens: the rows of all experts in use, one behind the other, are one long row times the tokens' h, each times
+// Up to four tokens: the rows of all experts in use, one behind the other, are one long row times the tokens' h, each times
 // its weight (0 for a token that did not choose the expert); the sum over a token's experts is the sum over the row.
-template <class F, int T, int CH>
+template <class F, class M>
 __global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ uint32_t items[4 * MOE_MAX_TOP_K];          // experts in use, in the order of their first pair
     __shared__ int32_t pair_at[4 * MOE_MAX_TOP_K][4];      // the pair of item and token, or -1
     __shared__ int32_t ids[4 * MOE_MAX_TOP_K];
     __shared__ uint64_t fresh_of[2];
-    typedef Tile<F, T, CH> M;
     typedef typename M::I I;
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t pairs = a.tokens * a.top_k, me_pair = threadIdx.x;      // at most 128: the first two waves
@@ -262,9 +272,9 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), each = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
     const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS, own = row < hidden ? row : hidden - 1;
     const uint32_t rows = hidden - own < M::ROWS ? hidden - own : M::ROWS;
-    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;
     typename M::Sums acc = no_sums<M>();
-    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes),
+    run_turns<M>(lds + wave * M::WAVE_BYTES, clear, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes),
                  Share{wave % a.ksplit, a.ksplit, a.chunk, each * count, a.tokens},
                  [&](uint32_t turn) {
                      const uint32_t item = turn / each, off = (turn - item * each) * I::TURN_BYTES;
@@ -282,24 +292,19 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
                  },
                  acc);
     float *part = (float *)(clear + M::CLEAR);
-    put_parts<M, T>(part, wave, acc);
+    put_parts<M>(part, wave, acc);
     for (uint32_t i = threadIdx.x; i < groups * M::ROWS * a.tokens; i += TILE_THREADS) {
         const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
+        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * M::TOKENS + t) * M::ROWS + r % M::ROWS];
         if (first_row + r < hidden) store_elem(a.y, t * a.y_stride + first_row + r, a.y_kind, v);
     }
 }
 
-// More tokens: expert by expert, up to T of its tokens at a time, into o[pair]; grid: (row groups, slots).
-template <class F, int T, int CH>
-__global__ __launch_bounds__(TILE_THREADS) void moe_down_many(MoeArgs a) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ SlotSpace space;
-    typedef Tile<F, T, CH> M;
+// More tokens: expert by expert, into o[pair]; grid: (row groups, slots).
+template <class F, class M>
+__device__ __forceinline__ void down_rows(const MoeArgs &a, uint8_t *lds, const Slot &slot, const uint32_t *pair, uint32_t chunk) {
     typedef typename M::I I;
-    const Slot slot = find_slot(space, a, blockIdx.y);
-    if (slot.count == 0) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t group = wave / a.ksplit, groups = TILE_WAVES / a.ksplit;
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), turns = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
@@ -307,26 +312,40 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_many(MoeArgs a) {
     const uint32_t rows = hidden - own < M::ROWS ? hidden - own : M::ROWS;
     const uint8_t *w = a.down + ((uint64_t)slot.expert * hidden + own) * row_bytes;
     const uint64_t behind = ((uint64_t)(a.experts - slot.expert) * hidden - own - 1) * row_bytes;
-    uint8_t *clear = lds + TILE_WAVES * I::BYTES;
+    uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;
     typename M::Sums acc = no_sums<M>();
-    run_turns<M>(lds + wave * I::BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
-                 Share{wave % a.ksplit, a.ksplit, a.chunk, turns, slot.count},
+    run_turns<M>(lds + wave * M::WAVE_BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
+                 Share{wave % a.ksplit, a.ksplit, chunk, turns, slot.count},
                  [&](uint32_t turn) {
                      const uint32_t off = turn * I::TURN_BYTES;
                      return Turn{w + off, row_bytes - off, behind + row_bytes - off};
                  },
                  [&](uint32_t turn, uint32_t t, uint32_t c, float (&v)[8]) {
-                     load8(a.h, space.pair[t] * a.ff, (uint64_t)turn * M::ELEMS + c, a.ff, EK_F32, v);
+                     load8(a.h, pair[t] * a.ff, (uint64_t)turn * M::ELEMS + c, a.ff, EK_F32, v);
                  },
                  acc);
     float *part = (float *)(clear + M::CLEAR);
-    put_parts<M, T>(part, wave, acc);
+    put_parts<M>(part, wave, acc);
     for (uint32_t i = threadIdx.x; i < groups * M::ROWS * slot.count; i += TILE_THREADS) {
         const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * T + t) * M::ROWS + r % M::ROWS];
-        if (first_row + r < hidden) a.o[(uint64_t)space.pair[t] * hidden + first_row + r] = v;
+        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * M::TOKENS + t) * M::ROWS + r % M::ROWS];
+        if (first_row + r < hidden) a.o[(uint64_t)pair[t] * hidden + first_row + r] = v;
     }
+}
+template <class F, class One, class Many>
+__global__ __launch_bounds__(TILE_THREADS) void moe_down_many(MoeArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    __shared__ SlotSpace space;
+    const Slot slot = find_slot(space, a, blockIdx.y);
+    if (slot.count == 0) return;
+    if constexpr (!__is_same(One, Many)) {
+        if (slot.count == 1) {
+            down_rows<F, One>(a, lds, slot, space.pair, a.chunk_one);
+            return;
+        }
+    }
+    down_rows<F, Many>(a, lds, slot, space.pair, a.chunk);
 }
 // ... and the sum over a token's experts, in order
 __global__ __launch_bounds__(MV_THREADS) static void moe_sum(MoeArgs a) {

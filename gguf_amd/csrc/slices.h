@@ -18,9 +18,9 @@
 //     HIGH            codes have a second plane
 //     STEP            packed bytes of a step
 //     TURN            steps that a wave takes at a time
-//     UNIT, UNITS     the bytes of a row's turn come into shared memory as UNITS pieces of UNIT bytes, each at a 16-byte
-//                     aligned place: whole blocks of the 256-element formats, so that their parts can be read with wide
-//                     aligned loads; everything at once for the others, whose slices are whole words
+//     BLOCKS          the steps of a turn come into shared memory at 16-byte aligned places, each a block of a 256-element
+//                     format, whose parts can then be read with wide aligned loads; otherwise a turn is one run of bytes,
+//                     whose slices are whole words
 //     Raw             the packed bytes of slice g of a step in registers; load(row, step, g, left): from the row's image in
 //                     shared memory, `left` bytes of the row from this turn on.  Blocks behind the row's end hold anything
 //                     there: they get the scale 0
@@ -84,7 +84,8 @@ template <uint32_t B, uint32_t T>
 struct SliceOfTwo {
     static constexpr bool PLANES = false;
     static constexpr int NSUB = 2, SUB = 32;
-    static constexpr uint32_t STEP = 8 * B, TURN = T, UNIT = STEP * T, UNITS = 1;
+    static constexpr uint32_t STEP = 8 * B, TURN = T;
+    static constexpr bool BLOCKS = false;
     GGQ_EXP(LOW_EXP, 9);
     GGQ_EXP(HIGH_EXP, 13);
     struct Raw {
@@ -192,7 +193,8 @@ template <> struct Slice<IQ4NL> : SliceOfTwo<18, 2> {
 // ---- 256-element formats: a block is a step, a lane's slice a quarter of it ----------------------------------
 template <uint32_t B, uint32_t T>
 struct SliceOfQuarter {
-    static constexpr uint32_t STEP = B, TURN = T, UNIT = B, UNITS = T;
+    static constexpr uint32_t STEP = B, TURN = T;
+    static constexpr bool BLOCKS = true;
     GGQ_EXP(LOW_EXP, 9);
     GGQ_EXP(HIGH_EXP, 13);
     // the block's image and whether there is such a block
@@ -412,7 +414,7 @@ template <> struct Slice<Q3K> : SliceOfPlanes<110, 2> {
     GGQ_LOW(4) {
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            b[i] = ((r.q[i] >> (2 * S)) & 0x03030303u) | ((S <= 2 ? r.f[i] << (2 - S) : r.f[i] >> (S - 2)) & 0x04040404u);
+            b[i] = ((r.q[i] >> (2 * S)) & 0x03030303u) | ((S == 3 ? r.f[i] >> 1 : r.f[i] << (S == 3 ? 0 : 2 - S)) & 0x04040404u);
     }
     GGQ_SCALE {
         const uint32_t sc = ((r.lo >> (8 * S)) & 0xFu) | (((r.hi >> (16 * (S & 1) + 2 * (S >> 1))) & 3u) << 4);
@@ -424,13 +426,14 @@ template <> struct Slice<Q3K> : SliceOfPlanes<110, 2> {
 // ---- 16-bit floats: rows of any length; a lane takes 64 elements ---------------------------------------------
 // The weights are their own codes, in bf16; a half has eleven significant bits and becomes two of them (WP pieces).
 struct SliceOfFloats {
-    static constexpr uint32_t STEP = 2048, TURN = 1, UNIT = STEP, UNITS = 1;      // a step of 16 slices
+    static constexpr uint32_t STEP = 512, TURN = 4;       // a turn of 16 slices
+    static constexpr bool BLOCKS = false;
     struct Raw {
         u32x4 q[8];
         __device__ __forceinline__ void load(const uint8_t *row, uint32_t quad, uint32_t left) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) q[i] = al16(row + 128 * quad + 16 * i);
-            if (left < STEP) {       // what lies behind the row may be anything, an infinity too
+            if (left < STEP * TURN) {      // what lies behind the row may be anything, an infinity too
                 const uint32_t n = left > 128 * quad ? (left - 128 * quad) / 2 : 0;
 #pragma unroll
                 for (uint32_t i = 0; i < 32; ++i) q[i / 4][i % 4] &= 2 * i + 1 < n ? ~0u : 2 * i < n ? 0xFFFFu : 0u;
