@@ -59,7 +59,7 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
 }
 
 // Shared memory of one workgroup for x, beside its waves' images.
-constexpr uint32_t X_LDS = 40 << 10;
+constexpr uint32_t X_LDS = 64 << 10;
 
 // The shape of a launch over `tiles` wave tiles, each of which takes `turns` turns: how many waves share a tile's turns,
 // the turns staged at a time (equal chunks, whole rounds of the waves), the shared memory.
@@ -125,6 +125,9 @@ uint64_t launch_some(MatvecArgs a, uint64_t tokens, hipStream_t st) {
 
 // ---- mixture of experts ---------------------------------------------------------------------------------
 namespace {
+
+// rows of 16-bit floats that are shorter than a piece of an image
+bool short_rows(uint32_t type, uint64_t cols) { return (type == GGQ_TYPE_F16 || type == GGQ_TYPE_BF16) && cols < 8; }
 
 uint64_t up256(uint64_t v) { return (v + 255) & ~255ull; }
 
@@ -353,8 +356,10 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     a.gelu = m->activation;
     a.scale = m->scale;
     hipStream_t st = (hipStream_t)hip_stream;
-    moe_logits<<<m->experts, MV_THREADS, 0, st>>>(a);
-    moe_route<<<(uint32_t)tokens, 64, 0, st>>>(a);
+    moe_logits<<<dim3(m->experts, ((uint32_t)tokens + LOGIT_TOKENS - 1) / LOGIT_TOKENS), MV_THREADS, 0, st>>>(a);
+    // Comparing each expert with each is on every workgroup's way; the launch that it saves takes about 2.5 us.
+    a.choose = tokens <= CHOOSE_TOKENS && m->experts <= 128 && !short_rows(m->up_type, m->hidden);
+    if (!a.choose) moe_route<<<(uint32_t)tokens, MV_THREADS, 0, st>>>(a);
     // groups of up to 16 pairs with the same expert: one for each pair, or one for each expert and one more for each 16 pairs
     const uint32_t pairs = (uint32_t)tokens * m->top_k, in_use = std::min(m->experts, pairs);
     a.slots = std::min(pairs, in_use + (pairs - in_use) / SLOT_TOKENS);

@@ -2,8 +2,8 @@
 //
 //     l = router x;  the top_k experts of each token;  h_e = act(gate_e x) * (up_e x);  y = sum of w_e down_e h_e
 //
-// The launches: logits, choice, gate and up of the experts in use, down with the sum over a token's experts (for more than
-// four tokens down and the sum apart).  Bound by the bytes of the experts in use: each is read once for up to 16 of its
+// The launches: logits; the choice, where it is not found on the way; gate and up of the experts in use; down with the sum
+// over a token's experts (for more than four tokens down and the sum apart).  Bound by the bytes of the experts in use: each is read once for up to 16 of its
 // tokens, and once more for each further 16.
 #pragma once
 #include "dense.h"
@@ -25,33 +25,64 @@ struct MoeArgs {
     uint32_t tokens, experts, top_k, router_kind, x_kind, y_kind;
     uint32_t sigmoid, normalize, gelu;
     uint32_t ksplit, chunk, chunk_one;        // as in MatvecArgs, of the launch; chunk_one: of experts with one token
+    uint32_t choose;                          // the workgroups of gate and up find the choice themselves
     uint32_t slots;                           // most slots there may be: workgroups along y
     float scale;
 };
 
-__device__ __forceinline__ double wave_sum(double v) {
+// ---- logits ---------------------------------------------------------------------------------------------
+// four elements from c on, 0 past the end
+__device__ __forceinline__ void load4(const void *p, uint64_t at, uint32_t c, uint32_t n, uint32_t kind, float (&v)[4]) {
+    if (c + 4 <= n && kind == EK_F32) {
+        const f32x4 a = __builtin_bit_cast(f32x4, ld16((const uint8_t *)p + 4 * (at + c)));
 #pragma unroll
-    for (int m = 32; m; m >>= 1) v += __shfl_xor(v, m);
-    return v;
-}
-
-// one workgroup per expert; a product of two f32 values is exact in 64 bits
-__global__ __launch_bounds__(MV_THREADS) static void moe_logits(MoeArgs a) {
-    __shared__ double part[MV_THREADS / 64];
-    const uint32_t e = blockIdx.x;
-    for (uint32_t t = 0; t < a.tokens; ++t) {
-        double s = 0.0;
-        for (uint64_t c = threadIdx.x; c < a.hidden; c += MV_THREADS)
-            s = __builtin_fma((double)load_elem(a.router, e * a.hidden + c, a.router_kind), (double)load_elem(a.x, t * a.x_stride + c, a.x_kind), s);
-        s = wave_sum(s);
-        if (threadIdx.x % 64 == 0) part[threadIdx.x / 64] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (uint32_t w = 1; w < MV_THREADS / 64; ++w) s += part[w];
-            a.logits[(uint64_t)t * a.experts + e] = (float)s;
-        }
-        __syncthreads();
+        for (int i = 0; i < 4; ++i) v[i] = a[i];
+    } else if (c + 4 <= n) {
+        const uint8_t *q = (const uint8_t *)p + 2 * (at + c);
+        const uint32_t a = ld4(q), b = ld4(q + 4);
+        v[0] = kind == EK_F16 ? h2f(a & 0xFFFFu) : bf2f(a & 0xFFFFu);
+        v[1] = kind == EK_F16 ? h2f(a >> 16) : bf2f(a >> 16);
+        v[2] = kind == EK_F16 ? h2f(b & 0xFFFFu) : bf2f(b & 0xFFFFu);
+        v[3] = kind == EK_F16 ? h2f(b >> 16) : bf2f(b >> 16);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = c + i < n ? load_elem(p, at + c + i, kind) : 0.0f;
     }
+}
+// One expert and four tokens a workgroup; grid: (experts, tokens / 4).  The choice hangs on the order of the logits, so
+// products (exact in 64 bits) are summed in 64 bits and rounded once.  Bound by its latency: 4 KiB of the router are on the
+// way at once in each workgroup, and the token's x with them.
+constexpr uint32_t LOGIT_TOKENS = 4;
+__global__ __launch_bounds__(MV_THREADS) static void moe_logits(MoeArgs a) {
+    __shared__ double part[LOGIT_TOKENS][MV_THREADS];
+    const uint32_t e = blockIdx.x, first = blockIdx.y * LOGIT_TOKENS, n = (uint32_t)a.hidden;
+    const uint32_t tokens = a.tokens - first < LOGIT_TOKENS ? a.tokens - first : LOGIT_TOKENS;
+    double sum[LOGIT_TOKENS] = {0.0, 0.0, 0.0, 0.0};
+    for (uint32_t c = threadIdx.x * 4; c < n; c += MV_THREADS * 16) {
+        float w[4][4];
+#pragma unroll
+        for (uint32_t k = 0; k < 4; ++k) load4(a.router, e * a.hidden, c + k * MV_THREADS * 4, n, a.router_kind, w[k]);
+#pragma unroll
+        for (uint32_t t = 0; t < LOGIT_TOKENS; ++t) {
+            if (t >= tokens) break;
+            float x[4][4];
+#pragma unroll
+            for (uint32_t k = 0; k < 4; ++k) load4(a.x, (first + t) * a.x_stride, c + k * MV_THREADS * 4, n, a.x_kind, x[k]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) sum[t] = __builtin_fma((double)w[k][i], (double)x[k][i], sum[t]);
+        }
+    }
+#pragma unroll
+    for (uint32_t t = 0; t < LOGIT_TOKENS; ++t) part[t][threadIdx.x] = sum[t];
+    __syncthreads();
+    const uint32_t t = threadIdx.x / 64, lane = threadIdx.x % 64;         // a wave for each token
+    if (t >= tokens) return;
+    double s = (part[t][lane] + part[t][lane + 64]) + (part[t][lane + 128] + part[t][lane + 192]);
+#pragma unroll
+    for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m);
+    if (lane == 0) a.logits[(uint64_t)(first + t) * a.experts + e] = (float)s;
 }
 
 // an order-preserving key of a logit: larger logit, larger key; NaN below everything; -0 equals +0
@@ -63,17 +94,22 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 
 // ---- the choice -----------------------------------------------------------------------------------------
 constexpr uint32_t MOE_MAX_EXPERTS = 512, MOE_MAX_TOP_K = 32, MOE_MAX_TOKENS = 64;
+constexpr uint32_t CHOOSE_TOKENS = 8;         // most tokens whose choice the workgroups of gate and up find themselves
 
-// One wave: the top_k experts of a token, ids[j] = the j-th.  An expert's place is the number of experts in front of it
-// (a larger key, or the same and a lower index), so all places are found at once, without a chain of k maxima; keys are
-// read four at a time, the same for all lanes.  `keys`: the wave's own, room for 512.
-__device__ __forceinline__ void choose(const float *logits, uint32_t experts, uint32_t top_k, uint32_t lane, uint32_t *keys, int32_t *ids) {
+// The top_k experts of a token, ids[j] = the j-th.  An expert's place is the number of experts in front of it (a larger key,
+// or the same and a lower index), so all places are found at once, without a chain of k maxima; keys are read four at a
+// time, the same for all lanes.  Threads `me`, me + threads, ... of `threads` share the work; `keys`: theirs, room for 512;
+// order(): what makes their writes to shared memory seen.
+template <class Order>
+__device__ __forceinline__ void choose(const float *logits, uint32_t experts, uint32_t top_k, uint32_t me, uint32_t threads, uint32_t *keys, int32_t *ids,
+                                       Order order) {
     const uint32_t padded = (experts + 3) & ~3u;
-    for (uint32_t e = lane; e < padded; e += 64) keys[e] = e < experts ? logit_key(logits[e]) : 0u;
-    wave_order();
-    for (uint32_t e = lane; e < experts; e += 64) {
+    for (uint32_t e = me; e < padded; e += threads) keys[e] = e < experts ? logit_key(logits[e]) : 0u;
+    order();
+    for (uint32_t e = me; e < experts; e += threads) {
         const uint32_t key = keys[e];
         uint32_t place = 0;
+#pragma unroll 4
         for (uint32_t q = 0; q < padded; q += 4) {
             const u32x4 k = *(const u32x4 *)(keys + q);
 #pragma unroll
@@ -81,43 +117,58 @@ __device__ __forceinline__ void choose(const float *logits, uint32_t experts, ui
         }
         if (place < top_k) ids[place] = (int32_t)e;
     }
-    wave_order();
+    order();
 }
 
-// One wave: the weights of a token's chosen experts, weight j in lane j.
-__device__ __forceinline__ float choice_weight(const float *l, const MoeArgs &a, const int32_t *ids, uint32_t lane) {
+__device__ __forceinline__ float wave_max(float v) {
+    v = __builtin_fmaxf(v, dpp<QUAD_XOR1>(v));
+    v = __builtin_fmaxf(v, dpp<QUAD_XOR2>(v));
+    v = __builtin_fmaxf(v, dpp<ROW_ROR4>(v));
+    v = __builtin_fmaxf(v, dpp<ROW_ROR8>(v));
+    v = __builtin_fmaxf(v, __shfl_xor(v, 16));
+    return __builtin_fmaxf(v, __shfl_xor(v, 32));
+}
+__device__ __forceinline__ float wave_total(float v) {
+    v += dpp<QUAD_XOR1>(v);
+    v += dpp<QUAD_XOR2>(v);
+    v += dpp<ROW_ROR4>(v);
+    v += dpp<ROW_ROR8>(v);
+    v += __shfl_xor(v, 16);
+    return v + __shfl_xor(v, 32);
+}
+// One wave: the choice of token t and its weights to the workspace and to the caller.
+__device__ __forceinline__ void put_choice(const MoeArgs &a, uint32_t t, const int32_t *ids, uint32_t lane) {
+    const float *l = a.logits + (uint64_t)t * a.experts;
     float top = -__builtin_inff(), total = 0.0f;
     if (!a.sigmoid) {
         for (uint32_t e = lane; e < a.experts; e += 64) top = __builtin_fmaxf(top, l[e]);
-#pragma unroll
-        for (int m = 32; m; m >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, m));
+        top = wave_max(top);
         for (uint32_t e = lane; e < a.experts; e += 64) total += expf(l[e] - top);
-        total = wave_sum(total);
+        total = wave_total(total);
     }
-    float mine = 0.0f;
+    float p = 0.0f;
     if (lane < a.top_k) {
         const float v = l[ids[lane]];
-        mine = a.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) / total;
+        p = a.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) / total;
     }
-    const float sum = wave_sum(mine);
-    return (a.normalize ? mine / sum : mine) * a.scale;
-}
-
-// The choice of all tokens, a wave per token; `out`: what the caller gets as well
-__global__ __launch_bounds__(64) static void moe_route(MoeArgs a) {
-    __shared__ uint32_t keys[MOE_MAX_EXPERTS];
-    __shared__ int32_t ids[MOE_MAX_TOP_K];
-    const uint32_t t = blockIdx.x, lane = threadIdx.x;
-    const float *l = a.logits + (uint64_t)t * a.experts;
-    choose(l, a.experts, a.top_k, lane, keys, ids);
-    const float w = choice_weight(l, a, ids, lane);
+    const float sum = wave_total(p);
     if (lane < a.top_k) {
         const uint32_t at = t * a.top_k + lane;
+        const float w = (a.normalize ? p / sum : p) * a.scale;
         a.ids[at] = ids[lane];
         a.weights[at] = w;
         if (a.out_ids) a.out_ids[at] = ids[lane];
         if (a.out_weights) a.out_weights[at] = w;
     }
+}
+
+// The choice of all tokens, a workgroup for each
+__global__ __launch_bounds__(MV_THREADS) static void moe_route(MoeArgs a) {
+    __shared__ uint32_t keys[MOE_MAX_EXPERTS];
+    __shared__ int32_t ids[MOE_MAX_TOP_K];
+    const uint32_t t = blockIdx.x;
+    choose(a.logits + (uint64_t)t * a.experts, a.experts, a.top_k, threadIdx.x, MV_THREADS, keys, ids, [] { __syncthreads(); });
+    if (threadIdx.x < 64) put_choice(a, t, ids, threadIdx.x);
 }
 
 __device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
@@ -135,20 +186,20 @@ struct Slot {
 };
 struct SlotSpace {
     uint32_t low[MOE_MAX_EXPERTS], high[MOE_MAX_EXPERTS];         // masks of tokens, by expert
-    uint32_t pair[SLOT_TOKENS];             // of the slot's tokens: token * top_k + place
+    uint32_t pair[SLOT_TOKENS];   // of the slot's tokens: token * top_k + place
 };
 __device__ __forceinline__ uint32_t nth_bit(uint64_t m, uint32_t n) {
     for (; n; --n) m &= m - 1;
     return (uint32_t)__builtin_ctzll(m);
 }
-// All threads of the workgroup, of 64 lanes or more; ids: the choices of all tokens.  The same answer in all of them.
-__device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, uint32_t slot) {
+// All threads of the workgroup; ids: the choices of all tokens.  The same answer in all of them.
+__device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, const int32_t *ids, uint32_t slot) {
     const uint32_t lane = threadIdx.x % 64;
     for (uint32_t e = threadIdx.x; e < a.experts; e += blockDim.x) s.low[e] = s.high[e] = 0;
     __syncthreads();
     for (uint32_t p = threadIdx.x; p < a.tokens * a.top_k; p += blockDim.x) {
         const uint32_t t = p / a.top_k;
-        atomicOr(t < 32 ? &s.low[a.ids[p]] : &s.high[a.ids[p]], 1u << (t & 31));
+        atomicOr(t < 32 ? &s.low[ids[p]] : &s.high[ids[p]], 1u << (t & 31));
     }
     __syncthreads();
     uint32_t seen = 0, expert = 0, count = 0;
@@ -173,7 +224,7 @@ __device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, uint32
             if (threadIdx.x < count) {
                 const uint32_t first = nth_bit(mask, group * SLOT_TOKENS + threadIdx.x) * a.top_k;
                 uint32_t pair = first;
-                for (uint32_t j = 0; j < a.top_k; ++j) pair = (uint32_t)a.ids[first + j] == expert ? first + j : pair;
+                for (uint32_t j = 0; j < a.top_k; ++j) pair = (uint32_t)ids[first + j] == expert ? first + j : pair;
                 s.pair[threadIdx.x] = pair;
             }
             break;
@@ -224,7 +275,21 @@ template <class F, class One, class Many>
 __global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ SlotSpace space;
-    const Slot slot = find_slot(space, a, blockIdx.y);
+    const int32_t *ids = a.ids;
+    if (a.choose) {
+        // few tokens and experts: each workgroup finds the choice by itself, a wave for each token, which costs it less than
+        // one more launch; one workgroup hands it on
+        __shared__ int32_t chosen[CHOOSE_TOKENS * MOE_MAX_TOP_K];
+        const uint32_t t = threadIdx.x / 64, lane = threadIdx.x % 64;
+        uint32_t *keys = (uint32_t *)lds + t * MOE_MAX_EXPERTS;
+        if (t < a.tokens) {
+            choose(a.logits + (uint64_t)t * a.experts, a.experts, a.top_k, lane, 64, keys, chosen + t * a.top_k, [] { wave_order(); });
+            if (blockIdx.x == 0 && blockIdx.y == 0) put_choice(a, t, chosen + t * a.top_k, lane);
+        }
+        ids = chosen;
+        __syncthreads();
+    }
+    const Slot slot = find_slot(space, a, ids, blockIdx.y);
     if (slot.count == 0) return;
     if constexpr (!__is_same(One, Many)) {
         if (slot.count == 1) {
@@ -337,7 +402,7 @@ template <class F, class One, class Many>
 __global__ __launch_bounds__(TILE_THREADS) void moe_down_many(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     __shared__ SlotSpace space;
-    const Slot slot = find_slot(space, a, blockIdx.y);
+    const Slot slot = find_slot(space, a, a.ids, blockIdx.y);
     if (slot.count == 0) return;
     if constexpr (!__is_same(One, Many)) {
         if (slot.count == 1) {
