@@ -53,6 +53,8 @@ constexpr uint64_t MAX_DIM = 1ull << 30;
 constexpr uint64_t MAX_COLS = 1ull << 26;
 // Workgroups of one launch: the grid's threads are counted in 32 bits
 constexpr uint64_t MAX_GRID = 1ull << 22;
+// ... and along y
+constexpr uint64_t MAX_GRID_Y = 65535;
 
 bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
     return stride < (1ull << 40) && (tokens <= 1 || stride >= width);
@@ -119,6 +121,18 @@ uint64_t launch_some(MatvecArgs a, uint64_t tokens, hipStream_t st) {
     if (a.x_kind == EK_BF16) return launch_tiles<F, DenseTile<F, 1>>(a, tokens, st);
     if (a.x_kind == EK_F16) return launch_tiles<F, DenseTile<F, 2>>(a, tokens, st);
     return launch_tiles<F, DenseTile<F, 3>>(a, tokens, st);
+}
+
+template <class F, class O>
+void launch_rows_as(const RowsArgs &a, uint32_t n, hipStream_t st) {
+    const uint64_t piece = WG_THREADS * STORES_PER_THREAD * O::EPL;
+    get_rows<F, O><<<dim3((uint32_t)((a.cols + piece - 1) / piece), n), WG_THREADS, 0, st>>>(a);
+}
+template <class F>
+void launch_rows(const RowsArgs &a, uint32_t y_kind, uint32_t n, hipStream_t st) {
+    if (y_kind == EK_F32) launch_rows_as<F, OutF32>(a, n, st);
+    else if (y_kind == EK_F16) launch_rows_as<F, OutF16>(a, n, st);
+    else launch_rows_as<F, OutBF16>(a, n, st);
 }
 
 }  // namespace
@@ -276,10 +290,10 @@ ggq_status ggq_get_rows_device(uint32_t ty, uint64_t rows, uint64_t cols, const 
                                const void *d_ids, uint64_t n, uint32_t y_type, void *d_y, uint64_t y_stride,
                                void *hip_stream) {
     RowsArgs a{};
-    uint32_t yb;
+    uint32_t y_kind, yb;
     const uint64_t be = ggq_block_elems(ty);
     const uint32_t idb = id_type == 26 ? 4 : id_type == 27 ? 8 : 0;     // GGmlType I32, I64
-    if (be == 0 || idb == 0 || !elem_kind(y_type, &a.y_kind, &yb)) return GGQ_UNSUPPORTED;
+    if (be == 0 || idb == 0 || !elem_kind(y_type, &y_kind, &yb)) return GGQ_UNSUPPORTED;
     if (cols % be != 0) return GGQ_INDIVISIBLE;
     if (rows >= MAX_DIM || cols >= MAX_COLS || n >= MAX_DIM || !strides_ok(y_stride, cols, n)) return GGQ_INVALID;
     if (cols == 0 || n == 0) return GGQ_OK;
@@ -294,10 +308,9 @@ ggq_status ggq_get_rows_device(uint32_t ty, uint64_t rows, uint64_t cols, const 
     a.y_stride = y_stride;
     a.row_bytes = cols / be * ggq_block_bytes(ty);
     a.wide_ids = idb == 8;
-    const uint64_t pieces = (cols + 3) / 4, total = pieces * n, step = MAX_GRID * MV_THREADS;
-    for (uint64_t p = 0; p < total; p += step) {
-        const uint32_t grid = (uint32_t)((std::min(step, total - p) + MV_THREADS - 1) / MV_THREADS);
-#define CASE(F) get_rows<F><<<grid, MV_THREADS, 0, (hipStream_t)hip_stream>>>(a, p, pieces)
+    for (; a.first < n; a.first += MAX_GRID_Y) {
+        const uint32_t now = (uint32_t)std::min<uint64_t>(MAX_GRID_Y, n - a.first);
+#define CASE(F) launch_rows<F>(a, y_kind, now, (hipStream_t)hip_stream)
         GGQ_FOR_TYPE(ty, CASE)
 #undef CASE
     }

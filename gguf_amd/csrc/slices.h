@@ -40,6 +40,8 @@ typedef u32x4 u32x4_any __attribute__((aligned(1), may_alias));
 
 // global memory, any alignment
 __device__ __forceinline__ u32x4 ld16(const uint8_t *p) { return *(const u32x4_any *)p; }
+// 16 bytes that nothing reads soon
+template <class V> __device__ __forceinline__ void st16_streaming(void *p, V v) { __builtin_nontemporal_store(__builtin_bit_cast(u32x4, v), (u32x4_any *)p); }
 __device__ __forceinline__ uint32_t ld4(const uint8_t *p) { return *(const u32_any *)p; }
 __device__ __forceinline__ uint32_t ld2(const uint8_t *p) { return *(const u16_any *)p; }
 // shared memory, aligned
