@@ -308,7 +308,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // Staged x, per turn: [piece][fragment of 8 elements][token] 16 bytes, 32 bytes between one fragment and the next for the
 // staging threads' banks; then the sums of x over each sub-block, [sub-block][token], f32.
 template <class F, int P>
-struct DenseTile {
+struct OldTile {
     typedef Step<F> S;
     static constexpr uint32_t ROWS = 16, ELEMS = 256, TOKENS = 16;
     typedef Image<F, ROWS, 1> I;
@@ -416,5 +416,274 @@ struct DenseTile {
         for (int r = 0; r < 4; ++r) part[(4 * (lane / 16) + r) * ROWS + lane % 16] = acc.v[r];
     }
 };
+
+
+// How x goes into the matrix unit: its type, and the bf16 pieces that a value is cut into
+enum XForm : int { X_BF16, X_F16, X_F32_2, X_F32_3 };
+
+// of a token's values; keep = 0: all of them are taken as zero, whatever they are
+struct Factor {
+    float by;
+    uint32_t keep;
+    __device__ __forceinline__ float of(float v) const { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & keep) * by; }
+};
+
+// Up to 16 tokens times R tiles of 16 rows.  A wave takes whole turns, 256 columns of all its rows and tokens, and nobody else
+// needs that part of x: it lies in the wave's own shared memory, as it comes from global memory, beside the images of its
+// tiles, and the waves of a workgroup meet only to add up their sums.  A fragment of x is read and cut into pieces once for
+// the R tiles.
+template <class F, int X, int R>
+struct DenseTile {
+    typedef Step<F> S;
+    static constexpr uint32_t ROWS = 16, ELEMS = 256, TOKENS = 16;
+    typedef Image<F, ROWS, 1> I;
+    static constexpr bool WIDE = X == X_F32_2 || X == X_F32_3;
+    static constexpr int P = X == X_BF16 ? 1 : X == X_F32_3 ? 3 : 2;
+    static constexpr uint32_t SUBS = 256 / S::SUB, EACH = SUBS / 4, N = S::SUB / 4;        // N: elements of a lane's fragment
+    static constexpr uint32_t X_SIZE = WIDE ? 4 : 2, X_ROW = 256 * X_SIZE + 16;              // an odd number of 16-byte places
+    static constexpr uint32_t X_LOADS = WIDE ? TOKENS : TOKENS / 2, X_EACH = 16 / X_SIZE;
+    static constexpr uint32_t SCALES = is_float_type<F> ? 0 : SUBS * ROWS * 4, PART = TOKENS * ROWS * 4;
+    static_assert(I::BYTES >= PART, "the sums take the place of the images");
+    // shared memory of a wave: images, scales [tile][4 sub-blocks][row][sub-block], x [token]
+    static constexpr uint32_t AT_X = R * (I::BYTES + SCALES);
+    static constexpr __host__ __device__ __forceinline__ uint32_t wave_bytes(uint32_t tokens) { return AT_X + (tokens + 1) / 2 * 2 * X_ROW; }
+
+    typedef float Values[N];
+    // N elements as pieces, in words of two
+    static __device__ __forceinline__ void cut(Values &v, uint32_t (&out)[P][N / 2]) {
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+#pragma unroll
+            for (uint32_t i = 0; i < N / 2; ++i) out[p][i] = upper_halves(v[2 * i], v[2 * i + 1]);
+            if (p + 1 < P)
+#pragma unroll
+                for (uint32_t i = 0; i < N; ++i) v[i] = below_bf16(v[i]);
+        }
+    }
+    // the fragment of sub-block s: elements SUB s + N g ..
+    static __device__ __forceinline__ void fragment(const uint8_t *x, uint32_t s, uint32_t g, const Factor *factor, uint32_t (&out)[P][N / 2]) {
+        const uint8_t *at = x + (S::SUB * s + N * g) * X_SIZE;
+        if constexpr (X == X_BF16) {
+            if constexpr (N == 8) {
+                const u32x4 w = al16(at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) out[0][i] = w[i];
+            } else {
+                const u32x2 w = al8(at);
+                out[0][0] = w[0];
+                out[0][1] = w[1];
+            }
+        } else {
+            Values v;
+            if constexpr (X == X_F16) {
+#pragma unroll
+                for (uint32_t i = 0; i < N; i += 4) {
+                    const u32x2 w = al8(at + 2 * i);
+                    const uint32_t w0 = w[0], w1 = w[1];
+                    v[i] = h2f(w0 & 0xFFFFu);
+                    v[i + 1] = h2f(w0 >> 16);
+                    v[i + 2] = h2f(w1 & 0xFFFFu);
+                    v[i + 3] = h2f(w1 >> 16);
+                }
+            } else {
+#pragma unroll
+                for (uint32_t i = 0; i < N; i += 4) {
+                    const f32x4 w = *(const f32x4 *)(at + 4 * i);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[i + j] = factor ? factor->of(w[j]) : w[j];
+                }
+            }
+            cut(v, out);
+        }
+    }
+    static __device__ __forceinline__ f32x4 multiply(const uint32_t (&a)[N / 2], const uint32_t (&b)[N / 2], f32x4 d) {
+        if constexpr (N == 8)
+            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{a[0], a[1], a[2], a[3]}), __builtin_bit_cast(bf16x8, u32x4{b[0], b[1], b[2], b[3]}), d, 0, 0, 0);
+        else
+            return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, u32x2{a[0], a[1]}), __builtin_bit_cast(s16x4, u32x2{b[0], b[1]}), d, 0, 0, 0);
+    }
+    // the products of one turn; `space`: the wave's shared memory, x: of the lane's token
+    static __device__ __forceinline__ void add(uint8_t *space, const uint8_t *x, uint32_t n, uint32_t g, uint32_t left, const Factor *factor, f32x4 (&acc)[R]) {
+        const uint8_t *row = space + n * I::ROW;
+        if constexpr (is_float_type<F>) {
+#pragma unroll
+            for (uint32_t s = 0; s < SUBS; ++s) {
+                uint32_t a[P][N / 2];
+                fragment(x, s, g, factor, a);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const u32x4 w = S::load(row + r * I::BYTES, s, g, left);
+                    uint32_t b[4] = {w[0], w[1], w[2], w[3]}, low[4];
+                    if constexpr (__is_same(F, WF16)) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float v0 = h2f(b[i] & 0xFFFFu), v1 = h2f(b[i] >> 16);
+                            b[i] = upper_halves(v0, v1);
+                            low[i] = upper_halves(below_bf16(v0), below_bf16(v1));
+                        }
+                    }
+#pragma unroll
+                    for (int p = 0; p < P; ++p) {
+                        acc[r] = multiply(a[p], b, acc[r]);
+                        if constexpr (__is_same(F, WF16)) acc[r] = multiply(a[p], low, acc[r]);
+                    }
+                }
+            }
+        } else {
+            float *scales = (float *)(space + R * I::BYTES);
+            float offset[R][EACH], sums[EACH];
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                SubScale mine[EACH];
+                S::scale(row + r * I::BYTES, g, left, mine);
+                float *to = scales + r * (SCALES / 4);
+                if constexpr (EACH == 2) *(f32x2 *)(to + (g / 2 * ROWS + n) * 4 + g % 2 * 2) = f32x2{mine[0].a, mine[1].a};
+                else *(f32x4 *)(to + (g * ROWS + n) * 4) = f32x4{mine[0].a, mine[1].a, mine[2].a, mine[3].a};
+#pragma unroll
+                for (uint32_t k = 0; k < EACH; ++k) offset[r][k] = -mine[k].c;
+            }
+            wave_order();
+            f32x4 scale[R];
+#pragma unroll
+            for (uint32_t s = 0; s < SUBS; ++s) {
+                uint32_t a[P][N / 2];
+                fragment(x, s, g, factor, a);
+                if constexpr (S::OFFSET) {
+                    // times ones: the sum of the lane's token, in all four of D's rows
+                    uint32_t ones[N / 2];
+#pragma unroll
+                    for (uint32_t i = 0; i < N / 2; ++i) ones[i] = 0x3F803F80u;
+                    f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int p = 0; p < P; ++p) d = multiply(ones, a[p], d);
+                    sums[s % EACH] = s / EACH == 0 || g == s / EACH ? d[0] : sums[s % EACH];
+                }
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    if (s % 4 == 0) scale[r] = *(const f32x4 *)(scales + r * (SCALES / 4) + (s / 4 * ROWS + n) * 4);
+                    uint32_t b[N / 2];
+                    S::codes(row + r * I::BYTES, s, g, b);
+                    f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int p = 0; p < P; ++p) d = multiply(a[p], b, d);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[r][i] = __builtin_fmaf(scale[r][s % 4], d[i], acc[r][i]);
+                }
+            }
+            if constexpr (S::OFFSET) {
+                // the offsets of a lane's row and sub-blocks meet the sums of its token and the same sub-blocks, in f32
+#pragma unroll
+                for (int r = 0; r < R; ++r)
+#pragma unroll
+                    for (uint32_t k = 0; k < EACH; ++k) acc[r] = __builtin_amdgcn_mfma_f32_16x16x4f32(sums[k], offset[r][k], acc[r], 0, 0, 0);
+            }
+        }
+    }
+};
+
+// The wave's turns kp, kp + waves, ..., the next one's bytes on the way while one is multiplied; then its sums, in the place of
+// the images, [tile][token][row].
+//     at(turn, r)        the packed bytes of tile r, as in run_turns
+//     src(turn, t)       the first element of token t in that turn
+//     col(turn)          its first column, of `cols`
+//     factor(turn, t)    of token t, for FACTOR
+template <class M, int R, bool FACTOR, class At, class Src, class Col, class FactorOf>
+__device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I::Places &places, uint32_t reach, uint32_t kp, uint32_t waves, uint32_t turns, uint32_t tokens,
+                                            uint32_t cols, At at, Src src, Col col, FactorOf factor) {
+    const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
+    uint8_t *xs = space + M::AT_X;
+    const uint32_t token = n < tokens ? n : tokens - 1;
+    const uint8_t *x = xs + token * M::X_ROW;
+    typename M::I in[R];
+    u32x4 xr[M::X_LOADS];
+    uint32_t left = 0;
+    const uint32_t x_need = M::WIDE ? tokens : (tokens + 1) / 2, x_slot = M::WIDE ? 0 : lane / 32, x_at = (M::WIDE ? lane : lane % 32) * M::X_EACH;
+    auto fetch = [&](uint32_t turn) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const Turn t = at(turn, r);
+            in[r].fetch(places, t.base, t.room, reach);
+            left = t.left;
+        }
+        const uint32_t c = col(turn);
+#pragma unroll
+        for (uint32_t i = 0; i < M::X_LOADS; ++i) {
+            if (i < x_need) {
+            const uint32_t slot = M::WIDE ? i : 2 * i + x_slot, t = slot < tokens ? slot : tokens - 1;
+            const uint8_t *p = src(turn, t) + x_at * M::X_SIZE;
+            u32x4 v = {0, 0, 0, 0};
+            if (c + x_at + M::X_EACH <= cols) {
+                v = ld16(p);
+            } else if (M::WIDE) {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) v[j] = c + x_at + j < cols ? ld4(p + 4 * j) : 0u;
+            } else {
+#pragma unroll
+                for (uint32_t j = 0; j < 4; ++j) {
+                    const uint32_t lo = c + x_at + 2 * j < cols ? ld2(p + 4 * j) : 0u, hi = c + x_at + 2 * j + 1 < cols ? ld2(p + 4 * j + 2) : 0u;
+                    v[j] = lo | (hi << 16);
+                }
+            }
+            xr[i] = v;
+            }
+        }
+    };
+    f32x4 acc[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) acc[r] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (kp < turns) fetch(kp);
+    for (uint32_t turn = kp; turn < turns; turn += waves) {
+        wave_order();
+#pragma unroll
+        for (int r = 0; r < R; ++r) in[r].put(places, space + r * M::I::BYTES);
+#pragma unroll
+        for (uint32_t i = 0; i < M::X_LOADS; ++i) {
+            if (i < x_need) *(u32x4 *)(xs + (M::WIDE ? i : 2 * i + x_slot) * M::X_ROW + x_at * M::X_SIZE) = xr[i];
+        }
+        wave_order();
+        const uint32_t here = left;
+        Factor by{};
+        if constexpr (FACTOR) by = factor(turn, token);
+        if (turn + waves < turns) fetch(turn + waves);
+        M::add(space, x, n, g, here, FACTOR ? &by : nullptr, acc);
+    }
+    wave_order();
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) *(float *)(space + r * M::PART + ((4 * g + i) * M::ROWS + n) * 4) = acc[r][i];
+}
+
+// ---- one matrix, several tokens ---------------------------------------------------------------------------------
+// A workgroup takes R tiles of rows, its waves share their columns.
+template <class F, int X, int R>
+__global__ __launch_bounds__(TILE_THREADS) void matvec_dense(MatvecArgs a) {
+    extern __shared__ __align__(16) uint8_t lds[];
+    typedef DenseTile<F, X, R> M;
+    typedef typename M::I I;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.tokens);
+    const uint32_t row_bytes = (uint32_t)(a.cols / F::N * F::BYTES), turns = (uint32_t)((a.cols + M::ELEMS - 1) / M::ELEMS);
+    const uint64_t first_row = (a.first_tile + (uint64_t)blockIdx.x * R) * M::ROWS;
+    const uint32_t rows = a.rows < M::ROWS ? (uint32_t)a.rows : M::ROWS;
+    const uint64_t last = a.rows - rows;                       // tiles that would end behind it begin with this row
+    auto begin = [&](int r) { const uint64_t row = first_row + r * M::ROWS; return row < last ? row : last; };
+    dense_turns<M, R, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, a.tokens,
+                             (uint32_t)a.cols,
+                             [&](uint32_t turn, int r) {
+                                 const uint64_t row = begin(r);
+                                 const uint32_t off = turn * I::TURN_BYTES;
+                                 return Turn{a.w + row * row_bytes + off, row_bytes - off, (a.rows - row) * row_bytes - off};
+                             },
+                             [&](uint32_t turn, uint32_t t) { return (const uint8_t *)a.x + (t * a.x_stride + turn * M::ELEMS) * M::X_SIZE; },
+                             [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < R * M::ROWS * a.tokens; i += blockDim.x) {
+        const uint32_t r = i % (R * M::ROWS) / M::ROWS, n = i % M::ROWS, t = i / (R * M::ROWS);
+        const uint64_t row = begin(r) + n;
+        float v = 0.0f;
+        for (uint32_t k = 0; k < waves; ++k) v += *(const float *)(lds + k * wave_bytes + r * M::PART + (t * M::ROWS + n) * 4);
+        if (row >= first_row + r * M::ROWS && row < a.rows) store_elem(a.y, t * a.y_stride + row, a.y_kind, v);
+    }
+}
 
 }  // namespace ggq

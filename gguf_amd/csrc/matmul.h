@@ -537,13 +537,6 @@ __global__ __launch_bounds__(MV_THREADS) void matvec_short(MatvecArgs a) {
     }
 }
 
-// a sum of nothing
-static __global__ __launch_bounds__(MV_THREADS) void fill_zero(MatvecArgs a) {
-    const uint64_t r = (uint64_t)blockIdx.x * MV_THREADS + threadIdx.x;
-    if (r >= a.rows) return;
-    for (uint32_t t = 0; t < a.tokens; ++t) store_elem(a.y, t * a.y_stride + r, a.y_kind, 0.0f);
-}
-
 // ---- rows by id -----------------------------------------------------------------------------------------
 struct RowsArgs {
     const uint8_t *w;

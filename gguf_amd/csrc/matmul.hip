@@ -1,15 +1,21 @@
 // matmul.hip -- entry points of the products with packed weights (include/ggq.h): argument checks and launches.
 #include "../../include/ggq.h"
 #include "internal.h"
-#include "dense.h"
-#include "matmul.h"
-#include "moe.h"
+#include "launch.h"
+#include "route.h"
 
 #include <algorithm>
 
 using namespace ggq;
 
 namespace {
+
+// a sum of nothing
+static __global__ __launch_bounds__(MV_THREADS) void fill_zero(MatvecArgs a) {
+    const uint64_t r = (uint64_t)blockIdx.x * MV_THREADS + threadIdx.x;
+    if (r >= a.rows) return;
+    for (uint32_t t = 0; t < a.tokens; ++t) store_elem(a.y, t * a.y_stride + r, a.y_kind, 0.0f);
+}
 
 #define HIP_TRY(call)                                       \
     do {                                                    \
@@ -51,88 +57,11 @@ bool elem_kind(uint32_t ty, uint32_t *kind, uint32_t *bytes) {
 constexpr uint64_t MAX_DIM = 1ull << 30;
 // Columns: eight packed rows of any type are within 32-bit offsets.
 constexpr uint64_t MAX_COLS = 1ull << 26;
-// Workgroups of one launch: the grid's threads are counted in 32 bits
-constexpr uint64_t MAX_GRID = 1ull << 22;
-// ... and along y
+// Workgroups of one launch along y
 constexpr uint64_t MAX_GRID_Y = 65535;
 
 bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
     return stride < (1ull << 40) && (tokens <= 1 || stride >= width);
-}
-
-// Shared memory of one workgroup for x, beside its waves' images.
-constexpr uint32_t X_LDS = 64 << 10;
-
-// The shape of a launch over `tiles` wave tiles, each of which takes `turns` turns: how many waves share a tile's turns,
-// the turns staged at a time (equal chunks, whole rounds of the waves), the shared memory.
-struct Shape {
-    uint32_t ksplit = 1, groups;
-    // `waves`: of a workgroup that may share a tile's turns; x_bytes: shared memory of a turn of x
-    Shape(uint64_t tiles, uint32_t turns, uint32_t waves, uint32_t x_bytes) {
-        // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
-        while (ksplit < waves && ksplit < turns && tiles * ksplit < 2048 && 2 * ksplit * x_bytes <= X_LDS) ksplit *= 2;
-        groups = waves / ksplit;
-    }
-    template <class M> uint32_t chunk(uint32_t turns) const {
-        const uint32_t rounds = (turns + ksplit - 1) / ksplit, most = std::max(1u, X_LDS / (M::X_BYTES * ksplit)), chunks = (rounds + most - 1) / most;
-        return (rounds + chunks - 1) / chunks * ksplit;
-    }
-    template <class M> uint32_t bytes(uint32_t turns) const {
-        return TILE_WAVES * M::WAVE_BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk<M>(turns), turns) * M::X_BYTES, TILE_WAVES * M::TOKENS * M::ROWS * 4);
-    }
-};
-template <class M> constexpr uint32_t turns_of(uint64_t cols) { return (uint32_t)((cols + M::ELEMS - 1) / M::ELEMS); }
-
-template <class F, class M>
-uint64_t launch_tiles(MatvecArgs a, uint64_t tokens, hipStream_t st) {
-    a.tokens = (uint32_t)std::min<uint64_t>(tokens, M::TOKENS);
-    const uint64_t tiles = (a.rows + M::ROWS - 1) / M::ROWS;
-    const uint32_t turns = turns_of<M>(a.cols);
-    const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
-    a.ksplit = sh.ksplit;
-    a.chunk = sh.chunk<M>(turns);
-    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * sh.groups) {
-        const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + sh.groups - 1) / sh.groups));
-        matvec_tiles<F, M><<<grid, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
-    }
-    return a.tokens;
-}
-
-// x is taken to 16 bits below an element, or the largest of 32, where the result is rounded to a 16-bit float anyway.
-bool to_16_bits(uint32_t x_kind, uint32_t y_kind) { return x_kind != EK_F32 && y_kind != EK_F32; }
-
-// One launch over the first of the tokens.  Returns how many it takes.
-template <class F>
-uint64_t launch_some(MatvecArgs a, uint64_t tokens, hipStream_t st) {
-    if constexpr (is_float_type<F>) {
-        if (a.cols < 8) {
-            a.tokens = (uint32_t)std::min<uint64_t>(tokens, 64);
-            matvec_short<F><<<(uint32_t)((a.rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
-            return a.tokens;
-        }
-        if (tokens == 1) {
-            if (a.x_kind == EK_BF16) return launch_tiles<F, FloatTile<F, 1>>(a, 1, st);
-            if (a.x_kind == EK_F16) return launch_tiles<F, FloatTile<F, 2>>(a, 1, st);
-            return launch_tiles<F, FloatTile<F, 3>>(a, 1, st);
-        }
-    } else if (tokens == 1) {
-        return to_16_bits(a.x_kind, a.y_kind) ? launch_tiles<F, CodeTile<F, 1>>(a, 1, st) : launch_tiles<F, CodeTile<F, 2>>(a, 1, st);
-    }
-    if (a.x_kind == EK_BF16) return launch_tiles<F, DenseTile<F, 1>>(a, tokens, st);
-    if (a.x_kind == EK_F16) return launch_tiles<F, DenseTile<F, 2>>(a, tokens, st);
-    return launch_tiles<F, DenseTile<F, 3>>(a, tokens, st);
-}
-
-template <class F, class O>
-void launch_rows_as(const RowsArgs &a, uint32_t n, hipStream_t st) {
-    const uint64_t piece = WG_THREADS * STORES_PER_THREAD * O::EPL;
-    get_rows<F, O><<<dim3((uint32_t)((a.cols + piece - 1) / piece), n), WG_THREADS, 0, st>>>(a);
-}
-template <class F>
-void launch_rows(const RowsArgs &a, uint32_t y_kind, uint32_t n, hipStream_t st) {
-    if (y_kind == EK_F32) launch_rows_as<F, OutF32>(a, n, st);
-    else if (y_kind == EK_F16) launch_rows_as<F, OutF16>(a, n, st);
-    else launch_rows_as<F, OutBF16>(a, n, st);
 }
 
 }  // namespace
@@ -171,82 +100,6 @@ struct MoeSpace {
     }
 };
 
-// One: the tile of experts with one token, Many: of the others
-template <class F, class One, class Many>
-void launch_up(MoeArgs a, hipStream_t st) {
-    const uint32_t tiles = (uint32_t)((a.ff + Many::ROWS - 1) / Many::ROWS);
-    static_assert(One::ROWS == Many::ROWS, "one grid for both");
-    const uint32_t one = turns_of<One>(a.hidden), many = turns_of<Many>(a.hidden);
-    const Shape sh(2 * (uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES / 2, std::max(One::X_BYTES, Many::X_BYTES));
-    a.ksplit = sh.ksplit;
-    a.chunk_one = sh.chunk<One>(one);
-    a.chunk = sh.chunk<Many>(many);
-    moe_up<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
-}
-
-template <class F>
-void launch_up_of(MoeArgs a, hipStream_t st) {
-    if constexpr (is_float_type<F>) {
-        if (a.hidden < 8) {
-            moe_up_short<F><<<dim3((uint32_t)((a.ff + MV_THREADS - 1) / MV_THREADS), a.tokens * a.top_k), MV_THREADS, 0, st>>>(a);
-        } else if (a.x_kind == EK_BF16) {
-            launch_up<F, DenseTile<F, 1>, DenseTile<F, 1>>(a, st);
-        } else if (a.x_kind == EK_F16) {
-            launch_up<F, DenseTile<F, 2>, DenseTile<F, 2>>(a, st);
-        } else {
-            launch_up<F, DenseTile<F, 3>, DenseTile<F, 3>>(a, st);
-        }
-    } else if (a.tokens == 1) {
-        if (to_16_bits(a.x_kind, a.y_kind)) launch_up<F, CodeTile<F, 1>, CodeTile<F, 1>>(a, st);
-        else launch_up<F, CodeTile<F, 2>, CodeTile<F, 2>>(a, st);
-    } else {
-        if (a.x_kind == EK_BF16) launch_up<F, CodeTile<F, 2>, DenseTile<F, 1>>(a, st);
-        else if (a.x_kind == EK_F16) launch_up<F, CodeTile<F, 2>, DenseTile<F, 2>>(a, st);
-        else launch_up<F, CodeTile<F, 2>, DenseTile<F, 3>>(a, st);
-    }
-}
-
-template <class F, class M>
-void launch_down_few(MoeArgs a, hipStream_t st) {
-    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.ff) * a.tokens * a.top_k;
-    const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
-    a.ksplit = sh.ksplit;
-    a.chunk = sh.chunk<M>(turns);
-    moe_down_few<F, M><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
-}
-
-template <class F, class One, class Many>
-void launch_down_many(MoeArgs a, hipStream_t st) {
-    const uint32_t tiles = (uint32_t)((a.hidden + Many::ROWS - 1) / Many::ROWS), one = turns_of<One>(a.ff), many = turns_of<Many>(a.ff);
-    const Shape sh((uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES, std::max(One::X_BYTES, Many::X_BYTES));
-    a.ksplit = sh.ksplit;
-    a.chunk_one = sh.chunk<One>(one);
-    a.chunk = sh.chunk<Many>(many);
-    moe_down_many<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
-    moe_sum<<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
-}
-
-template <class F>
-void launch_down_of(MoeArgs a, hipStream_t st) {
-    if constexpr (is_float_type<F>) {
-        if (a.ff < 8) {
-            moe_down_short<F><<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
-        } else if (a.tokens <= 4) {
-            launch_down_few<F, DenseTile<F, 3>>(a, st);
-        } else {
-            launch_down_many<F, DenseTile<F, 3>, DenseTile<F, 3>>(a, st);
-        }
-    } else if (to_16_bits(a.x_kind, a.y_kind)) {
-        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 1>>(a, st);
-        else if (a.tokens <= 4) launch_down_few<F, DenseTile<F, 2>>(a, st);
-        else launch_down_many<F, CodeTile<F, 1>, DenseTile<F, 2>>(a, st);
-    } else {
-        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 2>>(a, st);
-        else if (a.tokens <= 4) launch_down_few<F, DenseTile<F, 3>>(a, st);
-        else launch_down_many<F, CodeTile<F, 2>, DenseTile<F, 3>>(a, st);
-    }
-}
-
 }  // namespace
 
 extern "C" {
@@ -278,7 +131,7 @@ ggq_status ggq_matvec_device(uint32_t ty, uint64_t rows, uint64_t cols, const vo
             fill_zero<<<(uint32_t)((rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
             continue;
         }
-#define CASE(F) done = launch_some<F>(a, tokens - t, st)
+#define CASE(F) done = Launch<F>::matvec(a, tokens - t, st)
         GGQ_FOR_TYPE(ty, CASE)
 #undef CASE
     }
@@ -310,7 +163,7 @@ ggq_status ggq_get_rows_device(uint32_t ty, uint64_t rows, uint64_t cols, const 
     a.wide_ids = idb == 8;
     for (; a.first < n; a.first += MAX_GRID_Y) {
         const uint32_t now = (uint32_t)std::min<uint64_t>(MAX_GRID_Y, n - a.first);
-#define CASE(F) launch_rows<F>(a, y_kind, now, (hipStream_t)hip_stream)
+#define CASE(F) Launch<F>::rows(a, y_kind, now, (hipStream_t)hip_stream)
         GGQ_FOR_TYPE(ty, CASE)
 #undef CASE
     }
@@ -376,12 +229,14 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     // groups of up to 16 pairs with the same expert: one for each pair, or one for each expert and one more for each 16 pairs
     const uint32_t pairs = (uint32_t)tokens * m->top_k, in_use = std::min(m->experts, pairs);
     a.slots = std::min(pairs, in_use + (pairs - in_use) / SLOT_TOKENS);
-#define CASE(F) launch_up_of<F>(a, st)
+#define CASE(F) Launch<F>::up(a, st)
     GGQ_FOR_TYPE(m->up_type, CASE)
 #undef CASE
-#define CASE(F) launch_down_of<F>(a, st)
+#define CASE(F) Launch<F>::down(a, st)
     GGQ_FOR_TYPE(m->down_type, CASE)
 #undef CASE
+    if (tokens > FEW_TOKENS && !short_rows(m->down_type, m->ff))
+        moe_sum<<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
     HIP_TRY(hipGetLastError());
     return GGQ_OK;
 }

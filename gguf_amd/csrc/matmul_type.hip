@@ -1,0 +1,203 @@
+// matmul_type.hip -- the launches of the products with packed weights for one block type: compiled once for each, with
+// GGQ_FORMAT its struct in formats.h, so that they build side by side.
+#include "launch.h"
+#include "moe.h"
+
+#include <algorithm>
+
+namespace ggq {
+namespace {
+
+// Workgroups of one launch: the grid's threads are counted in 32 bits
+constexpr uint64_t MAX_GRID = 1ull << 22;
+// Shared memory of one workgroup for x, beside its waves' images.
+constexpr uint32_t X_LDS = 64 << 10;
+
+constexpr uint32_t DENSE_LDS = 152 << 10;
+
+// The shape of a launch over `tiles` wave tiles, each of which takes `turns` turns: how many waves share a tile's turns,
+// the turns staged at a time (equal chunks, whole rounds of the waves), the shared memory.
+struct Shape {
+    uint32_t ksplit = 1, groups;
+    // `waves`: of a workgroup that may share a tile's turns; x_bytes: shared memory of a turn of x
+    Shape(uint64_t tiles, uint32_t turns, uint32_t waves, uint32_t x_bytes) {
+        // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs
+        while (ksplit < waves && ksplit < turns && tiles * ksplit < 2048 && 2 * ksplit * x_bytes <= X_LDS) ksplit *= 2;
+        groups = waves / ksplit;
+    }
+    template <class M> uint32_t chunk(uint32_t turns) const {
+        const uint32_t rounds = (turns + ksplit - 1) / ksplit, most = std::max(1u, X_LDS / (M::X_BYTES * ksplit)), chunks = (rounds + most - 1) / most;
+        return (rounds + chunks - 1) / chunks * ksplit;
+    }
+    template <class M> uint32_t bytes(uint32_t turns) const {
+        return TILE_WAVES * M::WAVE_BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk<M>(turns), turns) * M::X_BYTES, TILE_WAVES * M::TOKENS * M::ROWS * 4);
+    }
+};
+template <class M> constexpr uint32_t turns_of(uint64_t cols) { return (uint32_t)((cols + M::ELEMS - 1) / M::ELEMS); }
+
+template <class F, class M>
+uint64_t launch_tiles(MatvecArgs a, uint64_t tokens, hipStream_t st) {
+    a.tokens = (uint32_t)std::min<uint64_t>(tokens, M::TOKENS);
+    const uint64_t tiles = (a.rows + M::ROWS - 1) / M::ROWS;
+    const uint32_t turns = turns_of<M>(a.cols);
+    const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
+    a.ksplit = sh.ksplit;
+    a.chunk = sh.chunk<M>(turns);
+    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * sh.groups) {
+        const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + sh.groups - 1) / sh.groups));
+        matvec_tiles<F, M><<<grid, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
+    }
+    return a.tokens;
+}
+
+// x is taken to 16 bits below an element, or the largest of 32, where the result is rounded to a 16-bit float anyway.
+[[maybe_unused]] bool to_16_bits(uint32_t x_kind, uint32_t y_kind) { return x_kind != EK_F32 && y_kind != EK_F32; }
+
+// Waves that share the columns of a dense tile: as many as there are turns and as fit, all with as many turns or one less.
+template <class M>
+uint32_t dense_waves(uint32_t turns, uint32_t tokens) {
+    const uint32_t most = std::min(std::min(TILE_WAVES, turns), DENSE_LDS / M::wave_bytes(tokens)), rounds = (turns + most - 1) / most;
+    return (turns + rounds - 1) / rounds;
+}
+template <class F, int X, int R>
+void launch_dense_tiles(MatvecArgs a, uint64_t tiles, hipStream_t st) {
+    typedef DenseTile<F, X, R> M;
+    static_assert(M::wave_bytes(M::TOKENS) <= DENSE_LDS, "a wave's shared memory");
+    const uint32_t waves = dense_waves<M>(turns_of<M>(a.cols), a.tokens);
+    for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * R) {
+        const uint32_t grid = (uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + R - 1) / R);
+        matvec_dense<F, X, R><<<grid, waves * 64, waves * M::wave_bytes(a.tokens), st>>>(a);
+    }
+}
+template <class F, int X>
+uint64_t launch_dense(MatvecArgs a, uint64_t tokens, hipStream_t st) {
+    a.tokens = (uint32_t)std::min<uint64_t>(tokens, 16);
+    const uint64_t tiles = (a.rows + 15) / 16;
+    // tiles of a workgroup: staging x costs as much as one more
+    uint32_t best = 1;
+    uint64_t least = ~0ull;
+    for (uint32_t r = 1; r <= 3; ++r) {
+        const uint64_t cost = ((tiles + r - 1) / r + 255) / 256 * (r + 1);
+        if (cost <= least) best = r, least = cost;
+    }
+    if (best == 1) launch_dense_tiles<F, X, 1>(a, tiles, st);
+    else if (best == 2) launch_dense_tiles<F, X, 2>(a, tiles, st);
+    else launch_dense_tiles<F, X, 3>(a, tiles, st);
+    return a.tokens;
+}
+
+}  // namespace
+
+// One launch over the first of the tokens.  Returns how many it takes.
+template <class F>
+uint64_t Launch<F>::matvec(MatvecArgs a, uint64_t tokens, hipStream_t st) {
+    if constexpr (is_float_type<F>) {
+        if (a.cols < 8) {
+            a.tokens = (uint32_t)std::min<uint64_t>(tokens, 64);
+            matvec_short<F><<<(uint32_t)((a.rows + MV_THREADS - 1) / MV_THREADS), MV_THREADS, 0, st>>>(a);
+            return a.tokens;
+        }
+        if (tokens == 1) {
+            if (a.x_kind == EK_BF16) return launch_tiles<F, FloatTile<F, 1>>(a, 1, st);
+            if (a.x_kind == EK_F16) return launch_tiles<F, FloatTile<F, 2>>(a, 1, st);
+            return launch_tiles<F, FloatTile<F, 3>>(a, 1, st);
+        }
+    } else if (tokens == 1) {
+        return to_16_bits(a.x_kind, a.y_kind) ? launch_tiles<F, CodeTile<F, 1>>(a, 1, st) : launch_tiles<F, CodeTile<F, 2>>(a, 1, st);
+    }
+    if (a.x_kind == EK_BF16) return launch_dense<F, X_BF16>(a, tokens, st);
+    if (a.x_kind == EK_F16) return launch_dense<F, X_F16>(a, tokens, st);
+    return launch_dense<F, X_F32_3>(a, tokens, st);
+}
+
+template <class F, class O>
+void launch_rows_as(const RowsArgs &a, uint32_t n, hipStream_t st) {
+    const uint64_t piece = WG_THREADS * STORES_PER_THREAD * O::EPL;
+    get_rows<F, O><<<dim3((uint32_t)((a.cols + piece - 1) / piece), n), WG_THREADS, 0, st>>>(a);
+}
+template <class F>
+void Launch<F>::rows(const RowsArgs &a, uint32_t y_kind, uint32_t n, hipStream_t st) {
+    if (y_kind == EK_F32) launch_rows_as<F, OutF32>(a, n, st);
+    else if (y_kind == EK_F16) launch_rows_as<F, OutF16>(a, n, st);
+    else launch_rows_as<F, OutBF16>(a, n, st);
+}
+
+// ---- mixture of experts ---------------------------------------------------------------------------------
+// One: the tile of experts with one token, Many: of the others
+template <class F, class One, class Many>
+void launch_up(MoeArgs a, hipStream_t st) {
+    const uint32_t tiles = (uint32_t)((a.ff + Many::ROWS - 1) / Many::ROWS);
+    static_assert(One::ROWS == Many::ROWS, "one grid for both");
+    const uint32_t one = turns_of<One>(a.hidden), many = turns_of<Many>(a.hidden);
+    const Shape sh(2 * (uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES / 2, std::max(One::X_BYTES, Many::X_BYTES));
+    a.ksplit = sh.ksplit;
+    a.chunk_one = sh.chunk<One>(one);
+    a.chunk = sh.chunk<Many>(many);
+    moe_up<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
+}
+
+template <class F>
+void Launch<F>::up(MoeArgs a, hipStream_t st) {
+    if constexpr (is_float_type<F>) {
+        if (a.hidden < 8) {
+            moe_up_short<F><<<dim3((uint32_t)((a.ff + MV_THREADS - 1) / MV_THREADS), a.tokens * a.top_k), MV_THREADS, 0, st>>>(a);
+        } else if (a.x_kind == EK_BF16) {
+            launch_up<F, OldTile<F, 1>, OldTile<F, 1>>(a, st);
+        } else if (a.x_kind == EK_F16) {
+            launch_up<F, OldTile<F, 2>, OldTile<F, 2>>(a, st);
+        } else {
+            launch_up<F, OldTile<F, 3>, OldTile<F, 3>>(a, st);
+        }
+    } else if (a.tokens == 1) {
+        if (to_16_bits(a.x_kind, a.y_kind)) launch_up<F, CodeTile<F, 1>, CodeTile<F, 1>>(a, st);
+        else launch_up<F, CodeTile<F, 2>, CodeTile<F, 2>>(a, st);
+    } else {
+        if (a.x_kind == EK_BF16) launch_up<F, CodeTile<F, 2>, OldTile<F, 1>>(a, st);
+        else if (a.x_kind == EK_F16) launch_up<F, CodeTile<F, 2>, OldTile<F, 2>>(a, st);
+        else launch_up<F, CodeTile<F, 2>, OldTile<F, 3>>(a, st);
+    }
+}
+
+template <class F, class M>
+void launch_down_few(MoeArgs a, hipStream_t st) {
+    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.ff) * a.tokens * a.top_k;
+    const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
+    a.ksplit = sh.ksplit;
+    a.chunk = sh.chunk<M>(turns);
+    moe_down_few<F, M><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
+}
+
+template <class F, class One, class Many>
+void launch_down_many(MoeArgs a, hipStream_t st) {
+    const uint32_t tiles = (uint32_t)((a.hidden + Many::ROWS - 1) / Many::ROWS), one = turns_of<One>(a.ff), many = turns_of<Many>(a.ff);
+    const Shape sh((uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES, std::max(One::X_BYTES, Many::X_BYTES));
+    a.ksplit = sh.ksplit;
+    a.chunk_one = sh.chunk<One>(one);
+    a.chunk = sh.chunk<Many>(many);
+    moe_down_many<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
+}
+
+template <class F>
+void Launch<F>::down(MoeArgs a, hipStream_t st) {
+    if constexpr (is_float_type<F>) {
+        if (a.ff < 8) {
+            moe_down_short<F><<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
+        } else if (a.tokens <= FEW_TOKENS) {
+            launch_down_few<F, OldTile<F, 3>>(a, st);
+        } else {
+            launch_down_many<F, OldTile<F, 3>, OldTile<F, 3>>(a, st);
+        }
+    } else if (to_16_bits(a.x_kind, a.y_kind)) {
+        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 1>>(a, st);
+        else if (a.tokens <= FEW_TOKENS) launch_down_few<F, OldTile<F, 2>>(a, st);
+        else launch_down_many<F, CodeTile<F, 1>, OldTile<F, 2>>(a, st);
+    } else {
+        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 2>>(a, st);
+        else if (a.tokens <= FEW_TOKENS) launch_down_few<F, OldTile<F, 3>>(a, st);
+        else launch_down_many<F, CodeTile<F, 2>, OldTile<F, 3>>(a, st);
+    }
+}
+
+template struct Launch<GGQ_FORMAT>;
+
+}  // namespace ggq

@@ -6,170 +6,10 @@
 // over a token's experts (for more than four tokens down and the sum apart).  Bound by the bytes of the experts in use: each is read once for up to 16 of its
 // tokens, and once more for each further 16.
 #pragma once
+#include "choice.h"
 #include "dense.h"
 
 namespace ggq {
-
-struct MoeArgs {
-    const uint8_t *gate, *up, *down;
-    const void *router, *x;
-    void *y;
-    float *logits;        // [tokens][experts]
-    int32_t *ids;         // [tokens][top_k]
-    float *weights;       // [tokens][top_k]
-    float *h;             // [tokens * top_k][ff]
-    float *o;             // [tokens * top_k][hidden], where tokens > 4
-    int32_t *out_ids;     // the caller's, or null
-    float *out_weights;
-    uint64_t hidden, ff, x_stride, y_stride;
-    uint32_t tokens, experts, top_k, router_kind, x_kind, y_kind;
-    uint32_t sigmoid, normalize, gelu;
-    uint32_t ksplit, chunk, chunk_one;        // as in MatvecArgs, of the launch; chunk_one: of experts with one token
-    uint32_t choose;                          // the workgroups of gate and up find the choice themselves
-    uint32_t slots;                           // most slots there may be: workgroups along y
-    float scale;
-};
-
-// ---- logits ---------------------------------------------------------------------------------------------
-// four elements from c on, 0 past the end
-__device__ __forceinline__ void load4(const void *p, uint64_t at, uint32_t c, uint32_t n, uint32_t kind, float (&v)[4]) {
-    if (c + 4 <= n && kind == EK_F32) {
-        const f32x4 a = __builtin_bit_cast(f32x4, ld16((const uint8_t *)p + 4 * (at + c)));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = a[i];
-    } else if (c + 4 <= n) {
-        const uint8_t *q = (const uint8_t *)p + 2 * (at + c);
-        const uint32_t a = ld4(q), b = ld4(q + 4);
-        v[0] = kind == EK_F16 ? h2f(a & 0xFFFFu) : bf2f(a & 0xFFFFu);
-        v[1] = kind == EK_F16 ? h2f(a >> 16) : bf2f(a >> 16);
-        v[2] = kind == EK_F16 ? h2f(b & 0xFFFFu) : bf2f(b & 0xFFFFu);
-        v[3] = kind == EK_F16 ? h2f(b >> 16) : bf2f(b >> 16);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = c + i < n ? load_elem(p, at + c + i, kind) : 0.0f;
-    }
-}
-// One expert and four tokens a workgroup; grid: (experts, tokens / 4).  The choice hangs on the order of the logits, so
-// products (exact in 64 bits) are summed in 64 bits and rounded once.  Bound by its latency: 4 KiB of the router are on the
-// way at once in each workgroup, and the token's x with them.
-constexpr uint32_t LOGIT_TOKENS = 4;
-__global__ __launch_bounds__(MV_THREADS) static void moe_logits(MoeArgs a) {
-    __shared__ double part[LOGIT_TOKENS][MV_THREADS];
-    const uint32_t e = blockIdx.x, first = blockIdx.y * LOGIT_TOKENS, n = (uint32_t)a.hidden;
-    const uint32_t tokens = a.tokens - first < LOGIT_TOKENS ? a.tokens - first : LOGIT_TOKENS;
-    double sum[LOGIT_TOKENS] = {0.0, 0.0, 0.0, 0.0};
-    for (uint32_t c = threadIdx.x * 4; c < n; c += MV_THREADS * 16) {
-        float w[4][4];
-#pragma unroll
-        for (uint32_t k = 0; k < 4; ++k) load4(a.router, e * a.hidden, c + k * MV_THREADS * 4, n, a.router_kind, w[k]);
-#pragma unroll
-        for (uint32_t t = 0; t < LOGIT_TOKENS; ++t) {
-            if (t >= tokens) break;
-            float x[4][4];
-#pragma unroll
-            for (uint32_t k = 0; k < 4; ++k) load4(a.x, (first + t) * a.x_stride, c + k * MV_THREADS * 4, n, a.x_kind, x[k]);
-#pragma unroll
-            for (int k = 0; k < 4; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) sum[t] = __builtin_fma((double)w[k][i], (double)x[k][i], sum[t]);
-        }
-    }
-#pragma unroll
-    for (uint32_t t = 0; t < LOGIT_TOKENS; ++t) part[t][threadIdx.x] = sum[t];
-    __syncthreads();
-    const uint32_t t = threadIdx.x / 64, lane = threadIdx.x % 64;         // a wave for each token
-    if (t >= tokens) return;
-    double s = (part[t][lane] + part[t][lane + 64]) + (part[t][lane + 128] + part[t][lane + 192]);
-#pragma unroll
-    for (int m = 32; m; m >>= 1) s += __shfl_xor(s, m);
-    if (lane == 0) a.logits[(uint64_t)(first + t) * a.experts + e] = (float)s;
-}
-
-// an order-preserving key of a logit: larger logit, larger key; NaN below everything; -0 equals +0
-__device__ __forceinline__ uint32_t logit_key(float v) {
-    if (v != v) return 0u;
-    const uint32_t b = __builtin_bit_cast(uint32_t, v + 0.0f);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-
-// ---- the choice -----------------------------------------------------------------------------------------
-constexpr uint32_t MOE_MAX_EXPERTS = 512, MOE_MAX_TOP_K = 32, MOE_MAX_TOKENS = 64;
-constexpr uint32_t CHOOSE_TOKENS = 8;         // most tokens whose choice the workgroups of gate and up find themselves
-
-// The top_k experts of a token, ids[j] = the j-th.  An expert's place is the number of experts in front of it (a larger key,
-// or the same and a lower index), so all places are found at once, without a chain of k maxima; keys are read four at a
-// time, the same for all lanes.  Threads `me`, me + threads, ... of `threads` share the work; `keys`: theirs, room for 512;
-// order(): what makes their writes to shared memory seen.
-template <class Order>
-__device__ __forceinline__ void choose(const float *logits, uint32_t experts, uint32_t top_k, uint32_t me, uint32_t threads, uint32_t *keys, int32_t *ids,
-                                       Order order) {
-    const uint32_t padded = (experts + 3) & ~3u;
-    for (uint32_t e = me; e < padded; e += threads) keys[e] = e < experts ? logit_key(logits[e]) : 0u;
-    order();
-    for (uint32_t e = me; e < experts; e += threads) {
-        const uint32_t key = keys[e];
-        uint32_t place = 0;
-#pragma unroll 4
-        for (uint32_t q = 0; q < padded; q += 4) {
-            const u32x4 k = *(const u32x4 *)(keys + q);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) place += (k[i] > key) || (k[i] == key && q + i < e);
-        }
-        if (place < top_k) ids[place] = (int32_t)e;
-    }
-    order();
-}
-
-__device__ __forceinline__ float wave_max(float v) {
-    v = __builtin_fmaxf(v, dpp<QUAD_XOR1>(v));
-    v = __builtin_fmaxf(v, dpp<QUAD_XOR2>(v));
-    v = __builtin_fmaxf(v, dpp<ROW_ROR4>(v));
-    v = __builtin_fmaxf(v, dpp<ROW_ROR8>(v));
-    v = __builtin_fmaxf(v, __shfl_xor(v, 16));
-    return __builtin_fmaxf(v, __shfl_xor(v, 32));
-}
-__device__ __forceinline__ float wave_total(float v) {
-    v += dpp<QUAD_XOR1>(v);
-    v += dpp<QUAD_XOR2>(v);
-    v += dpp<ROW_ROR4>(v);
-    v += dpp<ROW_ROR8>(v);
-    v += __shfl_xor(v, 16);
-    return v + __shfl_xor(v, 32);
-}
-// One wave: the choice of token t and its weights to the workspace and to the caller.
-__device__ __forceinline__ void put_choice(const MoeArgs &a, uint32_t t, const int32_t *ids, uint32_t lane) {
-    const float *l = a.logits + (uint64_t)t * a.experts;
-    float top = -__builtin_inff(), total = 0.0f;
-    if (!a.sigmoid) {
-        for (uint32_t e = lane; e < a.experts; e += 64) top = __builtin_fmaxf(top, l[e]);
-        top = wave_max(top);
-        for (uint32_t e = lane; e < a.experts; e += 64) total += expf(l[e] - top);
-        total = wave_total(total);
-    }
-    float p = 0.0f;
-    if (lane < a.top_k) {
-        const float v = l[ids[lane]];
-        p = a.sigmoid ? 1.0f / (1.0f + expf(-v)) : expf(v - top) / total;
-    }
-    const float sum = wave_total(p);
-    if (lane < a.top_k) {
-        const uint32_t at = t * a.top_k + lane;
-        const float w = (a.normalize ? p / sum : p) * a.scale;
-        a.ids[at] = ids[lane];
-        a.weights[at] = w;
-        if (a.out_ids) a.out_ids[at] = ids[lane];
-        if (a.out_weights) a.out_weights[at] = w;
-    }
-}
-
-// The choice of all tokens, a workgroup for each
-__global__ __launch_bounds__(MV_THREADS) static void moe_route(MoeArgs a) {
-    __shared__ uint32_t keys[MOE_MAX_EXPERTS];
-    __shared__ int32_t ids[MOE_MAX_TOP_K];
-    const uint32_t t = blockIdx.x;
-    choose(a.logits + (uint64_t)t * a.experts, a.experts, a.top_k, threadIdx.x, MV_THREADS, keys, ids, [] { __syncthreads(); });
-    if (threadIdx.x < 64) put_choice(a, t, ids, threadIdx.x);
-}
 
 __device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
     if (!gelu) return g / (1.0f + expf(-g));
@@ -180,7 +20,6 @@ __device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
 
 // ---- which expert, and which tokens ----------------------------------------------------------------------
 // Experts in use, in the order of their index, each with its tokens 16 at a time: a slot is one such group.
-constexpr uint32_t SLOT_TOKENS = 16;
 struct Slot {
     uint32_t expert, count;       // of tokens; 0: no such slot
 };
@@ -412,19 +251,6 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_many(MoeArgs a) {
     }
     down_rows<F, Many>(a, lds, slot, space.pair, a.chunk);
 }
-// ... and the sum over a token's experts, in order
-__global__ __launch_bounds__(MV_THREADS) static void moe_sum(MoeArgs a) {
-    const uint64_t r = (uint64_t)blockIdx.x * MV_THREADS + threadIdx.x;
-    if (r >= a.hidden) return;
-    const uint32_t t = blockIdx.y;
-    float y = 0.0f;
-    for (uint32_t j = 0; j < a.top_k; ++j) {
-        const uint64_t pair = t * a.top_k + j;
-        y = __builtin_fmaf(a.weights[pair], a.o[pair * a.hidden + r], y);
-    }
-    store_elem(a.y, t * a.y_stride + r, a.y_kind, y);
-}
-
 // Experts with rows of 16-bit floats shorter than a piece of an image: a thread per output.
 template <class F>
 __device__ __forceinline__ float short_dot(const uint8_t *row, uint32_t cols, const void *x, uint64_t at, uint32_t kind) {

@@ -72,8 +72,8 @@ template <class F> struct Slice;
 struct WF16 { static constexpr uint32_t N = 1, BYTES = 2; };
 struct WBF16 { static constexpr uint32_t N = 1, BYTES = 2; };
 template <class F> constexpr bool is_float_type = false;
-template <> constexpr bool is_float_type<WF16> = true;
-template <> constexpr bool is_float_type<WBF16> = true;
+template <> inline constexpr bool is_float_type<WF16> = true;
+template <> inline constexpr bool is_float_type<WBF16> = true;
 
 #define GGQ_LOW(N) template <int S> static __device__ __forceinline__ void low(const Raw &r, uint32_t (&b)[N])
 #define GGQ_HIGH(N) template <int S> static __device__ __forceinline__ void high(const Raw &r, uint32_t (&b)[N])
