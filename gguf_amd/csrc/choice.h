@@ -18,9 +18,9 @@ struct MoeArgs {
     uint64_t hidden, ff, x_stride, y_stride;
     uint32_t tokens, experts, top_k, router_kind, x_kind, y_kind;
     uint32_t sigmoid, normalize, gelu;
-    uint32_t ksplit, chunk, chunk_one;        // as in MatvecArgs, of the launch; chunk_one: of experts with one token
+    uint32_t ksplit, chunk;                   // as in MatvecArgs, of the launch
     uint32_t choose;                          // the workgroups of gate and up find the choice themselves
-    uint32_t slots;                           // most slots there may be: workgroups along y
+    uint32_t slots, slot_tokens;              // most slots there may be, workgroups along y; most tokens of one
     float scale;
 };
 
@@ -33,7 +33,7 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 
 // ---- the choice -----------------------------------------------------------------------------------------
 constexpr uint32_t MOE_MAX_EXPERTS = 512, MOE_MAX_TOP_K = 32, MOE_MAX_TOKENS = 64;
-constexpr uint32_t SLOT_TOKENS = 16;          // most tokens of one expert that a workgroup takes
+constexpr uint32_t SLOT_TOKENS = 16;          // most tokens of one expert that a workgroup may take
 constexpr uint32_t FEW_TOKENS = 4;            // most tokens whose sum over experts is made in the kernel of down
 constexpr uint32_t CHOOSE_TOKENS = 8;         // most tokens whose choice the workgroups of gate and up find themselves
 

@@ -304,120 +304,6 @@ template <> struct Step<WBF16> : StepOfFloats<WBF16> {};
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
-// The members of Tile (matmul.h), for up to 16 tokens.
-// Staged x, per turn: [piece][fragment of 8 elements][token] 16 bytes, 32 bytes between one fragment and the next for the
-// staging threads' banks; then the sums of x over each sub-block, [sub-block][token], f32.
-template <class F, int P>
-struct OldTile {
-    typedef Step<F> S;
-    static constexpr uint32_t ROWS = 16, ELEMS = 256, TOKENS = 16;
-    typedef Image<F, ROWS, 1> I;
-    static constexpr uint32_t FRAG = TOKENS * 16 + 32, PIECE = 32 * FRAG, SUBS = 256 / S::SUB;
-    static constexpr uint32_t SUMS = P * PIECE, X_BYTES = SUMS + (S::OFFSET ? SUBS * TOKENS * 4 : 0), CLEAR = 0;
-    static constexpr uint32_t WAVE_BYTES = I::BYTES + (is_float_type<F> ? 0 : SUBS * ROWS * 8);       // the image, then {a, c} [sub-block][row]
-
-    template <class Load>
-    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t tokens, Load load) {
-        // four lanes side by side take 32 neighbouring elements of a token
-        const uint32_t quads = turns * 8 * tokens;
-        for (uint32_t i = threadIdx.x; i < quads * 4; i += TILE_THREADS) {
-            const uint32_t q = i / 4, t = q % tokens, n = q / tokens, turn = n / 8, f = n % 8 * 4 + i % 4;
-            uint8_t *to = lds + turn * X_BYTES;
-            float v[8];
-            load(turn, t, f * 8, v);
-            if constexpr (S::OFFSET) {
-                float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-                sum += dpp<QUAD_XOR1>(sum);
-                if (S::SUB == 32) sum += dpp<QUAD_XOR2>(sum);
-                if (f % (S::SUB / 8) == 0) ((float *)(to + SUMS))[f / (S::SUB / 8) * TOKENS + t] = sum;
-            }
-            to += f * FRAG + t * 16;
-#pragma unroll
-            for (int p = 0; p < P; ++p) {
-                *(u32x4 *)(to + p * PIECE) = u32x4{upper_halves(v[0], v[1]), upper_halves(v[2], v[3]), upper_halves(v[4], v[5]), upper_halves(v[6], v[7])};
-                if (p + 1 < P)
-#pragma unroll
-                    for (int k = 0; k < 8; ++k) v[k] = below_bf16(v[k]);
-            }
-        }
-    }
-    struct Me {
-        uint32_t n, g;
-        __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) : n(lane % 16), g(lane / 16) {}
-    };
-    struct Sums { float v[4]; };                 // of tokens 4 g .. 4 g + 3
-    static __device__ __forceinline__ void add(uint8_t *image, const Me &me, const uint8_t *, const uint8_t *x, uint32_t left, uint32_t, Sums &acc) {
-        const uint8_t *row = image + me.n * I::ROW;
-        if constexpr (is_float_type<F>) {
-            f32x4 d = {acc.v[0], acc.v[1], acc.v[2], acc.v[3]};
-#pragma unroll
-            for (uint32_t s = 0; s < SUBS; ++s) {
-                u32x4 b = S::load(row, s, me.g, left), low = {0, 0, 0, 0};
-                if constexpr (__is_same(F, WF16)) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const uint32_t w = b[i];
-                        const float v0 = h2f(w & 0xFFFFu), v1 = h2f(w >> 16);
-                        b[i] = upper_halves(v0, v1);
-                        low[i] = upper_halves(below_bf16(v0), below_bf16(v1));
-                    }
-                }
-#pragma unroll
-                for (int p = 0; p < P; ++p) {
-                    const bf16x8 a = __builtin_bit_cast(bf16x8, al16(x + p * PIECE + (4 * s + me.g) * FRAG + me.n * 16));
-                    d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, b), d, 0, 0, 0);
-                    if constexpr (__is_same(F, WF16)) d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(bf16x8, low), d, 0, 0, 0);
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) acc.v[r] = d[r];
-        } else {
-            float *scales = (float *)(image + I::BYTES);
-            constexpr uint32_t EACH = SUBS / 4;
-            SubScale mine[EACH];
-            S::scale(row, me.g, left, mine);
-#pragma unroll
-            for (uint32_t k = 0; k < EACH; ++k) *(f32x2 *)(scales + ((me.g * EACH + k) * ROWS + me.n) * 2) = f32x2{mine[k].a, mine[k].c};
-            wave_order();
-#pragma unroll
-            for (uint32_t s = 0; s < SUBS; ++s) {
-                f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
-                if constexpr (S::SUB == 32) {
-                    uint32_t b[4];
-                    S::codes(row, s, me.g, b);
-                    const bf16x8 w = __builtin_bit_cast(bf16x8, u32x4{b[0], b[1], b[2], b[3]});
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        const u32x4 a = al16(x + p * PIECE + (4 * s + me.g) * FRAG + me.n * 16);
-                        d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), w, d, 0, 0, 0);
-                    }
-                } else {
-                    uint32_t b[2];
-                    S::codes(row, s, me.g, b);
-                    const s16x4 w = __builtin_bit_cast(s16x4, u32x2{b[0], b[1]});
-#pragma unroll
-                    for (int p = 0; p < P; ++p) {
-                        const u32x2 a = al8(x + p * PIECE + (2 * s + (me.g >> 1)) * FRAG + me.n * 16 + 8 * (me.g & 1));
-                        d = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), w, d, 0, 0, 0);
-                    }
-                }
-                const f32x2 k = *(const f32x2 *)(scales + (s * ROWS + me.n) * 2);
-                const f32x4 sum = *(const f32x4 *)(x + SUMS + (s * TOKENS + 4 * me.g) * 4);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    acc.v[r] = __builtin_fmaf(k[0], d[r], acc.v[r]);
-                    if constexpr (S::OFFSET) acc.v[r] = __builtin_fmaf(-k[1], sum[r], acc.v[r]);
-                }
-            }
-        }
-    }
-    static __device__ __forceinline__ void put(float *part, uint32_t lane, const Sums &acc) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) part[(4 * (lane / 16) + r) * ROWS + lane % 16] = acc.v[r];
-    }
-};
-
-
 // How x goes into the matrix unit: its type, and the bf16 pieces that a value is cut into
 enum XForm : int { X_BF16, X_F16, X_F32_2, X_F32_3 };
 
@@ -435,7 +321,7 @@ struct Factor {
 template <class F, int X, int R>
 struct DenseTile {
     typedef Step<F> S;
-    static constexpr uint32_t ROWS = 16, ELEMS = 256, TOKENS = 16;
+    static constexpr uint32_t TILES = R, ROWS = 16, ELEMS = 256, TOKENS = 16;
     typedef Image<F, ROWS, 1> I;
     static constexpr bool WIDE = X == X_F32_2 || X == X_F32_3;
     static constexpr int P = X == X_BF16 ? 1 : X == X_F32_3 ? 3 : 2;
@@ -448,6 +334,10 @@ struct DenseTile {
     static constexpr uint32_t AT_X = R * (I::BYTES + SCALES);
     static constexpr __host__ __device__ __forceinline__ uint32_t wave_bytes(uint32_t tokens) { return AT_X + (tokens + 1) / 2 * 2 * X_ROW; }
 
+    // a sum of the wave's, after dense_turns
+    static __device__ __forceinline__ float part(const uint8_t *space, uint32_t tile, uint32_t token, uint32_t row) {
+        return *(const float *)(space + tile * PART + (token * ROWS + row) * 4);
+    }
     typedef float Values[N];
     // N elements as pieces, in words of two
     static __device__ __forceinline__ void cut(Values &v, uint32_t (&out)[P][N / 2]) {
@@ -584,7 +474,7 @@ struct DenseTile {
 // The wave's turns kp, kp + waves, ..., the next one's bytes on the way while one is multiplied; then its sums, in the place of
 // the images, [tile][token][row].
 //     at(turn, r)        the packed bytes of tile r, as in run_turns
-//     src(turn, t)       the first element of token t in that turn
+//     src(turn, t)       the first element of token t's row
 //     col(turn)          its first column, of `cols`
 //     factor(turn, t)    of token t, for FACTOR
 template <class M, int R, bool FACTOR, class At, class Src, class Col, class FactorOf>
@@ -596,36 +486,25 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
     const uint8_t *x = xs + token * M::X_ROW;
     typename M::I in[R];
     u32x4 xr[M::X_LOADS];
-    uint32_t left = 0;
+    uint64_t room[R];
+    uint32_t left = 0, column = 0;
     const uint32_t x_need = M::WIDE ? tokens : (tokens + 1) / 2, x_slot = M::WIDE ? 0 : lane / 32, x_at = (M::WIDE ? lane : lane % 32) * M::X_EACH;
+    // 16 bytes of x that would end behind the row are moved back to end with it, and shifted when they are put
+    const uint32_t x_last = cols - M::X_EACH;
     auto fetch = [&](uint32_t turn) {
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const Turn t = at(turn, r);
-            in[r].fetch(places, t.base, t.room, reach);
+            in[r].fetch(places, t.base, t.room);
+            room[r] = t.room;
             left = t.left;
         }
-        const uint32_t c = col(turn);
+        column = col(turn);
+        const uint32_t from = (column + x_at < x_last ? column + x_at : x_last) * M::X_SIZE;
 #pragma unroll
         for (uint32_t i = 0; i < M::X_LOADS; ++i) {
-            if (i < x_need) {
-            const uint32_t slot = M::WIDE ? i : 2 * i + x_slot, t = slot < tokens ? slot : tokens - 1;
-            const uint8_t *p = src(turn, t) + x_at * M::X_SIZE;
-            u32x4 v = {0, 0, 0, 0};
-            if (c + x_at + M::X_EACH <= cols) {
-                v = ld16(p);
-            } else if (M::WIDE) {
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) v[j] = c + x_at + j < cols ? ld4(p + 4 * j) : 0u;
-            } else {
-#pragma unroll
-                for (uint32_t j = 0; j < 4; ++j) {
-                    const uint32_t lo = c + x_at + 2 * j < cols ? ld2(p + 4 * j) : 0u, hi = c + x_at + 2 * j + 1 < cols ? ld2(p + 4 * j + 2) : 0u;
-                    v[j] = lo | (hi << 16);
-                }
-            }
-            xr[i] = v;
-            }
+            const uint32_t slot = M::WIDE ? i : 2 * i + x_slot;
+            if (i < x_need) xr[i] = ld16(src(turn, slot < tokens ? slot : tokens - 1) + from);
         }
     };
     f32x4 acc[R];
@@ -635,10 +514,16 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
     for (uint32_t turn = kp; turn < turns; turn += waves) {
         wave_order();
 #pragma unroll
-        for (int r = 0; r < R; ++r) in[r].put(places, space + r * M::I::BYTES);
+        for (int r = 0; r < R; ++r) in[r].put(places, space + r * M::I::BYTES, room[r], reach);
+        if (column + M::ELEMS <= cols) {
 #pragma unroll
-        for (uint32_t i = 0; i < M::X_LOADS; ++i) {
-            if (i < x_need) *(u32x4 *)(xs + (M::WIDE ? i : 2 * i + x_slot) * M::X_ROW + x_at * M::X_SIZE) = xr[i];
+            for (uint32_t i = 0; i < M::X_LOADS; ++i)
+                if (i < x_need) *(u32x4 *)(xs + (M::WIDE ? i : 2 * i + x_slot) * M::X_ROW + x_at * M::X_SIZE) = xr[i];
+        } else {                                          // behind the row: zeros
+            const uint32_t c = column + x_at, back = c > x_last ? (c - x_last) * M::X_SIZE : 0u;
+#pragma unroll
+            for (uint32_t i = 0; i < M::X_LOADS; ++i)
+                if (i < x_need) *(u32x4 *)(xs + (M::WIDE ? i : 2 * i + x_slot) * M::X_ROW + x_at * M::X_SIZE) = back < 16 ? M::I::shifted(xr[i], back) : u32x4{0, 0, 0, 0};
         }
         wave_order();
         const uint32_t here = left;
@@ -654,10 +539,13 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
         for (uint32_t i = 0; i < 4; ++i) *(float *)(space + r * M::PART + ((4 * g + i) * M::ROWS + n) * 4) = acc[r][i];
 }
 
+// Waves of a CU that the registers of R tiles leave room for.
+constexpr int dense_waves_per_cu(int R) { return R == 1 ? 12 : 8; }
+
 // ---- one matrix, several tokens ---------------------------------------------------------------------------------
 // A workgroup takes R tiles of rows, its waves share their columns.
 template <class F, int X, int R>
-__global__ __launch_bounds__(TILE_THREADS) void matvec_dense(MatvecArgs a) {
+__global__ __launch_bounds__(TILE_THREADS) __attribute__((amdgpu_waves_per_eu(dense_waves_per_cu(R) / 4))) void matvec_dense(MatvecArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
     typedef DenseTile<F, X, R> M;
     typedef typename M::I I;
@@ -674,14 +562,14 @@ __global__ __launch_bounds__(TILE_THREADS) void matvec_dense(MatvecArgs a) {
                                  const uint32_t off = turn * I::TURN_BYTES;
                                  return Turn{a.w + row * row_bytes + off, row_bytes - off, (a.rows - row) * row_bytes - off};
                              },
-                             [&](uint32_t turn, uint32_t t) { return (const uint8_t *)a.x + (t * a.x_stride + turn * M::ELEMS) * M::X_SIZE; },
+                             [&](uint32_t turn, uint32_t t) { return (const uint8_t *)a.x + t * a.x_stride * M::X_SIZE; },
                              [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < R * M::ROWS * a.tokens; i += blockDim.x) {
         const uint32_t r = i % (R * M::ROWS) / M::ROWS, n = i % M::ROWS, t = i / (R * M::ROWS);
         const uint64_t row = begin(r) + n;
         float v = 0.0f;
-        for (uint32_t k = 0; k < waves; ++k) v += *(const float *)(lds + k * wave_bytes + r * M::PART + (t * M::ROWS + n) * 4);
+        for (uint32_t k = 0; k < waves; ++k) v += M::part(lds + k * wave_bytes, r, t, n);
         if (row >= first_row + r * M::ROWS && row < a.rows) store_elem(a.y, t * a.y_stride + row, a.y_kind, v);
     }
 }

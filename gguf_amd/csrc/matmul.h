@@ -129,24 +129,17 @@ struct Image {
     u32x4 v[LOADS];
 
     // The turn that begins at `base` (in the tile's first row).  A unit's last piece and a row's last turn may reach beyond
-    // them, into whatever follows in the tensor; `room` bytes of the tensor are left from base on, and where the furthest
-    // piece would end behind them, pieces are moved back to end with it and shifted into place.
-    __device__ __forceinline__ void fetch(const Places &at, const uint8_t *base, uint64_t room, uint32_t reach) {
-        if (room >= reach) {
+    // them, into whatever follows in the tensor; `room` bytes of the tensor are left from base on, and pieces that would end
+    // behind them are moved back to end with it.  put shifts those into place: without a second way through fetch the loads
+    // in flight keep their registers.
+    static __device__ __forceinline__ uint32_t limit(uint64_t room) { return room < (1u << 31) ? (uint32_t)room - 16 : (1u << 31) - 16; }
+    __device__ __forceinline__ void fetch(const Places &at, const uint8_t *base, uint64_t room) {
+        const uint32_t most = limit(room);
 #pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i) {
-                uint32_t o = at.src[i];
-                asm("" : "+v"(o));            // keeps the offset 32 bits wide, for a load with a scalar base
-                v[i] = ld16(base + o);
-            }
-        } else {
-            const int32_t limit = (int32_t)room - 16;
-#pragma unroll
-            for (uint32_t i = 0; i < LOADS; ++i) {
-                const int32_t from = (int32_t)at.src[i] < limit ? (int32_t)at.src[i] : limit;
-                const uint32_t back = at.src[i] - (uint32_t)from;
-                v[i] = shifted(ld16(base + from), back < 15 ? back : 15);
-            }
+        for (uint32_t i = 0; i < LOADS; ++i) {
+            uint32_t o = at.src[i] < most ? at.src[i] : most;
+            asm("" : "+v"(o));                // keeps the offset 32 bits wide, for a load with a scalar base
+            v[i] = ld16(base + o);
         }
     }
     static __device__ __forceinline__ u32x4 shifted(u32x4 a, uint32_t bytes) {
@@ -160,21 +153,30 @@ struct Image {
         }
         return {o[0], o[1], o[2], o[3]};
     }
-    __device__ __forceinline__ void put(const Places &at, uint8_t *image) const {
+    __device__ __forceinline__ void put(const Places &at, uint8_t *image, uint64_t room, uint32_t reach) const {
+        if (room >= reach) {
 #pragma unroll
-        for (uint32_t i = 0; i < LOADS; ++i) *(u32x4 *)(image + at.dst[i]) = v[i];
+            for (uint32_t i = 0; i < LOADS; ++i) *(u32x4 *)(image + at.dst[i]) = v[i];
+        } else {
+            const uint32_t most = limit(room);
+#pragma unroll
+            for (uint32_t i = 0; i < LOADS; ++i) {
+                const uint32_t back = at.src[i] > most ? at.src[i] - most : 0u;
+                *(u32x4 *)(image + at.dst[i]) = shifted(v[i], back < 15 ? back : 15);
+            }
+        }
     }
 };
 
-// What a wave does with a tile of rows, for up to TOKENS tokens.  Three kinds, with the same members (the third: dense.h):
+// What a wave does with a tile of rows and one token.  Two kinds, with the same members:
 //     ROWS, ELEMS       rows of the tile, elements of a turn
 //     X_BYTES           shared memory of a turn of x
 //     CLEAR             bytes of zeros in front of the staged x
+//     WAVE_BYTES        shared memory of a wave: its image
 //     stage             puts turns of x into shared memory
 //     Me                what a lane knows of its place
 //     add               the products of one turn
-//     put               the wave's sums to part[token][row]
-//     TOKENS            rows of part; WAVE_BYTES: shared memory of a wave, its image first
+//     put               the wave's sums to part[row]
 
 // ---- packed whole-number codes, one token: x in digits ------------------------------------------------------
 // The matrix unit multiplies e4m3 bytes with a block scale for each 32 of them.  Codes are such bytes already (slices.h),
@@ -197,20 +199,20 @@ struct Image {
 template <class F, int CH>
 struct CodeTile {
     typedef Slice<F> S;
-    static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN, TOKENS = 1;
+    static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN;
     typedef Image<F, ROWS, S::TURN> I;
     static constexpr uint32_t DIGITS = CH * 1024, EXPS = DIGITS * S::TURN, SUMS = EXPS + 8 * S::TURN + 8 * (S::TURN & 1);
     static constexpr uint32_t X_BYTES = SUMS + 16 * S::NSUB * S::TURN, CLEAR = DIGITS, WAVE_BYTES = I::BYTES;
 
     template <class Load>
-    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t, Load load) {
+    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, Load load) {
         constexpr uint32_t FRAGS = 32 * S::TURN;               // of eight elements; four lanes side by side have a block
         for (uint32_t i = threadIdx.x; i < FRAGS * turns; i += TILE_THREADS) {
             const uint32_t turn = i / FRAGS, f = i % FRAGS;
             const uint32_t step = f / 32, block = f / 4 % 8, half = f / 2 % 2;
             uint8_t *to = lds + turn * X_BYTES;
             float v[8];
-            load(turn, 0, f * 8, v);
+            load(turn, f * 8, v);
             float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
             sum += dpp<QUAD_XOR1>(sum);
             float *sums = (float *)(to + SUMS) + step * 4 * S::NSUB;
@@ -333,7 +335,7 @@ struct CodeTile {
     }
     // one turn: `image` the wave's bytes, `x` the turn's staged x, `clear` the zeros, `left` bytes of the row from the turn on
     static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *clear, const uint8_t *x, uint32_t left,
-                                               uint32_t, Sums &acc) {
+                                               Sums &acc) {
 #pragma unroll
         for (uint32_t step = 0; step < S::TURN; ++step) {
             typename S::Raw raw;
@@ -370,16 +372,16 @@ struct CodeTile {
 template <class F, int CH>
 struct FloatTile {
     typedef Slice<F> S;
-    static constexpr uint32_t ROWS = 4, ELEMS = 1024, TOKENS = 1;
+    static constexpr uint32_t ROWS = 4, ELEMS = 1024;
     typedef Image<F, ROWS, S::TURN> I;
     static constexpr uint32_t K = 256 + 16, X_BYTES = CH * 8 * K, CLEAR = 0, WAVE_BYTES = I::BYTES;
 
     template <class Load>
-    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, uint32_t, Load load) {
+    static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, Load load) {
         for (uint32_t i = threadIdx.x; i < 128 * turns; i += TILE_THREADS) {
             const uint32_t turn = i / 128, f = i % 128;
             float v[8];
-            load(turn, 0, f * 8, v);
+            load(turn, f * 8, v);
             uint8_t *to = lds + turn * X_BYTES + f % 8 * K + f / 8 * 16;
 #pragma unroll
             for (int p = 0; p < CH; ++p) {
@@ -395,7 +397,7 @@ struct FloatTile {
         __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) : quad(lane / 4), row(lane % 4 * I::ROW), x(lane / 4 * 16) {}
     };
     struct Sums { float v[1]; };
-    static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *, const uint8_t *x, uint32_t left, uint32_t, Sums &acc) {
+    static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *, const uint8_t *x, uint32_t left, Sums &acc) {
         typename S::Raw raw;
         raw.load(image + me.row, me.quad, left);
         f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -433,13 +435,13 @@ struct FloatTile {
 // The wave's part of a tile: turns kp, kp + ksplit, ... of `turns`, the next one's bytes on the way while one is multiplied.
 // All waves of the workgroup call this together, since they stage x for each other, `chunk` turns at a time.
 //     at(turn)           {where the turn begins in the tile's first row, bytes of the row and of the tensor from there on}
-//     load(turn, t, c, v)   elements [c, c + 8) of token t in that turn
+//     load(turn, c, v)   elements [c, c + 8) of x in that turn
 struct Turn {
     const uint8_t *base;
     uint32_t left;
     uint64_t room;
 };
-struct Share { uint32_t kp, ksplit, chunk, turns, tokens; };
+struct Share { uint32_t kp, ksplit, chunk, turns; };
 template <class M, class At, class Load>
 __device__ __forceinline__ void run_turns(uint8_t *image, uint8_t *clear, const typename M::I::Places &places, uint32_t reach, const Share &sh, At at, Load load,
                                           typename M::Sums &acc) {
@@ -447,34 +449,34 @@ __device__ __forceinline__ void run_turns(uint8_t *image, uint8_t *clear, const 
     uint8_t *xs = clear + M::CLEAR;
     const typename M::Me me(lane, clear);
     typename M::I in;
-    uint32_t left = 0, turn = sh.kp;
+    Turn next{};
+    uint32_t turn = sh.kp;
     auto fetch = [&](uint32_t n) {
-        const Turn t = at(n);
-        in.fetch(places, t.base, t.room, reach);
-        return t.left;
+        next = at(n);
+        in.fetch(places, next.base, next.room);
     };
-    if (turn < sh.turns) left = fetch(turn);
+    if (turn < sh.turns) fetch(turn);
     for (uint32_t i = threadIdx.x * 16; i < M::CLEAR; i += TILE_THREADS * 16) *(u32x4 *)(clear + i) = u32x4{0, 0, 0, 0};
     for (uint32_t first = 0; first < sh.turns; first += sh.chunk) {
         const uint32_t now = first + sh.chunk < sh.turns ? sh.chunk : sh.turns - first, end = first + now;
         if (first) __syncthreads();
-        M::stage(xs, now, sh.tokens, [&](uint32_t n, uint32_t t, uint32_t c, float (&v)[8]) { load(first + n, t, c, v); });
+        M::stage(xs, now, [&](uint32_t n, uint32_t c, float (&v)[8]) { load(first + n, c, v); });
         __syncthreads();
         for (; turn < end; turn += sh.ksplit) {
             wave_order();
-            in.put(places, image);
+            in.put(places, image, next.room, reach);
             wave_order();
-            const uint32_t here = left;
-            if (turn + sh.ksplit < sh.turns) left = fetch(turn + sh.ksplit);
-            M::add(image, me, clear, xs + (turn - first) * M::X_BYTES, here, sh.tokens, acc);
+            const uint32_t here = next.left;
+            if (turn + sh.ksplit < sh.turns) fetch(turn + sh.ksplit);
+            M::add(image, me, clear, xs + (turn - first) * M::X_BYTES, here, acc);
         }
     }
 }
-// The waves' sums to part[wave][token][row].
+// The waves' sums to part[wave][row].
 template <class M>
 __device__ __forceinline__ void put_parts(float *part, uint32_t wave, const typename M::Sums &acc) {
     __syncthreads();                                   // the staged x is no longer needed
-    M::put(part + wave * M::TOKENS * M::ROWS, threadIdx.x % 64, acc);
+    M::put(part + wave * M::ROWS, threadIdx.x % 64, acc);
     __syncthreads();
 }
 template <class M>
@@ -486,7 +488,7 @@ __device__ __forceinline__ typename M::Sums no_sums() {
 }
 
 // ---- one matrix -----------------------------------------------------------------------------------------------
-// Up to M::TOKENS tokens.  A wave owns a tile of rows, or shares it with others that take other turns of its columns.
+// One token.  A wave owns a tile of rows, or shares it with others that take other turns of its columns.
 template <class F, class M>
 __global__ __launch_bounds__(TILE_THREADS) void matvec_tiles(MatvecArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
@@ -503,22 +505,20 @@ __global__ __launch_bounds__(TILE_THREADS) void matvec_tiles(MatvecArgs a) {
     uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;
     typename M::Sums acc = no_sums<M>();
     run_turns<M>(lds + wave * M::WAVE_BYTES, clear, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes),
-                 Share{wave % a.ksplit, a.ksplit, a.chunk, turns, a.tokens},
+                 Share{wave % a.ksplit, a.ksplit, a.chunk, turns},
                  [&](uint32_t turn) {
                      const uint32_t off = turn * I::TURN_BYTES;
                      return Turn{w + off, row_bytes - off, behind + row_bytes - off};
                  },
-                 [&](uint32_t turn, uint32_t t, uint32_t c, float (&v)[8]) {
-                     load8(a.x, t * a.x_stride, (uint64_t)turn * M::ELEMS + c, a.cols, a.x_kind, v);
-                 },
+                 [&](uint32_t turn, uint32_t c, float (&v)[8]) { load8(a.x, 0, (uint64_t)turn * M::ELEMS + c, a.cols, a.x_kind, v); },
                  acc);
     float *part = (float *)(clear + M::CLEAR);
     put_parts<M>(part, wave, acc);
-    for (uint32_t i = threadIdx.x; i < groups * M::ROWS * a.tokens; i += TILE_THREADS) {
-        const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
+    for (uint32_t r = threadIdx.x; r < groups * M::ROWS; r += TILE_THREADS) {
+        const uint32_t g = r / M::ROWS;
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[((g * a.ksplit + k) * M::TOKENS + t) * M::ROWS + r % M::ROWS];
-        if (first_row + r < a.rows) store_elem(a.y, t * a.y_stride + first_row + r, a.y_kind, v);
+        for (uint32_t k = 0; k < a.ksplit; ++k) v += part[(g * a.ksplit + k) * M::ROWS + r % M::ROWS];
+        if (first_row + r < a.rows) store_elem(a.y, first_row + r, a.y_kind, v);
     }
 }
 

@@ -226,9 +226,11 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     // Comparing each expert with each is on every workgroup's way; the launch that it saves takes about 2.5 us.
     a.choose = tokens <= CHOOSE_TOKENS && m->experts <= 128 && !short_rows(m->up_type, m->hidden);
     if (!a.choose) moe_route<<<(uint32_t)tokens, MV_THREADS, 0, st>>>(a);
-    // groups of up to 16 pairs with the same expert: one for each pair, or one for each expert and one more for each 16 pairs
+    // groups of pairs with the same expert: one for each pair, or one for each expert and one more for each slot_tokens pairs.
+    // Shared memory is kept for as many tokens: where experts have four on average, or fewer, more than eight are rare.
     const uint32_t pairs = (uint32_t)tokens * m->top_k, in_use = std::min(m->experts, pairs);
-    a.slots = std::min(pairs, in_use + (pairs - in_use) / SLOT_TOKENS);
+    a.slot_tokens = std::min((uint32_t)tokens, pairs > 4 * m->experts ? SLOT_TOKENS : SLOT_TOKENS / 2);
+    a.slots = std::min(pairs, in_use + (pairs - in_use) / a.slot_tokens);
 #define CASE(F) Launch<F>::up(a, st)
     GGQ_FOR_TYPE(m->up_type, CASE)
 #undef CASE

@@ -30,14 +30,13 @@ struct Shape {
         return (rounds + chunks - 1) / chunks * ksplit;
     }
     template <class M> uint32_t bytes(uint32_t turns) const {
-        return TILE_WAVES * M::WAVE_BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk<M>(turns), turns) * M::X_BYTES, TILE_WAVES * M::TOKENS * M::ROWS * 4);
+        return TILE_WAVES * M::WAVE_BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk<M>(turns), turns) * M::X_BYTES, TILE_WAVES * M::ROWS * 4);
     }
 };
 template <class M> constexpr uint32_t turns_of(uint64_t cols) { return (uint32_t)((cols + M::ELEMS - 1) / M::ELEMS); }
 
 template <class F, class M>
-uint64_t launch_tiles(MatvecArgs a, uint64_t tokens, hipStream_t st) {
-    a.tokens = (uint32_t)std::min<uint64_t>(tokens, M::TOKENS);
+uint64_t launch_tiles(MatvecArgs a, hipStream_t st) {
     const uint64_t tiles = (a.rows + M::ROWS - 1) / M::ROWS;
     const uint32_t turns = turns_of<M>(a.cols);
     const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
@@ -47,23 +46,40 @@ uint64_t launch_tiles(MatvecArgs a, uint64_t tokens, hipStream_t st) {
         const dim3 grid((uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + sh.groups - 1) / sh.groups));
         matvec_tiles<F, M><<<grid, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
     }
-    return a.tokens;
+    return 1;
 }
 
 // x is taken to 16 bits below an element, or the largest of 32, where the result is rounded to a 16-bit float anyway.
 [[maybe_unused]] bool to_16_bits(uint32_t x_kind, uint32_t y_kind) { return x_kind != EK_F32 && y_kind != EK_F32; }
 
-// Waves that share the columns of a dense tile: as many as there are turns and as fit, all with as many turns or one less.
+// Waves that share the columns of R tiles: no more than `most`, or turns, or fit; all with as many turns or one less.
 template <class M>
-uint32_t dense_waves(uint32_t turns, uint32_t tokens) {
-    const uint32_t most = std::min(std::min(TILE_WAVES, turns), DENSE_LDS / M::wave_bytes(tokens)), rounds = (turns + most - 1) / most;
+uint32_t dense_waves(uint32_t most, uint32_t turns, uint32_t tokens) {
+    most = std::min(std::min(most, turns), DENSE_LDS / M::wave_bytes(tokens));
+    const uint32_t rounds = (turns + most - 1) / most;
     return (turns + rounds - 1) / rounds;
 }
+// How a dense product is cut: R tiles of rows for a workgroup, waves that share their columns.
+struct DenseCut {
+    uint64_t cost = ~0ull;
+    uint32_t R = 0, waves = 0;
+    // `groups`: of waves that share columns.  They run in rounds of what 256 CUs hold; each takes its turns, whose x costs as
+    // much as one more tile, and what a tile and a half takes to begin and end; and the waves of a CU slow each other down.
+    template <class M>
+    void consider(uint64_t groups, uint32_t turns, uint32_t tokens) {
+        for (uint32_t most = TILE_WAVES; most; most /= 2) {
+            const uint32_t w = dense_waves<M>(most, turns, tokens), each = (turns + w - 1) / w;
+            const uint32_t fit = std::max(1u, std::min<uint32_t>(dense_waves_per_cu(M::TILES) / w, DENSE_LDS / (w * M::wave_bytes(tokens))));
+            const uint64_t rounds = (groups + 256 * fit - 1) / (256 * fit), of_cu = (groups + 255) / 256;
+            const uint64_t c = rounds * (2 * each * (M::TILES + 1) + 3) + of_cu * turns * (M::TILES + 1) / 8;
+            if (c < cost) cost = c, R = M::TILES, waves = w;
+        }
+    }
+};
 template <class F, int X, int R>
-void launch_dense_tiles(MatvecArgs a, uint64_t tiles, hipStream_t st) {
+void launch_dense_tiles(MatvecArgs a, uint64_t tiles, uint32_t waves, hipStream_t st) {
     typedef DenseTile<F, X, R> M;
     static_assert(M::wave_bytes(M::TOKENS) <= DENSE_LDS, "a wave's shared memory");
-    const uint32_t waves = dense_waves<M>(turns_of<M>(a.cols), a.tokens);
     for (a.first_tile = 0; a.first_tile < tiles; a.first_tile += MAX_GRID * R) {
         const uint32_t grid = (uint32_t)std::min<uint64_t>(MAX_GRID, (tiles - a.first_tile + R - 1) / R);
         matvec_dense<F, X, R><<<grid, waves * 64, waves * M::wave_bytes(a.tokens), st>>>(a);
@@ -73,16 +89,14 @@ template <class F, int X>
 uint64_t launch_dense(MatvecArgs a, uint64_t tokens, hipStream_t st) {
     a.tokens = (uint32_t)std::min<uint64_t>(tokens, 16);
     const uint64_t tiles = (a.rows + 15) / 16;
-    // tiles of a workgroup: staging x costs as much as one more
-    uint32_t best = 1;
-    uint64_t least = ~0ull;
-    for (uint32_t r = 1; r <= 3; ++r) {
-        const uint64_t cost = ((tiles + r - 1) / r + 255) / 256 * (r + 1);
-        if (cost <= least) best = r, least = cost;
-    }
-    if (best == 1) launch_dense_tiles<F, X, 1>(a, tiles, st);
-    else if (best == 2) launch_dense_tiles<F, X, 2>(a, tiles, st);
-    else launch_dense_tiles<F, X, 3>(a, tiles, st);
+    const uint32_t turns = (uint32_t)((a.cols + 255) / 256);
+    DenseCut cut;
+    cut.consider<DenseTile<F, X, 1>>(tiles, turns, a.tokens);
+    cut.consider<DenseTile<F, X, 2>>((tiles + 1) / 2, turns, a.tokens);
+    cut.consider<DenseTile<F, X, 3>>((tiles + 2) / 3, turns, a.tokens);
+    if (cut.R == 1) launch_dense_tiles<F, X, 1>(a, tiles, cut.waves, st);
+    else if (cut.R == 2) launch_dense_tiles<F, X, 2>(a, tiles, cut.waves, st);
+    else launch_dense_tiles<F, X, 3>(a, tiles, cut.waves, st);
     return a.tokens;
 }
 
@@ -98,12 +112,12 @@ uint64_t Launch<F>::matvec(MatvecArgs a, uint64_t tokens, hipStream_t st) {
             return a.tokens;
         }
         if (tokens == 1) {
-            if (a.x_kind == EK_BF16) return launch_tiles<F, FloatTile<F, 1>>(a, 1, st);
-            if (a.x_kind == EK_F16) return launch_tiles<F, FloatTile<F, 2>>(a, 1, st);
-            return launch_tiles<F, FloatTile<F, 3>>(a, 1, st);
+            if (a.x_kind == EK_BF16) return launch_tiles<F, FloatTile<F, 1>>(a, st);
+            if (a.x_kind == EK_F16) return launch_tiles<F, FloatTile<F, 2>>(a, st);
+            return launch_tiles<F, FloatTile<F, 3>>(a, st);
         }
     } else if (tokens == 1) {
-        return to_16_bits(a.x_kind, a.y_kind) ? launch_tiles<F, CodeTile<F, 1>>(a, 1, st) : launch_tiles<F, CodeTile<F, 2>>(a, 1, st);
+        return to_16_bits(a.x_kind, a.y_kind) ? launch_tiles<F, CodeTile<F, 1>>(a, st) : launch_tiles<F, CodeTile<F, 2>>(a, st);
     }
     if (a.x_kind == EK_BF16) return launch_dense<F, X_BF16>(a, tokens, st);
     if (a.x_kind == EK_F16) return launch_dense<F, X_F16>(a, tokens, st);
@@ -123,78 +137,91 @@ void Launch<F>::rows(const RowsArgs &a, uint32_t y_kind, uint32_t n, hipStream_t
 }
 
 // ---- mixture of experts ---------------------------------------------------------------------------------
-// One: the tile of experts with one token, Many: of the others
-template <class F, class One, class Many>
+namespace {
+// one token
+template <class F, class M>
 void launch_up(MoeArgs a, hipStream_t st) {
-    const uint32_t tiles = (uint32_t)((a.ff + Many::ROWS - 1) / Many::ROWS);
-    static_assert(One::ROWS == Many::ROWS, "one grid for both");
-    const uint32_t one = turns_of<One>(a.hidden), many = turns_of<Many>(a.hidden);
-    const Shape sh(2 * (uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES / 2, std::max(One::X_BYTES, Many::X_BYTES));
+    const uint32_t tiles = (uint32_t)((a.ff + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.hidden);
+    const Shape sh(2 * (uint64_t)tiles * a.slots, turns, TILE_WAVES / 2, M::X_BYTES);
     a.ksplit = sh.ksplit;
-    a.chunk_one = sh.chunk<One>(one);
-    a.chunk = sh.chunk<Many>(many);
-    moe_up<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
+    a.chunk = sh.chunk<M>(turns);
+    moe_up<F, M><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
 }
-
-template <class F>
-void Launch<F>::up(MoeArgs a, hipStream_t st) {
-    if constexpr (is_float_type<F>) {
-        if (a.hidden < 8) {
-            moe_up_short<F><<<dim3((uint32_t)((a.ff + MV_THREADS - 1) / MV_THREADS), a.tokens * a.top_k), MV_THREADS, 0, st>>>(a);
-        } else if (a.x_kind == EK_BF16) {
-            launch_up<F, OldTile<F, 1>, OldTile<F, 1>>(a, st);
-        } else if (a.x_kind == EK_F16) {
-            launch_up<F, OldTile<F, 2>, OldTile<F, 2>>(a, st);
-        } else {
-            launch_up<F, OldTile<F, 3>, OldTile<F, 3>>(a, st);
-        }
-    } else if (a.tokens == 1) {
-        if (to_16_bits(a.x_kind, a.y_kind)) launch_up<F, CodeTile<F, 1>, CodeTile<F, 1>>(a, st);
-        else launch_up<F, CodeTile<F, 2>, CodeTile<F, 2>>(a, st);
-    } else {
-        if (a.x_kind == EK_BF16) launch_up<F, CodeTile<F, 2>, OldTile<F, 1>>(a, st);
-        else if (a.x_kind == EK_F16) launch_up<F, CodeTile<F, 2>, OldTile<F, 2>>(a, st);
-        else launch_up<F, CodeTile<F, 2>, OldTile<F, 3>>(a, st);
-    }
+// Several: as many groups of waves in a workgroup as eight waves are, since each workgroup looks for its slot.
+template <class M>
+uint32_t cut_slots(MoeArgs &a, uint32_t tiles, uint32_t turns) {
+    DenseCut cut;
+    cut.consider<M>((uint64_t)tiles * a.slots, turns, a.slot_tokens);
+    a.ksplit = cut.waves;
+    const uint32_t fit = DENSE_LDS / (cut.waves * M::wave_bytes(a.slot_tokens));
+    return std::max(1u, std::min(std::min(TILE_WAVES / cut.waves, tiles), fit));
 }
-
+template <class F, int X>
+void launch_up_dense(MoeArgs a, hipStream_t st) {
+    typedef DenseTile<F, X, 2> M;
+    const uint32_t tiles = (uint32_t)((a.ff + 15) / 16), groups = cut_slots<M>(a, tiles, turns_of<M>(a.hidden)), waves = groups * a.ksplit;
+    moe_up_dense<F, X><<<dim3((tiles + groups - 1) / groups, a.slots), waves * 64, waves * M::wave_bytes(a.slot_tokens), st>>>(a);
+}
+template <class F, int X>
+void launch_down_dense(MoeArgs a, hipStream_t st) {
+    typedef DenseTile<F, X, DOWN_TILES> M;
+    const uint32_t tiles = (uint32_t)((a.hidden + 16 * DOWN_TILES - 1) / (16 * DOWN_TILES)), groups = cut_slots<M>(a, tiles, turns_of<M>(a.ff)), waves = groups * a.ksplit;
+    moe_down_dense<F, X><<<dim3((tiles + groups - 1) / groups, a.slots), waves * 64, waves * M::wave_bytes(a.slot_tokens), st>>>(a);
+}
 template <class F, class M>
 void launch_down_few(MoeArgs a, hipStream_t st) {
     const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.ff) * a.tokens * a.top_k;
     const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
     a.ksplit = sh.ksplit;
     a.chunk = sh.chunk<M>(turns);
-    moe_down_few<F, M><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
+    moe_down_one<F, M><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
 }
+template <class F, int X>
+void launch_down_few_dense(MoeArgs a, hipStream_t st) {
+    typedef DenseTile<F, X, 1> M;
+    const uint32_t tiles = (uint32_t)((a.hidden + 15) / 16), turns = turns_of<M>(a.ff) * std::min(a.tokens * a.top_k, a.experts);
+    DenseCut cut;
+    cut.consider<M>(tiles, turns, a.tokens);
+    moe_down_few<F, X><<<tiles, cut.waves * 64, cut.waves * M::wave_bytes(a.tokens), st>>>(a);
+}
+}  // namespace
 
-template <class F, class One, class Many>
-void launch_down_many(MoeArgs a, hipStream_t st) {
-    const uint32_t tiles = (uint32_t)((a.hidden + Many::ROWS - 1) / Many::ROWS), one = turns_of<One>(a.ff), many = turns_of<Many>(a.ff);
-    const Shape sh((uint64_t)tiles * a.slots, std::min(one, many), TILE_WAVES, std::max(One::X_BYTES, Many::X_BYTES));
-    a.ksplit = sh.ksplit;
-    a.chunk_one = sh.chunk<One>(one);
-    a.chunk = sh.chunk<Many>(many);
-    moe_down_many<F, One, Many><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, std::max(sh.bytes<One>(one), sh.bytes<Many>(many)), st>>>(a);
+template <class F>
+void Launch<F>::up(MoeArgs a, hipStream_t st) {
+    if constexpr (is_float_type<F>) {
+        if (a.hidden < 8) {
+            moe_up_short<F><<<dim3((uint32_t)((a.ff + MV_THREADS - 1) / MV_THREADS), a.tokens * a.top_k), MV_THREADS, 0, st>>>(a);
+            return;
+        }
+    } else if (a.tokens == 1) {
+        if (to_16_bits(a.x_kind, a.y_kind)) launch_up<F, CodeTile<F, 1>>(a, st);
+        else launch_up<F, CodeTile<F, 2>>(a, st);
+        return;
+    }
+    if (a.x_kind == EK_BF16) launch_up_dense<F, X_BF16>(a, st);
+    else if (a.x_kind == EK_F16) launch_up_dense<F, X_F16>(a, st);
+    else launch_up_dense<F, X_F32_3>(a, st);
 }
 
 template <class F>
 void Launch<F>::down(MoeArgs a, hipStream_t st) {
+    const bool to_16 = to_16_bits(a.x_kind, a.y_kind);
     if constexpr (is_float_type<F>) {
         if (a.ff < 8) {
             moe_down_short<F><<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
-        } else if (a.tokens <= FEW_TOKENS) {
-            launch_down_few<F, OldTile<F, 3>>(a, st);
-        } else {
-            launch_down_many<F, OldTile<F, 3>, OldTile<F, 3>>(a, st);
+            return;
         }
-    } else if (to_16_bits(a.x_kind, a.y_kind)) {
-        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 1>>(a, st);
-        else if (a.tokens <= FEW_TOKENS) launch_down_few<F, OldTile<F, 2>>(a, st);
-        else launch_down_many<F, CodeTile<F, 1>, OldTile<F, 2>>(a, st);
+    } else if (a.tokens == 1) {
+        if (to_16) launch_down_few<F, CodeTile<F, 1>>(a, st);
+        else launch_down_few<F, CodeTile<F, 2>>(a, st);
+        return;
+    }
+    if (a.tokens <= FEW_TOKENS) {
+        if (to_16) launch_down_few_dense<F, X_F32_2>(a, st);
+        else launch_down_few_dense<F, X_F32_3>(a, st);
     } else {
-        if (a.tokens == 1) launch_down_few<F, CodeTile<F, 2>>(a, st);
-        else if (a.tokens <= FEW_TOKENS) launch_down_few<F, OldTile<F, 3>>(a, st);
-        else launch_down_many<F, CodeTile<F, 2>, OldTile<F, 3>>(a, st);
+        if (to_16) launch_down_dense<F, X_F32_2>(a, st);
+        else launch_down_dense<F, X_F32_3>(a, st);
     }
 }
 
