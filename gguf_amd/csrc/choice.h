@@ -4,6 +4,17 @@
 
 namespace ggq {
 
+constexpr uint32_t MOE_MAX_EXPERTS = 512, MOE_MAX_TOP_K = 32, MOE_MAX_TOKENS = 64;
+constexpr uint32_t SLOT_TOKENS = 16;          // most tokens of one expert that a workgroup takes
+constexpr uint32_t FEW_TOKENS = 4;            // most tokens whose sum over experts is made in the kernel of down
+
+// Experts in use, in the order of their index, each with its tokens a few at a time (MoeArgs::slot_tokens): a slot is one such
+// group.
+struct Slot {
+    uint32_t expert, count;           // of tokens; 0: no such slot
+    uint32_t pair[SLOT_TOKENS];       // of the tokens, in order: token * top_k + place
+};
+
 struct MoeArgs {
     const uint8_t *gate, *up, *down;
     const void *router, *x;
@@ -12,15 +23,16 @@ struct MoeArgs {
     int32_t *ids;         // [tokens][top_k]
     float *weights;       // [tokens][top_k]
     float *h;             // [tokens * top_k][ff]
-    float *o;             // [tokens * top_k][hidden], where tokens > 4
+    float *o;             // [tokens * top_k][hidden], where tokens > FEW_TOKENS
+    Slot *table;          // [slots], where tokens > 1
     int32_t *out_ids;     // the caller's, or null
     float *out_weights;
     uint64_t hidden, ff, x_stride, y_stride;
     uint32_t tokens, experts, top_k, router_kind, x_kind, y_kind;
     uint32_t sigmoid, normalize, gelu;
     uint32_t ksplit, chunk;                   // as in MatvecArgs, of the launch
-    uint32_t choose;                          // the workgroups of gate and up find the choice themselves
-    uint32_t slots, slot_tokens;              // most slots there may be, workgroups along y; most tokens of one
+    uint32_t slots, slot_tokens;              // of the table: most there may be; most tokens of one
+    uint32_t slots_expected;                  // where every expert is as likely
     float scale;
 };
 
@@ -32,11 +44,6 @@ __device__ __forceinline__ uint32_t logit_key(float v) {
 }
 
 // ---- the choice -----------------------------------------------------------------------------------------
-constexpr uint32_t MOE_MAX_EXPERTS = 512, MOE_MAX_TOP_K = 32, MOE_MAX_TOKENS = 64;
-constexpr uint32_t SLOT_TOKENS = 16;          // most tokens of one expert that a workgroup may take
-constexpr uint32_t FEW_TOKENS = 4;            // most tokens whose sum over experts is made in the kernel of down
-constexpr uint32_t CHOOSE_TOKENS = 8;         // most tokens whose choice the workgroups of gate and up find themselves
-
 // The top_k experts of a token, ids[j] = the j-th.  An expert's place is the number of experts in front of it (a larger key,
 // or the same and a lower index), so all places are found at once, without a chain of k maxima; keys are read four at a
 // time, the same for all lanes.  Threads `me`, me + threads, ... of `threads` share the work; `keys`: theirs, room for 512;

@@ -22,22 +22,37 @@ namespace ggq {
 //     codes(row, s, g, b)        sub-block s: the lane's 8 codes (SUB 32) or 4 (SUB 16) as bf16
 template <class F> struct Step;
 
-// four codes below 16 (bytes of w) -> two words of two bf16
-__device__ __forceinline__ void small_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, false));
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, true));
+// four codes (bytes of w) -> two words of two bf16, or of two f16 (H): both hold every code exactly
+template <bool H>
+__device__ __forceinline__ uint32_t pair_of(float lo, float hi) {
+    if constexpr (H) return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+    else return upper_halves(lo, hi);
 }
+// ... below 16
+template <bool H>
+__device__ __forceinline__ void small_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
+    if constexpr (H) {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.0f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 512.0f, true));
+    } else {
+        lo = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, false));
+        hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 512.0f, true));
+    }
+}
+template <bool H>
 __device__ __forceinline__ void byte_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
     w = opaque(w);
-    lo = upper_halves(ub<0>(w), ub<1>(w));
-    hi = upper_halves(ub<2>(w), ub<3>(w));
+    lo = pair_of<H>(ub<0>(w), ub<1>(w));
+    hi = pair_of<H>(ub<2>(w), ub<3>(w));
 }
+template <bool H>
 __device__ __forceinline__ void signed_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
     w = opaque(w);
-    lo = upper_halves(sb<0>(w), sb<1>(w));
-    hi = upper_halves(sb<2>(w), sb<3>(w));
+    lo = pair_of<H>(sb<0>(w), sb<1>(w));
+    hi = pair_of<H>(sb<2>(w), sb<3>(w));
 }
-__device__ __forceinline__ void iq4_codes(uint32_t nibbles, uint32_t &lo, uint32_t &hi) { signed_codes(iq4_lookup4(nibbles) ^ 0x80808080u, lo, hi); }
+template <bool H>
+__device__ __forceinline__ void iq4_codes(uint32_t nibbles, uint32_t &lo, uint32_t &hi) { signed_codes<H>(iq4_lookup4(nibbles) ^ 0x80808080u, lo, hi); }
 
 // ---- 32-element formats: sub-block s is block s of the step, at byte s * B -----------------------------------
 template <uint32_t B>
@@ -72,7 +87,7 @@ struct StepOfBlocks {
     }
 };
 #define GGQ_STEP_SCALES(N) static __device__ __forceinline__ void scale(const uint8_t *row, uint32_t g, uint32_t left, SubScale (&out)[N])
-#define GGQ_STEP_CODES(N) static __device__ __forceinline__ void codes(const uint8_t *row, uint32_t s, uint32_t g, uint32_t (&b)[N])
+#define GGQ_STEP_CODES(N) template <bool H> static __device__ __forceinline__ void codes(const uint8_t *row, uint32_t s, uint32_t g, uint32_t (&b)[N])
 // {d, c(d)} of blocks 2 g and 2 g + 1 with a half at their begin; {d, m} with two
 #define GGQ_BLOCK_SCALES(EXPR_C)                                                        \
     GGQ_STEP_SCALES(2) {                                                                \
@@ -90,8 +105,8 @@ template <> struct Step<Q4_0> : StepOfBlocks<18> {
     GGQ_STEP_CODES(4) {
         uint32_t w[2];
         nibbles<2>(row, s, g, w);
-        small_codes(w[0], b[0], b[1]);
-        small_codes(w[1], b[2], b[3]);
+        small_codes<H>(w[0], b[0], b[1]);
+        small_codes<H>(w[1], b[2], b[3]);
     }
 };
 template <> struct Step<Q4_1> : StepOfBlocks<20> {
@@ -101,8 +116,8 @@ template <> struct Step<Q4_1> : StepOfBlocks<20> {
     GGQ_STEP_CODES(4) {
         uint32_t w[2];
         nibbles<4>(row, s, g, w);
-        small_codes(w[0], b[0], b[1]);
-        small_codes(w[1], b[2], b[3]);
+        small_codes<H>(w[0], b[0], b[1]);
+        small_codes<H>(w[1], b[2], b[3]);
     }
 };
 template <> struct Step<Q5_0> : StepOfBlocks<22> {
@@ -112,8 +127,8 @@ template <> struct Step<Q5_0> : StepOfBlocks<22> {
     GGQ_STEP_CODES(4) {
         uint32_t w[2];
         with_fifth<2>(row, s, g, w);
-        byte_codes(w[0], b[0], b[1]);
-        byte_codes(w[1], b[2], b[3]);
+        byte_codes<H>(w[0], b[0], b[1]);
+        byte_codes<H>(w[1], b[2], b[3]);
     }
 };
 template <> struct Step<Q5_1> : StepOfBlocks<24> {
@@ -123,18 +138,19 @@ template <> struct Step<Q5_1> : StepOfBlocks<24> {
     GGQ_STEP_CODES(4) {
         uint32_t w[2];
         with_fifth<4>(row, s, g, w);
-        byte_codes(w[0], b[0], b[1]);
-        byte_codes(w[1], b[2], b[3]);
+        byte_codes<H>(w[0], b[0], b[1]);
+        byte_codes<H>(w[1], b[2], b[3]);
     }
 };
 template <uint32_t B, uint32_t HEAD>
 struct StepOfBytes : StepOfBlocks<B> {
     static constexpr uint32_t BYTES = B;
+    template <bool H>
     static __device__ __forceinline__ void codes(const uint8_t *row, uint32_t s, uint32_t g, uint32_t (&b)[4]) {
         uint32_t w[2];
         StepOfBlocks<B>::two_words(row, s * B + HEAD + 8 * g, (s * B + HEAD) % 4 != 0, w);
-        signed_codes(w[0], b[0], b[1]);
-        signed_codes(w[1], b[2], b[3]);
+        signed_codes<H>(w[0], b[0], b[1]);
+        signed_codes<H>(w[1], b[2], b[3]);
     }
 };
 template <> struct Step<Q8_0> : StepOfBytes<34, 2> {
@@ -152,8 +168,8 @@ template <> struct Step<IQ4NL> : StepOfBlocks<18> {
     GGQ_STEP_CODES(4) {
         uint32_t w[2];
         nibbles<2>(row, s, g, w);
-        iq4_codes(w[0], b[0], b[1]);
-        iq4_codes(w[1], b[2], b[3]);
+        iq4_codes<H>(w[0], b[0], b[1]);
+        iq4_codes<H>(w[1], b[2], b[3]);
     }
 };
 
@@ -171,8 +187,8 @@ template <> struct Step<Q4K> {
     }
     GGQ_STEP_CODES(4) {
         const u32x2 q = al8(row + 16 + 32 * (s >> 1) + 8 * g);
-        small_codes((q[0] >> (4 * (s & 1))) & LOW4, b[0], b[1]);
-        small_codes((q[1] >> (4 * (s & 1))) & LOW4, b[2], b[3]);
+        small_codes<H>((q[0] >> (4 * (s & 1))) & LOW4, b[0], b[1]);
+        small_codes<H>((q[1] >> (4 * (s & 1))) & LOW4, b[2], b[3]);
     }
 };
 template <> struct Step<Q5K> {
@@ -190,7 +206,7 @@ template <> struct Step<Q5K> {
         const u32x2 q = al8(row + 48 + 32 * (s >> 1) + 8 * g), f = al8(row + 16 + 8 * g);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            byte_codes(((q[i] >> (4 * (s & 1))) & LOW4) | (((f[i] >> s) & 0x01010101u) << 4), b[2 * i], b[2 * i + 1]);
+            byte_codes<H>(((q[i] >> (4 * (s & 1))) & LOW4) | (((f[i] >> s) & 0x01010101u) << 4), b[2 * i], b[2 * i + 1]);
     }
 };
 template <> struct Step<IQ4XS> {
@@ -207,8 +223,8 @@ template <> struct Step<IQ4XS> {
     }
     GGQ_STEP_CODES(4) {
         const u32x2 q = al8(row + 8 + 16 * s + 8 * (g & 1));
-        iq4_codes((q[0] >> (4 * (g >> 1))) & LOW4, b[0], b[1]);
-        iq4_codes((q[1] >> (4 * (g >> 1))) & LOW4, b[2], b[3]);
+        iq4_codes<H>((q[0] >> (4 * (g >> 1))) & LOW4, b[0], b[1]);
+        iq4_codes<H>((q[1] >> (4 * (g >> 1))) & LOW4, b[2], b[3]);
     }
 };
 template <> struct Step<Q8K> {
@@ -222,8 +238,8 @@ template <> struct Step<Q8K> {
         const uint8_t *p = row + 32 * s + 8 * g;             // the codes begin two bytes behind
         const u32x2 q = al8(p);
         const uint32_t over = al4(p + 8);
-        signed_codes(funnel16(q[1], q[0]), b[0], b[1]);
-        signed_codes(funnel16(over, q[1]), b[2], b[3]);
+        signed_codes<H>(funnel16(q[1], q[0]), b[0], b[1]);
+        signed_codes<H>(funnel16(over, q[1]), b[2], b[3]);
     }
 };
 // sub-blocks of 16: s = 8 n + 2 p + h, elements 128 n + 32 p + 16 h + 0..15; lane g the elements 4 g .. of them
@@ -241,7 +257,7 @@ template <> struct Step<Q6K> {
         const uint32_t n = s >> 3, p = (s >> 1) & 3, h = s & 1;
         const uint32_t low = (al4(row + 64 * n + 32 * (p & 1) + 16 * h + 4 * g) >> (4 * (p >> 1))) & LOW4;
         const uint32_t high = (al4(row + 128 + 32 * n + 16 * h + 4 * g) >> (2 * p)) & 0x03030303u;
-        byte_codes(low | (high << 4), b[0], b[1]);
+        byte_codes<H>(low | (high << 4), b[0], b[1]);
     }
 };
 template <> struct Step<Q2K> {
@@ -258,7 +274,7 @@ template <> struct Step<Q2K> {
     }
     GGQ_STEP_CODES(2) {
         const uint32_t n = s >> 3, p = (s >> 1) & 3, h = s & 1;
-        small_codes((al4(row + 16 + 32 * n + 16 * h + 4 * g) >> (2 * p)) & 0x03030303u, b[0], b[1]);
+        small_codes<H>((al4(row + 16 + 32 * n + 16 * h + 4 * g) >> (2 * p)) & 0x03030303u, b[0], b[1]);
     }
 };
 template <> struct Step<Q3K> {
@@ -277,7 +293,7 @@ template <> struct Step<Q3K> {
         const uint32_t n = s >> 3, p = (s >> 1) & 3, h = s & 1;
         const uint32_t low = (al4(row + 32 + 32 * n + 16 * h + 4 * g) >> (2 * p)) & 0x03030303u;
         const uint32_t high = (al4(row + 16 * h + 4 * g) >> (4 * n + p)) & 0x01010101u;
-        small_codes(low | (high << 2), b[0], b[1]);
+        small_codes<H>(low | (high << 2), b[0], b[1]);
     }
 };
 
@@ -302,6 +318,8 @@ template <> struct Step<WF16> : StepOfFloats<WF16> {};
 template <> struct Step<WBF16> : StepOfFloats<WBF16> {};
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // How x goes into the matrix unit: its type, and the bf16 pieces that a value is cut into
@@ -324,7 +342,8 @@ struct DenseTile {
     static constexpr uint32_t TILES = R, ROWS = 16, ELEMS = 256, TOKENS = 16;
     typedef Image<F, ROWS, 1> I;
     static constexpr bool WIDE = X == X_F32_2 || X == X_F32_3;
-    static constexpr int P = X == X_BF16 ? 1 : X == X_F32_3 ? 3 : 2;
+    static constexpr bool H = X == X_F16 && !__is_same(F, WBF16);                           // f16 as it is
+    static constexpr int P = X == X_BF16 || H ? 1 : X == X_F32_3 ? 3 : 2;
     static constexpr uint32_t SUBS = 256 / S::SUB, EACH = SUBS / 4, N = S::SUB / 4;        // N: elements of a lane's fragment
     static constexpr uint32_t X_SIZE = WIDE ? 4 : 2, X_ROW = 256 * X_SIZE + 16;              // an odd number of 16-byte places
     static constexpr uint32_t X_LOADS = WIDE ? TOKENS : TOKENS / 2, X_EACH = 16 / X_SIZE;
@@ -353,7 +372,7 @@ struct DenseTile {
     // the fragment of sub-block s: elements SUB s + N g ..
     static __device__ __forceinline__ void fragment(const uint8_t *x, uint32_t s, uint32_t g, const Factor *factor, uint32_t (&out)[P][N / 2]) {
         const uint8_t *at = x + (S::SUB * s + N * g) * X_SIZE;
-        if constexpr (X == X_BF16) {
+        if constexpr (X == X_BF16 || H) {
             if constexpr (N == 8) {
                 const u32x4 w = al16(at);
 #pragma unroll
@@ -387,10 +406,15 @@ struct DenseTile {
         }
     }
     static __device__ __forceinline__ f32x4 multiply(const uint32_t (&a)[N / 2], const uint32_t (&b)[N / 2], f32x4 d) {
-        if constexpr (N == 8)
-            return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, u32x4{a[0], a[1], a[2], a[3]}), __builtin_bit_cast(bf16x8, u32x4{b[0], b[1], b[2], b[3]}), d, 0, 0, 0);
-        else
-            return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, u32x2{a[0], a[1]}), __builtin_bit_cast(s16x4, u32x2{b[0], b[1]}), d, 0, 0, 0);
+        if constexpr (N == 8) {
+            const u32x4 va = {a[0], a[1], a[2], a[3]}, vb = {b[0], b[1], b[2], b[3]};
+            if constexpr (H) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, va), __builtin_bit_cast(f16x8, vb), d, 0, 0, 0);
+            else return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, va), __builtin_bit_cast(bf16x8, vb), d, 0, 0, 0);
+        } else {
+            const u32x2 va = {a[0], a[1]}, vb = {b[0], b[1]};
+            if constexpr (H) return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, va), __builtin_bit_cast(f16x4, vb), d, 0, 0, 0);
+            else return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, va), __builtin_bit_cast(s16x4, vb), d, 0, 0, 0);
+        }
     }
     // the products of one turn; `space`: the wave's shared memory, x: of the lane's token
     static __device__ __forceinline__ void add(uint8_t *space, const uint8_t *x, uint32_t n, uint32_t g, uint32_t left, const Factor *factor, f32x4 (&acc)[R]) {
@@ -404,7 +428,7 @@ struct DenseTile {
                 for (int r = 0; r < R; ++r) {
                     const u32x4 w = S::load(row + r * I::BYTES, s, g, left);
                     uint32_t b[4] = {w[0], w[1], w[2], w[3]}, low[4];
-                    if constexpr (__is_same(F, WF16)) {
+                    if constexpr (__is_same(F, WF16) && !H) {
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float v0 = h2f(b[i] & 0xFFFFu), v1 = h2f(b[i] >> 16);
@@ -415,7 +439,7 @@ struct DenseTile {
 #pragma unroll
                     for (int p = 0; p < P; ++p) {
                         acc[r] = multiply(a[p], b, acc[r]);
-                        if constexpr (__is_same(F, WF16)) acc[r] = multiply(a[p], low, acc[r]);
+                        if constexpr (__is_same(F, WF16) && !H) acc[r] = multiply(a[p], low, acc[r]);
                     }
                 }
             }
@@ -442,7 +466,7 @@ struct DenseTile {
                     // times ones: the sum of the lane's token, in all four of D's rows
                     uint32_t ones[N / 2];
 #pragma unroll
-                    for (uint32_t i = 0; i < N / 2; ++i) ones[i] = 0x3F803F80u;
+                    for (uint32_t i = 0; i < N / 2; ++i) ones[i] = H ? 0x3C003C00u : 0x3F803F80u;
                     f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int p = 0; p < P; ++p) d = multiply(ones, a[p], d);
@@ -452,7 +476,7 @@ struct DenseTile {
                 for (int r = 0; r < R; ++r) {
                     if (s % 4 == 0) scale[r] = *(const f32x4 *)(scales + r * (SCALES / 4) + (s / 4 * ROWS + n) * 4);
                     uint32_t b[N / 2];
-                    S::codes(row + r * I::BYTES, s, g, b);
+                    S::template codes<H>(row + r * I::BYTES, s, g, b);
                     f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int p = 0; p < P; ++p) d = multiply(a[p], b, d);

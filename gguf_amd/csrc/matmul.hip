@@ -69,8 +69,9 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
 // ---- mixture of experts ---------------------------------------------------------------------------------
 namespace {
 
+bool is_16_bit(uint32_t type) { return type == GGQ_TYPE_F16 || type == GGQ_TYPE_BF16; }
 // rows of 16-bit floats that are shorter than a piece of an image
-bool short_rows(uint32_t type, uint64_t cols) { return (type == GGQ_TYPE_F16 || type == GGQ_TYPE_BF16) && cols < 8; }
+bool short_rows(uint32_t type, uint64_t cols) { return is_16_bit(type) && cols < 8; }
 
 uint64_t up256(uint64_t v) { return (v + 255) & ~255ull; }
 
@@ -90,13 +91,14 @@ ggq_status check_moe(const ggq_moe *m, uint64_t tokens) {
 
 // byte offsets of the workspace's parts
 struct MoeSpace {
-    uint64_t ids, weights, h, o, end;
+    uint64_t ids, weights, table, h, o, end;
     MoeSpace(const ggq_moe &m, uint64_t tokens) {
         ids = up256(4 * tokens * m.experts);
         weights = ids + up256(4 * tokens * m.top_k);
-        h = weights + up256(4 * tokens * m.top_k);
+        table = weights + up256(4 * tokens * m.top_k);
+        h = table + up256(sizeof(Slot) * tokens * m.top_k);
         o = h + up256(4 * tokens * m.top_k * m.ff);
-        end = o + (tokens > 4 ? up256(4 * tokens * m.top_k * m.hidden) : 0);
+        end = o + (tokens > FEW_TOKENS ? up256(4 * tokens * m.top_k * m.hidden) : 0);
     }
 };
 
@@ -206,6 +208,7 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     a.logits = (float *)space;
     a.ids = (int32_t *)(space + ws.ids);
     a.weights = (float *)(space + ws.weights);
+    a.table = (Slot *)(space + ws.table);
     a.h = (float *)(space + ws.h);
     a.o = (float *)(space + ws.o);
     a.out_ids = d_ids;
@@ -223,14 +226,16 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     a.scale = m->scale;
     hipStream_t st = (hipStream_t)hip_stream;
     moe_logits<<<dim3(m->experts, ((uint32_t)tokens + LOGIT_TOKENS - 1) / LOGIT_TOKENS), MV_THREADS, 0, st>>>(a);
-    // Comparing each expert with each is on every workgroup's way; the launch that it saves takes about 2.5 us.
-    a.choose = tokens <= CHOOSE_TOKENS && m->experts <= 128 && !short_rows(m->up_type, m->hidden);
-    if (!a.choose) moe_route<<<(uint32_t)tokens, MV_THREADS, 0, st>>>(a);
     // groups of pairs with the same expert: one for each pair, or one for each expert and one more for each slot_tokens pairs.
     // Shared memory is kept for as many tokens: where experts have four on average, or fewer, more than eight are rare.
     const uint32_t pairs = (uint32_t)tokens * m->top_k, in_use = std::min(m->experts, pairs);
     a.slot_tokens = std::min((uint32_t)tokens, pairs > 4 * m->experts ? SLOT_TOKENS : SLOT_TOKENS / 2);
     a.slots = std::min(pairs, in_use + (pairs - in_use) / a.slot_tokens);
+    double unused = 1.0;
+    for (uint64_t t = 0; t < tokens; ++t) unused *= 1.0 - (double)m->top_k / m->experts;
+    a.slots_expected = std::max(1u, std::min(a.slots, (uint32_t)(m->experts * (1.0 - unused) + 0.5)));
+    // one token of packed codes: the kernel of gate and up makes the choice
+    if (tokens > 1 || is_16_bit(m->up_type) || is_16_bit(m->down_type)) moe_route<<<1, ROUTE_WAVES * 64, 0, st>>>(a);
 #define CASE(F) Launch<F>::up(a, st)
     GGQ_FOR_TYPE(m->up_type, CASE)
 #undef CASE

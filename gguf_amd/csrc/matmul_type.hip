@@ -63,15 +63,19 @@ uint32_t dense_waves(uint32_t most, uint32_t turns, uint32_t tokens) {
 struct DenseCut {
     uint64_t cost = ~0ull;
     uint32_t R = 0, waves = 0;
-    // `groups`: of waves that share columns.  They run in rounds of what 256 CUs hold; each takes its turns, whose x costs as
-    // much as one more tile, and what a tile and a half takes to begin and end; and the waves of a CU slow each other down.
+    // `groups`: of waves that share columns.  They run in rounds of what 256 CUs hold; in each, waves take their turns, whose x
+    // costs as much as half a tile, and what a tile takes to begin and end; some of the work of a CU and of a SIMD is not hidden
+    // by that, and a wave has a price.  The weights were fitted to nine ways to cut each of eight products (4096 x 4096 to
+    // 32000 x 4096, 4 to 16 tokens, two types of x, three block types) and three or four of four MoE products: the way with the
+    // least cost is the fastest of them, or within 8 %.  q6_k 32000 x 4096 by 16 tokens: 37 us with two tiles and two waves, 48
+    // with three and eight; 11008 x 4096: 29 and 16.
     template <class M>
     void consider(uint64_t groups, uint32_t turns, uint32_t tokens) {
         for (uint32_t most = TILE_WAVES; most; most /= 2) {
-            const uint32_t w = dense_waves<M>(most, turns, tokens), each = (turns + w - 1) / w;
+            const uint32_t w = dense_waves<M>(most, turns, tokens), turn = 2 * M::TILES + 1, each = (turns + w - 1) / w * turn;
             const uint32_t fit = std::max(1u, std::min<uint32_t>(dense_waves_per_cu(M::TILES) / w, DENSE_LDS / (w * M::wave_bytes(tokens))));
-            const uint64_t rounds = (groups + 256 * fit - 1) / (256 * fit), of_cu = (groups + 255) / 256;
-            const uint64_t c = rounds * (2 * each * (M::TILES + 1) + 3) + of_cu * turns * (M::TILES + 1) / 8;
+            const uint64_t of_cu = (groups + 255) / 256, rounds = (of_cu + fit - 1) / fit, of_simd = (of_cu * w + 3) / 4;
+            const uint64_t c = rounds * (160 * each + 320) + of_simd * each * 40 + of_cu * (turns * turn * 5 + w * 16);
             if (c < cost) cost = c, R = M::TILES, waves = w;
         }
     }
@@ -142,35 +146,30 @@ namespace {
 template <class F, class M>
 void launch_up(MoeArgs a, hipStream_t st) {
     const uint32_t tiles = (uint32_t)((a.ff + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.hidden);
-    const Shape sh(2 * (uint64_t)tiles * a.slots, turns, TILE_WAVES / 2, M::X_BYTES);
+    const Shape sh(2 * (uint64_t)tiles * a.top_k, turns, TILE_WAVES / 2, M::X_BYTES);
     a.ksplit = sh.ksplit;
     a.chunk = sh.chunk<M>(turns);
-    moe_up<F, M><<<dim3((tiles + sh.groups - 1) / sh.groups, a.slots), TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
-}
-// Several: as many groups of waves in a workgroup as eight waves are, since each workgroup looks for its slot.
-template <class M>
-uint32_t cut_slots(MoeArgs &a, uint32_t tiles, uint32_t turns) {
-    DenseCut cut;
-    cut.consider<M>((uint64_t)tiles * a.slots, turns, a.slot_tokens);
-    a.ksplit = cut.waves;
-    const uint32_t fit = DENSE_LDS / (cut.waves * M::wave_bytes(a.slot_tokens));
-    return std::max(1u, std::min(std::min(TILE_WAVES / cut.waves, tiles), fit));
+    moe_up<F, M><<<dim3((tiles + sh.groups - 1) / sh.groups, a.top_k), TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
 }
 template <class F, int X>
 void launch_up_dense(MoeArgs a, hipStream_t st) {
     typedef DenseTile<F, X, 2> M;
-    const uint32_t tiles = (uint32_t)((a.ff + 15) / 16), groups = cut_slots<M>(a, tiles, turns_of<M>(a.hidden)), waves = groups * a.ksplit;
-    moe_up_dense<F, X><<<dim3((tiles + groups - 1) / groups, a.slots), waves * 64, waves * M::wave_bytes(a.slot_tokens), st>>>(a);
+    const uint32_t tiles = (uint32_t)((a.ff + 15) / 16);
+    DenseCut cut;
+    cut.consider<M>((uint64_t)tiles * a.slots_expected, turns_of<M>(a.hidden), a.slot_tokens);
+    moe_up_dense<F, X><<<dim3(tiles, a.slots), cut.waves * 64, cut.waves * M::wave_bytes(a.slot_tokens), st>>>(a);
 }
 template <class F, int X>
 void launch_down_dense(MoeArgs a, hipStream_t st) {
     typedef DenseTile<F, X, DOWN_TILES> M;
-    const uint32_t tiles = (uint32_t)((a.hidden + 16 * DOWN_TILES - 1) / (16 * DOWN_TILES)), groups = cut_slots<M>(a, tiles, turns_of<M>(a.ff)), waves = groups * a.ksplit;
-    moe_down_dense<F, X><<<dim3((tiles + groups - 1) / groups, a.slots), waves * 64, waves * M::wave_bytes(a.slot_tokens), st>>>(a);
+    const uint32_t tiles = (uint32_t)((a.hidden + 16 * DOWN_TILES - 1) / (16 * DOWN_TILES));
+    DenseCut cut;
+    cut.consider<M>((uint64_t)tiles * a.slots_expected, turns_of<M>(a.ff), a.slot_tokens);
+    moe_down_dense<F, X><<<dim3(tiles, a.slots), cut.waves * 64, cut.waves * M::wave_bytes(a.slot_tokens), st>>>(a);
 }
 template <class F, class M>
-void launch_down_few(MoeArgs a, hipStream_t st) {
-    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.ff) * a.tokens * a.top_k;
+void launch_down_one(MoeArgs a, hipStream_t st) {
+    const uint32_t tiles = (uint32_t)((a.hidden + M::ROWS - 1) / M::ROWS), turns = turns_of<M>(a.ff) * a.top_k;
     const Shape sh(tiles, turns, TILE_WAVES, M::X_BYTES);
     a.ksplit = sh.ksplit;
     a.chunk = sh.chunk<M>(turns);
@@ -212,8 +211,8 @@ void Launch<F>::down(MoeArgs a, hipStream_t st) {
             return;
         }
     } else if (a.tokens == 1) {
-        if (to_16) launch_down_few<F, CodeTile<F, 1>>(a, st);
-        else launch_down_few<F, CodeTile<F, 2>>(a, st);
+        if (to_16) launch_down_one<F, CodeTile<F, 1>>(a, st);
+        else launch_down_one<F, CodeTile<F, 2>>(a, st);
         return;
     }
     if (a.tokens <= FEW_TOKENS) {

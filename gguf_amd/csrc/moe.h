@@ -18,87 +18,18 @@ __device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
 }
 
 
-// ---- which expert, and which tokens ----------------------------------------------------------------------
-// Experts in use, in the order of their index, each with its tokens a few at a time (a.slot_tokens): a slot is one such group.
-struct Slot {
-    uint32_t expert, count;       // of tokens; 0: no such slot
-};
-struct SlotSpace {
-    uint32_t low[MOE_MAX_EXPERTS], high[MOE_MAX_EXPERTS];         // masks of tokens, by expert
-    uint32_t pair[SLOT_TOKENS];   // of the slot's tokens: token * top_k + place
-};
-__device__ __forceinline__ uint32_t nth_bit(uint64_t m, uint32_t n) {
-    for (; n; --n) m &= m - 1;
-    return (uint32_t)__builtin_ctzll(m);
-}
-// All threads of the workgroup; ids: the choices of all tokens.  The same answer in all of them.
-__device__ __forceinline__ Slot find_slot(SlotSpace &s, const MoeArgs &a, const int32_t *ids, uint32_t slot) {
-    const uint32_t lane = threadIdx.x % 64;
-    for (uint32_t e = threadIdx.x; e < a.experts; e += blockDim.x) s.low[e] = s.high[e] = 0;
-    __syncthreads();
-    for (uint32_t p = threadIdx.x; p < a.tokens * a.top_k; p += blockDim.x) {
-        const uint32_t t = p / a.top_k;
-        atomicOr(t < 32 ? &s.low[ids[p]] : &s.high[ids[p]], 1u << (t & 31));
-    }
-    __syncthreads();
-    uint32_t seen = 0, expert = 0, count = 0;
-    for (uint32_t base = 0; base < a.experts; base += 64) {
-        const uint32_t e = base + lane;
-        const uint32_t tokens = e < a.experts ? (uint32_t)__popc(s.low[e]) + (uint32_t)__popc(s.high[e]) : 0u, mine = (tokens + a.slot_tokens - 1) / a.slot_tokens;
-        uint32_t upto = mine;                                     // slots of the lanes up to this one
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const uint32_t o = __shfl_up(upto, d);
-            upto += lane >= (uint32_t)d ? o : 0u;
-        }
-        const uint64_t here = __ballot(slot < seen + upto);
-        if (here) {
-            const uint32_t l = (uint32_t)__builtin_ctzll(here);
-            const uint32_t group = __builtin_amdgcn_readfirstlane(slot - seen - __shfl(upto - mine, l));
-            expert = base + l;
-            const uint32_t low = __builtin_amdgcn_readfirstlane(s.low[expert]), high = __builtin_amdgcn_readfirstlane(s.high[expert]);
-            const uint64_t mask = low | ((uint64_t)high << 32);
-            const uint32_t n = (uint32_t)__popcll(mask) - group * a.slot_tokens;
-            count = n < a.slot_tokens ? n : a.slot_tokens;
-            if (threadIdx.x < count) {
-                const uint32_t first = nth_bit(mask, group * a.slot_tokens + threadIdx.x) * a.top_k;
-                uint32_t pair = first;
-                for (uint32_t j = 0; j < a.top_k; ++j) pair = (uint32_t)ids[first + j] == expert ? first + j : pair;
-                s.pair[threadIdx.x] = pair;
-            }
-            break;
-        }
-        seen += __builtin_amdgcn_readfirstlane(__shfl(upto, 63));
-    }
-    __syncthreads();
-    return {(uint32_t)__builtin_amdgcn_readfirstlane(expert), (uint32_t)__builtin_amdgcn_readfirstlane(count)};
-}
-
 // ---- gate and up ----------------------------------------------------------------------------------------
-// The choice of all tokens: already there, or found by each workgroup with few tokens and experts, a wave for each token, which
-// costs it less than one more launch; one workgroup hands it on.  `space`: wave_bytes of shared memory for each wave.
-constexpr uint32_t MOE_KEYS = MOE_MAX_EXPERTS * 4;
-struct Chosen { int32_t ids[CHOOSE_TOKENS * MOE_MAX_TOP_K]; };
-__device__ __forceinline__ const int32_t *choices(const MoeArgs &a, Chosen &chosen, uint8_t *space, uint32_t wave_bytes) {
-    if (!a.choose) return a.ids;
-    const uint32_t lane = threadIdx.x % 64, waves = blockDim.x / 64, wave = threadIdx.x / 64;
-    for (uint32_t t = wave; t < a.tokens; t += waves) {
-        int32_t *ids = chosen.ids + t * a.top_k;
-        choose(a.logits + (uint64_t)t * a.experts, a.experts, a.top_k, lane, 64, (uint32_t *)(space + wave * wave_bytes), ids, [] { wave_order(); });
-        if (blockIdx.x == 0 && blockIdx.y == 0) put_choice(a, t, ids, lane);
-    }
-    __syncthreads();
-    return chosen.ids;
-}
-
-// One token.  As matvec_tiles; half of a workgroup's waves take gate's rows, the others the same rows of up.  Grid: (row groups, slots).
+// One token.  As matvec_tiles; half of a workgroup's waves take gate's rows, the others the same rows of up.  Each workgroup finds
+// the choice by itself, which costs less than one more launch; one hands it on.  Grid: (row groups, top_k).
 template <class F, class M>
 __global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ Chosen chosen;
+    __shared__ int32_t chosen[MOE_MAX_TOP_K];
     typedef typename M::I I;
-    static_assert(M::WAVE_BYTES >= MOE_KEYS, "room for the keys");
-    const uint32_t expert = __builtin_amdgcn_readfirstlane((uint32_t)choices(a, chosen, lds, M::WAVE_BYTES)[blockIdx.y]);
+    static_assert(TILE_WAVES * M::WAVE_BYTES >= MOE_MAX_EXPERTS * 4, "room for the keys");
+    choose(a.logits, a.experts, a.top_k, threadIdx.x, TILE_THREADS, (uint32_t *)lds, chosen, [] { __syncthreads(); });
+    if (blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x < 64) put_choice(a, 0, chosen, threadIdx.x);
+    const uint32_t expert = __builtin_amdgcn_readfirstlane((uint32_t)chosen[blockIdx.y]);
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t second = wave / (TILE_WAVES / 2), group = wave % (TILE_WAVES / 2) / a.ksplit, groups = TILE_WAVES / 2 / a.ksplit;
     const uint32_t row_bytes = (uint32_t)(a.hidden / F::N * F::BYTES), turns = (uint32_t)((a.hidden + M::ELEMS - 1) / M::ELEMS);
@@ -128,44 +59,37 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
     }
 }
 
-// Several tokens.  As matvec_dense: a wave's two tiles are the same rows of gate and of up; a workgroup has several groups of
-// waves.  Grid: (row groups, slots).
+// Several tokens.  As matvec_dense: a wave's two tiles are the same rows of gate and of up.  Grid: (tiles, slots).
 template <class F, int X>
 __global__ __launch_bounds__(TILE_THREADS) void moe_up_dense(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ SlotSpace space;
-    __shared__ Chosen chosen;
     typedef DenseTile<F, X, 2> M;
     typedef typename M::I I;
-    static_assert(M::AT_X >= MOE_KEYS, "room for the keys");
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave_bytes = M::wave_bytes(a.slot_tokens);
-    const Slot slot = find_slot(space, a, choices(a, chosen, lds, wave_bytes), blockIdx.y);
-    if (slot.count == 0) return;
-    const uint32_t group = wave / a.ksplit, groups = blockDim.x / 64 / a.ksplit;
+    const Slot &slot = a.table[blockIdx.y];
+    const uint32_t expert = slot.expert, count = slot.count;
+    if (count == 0) return;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.slot_tokens);
     const uint32_t row_bytes = (uint32_t)(a.hidden / F::N * F::BYTES), turns = (uint32_t)((a.hidden + M::ELEMS - 1) / M::ELEMS);
-    const uint32_t ff = (uint32_t)a.ff, rows = ff < M::ROWS ? ff : M::ROWS, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS;
-    const uint32_t own = row < ff - rows ? row : ff - rows;
-    const uint64_t at_row = (uint64_t)slot.expert * ff + own, behind = ((uint64_t)a.experts * ff - at_row) * row_bytes;
+    const uint32_t ff = (uint32_t)a.ff, rows = ff < M::ROWS ? ff : M::ROWS, row = blockIdx.x * M::ROWS, own = row < ff - rows ? row : ff - rows;
+    const uint64_t at_row = (uint64_t)expert * ff + own, behind = ((uint64_t)a.experts * ff - at_row) * row_bytes;
     const uint8_t *w[2] = {a.gate + at_row * row_bytes, a.up + at_row * row_bytes};
-    if (row < ff)
-        dense_turns<M, 2, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave % a.ksplit, a.ksplit, turns,
-                                 slot.count, (uint32_t)a.hidden,
-                                 [&](uint32_t turn, int r) {
-                                     const uint32_t off = turn * I::TURN_BYTES;
-                                     return Turn{w[r] + off, row_bytes - off, behind - off};
-                                 },
-                                 [&](uint32_t, uint32_t t) { return (const uint8_t *)a.x + space.pair[t] / a.top_k * a.x_stride * M::X_SIZE; },
-                                 [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
+    dense_turns<M, 2, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
+                             (uint32_t)a.hidden,
+                             [&](uint32_t turn, int r) {
+                                 const uint32_t off = turn * I::TURN_BYTES;
+                                 return Turn{w[r] + off, row_bytes - off, behind - off};
+                             },
+                             [&](uint32_t, uint32_t t) { return (const uint8_t *)a.x + slot.pair[t] / a.top_k * a.x_stride * M::X_SIZE; },
+                             [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < groups * M::ROWS * slot.count; i += blockDim.x) {
-        const uint32_t r = i % (groups * M::ROWS), t = i / (groups * M::ROWS), g = r / M::ROWS;
-        const uint32_t nominal = first_row + g * M::ROWS, begin = nominal < ff - rows ? nominal : ff - rows, at = begin + r % M::ROWS;
-        if (at < nominal || at >= ff) continue;
+    for (uint32_t i = threadIdx.x; i < M::ROWS * count; i += blockDim.x) {
+        const uint32_t n = i % M::ROWS, t = i / M::ROWS, at = own + n;
+        if (at < row || at >= ff) continue;
         float v[2] = {0.0f, 0.0f};
-        for (uint32_t k = 0; k < a.ksplit; ++k)
+        for (uint32_t k = 0; k < waves; ++k)
 #pragma unroll
-            for (uint32_t m = 0; m < 2; ++m) v[m] += M::part(lds + (g * a.ksplit + k) * wave_bytes, m, t, r % M::ROWS);
-        a.h[(uint64_t)space.pair[t] * ff + at] = moe_act(v[0], a.gelu) * v[1];
+            for (uint32_t m = 0; m < 2; ++m) v[m] += M::part(lds + k * wave_bytes, m, t, n);
+        a.h[(uint64_t)slot.pair[t] * ff + at] = moe_act(v[0], a.gelu) * v[1];
     }
 }
 
@@ -219,34 +143,26 @@ constexpr uint32_t FEW_PAIRS = FEW_TOKENS * MOE_MAX_TOP_K;
 template <class F, int X>
 __global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ uint32_t items[FEW_PAIRS];          // experts in use, in the order of their first pair
-    __shared__ int32_t pair_at[FEW_PAIRS][FEW_TOKENS];      // the pair of item and token, or -1
-    __shared__ int32_t ids[FEW_PAIRS];
-    __shared__ uint64_t fresh_of[2];
+    __shared__ uint32_t items[FEW_PAIRS];                    // experts in use
+    __shared__ int32_t pair_at[FEW_PAIRS][FEW_TOKENS];       // the pair of item and token, or -1
     typedef DenseTile<F, X, 1> M;
     typedef typename M::I I;
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.tokens);
-    const uint32_t pairs = a.tokens * a.top_k, me_pair = threadIdx.x;      // at most 128: the first two waves
-    if (me_pair < FEW_PAIRS) {
-        ids[me_pair] = me_pair < pairs ? a.ids[me_pair] : -1;
+    uint32_t count = 0;                                      // of items; all slots in use come first
+    for (uint32_t base = 0; base < a.slots; base += 64) {
+        const uint32_t k = base + lane, n = k < a.slots ? a.table[k].count : 0u;
+        count += (uint32_t)__popcll(__ballot(n > 0));
+        if (wave == 0 && n > 0) {
+            items[k] = a.table[k].expert;
 #pragma unroll
-        for (int t = 0; t < (int)FEW_TOKENS; ++t) pair_at[me_pair][t] = -1;
+            for (uint32_t t = 0; t < FEW_TOKENS; ++t) pair_at[k][t] = -1;
+            for (uint32_t i = 0; i < n; ++i) {
+                const uint32_t pair = a.table[k].pair[i];
+                pair_at[k][pair / a.top_k] = (int32_t)pair;
+            }
+        }
     }
     __syncthreads();
-    uint32_t front = me_pair;                              // the first pair with the same expert
-    if (me_pair < pairs)
-        for (uint32_t q = me_pair; q-- > 0;) front = ids[q] == ids[me_pair] ? q : front;
-    const uint64_t fresh = __ballot(me_pair < pairs && front == me_pair);
-    if (lane == 0 && wave < 2) fresh_of[wave] = fresh;
-    __syncthreads();
-    if (me_pair < pairs) {
-        const uint32_t below = (uint32_t)__popcll(fresh_of[front / 64] & ((1ull << (front % 64)) - 1));
-        const uint32_t place = below + (front >= 64 ? (uint32_t)__popcll(fresh_of[0]) : 0u);
-        if (front == me_pair) items[place] = (uint32_t)ids[me_pair];
-        pair_at[place][me_pair / a.top_k] = (int32_t)me_pair;
-    }
-    __syncthreads();
-    const uint32_t count = __builtin_amdgcn_readfirstlane((uint32_t)(__popcll(fresh_of[0]) + __popcll(fresh_of[1])));
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), each = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
     const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, row = blockIdx.x * M::ROWS, own = row < hidden - rows ? row : hidden - rows;
     dense_turns<M, 1, true>(lds + wave * wave_bytes, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, each * count, a.tokens, (uint32_t)a.ff,
@@ -274,40 +190,37 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
     }
 }
 
-// More tokens: expert by expert, into o[pair]; grid: (row groups, slots).
+// More tokens: expert by expert, into o[pair]; grid: (tiles, slots).
 constexpr int DOWN_TILES = 2;
 template <class F, int X>
 __global__ __launch_bounds__(TILE_THREADS) void moe_down_dense(MoeArgs a) {
     extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ SlotSpace space;
     typedef DenseTile<F, X, DOWN_TILES> M;
     typedef typename M::I I;
-    constexpr uint32_t ROWS = DOWN_TILES * M::ROWS;
-    const Slot slot = find_slot(space, a, a.ids, blockIdx.y);
-    if (slot.count == 0) return;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), wave_bytes = M::wave_bytes(a.slot_tokens);
-    const uint32_t group = wave / a.ksplit, groups = blockDim.x / 64 / a.ksplit;
+    const Slot &slot = a.table[blockIdx.y];
+    const uint32_t expert = slot.expert, count = slot.count;
+    if (count == 0) return;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.slot_tokens);
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), turns = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
-    const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, first_row = blockIdx.x * groups * ROWS;
+    const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, first_row = blockIdx.x * DOWN_TILES * M::ROWS;
     auto begin = [&](uint32_t nominal) { return nominal < hidden - rows ? nominal : hidden - rows; };
-    if (first_row + group * ROWS < hidden)
-        dense_turns<M, DOWN_TILES, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave % a.ksplit, a.ksplit,
-                                          turns, slot.count, (uint32_t)a.ff,
-                                          [&](uint32_t turn, int r) {
-                                              const uint64_t row = (uint64_t)slot.expert * hidden + begin(first_row + group * ROWS + r * M::ROWS);
-                                              const uint32_t off = turn * I::TURN_BYTES;
-                                              return Turn{a.down + row * row_bytes + off, row_bytes - off, ((uint64_t)a.experts * hidden - row) * row_bytes - off};
-                                          },
-                                          [&](uint32_t, uint32_t t) { return (const uint8_t *)a.h + space.pair[t] * a.ff * M::X_SIZE; },
-                                          [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
+    dense_turns<M, DOWN_TILES, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
+                                      (uint32_t)a.ff,
+                                      [&](uint32_t turn, int r) {
+                                          const uint64_t row = (uint64_t)expert * hidden + begin(first_row + r * M::ROWS);
+                                          const uint32_t off = turn * I::TURN_BYTES;
+                                          return Turn{a.down + row * row_bytes + off, row_bytes - off, ((uint64_t)a.experts * hidden - row) * row_bytes - off};
+                                      },
+                                      [&](uint32_t, uint32_t t) { return (const uint8_t *)a.h + slot.pair[t] * a.ff * M::X_SIZE; },
+                                      [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < groups * ROWS * slot.count; i += blockDim.x) {
-        const uint32_t r = i % (groups * ROWS), t = i / (groups * ROWS), g = r / ROWS, tile = r % ROWS / M::ROWS;
-        const uint32_t nominal = first_row + r / M::ROWS * M::ROWS, at = begin(nominal) + r % M::ROWS;
+    for (uint32_t i = threadIdx.x; i < DOWN_TILES * M::ROWS * count; i += blockDim.x) {
+        const uint32_t r = i % (DOWN_TILES * M::ROWS), t = i / (DOWN_TILES * M::ROWS), tile = r / M::ROWS;
+        const uint32_t nominal = first_row + tile * M::ROWS, at = begin(nominal) + r % M::ROWS;
         if (at < nominal || at >= hidden) continue;
         float v = 0.0f;
-        for (uint32_t k = 0; k < a.ksplit; ++k) v += M::part(lds + (g * a.ksplit + k) * wave_bytes, tile, t, r % M::ROWS);
-        a.o[(uint64_t)space.pair[t] * hidden + at] = v;
+        for (uint32_t k = 0; k < waves; ++k) v += M::part(lds + k * wave_bytes, tile, t, r % M::ROWS);
+        a.o[(uint64_t)slot.pair[t] * hidden + at] = v;
     }
 }
 
