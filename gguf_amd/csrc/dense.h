@@ -370,7 +370,8 @@ struct DenseTile {
         }
     }
     // the fragment of sub-block s: elements SUB s + N g ..
-    static __device__ __forceinline__ void fragment(const uint8_t *x, uint32_t s, uint32_t g, const Factor *factor, uint32_t (&out)[P][N / 2]) {
+    template <bool FACTOR>
+    static __device__ __forceinline__ void fragment(const uint8_t *x, uint32_t s, uint32_t g, const Factor &factor, uint32_t (&out)[P][N / 2]) {
         const uint8_t *at = x + (S::SUB * s + N * g) * X_SIZE;
         if constexpr (X == X_BF16 || H) {
             if constexpr (N == 8) {
@@ -399,7 +400,7 @@ struct DenseTile {
                 for (uint32_t i = 0; i < N; i += 4) {
                     const f32x4 w = *(const f32x4 *)(at + 4 * i);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[i + j] = factor ? factor->of(w[j]) : w[j];
+                    for (int j = 0; j < 4; ++j) v[i + j] = FACTOR ? factor.of(w[j]) : w[j];
                 }
             }
             cut(v, out);
@@ -417,13 +418,14 @@ struct DenseTile {
         }
     }
     // the products of one turn; `space`: the wave's shared memory, x: of the lane's token
-    static __device__ __forceinline__ void add(uint8_t *space, const uint8_t *x, uint32_t n, uint32_t g, uint32_t left, const Factor *factor, f32x4 (&acc)[R]) {
+    template <bool FACTOR>
+    static __device__ __forceinline__ void add(uint8_t *space, const uint8_t *x, uint32_t n, uint32_t g, uint32_t left, const Factor &factor, f32x4 (&acc)[R]) {
         const uint8_t *row = space + n * I::ROW;
         if constexpr (is_float_type<F>) {
 #pragma unroll
             for (uint32_t s = 0; s < SUBS; ++s) {
                 uint32_t a[P][N / 2];
-                fragment(x, s, g, factor, a);
+                fragment<FACTOR>(x, s, g, factor, a);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const u32x4 w = S::load(row + r * I::BYTES, s, g, left);
@@ -461,7 +463,7 @@ struct DenseTile {
 #pragma unroll
             for (uint32_t s = 0; s < SUBS; ++s) {
                 uint32_t a[P][N / 2];
-                fragment(x, s, g, factor, a);
+                fragment<FACTOR>(x, s, g, factor, a);
                 if constexpr (S::OFFSET) {
                     // times ones: the sum of the lane's token, in all four of D's rows
                     uint32_t ones[N / 2];
@@ -498,10 +500,10 @@ struct DenseTile {
 // The wave's turns kp, kp + waves, ..., the next one's bytes on the way while one is multiplied; then its sums, in the place of
 // the images, [tile][token][row].
 //     at(turn, r)        the packed bytes of tile r, as in run_turns
-//     src(turn, t)       the first element of token t's row
+//     src(turn, t)       the first element of token t's row; KEEP: the same in all turns, and not found by arithmetic alone
 //     col(turn)          its first column, of `cols`
 //     factor(turn, t)    of token t, for FACTOR
-template <class M, int R, bool FACTOR, class At, class Src, class Col, class FactorOf>
+template <class M, int R, bool KEEP, bool FACTOR, class At, class Src, class Col, class FactorOf>
 __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I::Places &places, uint32_t reach, uint32_t kp, uint32_t waves, uint32_t turns, uint32_t tokens,
                                             uint32_t cols, At at, Src src, Col col, FactorOf factor) {
     const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
@@ -513,6 +515,16 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
     uint64_t room[R];
     uint32_t left = 0, column = 0;
     const uint32_t x_need = M::WIDE ? tokens : (tokens + 1) / 2, x_slot = M::WIDE ? 0 : lane / 32, x_at = (M::WIDE ? lane : lane % 32) * M::X_EACH;
+    const uint8_t *x_row[KEEP ? M::X_LOADS : 1];
+    auto of = [&](uint32_t turn, uint32_t i) {
+        const uint32_t slot = M::WIDE ? i : 2 * i + x_slot;
+        return src(turn, slot < tokens ? slot : tokens - 1);
+    };
+    if constexpr (KEEP) {
+#pragma unroll
+        for (uint32_t i = 0; i < M::X_LOADS; ++i)
+            if (i < x_need) x_row[i] = of(0, i);
+    }
     // 16 bytes of x that would end behind the row are moved back to end with it, and shifted when they are put
     const uint32_t x_last = cols - M::X_EACH;
     auto fetch = [&](uint32_t turn) {
@@ -526,10 +538,8 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
         column = col(turn);
         const uint32_t from = (column + x_at < x_last ? column + x_at : x_last) * M::X_SIZE;
 #pragma unroll
-        for (uint32_t i = 0; i < M::X_LOADS; ++i) {
-            const uint32_t slot = M::WIDE ? i : 2 * i + x_slot;
-            if (i < x_need) xr[i] = ld16(src(turn, slot < tokens ? slot : tokens - 1) + from);
-        }
+        for (uint32_t i = 0; i < M::X_LOADS; ++i)
+            if (i < x_need) xr[i] = ld16((KEEP ? x_row[KEEP ? i : 0] : of(turn, i)) + from);
     };
     f32x4 acc[R];
 #pragma unroll
@@ -554,7 +564,7 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
         Factor by{};
         if constexpr (FACTOR) by = factor(turn, token);
         if (turn + waves < turns) fetch(turn + waves);
-        M::add(space, x, n, g, here, FACTOR ? &by : nullptr, acc);
+        M::template add<FACTOR>(space, x, n, g, here, by, acc);
     }
     wave_order();
 #pragma unroll
@@ -579,7 +589,7 @@ __global__ __launch_bounds__(TILE_THREADS) __attribute__((amdgpu_waves_per_eu(de
     const uint32_t rows = a.rows < M::ROWS ? (uint32_t)a.rows : M::ROWS;
     const uint64_t last = a.rows - rows;                       // tiles that would end behind it begin with this row
     auto begin = [&](int r) { const uint64_t row = first_row + r * M::ROWS; return row < last ? row : last; };
-    dense_turns<M, R, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, a.tokens,
+    dense_turns<M, R, false, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, a.tokens,
                              (uint32_t)a.cols,
                              [&](uint32_t turn, int r) {
                                  const uint64_t row = begin(r);

@@ -73,7 +73,7 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_up_dense(MoeArgs a) {
     const uint32_t ff = (uint32_t)a.ff, rows = ff < M::ROWS ? ff : M::ROWS, row = blockIdx.x * M::ROWS, own = row < ff - rows ? row : ff - rows;
     const uint64_t at_row = (uint64_t)expert * ff + own, behind = ((uint64_t)a.experts * ff - at_row) * row_bytes;
     const uint8_t *w[2] = {a.gate + at_row * row_bytes, a.up + at_row * row_bytes};
-    dense_turns<M, 2, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
+    dense_turns<M, 2, true, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
                              (uint32_t)a.hidden,
                              [&](uint32_t turn, int r) {
                                  const uint32_t off = turn * I::TURN_BYTES;
@@ -165,7 +165,7 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
     __syncthreads();
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), each = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
     const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, row = blockIdx.x * M::ROWS, own = row < hidden - rows ? row : hidden - rows;
-    dense_turns<M, 1, true>(lds + wave * wave_bytes, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, each * count, a.tokens, (uint32_t)a.ff,
+    dense_turns<M, 1, false, true>(lds + wave * wave_bytes, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, each * count, a.tokens, (uint32_t)a.ff,
                             [&](uint32_t turn, int) {
                                 const uint32_t item = turn / each, off = (turn - item * each) * I::TURN_BYTES;
                                 const uint64_t e = __builtin_amdgcn_readfirstlane(items[item]);
@@ -204,7 +204,7 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_dense(MoeArgs a) {
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), turns = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
     const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, first_row = blockIdx.x * DOWN_TILES * M::ROWS;
     auto begin = [&](uint32_t nominal) { return nominal < hidden - rows ? nominal : hidden - rows; };
-    dense_turns<M, DOWN_TILES, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
+    dense_turns<M, DOWN_TILES, true, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
                                       (uint32_t)a.ff,
                                       [&](uint32_t turn, int r) {
                                           const uint64_t row = (uint64_t)expert * hidden + begin(first_row + r * M::ROWS);
