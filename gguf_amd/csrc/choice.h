@@ -6,7 +6,6 @@ namespace ggq {
 
 constexpr uint32_t MOE_MAX_EXPERTS = 512, MOE_MAX_TOP_K = 32, MOE_MAX_TOKENS = 64;
 constexpr uint32_t SLOT_TOKENS = 16;          // most tokens of one expert that a workgroup takes
-constexpr uint32_t FEW_TOKENS = 4;            // most tokens whose sum over experts is made in the kernel of down
 
 // Experts in use, in the order of their index, each with its tokens a few at a time (MoeArgs::slot_tokens): a slot is one such
 // group.
@@ -23,8 +22,8 @@ struct MoeArgs {
     int32_t *ids;         // [tokens][top_k]
     float *weights;       // [tokens][top_k]
     float *h;             // [tokens * top_k][ff]
-    float *o;             // [tokens * top_k][hidden], where tokens > FEW_TOKENS
-    Slot *table;          // [slots], where tokens > 1
+    float *o;             // [tokens * top_k][hidden]
+    Slot *table;          // [slots]
     int32_t *out_ids;     // the caller's, or null
     float *out_weights;
     uint64_t hidden, ff, x_stride, y_stride;

@@ -1,16 +1,19 @@
-// dense.h -- two to sixteen tokens at once: the tile of a wave for the products with packed weights (matmul.h).
+// dense.h -- two to sixteen tokens at once: products with packed weights (matmul.h).
 //
-// With several tokens the matrix unit's rows are tokens, all of them in use: v_mfma_f32_16x16x32_bf16 multiplies 32 codes of
-// 16 rows, one sub-block, with 16 tokens (16x16x16 for sub-blocks of 16).  Codes are turned into bf16, which holds every code
-// exactly (two at a time by v_cvt_scalef32_pk_bf16_fp8 where they are below 16: an e4m3 byte of 0..15 times 2^9 is itself);
-// x is in bf16 pieces, P of them: one for bf16, two for f16 and three for f32, exactly, and two for f32 where the result is
-// rounded to 16 bits anyway (2^-17 of an element).  Lane (n, g), n = lane % 16, g = lane / 16, brings the codes k = 8 g ..
-// 8 g + 7 (4 g .. 4 g + 3) of row n and receives the sums of tokens 4 g .. 4 g + 3, which it scales: two multiply-adds for
-// each eight codes and token, whatever the format, are most of the vector work.  The scales of a step are unpacked once,
-// each lane a quarter of its row's, and handed round through shared memory.
+// With several tokens the matrix unit's rows are tokens: v_mfma_f32_16x16x32_bf16 multiplies 32 codes of 16 rows, one
+// sub-block, with 16 tokens (16x16x16 for sub-blocks of 16).  Codes are turned into bf16, which holds every code exactly (two at
+// a time by v_cvt_scalef32_pk_bf16_fp8 where they are below 16: an e4m3 byte of 0..15 times 2^9 is itself).  x goes in as bf16,
+// in pieces where its type is wider: three of f32, exactly, or two where the result is rounded to 16 bits anyway; f16 goes in as
+// it is, with codes as f16.  Lane (n, g), n = lane % 16, g = lane / 16, brings the codes k = 8 g .. 8 g + 7 (4 g .. 4 g + 3) of
+// row n and receives the sums of tokens 4 g .. 4 g + 3, which it scales: a multiply-add for each eight codes and token.  The
+// offsets' part, sum over sub-blocks of c times the sum of x, is a product too: the sums come from a multiplication with ones,
+// and v_mfma_f32_16x16x4_f32 adds them up in f32.  The scales of 256 columns are unpacked once, each lane a quarter of its
+// row's, and handed round through shared memory.
 //
-// Against the digits of one token (matmul.h), whose work grows with the tokens: q4_k 11008 x 4096, two tokens 9.6 against
-// 11.1 us.
+// Bound by the vector instructions that unpack and scale (about 150 for 256 columns of 16 rows), and for few rows by the time
+// that a workgroup takes to begin and end.  Against all waves of a workgroup staging x for each other: q4_k 11008 x 4096 by 16
+// tokens (bf16) 11.4 against 20.5 us, q6_k 15.5 against 36.8.  Against one token's digits (matmul.h): q4_k 28672 x 8192 by one
+// token 42 against 27 us here, so one token is left to those.
 #pragma once
 #include "matmul.h"
 
@@ -325,13 +328,6 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 // How x goes into the matrix unit: its type, and the bf16 pieces that a value is cut into
 enum XForm : int { X_BF16, X_F16, X_F32_2, X_F32_3 };
 
-// of a token's values; keep = 0: all of them are taken as zero, whatever they are
-struct Factor {
-    float by;
-    uint32_t keep;
-    __device__ __forceinline__ float of(float v) const { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & keep) * by; }
-};
-
 // Up to 16 tokens times R tiles of 16 rows.  A wave takes whole turns, 256 columns of all its rows and tokens, and nobody else
 // needs that part of x: it lies in the wave's own shared memory, as it comes from global memory, beside the images of its
 // tiles, and the waves of a workgroup meet only to add up their sums.  A fragment of x is read and cut into pieces once for
@@ -358,20 +354,27 @@ struct DenseTile {
         return *(const float *)(space + tile * PART + (token * ROWS + row) * 4);
     }
     typedef float Values[N];
-    // N elements as pieces, in words of two
+    // N elements as pieces, in words of two: cut off behind eight bits each, which three pieces hold exactly (two, of f16); two
+    // of f32 are rounded, to 2^-18 of the element
     static __device__ __forceinline__ void cut(Values &v, uint32_t (&out)[P][N / 2]) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
+        for (int p = 0; p < P; ++p)
 #pragma unroll
-            for (uint32_t i = 0; i < N / 2; ++i) out[p][i] = upper_halves(v[2 * i], v[2 * i + 1]);
-            if (p + 1 < P)
-#pragma unroll
-                for (uint32_t i = 0; i < N; ++i) v[i] = below_bf16(v[i]);
-        }
+            for (uint32_t i = 0; i < N; i += 2) {
+                if constexpr (X == X_F32_2) {
+                    const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[i], v[i + 1]}, bf16x2v));
+                    out[p][i / 2] = w;
+                    v[i] -= bf2f(w & 0xFFFFu);
+                    v[i + 1] -= __builtin_bit_cast(float, w & 0xFFFF0000u);
+                } else {
+                    out[p][i / 2] = upper_halves(v[i], v[i + 1]);
+                    v[i] = below_bf16(v[i]);
+                    v[i + 1] = below_bf16(v[i + 1]);
+                }
+            }
     }
     // the fragment of sub-block s: elements SUB s + N g ..
-    template <bool FACTOR>
-    static __device__ __forceinline__ void fragment(const uint8_t *x, uint32_t s, uint32_t g, const Factor &factor, uint32_t (&out)[P][N / 2]) {
+    static __device__ __forceinline__ void fragment(const uint8_t *x, uint32_t s, uint32_t g, uint32_t (&out)[P][N / 2]) {
         const uint8_t *at = x + (S::SUB * s + N * g) * X_SIZE;
         if constexpr (X == X_BF16 || H) {
             if constexpr (N == 8) {
@@ -400,7 +403,7 @@ struct DenseTile {
                 for (uint32_t i = 0; i < N; i += 4) {
                     const f32x4 w = *(const f32x4 *)(at + 4 * i);
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) v[i + j] = FACTOR ? factor.of(w[j]) : w[j];
+                    for (int j = 0; j < 4; ++j) v[i + j] = w[j];
                 }
             }
             cut(v, out);
@@ -418,14 +421,13 @@ struct DenseTile {
         }
     }
     // the products of one turn; `space`: the wave's shared memory, x: of the lane's token
-    template <bool FACTOR>
-    static __device__ __forceinline__ void add(uint8_t *space, const uint8_t *x, uint32_t n, uint32_t g, uint32_t left, const Factor &factor, f32x4 (&acc)[R]) {
+    static __device__ __forceinline__ void add(uint8_t *space, const uint8_t *x, uint32_t n, uint32_t g, uint32_t left, f32x4 (&acc)[R]) {
         const uint8_t *row = space + n * I::ROW;
         if constexpr (is_float_type<F>) {
 #pragma unroll
             for (uint32_t s = 0; s < SUBS; ++s) {
                 uint32_t a[P][N / 2];
-                fragment<FACTOR>(x, s, g, factor, a);
+                fragment(x, s, g, a);
 #pragma unroll
                 for (int r = 0; r < R; ++r) {
                     const u32x4 w = S::load(row + r * I::BYTES, s, g, left);
@@ -463,7 +465,7 @@ struct DenseTile {
 #pragma unroll
             for (uint32_t s = 0; s < SUBS; ++s) {
                 uint32_t a[P][N / 2];
-                fragment<FACTOR>(x, s, g, factor, a);
+                fragment(x, s, g, a);
                 if constexpr (S::OFFSET) {
                     // times ones: the sum of the lane's token, in all four of D's rows
                     uint32_t ones[N / 2];
@@ -500,12 +502,10 @@ struct DenseTile {
 // The wave's turns kp, kp + waves, ..., the next one's bytes on the way while one is multiplied; then its sums, in the place of
 // the images, [tile][token][row].
 //     at(turn, r)        the packed bytes of tile r, as in run_turns
-//     src(turn, t)       the first element of token t's row; KEEP: the same in all turns, and not found by arithmetic alone
-//     col(turn)          its first column, of `cols`
-//     factor(turn, t)    of token t, for FACTOR
-template <class M, int R, bool KEEP, bool FACTOR, class At, class Src, class Col, class FactorOf>
+//     src(t)             the first element of token t's row of `cols`; KEEP: not found by arithmetic alone
+template <class M, int R, bool KEEP, class At, class Src>
 __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I::Places &places, uint32_t reach, uint32_t kp, uint32_t waves, uint32_t turns, uint32_t tokens,
-                                            uint32_t cols, At at, Src src, Col col, FactorOf factor) {
+                                            uint32_t cols, At at, Src src) {
     const uint32_t lane = threadIdx.x % 64, n = lane % 16, g = lane / 16;
     uint8_t *xs = space + M::AT_X;
     const uint32_t token = n < tokens ? n : tokens - 1;
@@ -516,14 +516,14 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
     uint32_t left = 0, column = 0;
     const uint32_t x_need = M::WIDE ? tokens : (tokens + 1) / 2, x_slot = M::WIDE ? 0 : lane / 32, x_at = (M::WIDE ? lane : lane % 32) * M::X_EACH;
     const uint8_t *x_row[KEEP ? M::X_LOADS : 1];
-    auto of = [&](uint32_t turn, uint32_t i) {
+    auto of = [&](uint32_t i) {
         const uint32_t slot = M::WIDE ? i : 2 * i + x_slot;
-        return src(turn, slot < tokens ? slot : tokens - 1);
+        return src(slot < tokens ? slot : tokens - 1);
     };
     if constexpr (KEEP) {
 #pragma unroll
         for (uint32_t i = 0; i < M::X_LOADS; ++i)
-            if (i < x_need) x_row[i] = of(0, i);
+            if (i < x_need) x_row[i] = of(i);
     }
     // 16 bytes of x that would end behind the row are moved back to end with it, and shifted when they are put
     const uint32_t x_last = cols - M::X_EACH;
@@ -535,11 +535,11 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
             room[r] = t.room;
             left = t.left;
         }
-        column = col(turn);
+        column = turn * M::ELEMS;
         const uint32_t from = (column + x_at < x_last ? column + x_at : x_last) * M::X_SIZE;
 #pragma unroll
         for (uint32_t i = 0; i < M::X_LOADS; ++i)
-            if (i < x_need) xr[i] = ld16((KEEP ? x_row[KEEP ? i : 0] : of(turn, i)) + from);
+            if (i < x_need) xr[i] = ld16((KEEP ? x_row[KEEP ? i : 0] : of(i)) + from);
     };
     f32x4 acc[R];
 #pragma unroll
@@ -561,10 +561,8 @@ __device__ __forceinline__ void dense_turns(uint8_t *space, const typename M::I:
         }
         wave_order();
         const uint32_t here = left;
-        Factor by{};
-        if constexpr (FACTOR) by = factor(turn, token);
         if (turn + waves < turns) fetch(turn + waves);
-        M::template add<FACTOR>(space, x, n, g, here, by, acc);
+        M::add(space, x, n, g, here, acc);
     }
     wave_order();
 #pragma unroll
@@ -589,15 +587,14 @@ __global__ __launch_bounds__(TILE_THREADS) __attribute__((amdgpu_waves_per_eu(de
     const uint32_t rows = a.rows < M::ROWS ? (uint32_t)a.rows : M::ROWS;
     const uint64_t last = a.rows - rows;                       // tiles that would end behind it begin with this row
     auto begin = [&](int r) { const uint64_t row = first_row + r * M::ROWS; return row < last ? row : last; };
-    dense_turns<M, R, false, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, a.tokens,
+    dense_turns<M, R, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, a.tokens,
                              (uint32_t)a.cols,
                              [&](uint32_t turn, int r) {
                                  const uint64_t row = begin(r);
                                  const uint32_t off = turn * I::TURN_BYTES;
                                  return Turn{a.w + row * row_bytes + off, row_bytes - off, (a.rows - row) * row_bytes - off};
                              },
-                             [&](uint32_t turn, uint32_t t) { return (const uint8_t *)a.x + t * a.x_stride * M::X_SIZE; },
-                             [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
+                             [&](uint32_t t) { return (const uint8_t *)a.x + t * a.x_stride * M::X_SIZE; });
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < R * M::ROWS * a.tokens; i += blockDim.x) {
         const uint32_t r = i % (R * M::ROWS) / M::ROWS, n = i % M::ROWS, t = i / (R * M::ROWS);

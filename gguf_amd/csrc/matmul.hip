@@ -69,9 +69,9 @@ bool strides_ok(uint64_t stride, uint64_t width, uint64_t tokens) {
 // ---- mixture of experts ---------------------------------------------------------------------------------
 namespace {
 
-bool is_16_bit(uint32_t type) { return type == GGQ_TYPE_F16 || type == GGQ_TYPE_BF16; }
+bool is_float(uint32_t type) { return type == GGQ_TYPE_F16 || type == GGQ_TYPE_BF16; }
 // rows of 16-bit floats that are shorter than a piece of an image
-bool short_rows(uint32_t type, uint64_t cols) { return is_16_bit(type) && cols < 8; }
+bool short_rows(uint32_t type, uint64_t cols) { return is_float(type) && cols < 8; }
 
 uint64_t up256(uint64_t v) { return (v + 255) & ~255ull; }
 
@@ -98,7 +98,7 @@ struct MoeSpace {
         table = weights + up256(4 * tokens * m.top_k);
         h = table + up256(sizeof(Slot) * tokens * m.top_k);
         o = h + up256(4 * tokens * m.top_k * m.ff);
-        end = o + (tokens > FEW_TOKENS ? up256(4 * tokens * m.top_k * m.hidden) : 0);
+        end = o + up256(4 * tokens * m.top_k * m.hidden);
     }
 };
 
@@ -235,14 +235,14 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     for (uint64_t t = 0; t < tokens; ++t) unused *= 1.0 - (double)m->top_k / m->experts;
     a.slots_expected = std::max(1u, std::min(a.slots, (uint32_t)(m->experts * (1.0 - unused) + 0.5)));
     // one token of packed codes: the kernel of gate and up makes the choice
-    if (tokens > 1 || is_16_bit(m->up_type) || is_16_bit(m->down_type)) moe_route<<<1, ROUTE_WAVES * 64, 0, st>>>(a);
+    if (tokens > 1 || is_float(m->up_type) || is_float(m->down_type)) moe_route<<<1, ROUTE_WAVES * 64, 0, st>>>(a);
 #define CASE(F) Launch<F>::up(a, st)
     GGQ_FOR_TYPE(m->up_type, CASE)
 #undef CASE
 #define CASE(F) Launch<F>::down(a, st)
     GGQ_FOR_TYPE(m->down_type, CASE)
 #undef CASE
-    if (tokens > FEW_TOKENS && !short_rows(m->down_type, m->ff))
+    if ((tokens > 1 || is_float(m->down_type)) && !short_rows(m->down_type, m->ff))
         moe_sum<<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
     HIP_TRY(hipGetLastError());
     return GGQ_OK;

@@ -175,14 +175,6 @@ void launch_down_one(MoeArgs a, hipStream_t st) {
     a.chunk = sh.chunk<M>(turns);
     moe_down_one<F, M><<<(tiles + sh.groups - 1) / sh.groups, TILE_THREADS, sh.bytes<M>(turns), st>>>(a);
 }
-template <class F, int X>
-void launch_down_few_dense(MoeArgs a, hipStream_t st) {
-    typedef DenseTile<F, X, 1> M;
-    const uint32_t tiles = (uint32_t)((a.hidden + 15) / 16), turns = turns_of<M>(a.ff) * std::min(a.tokens * a.top_k, a.experts);
-    DenseCut cut;
-    cut.consider<M>(tiles, turns, a.tokens);
-    moe_down_few<F, X><<<tiles, cut.waves * 64, cut.waves * M::wave_bytes(a.tokens), st>>>(a);
-}
 }  // namespace
 
 template <class F>
@@ -215,13 +207,8 @@ void Launch<F>::down(MoeArgs a, hipStream_t st) {
         else launch_down_one<F, CodeTile<F, 2>>(a, st);
         return;
     }
-    if (a.tokens <= FEW_TOKENS) {
-        if (to_16) launch_down_few_dense<F, X_F32_2>(a, st);
-        else launch_down_few_dense<F, X_F32_3>(a, st);
-    } else {
-        if (to_16) launch_down_dense<F, X_F32_2>(a, st);
-        else launch_down_dense<F, X_F32_3>(a, st);
-    }
+    if (to_16) launch_down_dense<F, X_F32_2>(a, st);
+    else launch_down_dense<F, X_F32_3>(a, st);
 }
 
 template struct Launch<GGQ_FORMAT>;

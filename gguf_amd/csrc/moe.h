@@ -73,14 +73,13 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_up_dense(MoeArgs a) {
     const uint32_t ff = (uint32_t)a.ff, rows = ff < M::ROWS ? ff : M::ROWS, row = blockIdx.x * M::ROWS, own = row < ff - rows ? row : ff - rows;
     const uint64_t at_row = (uint64_t)expert * ff + own, behind = ((uint64_t)a.experts * ff - at_row) * row_bytes;
     const uint8_t *w[2] = {a.gate + at_row * row_bytes, a.up + at_row * row_bytes};
-    dense_turns<M, 2, true, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
+    dense_turns<M, 2, true>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
                              (uint32_t)a.hidden,
                              [&](uint32_t turn, int r) {
                                  const uint32_t off = turn * I::TURN_BYTES;
                                  return Turn{w[r] + off, row_bytes - off, behind - off};
                              },
-                             [&](uint32_t, uint32_t t) { return (const uint8_t *)a.x + slot.pair[t] / a.top_k * a.x_stride * M::X_SIZE; },
-                             [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
+                             [&](uint32_t t) { return (const uint8_t *)a.x + slot.pair[t] / a.top_k * a.x_stride * M::X_SIZE; });
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < M::ROWS * count; i += blockDim.x) {
         const uint32_t n = i % M::ROWS, t = i / M::ROWS, at = own + n;
@@ -138,59 +137,7 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_one(MoeArgs a) {
     }
 }
 
-constexpr uint32_t FEW_PAIRS = FEW_TOKENS * MOE_MAX_TOP_K;
-// Up to FEW_TOKENS: the same with the rows of all experts in use; a token that did not choose an expert meets zeros.
-template <class F, int X>
-__global__ __launch_bounds__(TILE_THREADS) void moe_down_few(MoeArgs a) {
-    extern __shared__ __align__(16) uint8_t lds[];
-    __shared__ uint32_t items[FEW_PAIRS];                    // experts in use
-    __shared__ int32_t pair_at[FEW_PAIRS][FEW_TOKENS];       // the pair of item and token, or -1
-    typedef DenseTile<F, X, 1> M;
-    typedef typename M::I I;
-    const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.tokens);
-    uint32_t count = 0;                                      // of items; all slots in use come first
-    for (uint32_t base = 0; base < a.slots; base += 64) {
-        const uint32_t k = base + lane, n = k < a.slots ? a.table[k].count : 0u;
-        count += (uint32_t)__popcll(__ballot(n > 0));
-        if (wave == 0 && n > 0) {
-            items[k] = a.table[k].expert;
-#pragma unroll
-            for (uint32_t t = 0; t < FEW_TOKENS; ++t) pair_at[k][t] = -1;
-            for (uint32_t i = 0; i < n; ++i) {
-                const uint32_t pair = a.table[k].pair[i];
-                pair_at[k][pair / a.top_k] = (int32_t)pair;
-            }
-        }
-    }
-    __syncthreads();
-    const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), each = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
-    const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, row = blockIdx.x * M::ROWS, own = row < hidden - rows ? row : hidden - rows;
-    dense_turns<M, 1, false, true>(lds + wave * wave_bytes, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, each * count, a.tokens, (uint32_t)a.ff,
-                            [&](uint32_t turn, int) {
-                                const uint32_t item = turn / each, off = (turn - item * each) * I::TURN_BYTES;
-                                const uint64_t e = __builtin_amdgcn_readfirstlane(items[item]);
-                                return Turn{a.down + (e * hidden + own) * row_bytes + off, row_bytes - off, ((a.experts - e) * hidden - own) * row_bytes - off};
-                            },
-                            [&](uint32_t turn, uint32_t t) {
-                                const int32_t pair = pair_at[turn / each][t];
-                                return (const uint8_t *)a.h + (pair < 0 ? 0 : pair) * a.ff * M::X_SIZE;
-                            },
-                            [&](uint32_t turn) { return turn % each * M::ELEMS; },
-                            [&](uint32_t turn, uint32_t t) {
-                                const int32_t pair = pair_at[turn / each][t];
-                                return pair < 0 ? Factor{0.0f, 0u} : Factor{a.weights[pair], ~0u};
-                            });
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < M::ROWS * a.tokens; i += blockDim.x) {
-        const uint32_t n = i % M::ROWS, t = i / M::ROWS, at = own + n;
-        if (at < row || at >= hidden) continue;
-        float v = 0.0f;
-        for (uint32_t k = 0; k < waves; ++k) v += M::part(lds + k * wave_bytes, 0, t, n);
-        store_elem(a.y, t * a.y_stride + at, a.y_kind, v);
-    }
-}
-
-// More tokens: expert by expert, into o[pair]; grid: (tiles, slots).
+// Several tokens: expert by expert, into o[pair]; grid: (tiles, slots).
 constexpr int DOWN_TILES = 2;
 template <class F, int X>
 __global__ __launch_bounds__(TILE_THREADS) void moe_down_dense(MoeArgs a) {
@@ -204,15 +151,14 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_dense(MoeArgs a) {
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), turns = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
     const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, first_row = blockIdx.x * DOWN_TILES * M::ROWS;
     auto begin = [&](uint32_t nominal) { return nominal < hidden - rows ? nominal : hidden - rows; };
-    dense_turns<M, DOWN_TILES, true, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
+    dense_turns<M, DOWN_TILES, true>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
                                       (uint32_t)a.ff,
                                       [&](uint32_t turn, int r) {
                                           const uint64_t row = (uint64_t)expert * hidden + begin(first_row + r * M::ROWS);
                                           const uint32_t off = turn * I::TURN_BYTES;
                                           return Turn{a.down + row * row_bytes + off, row_bytes - off, ((uint64_t)a.experts * hidden - row) * row_bytes - off};
                                       },
-                                      [&](uint32_t, uint32_t t) { return (const uint8_t *)a.h + slot.pair[t] * a.ff * M::X_SIZE; },
-                                      [](uint32_t turn) { return turn * M::ELEMS; }, [](uint32_t, uint32_t) { return Factor{}; });
+                                      [&](uint32_t t) { return (const uint8_t *)a.h + slot.pair[t] * a.ff * M::X_SIZE; });
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < DOWN_TILES * M::ROWS * count; i += blockDim.x) {
         const uint32_t r = i % (DOWN_TILES * M::ROWS), t = i / (DOWN_TILES * M::ROWS), tile = r / M::ROWS;
