@@ -266,6 +266,40 @@ def test_matrix_beyond_32_bit_offsets(oracle):
     assert same_bits(got[0], dec[-1]) and same_bits(got[1], dec[0]) and not got[2:].any()
 
 
+@pytest.mark.parametrize("ty", [1, 2, 8, 12, 14])
+@pytest.mark.parametrize("rows", [15, 16, 17, 31, 47, 48, 49])
+@pytest.mark.parametrize("tokens", [2, 7, 16])
+def test_matvec_rows_beside_a_tile(oracle, ty, rows, tokens):
+    """Tiles that end with the matrix are moved back to end with it: no row twice, none behind the last."""
+    run_matvec(oracle, ty, rows, 512, tokens, ("f32", "f16", "bf16")[rows % 3], "f32", rows + tokens, y_stride=rows + 5)
+
+
+@pytest.mark.parametrize("ty,rows,cols,tokens,xk", [
+    (12, 4097, 256, 2, "bf16"), (12, 8195, 2304, 16, "bf16"), (14, 12003, 512, 9, "f32"), (8, 30001, 256, 3, "f16"), (2, 4100, 4128, 16, "f32"),
+    (30, 9001, 264, 5, "f16"), (1, 6005, 777, 8, "bf16"), (23, 5001, 2816, 16, "f16"), (10, 70001, 256, 2, "f32"), (15, 300, 16640, 16, "f32")])
+def test_matvec_cuts(oracle, ty, rows, cols, tokens, xk):
+    """From few to many rows and columns: one to three tiles a workgroup, one to eight waves that share its columns."""
+    run_matvec(oracle, ty, rows, cols, tokens, xk, "f32", rows + cols)
+
+
+@pytest.mark.parametrize("ty", [2, 12, 14, 20, 1, 30])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_matvec_subnormal_x(oracle, ty, tokens):
+    """f16 x below 2^-14, whose every bit counts.  The products are far above the bounds of f32 sums."""
+    import torch
+    import gguf_amd as g
+    rows, cols = 33, 512
+    p = weights(ty, rows, cols, ty)
+    v = np.random.default_rng(ty).integers(-1023, 1024, (tokens, cols)) * 2.0 ** -24
+    x = torch.from_numpy(v).cuda().to(torch.float16)
+    assert bool((x.double().cpu().numpy() == v).all())
+    y = torch.empty(tokens, rows, device="cuda")
+    g.matvec(ty, y, on_device(p), x)
+    torch.cuda.synchronize()
+    want, bound = ref.product(*ref.decode(oracle, ty, p, rows, cols), v)
+    assert ref.outside(y.cpu().numpy(), want, bound, "f32") == 0
+
+
 # ---- rows by id --------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("ty", TYPES)
@@ -416,6 +450,47 @@ def test_moe_non_finite_token_stays_alone(oracle):
     assert np.isnan(y[1]).all() and not np.isfinite(y[3]).any()
     want, bound, *_ = ref.moe(m.router.double().cpu().numpy(), *m.ref, x[[0, 2, 4]].double().cpu().numpy(), **m.kw)
     assert ref.outside(y[[0, 2, 4]], want, bound, "f32") == 0
+
+
+@pytest.mark.parametrize("experts,top_k,tokens", [
+    (2, 1, 6), (2, 2, 64), (2, 1, 33), (1, 1, 17), (7, 3, 9), (4, 1, 16), (4, 1, 17), (300, 4, 12), (64, 32, 4), (512, 2, 64), (65, 8, 8)])
+def test_moe_tokens_of_an_expert(oracle, experts, top_k, tokens):
+    """Experts with one token to all of them, some with more than a workgroup takes, and experts with none."""
+    m = Moe(oracle, experts, 64, 96, 2, 8, seed=experts + tokens, top_k=top_k)
+    for xk in ("f32", "bf16"):
+        x, _ = activations(tokens, 64, xk, tokens)
+        m.check(x, "f32", pad=1)
+
+
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_moe_nan_logits_come_last(oracle, tokens):
+    """Experts whose logit is NaN are chosen behind all others, the lowest index first."""
+    import torch
+    m = Moe(oracle, 6, 256, 256, 2, 2, seed=8, top_k=5)
+    m.router[1] = m.router[2] = m.router[4] = float("nan")
+    x, _ = activations(tokens, 256, "f32", 2)
+    y, ids = torch.empty(tokens, 256, device="cuda"), torch.empty(tokens, 5, dtype=torch.int32, device="cuda")
+    m.layer.run(y, x, ids=ids)
+    got = ids.cpu().numpy()
+    assert (np.sort(got[:, :3]) == [0, 3, 5]).all() and (got[:, 3:] == [1, 2]).all()
+    logits = (x.double().cpu().numpy() @ np.nan_to_num(m.router.double().cpu().numpy()).T)
+    assert all((np.diff(logits[t, got[t, :3]]) <= 0).all() for t in range(tokens))
+
+
+def test_moe_same_result_alone_and_with_others(oracle):
+    """A token's ids and weights do not depend on the tokens beside it."""
+    import torch
+    m = Moe(oracle, 20, 256, 256, 12, 12, seed=3, top_k=4)
+    x, _ = activations(16, 256, "f32", 5)
+    def run(x):
+        n = x.shape[0]
+        y, ids, w = torch.empty(n, 256, device="cuda"), torch.empty(n, 4, dtype=torch.int32, device="cuda"), torch.empty(n, 4, device="cuda")
+        m.layer.run(y, x, ids=ids, weights=w)
+        return ids, w
+    ids, w = run(x)
+    for n in (1, 2, 5):
+        i, v = run(x[:n])
+        assert torch.equal(i, ids[:n]) and same_bits(v.cpu().numpy(), w[:n].cpu().numpy())
 
 
 def test_moe_graph_and_streams(oracle):
