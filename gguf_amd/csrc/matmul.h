@@ -191,10 +191,12 @@ struct Image {
 // the scale that a lane has unpacked is applied where it is.  The lanes of A whose slice is not m / 4's read zeros.  Digits
 // carry their weight 16^-d in A's block scale, so a sub-block's sum is the sum of the four.
 //
-// Against codes in bf16 (x as three pieces, v_mfma_f32_4x4x4, what 16-bit float weights take below) it needs a third of the
-// vector instructions, which bound those: q6_k 4096 x 11008 11.2 against 12.6 us, q5_k 11008 x 4096 8.8 against 11.4.
+// Codes need no conversion, and a sub-block's four digits one addition each: against codes in bf16 (x as three pieces,
+// v_mfma_f32_4x4x4, what 16-bit float weights take below) q6_k 4096 x 11008 took 11.2 instead of 12.6 us, q5_k 11008 x 4096 8.8
+// instead of 11.4.  Large matrices are bound by the bytes that the loads in flight bring (q4_k 28672 x 8192, f32: 26.8 us, 4.9
+// TB/s of 7.05), small ones by the way from the launch to the staged x (q4_0 256 x 2048: 4.2 us, an empty kernel 2.5).
 //
-// Staged x, per turn and token: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e - 2 as a byte, then
+// Staged x, per turn: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e - 2 as a byte, then
 // the sums of x, f32: [step][slice][sub-block].
 template <class F, int CH>
 struct CodeTile {

@@ -93,8 +93,8 @@ def matvec(ty, dst, w, x, stream=None):
     """dst[t, r] = sum over c of W[r, c] * x[t, c].
 
     `w`: packed rows of block type `ty`, dst.shape[-1] rows of x.shape[-1] elements.  `x` and `dst`: [tokens, ...] or one
-    vector, float32, float16 or bfloat16 each, with contiguous rows and any stride between them.  Products are exact,
-    sums are held in 32 bits; see ggq_matvec_device in include/ggq.h."""
+    vector, float32, float16 or bfloat16 each, with contiguous rows and any stride between them.  Sums are held in 32 bits;
+    see ggq_matvec_device in include/ggq.h for what is rounded before."""
     be, bb = _block(ty)
     n, cols, xs = _rows_of(x, "x")
     m, rows, ys = _rows_of(dst, "dst")

@@ -281,13 +281,15 @@ ggq_status ggq_dequantize_noalloc(uint32_t ggml_type, uint32_t out_type,
  * Element types x_type and y_type: F32 (0), F16 (1) or BF16 (30); other types: GGQ_UNSUPPORTED.
  * Strides are in elements, from one token's row to the next one's.
  *
- * ggq_matvec_device: y[t][r] = sum over c of W[r][c] * x[t][c], for t < tokens.  Products are exact, sums are held in
- *   32 bits in an order that depends on the sizes alone, and one rounding to y_type ends each.  Made for the few
- *   tokens of decoding; any number is computed.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
+ * ggq_matvec_device: y[t][r] = sum over c of W[r][c] * x[t][c], for t < tokens.  x is taken exactly by two tokens and
+ *   more; for one token and packed codes to 2^-32 of the largest of 32 neighbours, or to 2^-17 of it where x and y are both
+ *   F16 or BF16.  Products of that are exact, sums are held in 32 bits in an order that depends on the sizes alone, and one
+ *   rounding to y_type ends each.  Made for the few tokens of decoding (up to 16 share one pass over W); any number is
+ *   computed.  A token's result may differ in its last bits with the number of tokens of the call.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
  *   there are two tokens or more (GGQ_INVALID).  cols must be whole blocks (GGQ_INDIVISIBLE) and below 2^26, rows and tokens below
  *   2^30 (GGQ_INVALID); cols == 0 gives zeros.
  *   Intermediate sums are those of whole-number codes times x: |x| stays below 2^100, and non-finite x makes the
- *   token's outputs non-finite where the row's codes reach it, of either kind.
+ *   token's outputs non-finite, NaN or infinite; other tokens are not touched by it.
  * ggq_get_rows_device: y[i] = the decoded row ids[i] of W, i < n: the token embeddings of n ids.  id_type is the
  *   GGmlType of the ids: I32 (26) or I64 (27); an id outside [0, rows) gives a row of zeros.  y_stride >= cols where
  *   n > 1.  Values equal ggq_dequantize_device's bit for bit. */
@@ -304,7 +306,8 @@ ggq_status ggq_get_rows_device(uint32_t ggml_type, uint64_t rows, uint64_t cols,
  *   p = softmax(l) or sigmoid(l);  the top_k experts of the largest l, equal ones by the lowest index (a NaN counts as
  *   lowest);  w = p of those, divided by their sum if `normalize`, times `scale`;
  *   y = sum over the chosen e, in order, of w_e * down_e (act(gate_e x) * (up_e x)).
- * The products between are held in 32 bits. */
+ * The products between are held in 32 bits; where x and y are both F16 or BF16, act(gate_e x) * (up_e x) goes into down to
+ * 2^-17 of its largest of 32 neighbours.  Weights whose sum is 0 (a sigmoid of large negative logits) are NaN if `normalize`. */
 typedef struct ggq_moe {
     uint32_t router_type;           /* F32, F16 or BF16: [experts][hidden], row-major      */
     uint32_t up_type;               /* block type of gate and of up, [experts][ff][hidden] */
