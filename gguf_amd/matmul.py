@@ -20,20 +20,19 @@ from .quants import GGmlType, LengthMismatch, Indivisible, Unsupported, block_by
 
 _ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _IDS = {torch.int32: 26, torch.int64: 27}
-_BLOCK = {}          # type id -> (elements, bytes) of a block
-
-
-# a call is over in about 7 us of the host's time, of which torch.cuda's own lookups were 1.3; where this torch has the
-# functions behind them, those are asked
+_BLOCK = {}          # type id -> (elements, bytes of a block, the id as a plain number)
+# A call takes about 5 us of the host's time, 3.9 of them for the launch; torch.cuda's own lookups would add 1.3.  Where this
+# torch has the functions behind them, those are asked.
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+_matvec_device, _get_rows_device = lib.ggq_matvec_device, lib.ggq_get_rows_device
 
 
 def _block(ty):
     b = _BLOCK.get(ty)
     if b is None:
         ty = int(ty)
-        b = _BLOCK[ty] = (block_elems(ty), block_bytes(ty))
+        b = _BLOCK[ty] = (block_elems(ty), block_bytes(ty), ty)
     if b[0] == 0:
         raise Unsupported()
     return b
@@ -86,7 +85,9 @@ def _call(dev, stream, fn, *args):
             return _call(dev, stream, fn, *args)
     if stream is None:
         stream = _current_stream(dev)
-    check(fn(*args, stream))
+    status = fn(*args, stream)
+    if status:
+        check(status)
 
 
 def matvec(ty, dst, w, x, stream=None):
@@ -95,7 +96,7 @@ def matvec(ty, dst, w, x, stream=None):
     `w`: packed rows of block type `ty`, dst.shape[-1] rows of x.shape[-1] elements.  `x` and `dst`: [tokens, ...] or one
     vector, float32, float16 or bfloat16 each, with contiguous rows and any stride between them.  Sums are held in 32 bits;
     see ggq_matvec_device in include/ggq.h for what is rounded before."""
-    be, bb = _block(ty)
+    be, bb, ty = _block(ty)
     n, cols, xs = _rows_of(x, "x")
     m, rows, ys = _rows_of(dst, "dst")
     if n != m:
@@ -104,7 +105,7 @@ def matvec(ty, dst, w, x, stream=None):
         raise Indivisible()
     if _packed_bytes(w) != rows * (cols // be) * bb:
         raise LengthMismatch()
-    _call(_device_of(dst, w, x), stream, lib.ggq_matvec_device, int(ty), rows, cols, w.data_ptr(), _elem(x), x.data_ptr(), xs, n,
+    _call(_device_of(dst, w, x), stream, _matvec_device, ty, rows, cols, w.data_ptr(), _elem(x), x.data_ptr(), xs, n,
           _elem(dst), dst.data_ptr(), ys)
 
 
@@ -113,7 +114,7 @@ def get_rows(ty, dst, w, ids, stream=None):
 
     `ids`: int32 or int64, contiguous; an id outside the table gives a row of zeros.  The values are those of
     `dequantize_slice`, bit for bit."""
-    be, bb = _block(ty)
+    be, bb, ty = _block(ty)
     n, cols, ys = _rows_of(dst, "dst")
     kind = _IDS.get(ids.dtype)
     if kind is None:
@@ -128,7 +129,7 @@ def get_rows(ty, dst, w, ids, stream=None):
     size = _packed_bytes(w)
     if row and size % row:
         raise LengthMismatch()
-    _call(_device_of(dst, w, ids), stream, lib.ggq_get_rows_device, int(ty), size // row if row else 0, cols, w.data_ptr(), kind,
+    _call(_device_of(dst, w, ids), stream, _get_rows_device, ty, size // row if row else 0, cols, w.data_ptr(), kind,
           ids.data_ptr(), n, _elem(dst), dst.data_ptr(), ys)
 
 
@@ -154,7 +155,7 @@ class MoeLayer:
         if router.dim() != 2 or router.shape[1] != hidden or not router.is_contiguous():
             raise ValueError("router must be a contiguous [experts, hidden] matrix")
         experts = router.shape[0]
-        (ue, ub), (de, db) = _block(ut), _block(dt)
+        (ue, ub, _), (de, db, _) = _block(ut), _block(dt)
         if hidden % ue or ff % de:
             raise Indivisible()
         for w, size in ((gw, experts * ff * (hidden // ue) * ub), (uw, experts * ff * (hidden // ue) * ub), (dw, experts * hidden * (ff // de) * db)):
