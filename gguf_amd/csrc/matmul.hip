@@ -225,7 +225,8 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     a.gelu = m->activation;
     a.scale = m->scale;
     hipStream_t st = (hipStream_t)hip_stream;
-    moe_logits<<<dim3(m->experts, ((uint32_t)tokens + LOGIT_TOKENS - 1) / LOGIT_TOKENS), MV_THREADS, 0, st>>>(a);
+    if (tokens == 1) moe_logits<1><<<m->experts, MV_THREADS, 0, st>>>(a);
+    else moe_logits<LOGIT_TOKENS><<<dim3(m->experts, ((uint32_t)tokens + LOGIT_TOKENS - 1) / LOGIT_TOKENS), MV_THREADS, 0, st>>>(a);
     // groups of pairs with the same expert: one for each pair, or one for each expert and one more for each slot_tokens pairs.
     // Shared memory is kept for as many tokens: where experts have four on average, or fewer, more than eight are rare (128
     // experts, 8 chosen, 2048/768 by 16 tokens: 99 us; with room for 16 113).
