@@ -7,8 +7,8 @@
 // An expert's bytes are read once for each slot: for up to 16 of its tokens, or 8.
 //
 // Bound, for one token and large experts, by the bytes of the experts in use (8 experts, 2 chosen, 4096/11008: gate and up 101 MB
-// in 25 us, down 74 MB in 21); for small ones by the time that three launches take to begin and end (64, 8, 2048/1024: 20.7 us
-// for 29 MB); for several tokens by the instructions that unpack (128, 8, 2048/768 by 16 tokens: 99 us for 235 MB).
+// in 25 us, down 74 MB in 21); for small ones by the time that three launches take to begin and end (64, 8, 2048/1024: 20.6 us
+// for 29 MB); for several tokens by the instructions that unpack (128, 8, 2048/768 by 16 tokens: 98 us for 235 MB).
 #pragma once
 #include "choice.h"
 #include "dense.h"
