@@ -584,9 +584,8 @@ __global__ __launch_bounds__(TILE_THREADS) __attribute__((amdgpu_waves_per_eu(de
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.tokens);
     const uint32_t row_bytes = (uint32_t)(a.cols / F::N * F::BYTES), turns = (uint32_t)((a.cols + M::ELEMS - 1) / M::ELEMS);
     const uint64_t first_row = (a.first_tile + (uint64_t)blockIdx.x * R) * M::ROWS;
-    const uint32_t rows = a.rows < M::ROWS ? (uint32_t)a.rows : M::ROWS;
-    const uint64_t last = a.rows - rows;                       // tiles that would end behind it begin with this row
-    auto begin = [&](int r) { const uint64_t row = first_row + r * M::ROWS; return row < last ? row : last; };
+    const uint32_t rows = full_tile_at<M::ROWS>(first_row, a.rows).rows;
+    auto begin = [&](int r) { return full_tile_at<M::ROWS>(first_row + r * M::ROWS, a.rows).own; };
     dense_turns<M, R, false>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, a.tokens,
                              (uint32_t)a.cols,
                              [&](uint32_t turn, int r) {

@@ -113,7 +113,7 @@ struct Image {
     struct Places {
         uint32_t src[LOADS], dst[LOADS];      // from the tile's first row on; in the image
         // `rows` of the tile's rows exist; the others are the last one again
-        __device__ __forceinline__ Places(uint32_t lane, uint32_t rows, uint32_t row_bytes) {
+        __host__ __device__ __forceinline__ Places(uint32_t lane, uint32_t rows, uint32_t row_bytes) {
 #pragma unroll
             for (uint32_t i = 0; i < LOADS; ++i) {
                 uint32_t p = i * 64 + lane;
@@ -125,21 +125,32 @@ struct Image {
         }
     };
     // bytes from a turn's begin in the tile's first row to the end of its furthest piece
-    static __device__ __forceinline__ uint32_t reach(uint32_t rows, uint32_t row_bytes) { return (rows - 1) * row_bytes + (UNITS - 1) * UNIT_BYTES + UNIT; }
+    static __host__ __device__ __forceinline__ uint32_t reach(uint32_t rows, uint32_t row_bytes) { return (rows - 1) * row_bytes + (UNITS - 1) * UNIT_BYTES + UNIT; }
     u32x4 v[LOADS];
 
     // The turn that begins at `base` (in the tile's first row).  A unit's last piece and a row's last turn may reach beyond
     // them, into whatever follows in the tensor; `room` bytes of the tensor are left from base on, and pieces that would end
     // behind them are moved back to end with it.  put shifts those into place: without a second way through fetch the loads
-    // in flight keep their registers.
-    static __device__ __forceinline__ uint32_t limit(uint64_t room) { return room < (1u << 31) ? (uint32_t)room - 16 : (1u << 31) - 16; }
+    // in flight keep their registers.  A turn begins with a whole block, so that only blocks of less than 16 bytes, the 16-bit
+    // floats, may leave less room than a piece takes; then all pieces begin in front of base, in the same row, which has 16 bytes.
+    static constexpr bool SHORT = F::BYTES < 16;
+    // the last place from base on where a piece may begin
+    static __host__ __device__ __forceinline__ int32_t last(uint64_t room) { return room < (1u << 31) ? (int32_t)room - 16 : (int32_t)((1u << 31) - 16); }
+    // where a piece begins, and how far that is in front of its place
+    static __host__ __device__ __forceinline__ uint32_t begin(uint32_t src, int32_t last) {
+        const uint32_t most = SHORT && last < 0 ? 0u : (uint32_t)last;
+        return src < most ? src : most;
+    }
+    static __host__ __device__ __forceinline__ int32_t begin_of_turn(int32_t last) { return SHORT && last < 0 ? last : 0; }       // from base on
+    static __host__ __device__ __forceinline__ uint32_t moved(uint32_t src, int32_t last) { return (int32_t)src > last ? (uint32_t)((int32_t)src - last) : 0u; }
     __device__ __forceinline__ void fetch(const Places &at, const uint8_t *base, uint64_t room) {
-        const uint32_t most = limit(room);
+        const int32_t end = last(room);
+        const uint8_t *from = base + begin_of_turn(end);
 #pragma unroll
         for (uint32_t i = 0; i < LOADS; ++i) {
-            uint32_t o = at.src[i] < most ? at.src[i] : most;
+            uint32_t o = begin(at.src[i], end);
             asm("" : "+v"(o));                // keeps the offset 32 bits wide, for a load with a scalar base
-            v[i] = ld16(base + o);
+            v[i] = ld16(from + o);
         }
     }
     static __device__ __forceinline__ u32x4 shifted(u32x4 a, uint32_t bytes) {
@@ -158,15 +169,34 @@ struct Image {
 #pragma unroll
             for (uint32_t i = 0; i < LOADS; ++i) *(u32x4 *)(image + at.dst[i]) = v[i];
         } else {
-            const uint32_t most = limit(room);
+            const int32_t end = last(room);
 #pragma unroll
             for (uint32_t i = 0; i < LOADS; ++i) {
-                const uint32_t back = at.src[i] > most ? at.src[i] - most : 0u;
+                const uint32_t back = moved(at.src[i], end);
                 *(u32x4 *)(image + at.dst[i]) = shifted(v[i], back < 15 ? back : 15);
             }
         }
     }
 };
+
+// A wave's tile of at most N rows, from `row` on, in a matrix of `total` rows
+template <class T>
+struct RowTile {
+    T own;                // its first row
+    uint32_t rows;
+};
+// ... of one token: fewer rows at the matrix' end; a wave that has nothing to do takes the last row
+template <uint32_t N, class T>
+__host__ __device__ __forceinline__ RowTile<T> tile_at(T row, T total) {
+    const T own = row < total ? row : total - 1;
+    return {own, total - own < N ? (uint32_t)(total - own) : N};
+}
+// ... of several: moved back to end with the matrix
+template <uint32_t N, class T>
+__host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
+    const uint32_t rows = total < N ? (uint32_t)total : N;
+    return {row < total - rows ? row : total - rows, rows};
+}
 
 // What a wave does with a tile of rows and one token.  Two kinds, with the same members:
 //     ROWS, ELEMS       rows of the tile, elements of a turn
@@ -500,8 +530,9 @@ __global__ __launch_bounds__(TILE_THREADS) void matvec_tiles(MatvecArgs a) {
     const uint32_t row_bytes = (uint32_t)(a.cols / F::N * F::BYTES), turns = (uint32_t)((a.cols + M::ELEMS - 1) / M::ELEMS);
     const uint64_t first_row = (a.first_tile + (uint64_t)blockIdx.x * groups) * M::ROWS;      // of the workgroup
     const uint64_t row = first_row + group * M::ROWS;                                         // of the wave
-    const uint64_t own = row < a.rows ? row : a.rows - 1;
-    const uint32_t rows = a.rows - own < M::ROWS ? (uint32_t)(a.rows - own) : M::ROWS;
+    const RowTile<uint64_t> tile = tile_at<M::ROWS>(row, a.rows);
+    const uint64_t own = tile.own;
+    const uint32_t rows = tile.rows;
     const uint8_t *w = a.w + own * row_bytes;
     const uint64_t behind = (a.rows - own - 1) * row_bytes;                                   // of the tensor, behind the row
     uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;

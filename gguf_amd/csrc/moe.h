@@ -37,8 +37,9 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_up(MoeArgs a) {
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t second = wave / (TILE_WAVES / 2), group = wave % (TILE_WAVES / 2) / a.ksplit, groups = TILE_WAVES / 2 / a.ksplit;
     const uint32_t row_bytes = (uint32_t)(a.hidden / F::N * F::BYTES), turns = (uint32_t)((a.hidden + M::ELEMS - 1) / M::ELEMS);
-    const uint32_t ff = (uint32_t)a.ff, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS, own = row < ff ? row : ff - 1;
-    const uint32_t rows = ff - own < M::ROWS ? ff - own : M::ROWS;
+    const uint32_t ff = (uint32_t)a.ff, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS;
+    const RowTile<uint32_t> tile = tile_at<M::ROWS>(row, ff);
+    const uint32_t own = tile.own, rows = tile.rows;
     const uint8_t *w = (second ? a.up : a.gate) + ((uint64_t)expert * ff + own) * row_bytes;
     const uint64_t behind = ((uint64_t)(a.experts - expert) * ff - own - 1) * row_bytes;
     uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;
@@ -74,7 +75,9 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_up_dense(MoeArgs a) {
     if (count == 0) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.slot_tokens);
     const uint32_t row_bytes = (uint32_t)(a.hidden / F::N * F::BYTES), turns = (uint32_t)((a.hidden + M::ELEMS - 1) / M::ELEMS);
-    const uint32_t ff = (uint32_t)a.ff, rows = ff < M::ROWS ? ff : M::ROWS, row = blockIdx.x * M::ROWS, own = row < ff - rows ? row : ff - rows;
+    const uint32_t ff = (uint32_t)a.ff, row = blockIdx.x * M::ROWS;
+    const RowTile<uint32_t> tile = full_tile_at<M::ROWS>(row, ff);
+    const uint32_t own = tile.own, rows = tile.rows;
     const uint64_t at_row = (uint64_t)expert * ff + own, behind = ((uint64_t)a.experts * ff - at_row) * row_bytes;
     const uint8_t *w[2] = {a.gate + at_row * row_bytes, a.up + at_row * row_bytes};
     dense_turns<M, 2, true>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
@@ -113,8 +116,9 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_one(MoeArgs a) {
     const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
     const uint32_t group = wave / a.ksplit, groups = TILE_WAVES / a.ksplit;
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), each = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
-    const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS, own = row < hidden ? row : hidden - 1;
-    const uint32_t rows = hidden - own < M::ROWS ? hidden - own : M::ROWS;
+    const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * groups * M::ROWS, row = first_row + group * M::ROWS;
+    const RowTile<uint32_t> tile = tile_at<M::ROWS>(row, hidden);
+    const uint32_t own = tile.own, rows = tile.rows;
     uint8_t *clear = lds + TILE_WAVES * M::WAVE_BYTES;
     typename M::Sums acc = no_sums<M>();
     run_turns<M>(lds + wave * M::WAVE_BYTES, clear, typename I::Places(lane, rows, row_bytes), I::reach(rows, row_bytes),
@@ -153,8 +157,8 @@ __global__ __launch_bounds__(TILE_THREADS) void moe_down_dense(MoeArgs a) {
     if (count == 0) return;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), waves = blockDim.x / 64, wave_bytes = M::wave_bytes(a.slot_tokens);
     const uint32_t row_bytes = (uint32_t)(a.ff / F::N * F::BYTES), turns = (uint32_t)((a.ff + M::ELEMS - 1) / M::ELEMS);
-    const uint32_t hidden = (uint32_t)a.hidden, rows = hidden < M::ROWS ? hidden : M::ROWS, first_row = blockIdx.x * DOWN_TILES * M::ROWS;
-    auto begin = [&](uint32_t nominal) { return nominal < hidden - rows ? nominal : hidden - rows; };
+    const uint32_t hidden = (uint32_t)a.hidden, first_row = blockIdx.x * DOWN_TILES * M::ROWS, rows = full_tile_at<M::ROWS>(first_row, hidden).rows;
+    auto begin = [&](uint32_t nominal) { return full_tile_at<M::ROWS>(nominal, hidden).own; };
     dense_turns<M, DOWN_TILES, true>(lds + wave * wave_bytes, typename I::Places(threadIdx.x % 64, rows, row_bytes), I::reach(rows, row_bytes), wave, waves, turns, count,
                                       (uint32_t)a.ff,
                                       [&](uint32_t turn, int r) {
