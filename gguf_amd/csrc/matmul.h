@@ -211,9 +211,10 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 // ---- packed whole-number codes, one token: x in digits ------------------------------------------------------
 // The matrix unit multiplies e4m3 bytes with a block scale for each 32 of them.  Codes are such bytes already (slices.h),
 // and so are the digits of x: 32 neighbouring elements share an exponent e, the largest one's; each becomes a whole number
-// of 16 CH bits (truncated, 2^-32 of the largest element, for CH = 2; rounded, 2^-17 of it, for CH = 1, which is taken where
-// the result is rounded to 16 bits anyway) and that CH * 4 hexadecimal digits, each a byte 0..15 with x's sign.  All
-// products and their sums over a sub-block are whole numbers below 2^13, so nothing is rounded before a sub-block's scale.
+// of 32 bits (truncated, 2^-32 of the largest element) and that eight hexadecimal digits, each a byte 0..15 with x's sign, in
+// two chains of four.  All products are exact, and a digit's sums over a sub-block are whole numbers below 2^13.  Sixteen bits,
+// one chain, would do for 16-bit results of ordinary x (q6_k 32000 x 4096, 22.8 instead of 24.0 us), but beside an outlier the
+// small elements would lose bits that the caller gave.
 //
 // v_mfma_scale_f32_16x16x128: A is x, B the codes of 16 rows.  Lane (n, g), n = lane % 16, g = lane / 16, brings 32 codes of
 // row n, slice g.  Row m of A is digit m % 4 of the slices g = m / 4 and zero for the other slices, so that D's rows
@@ -228,12 +229,12 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 //
 // Staged x, per turn: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e - 2 as a byte, then
 // the sums of x, f32: [step][slice][sub-block].
-template <class F, int CH>
+template <class F>
 struct CodeTile {
     typedef Slice<F> S;
-    static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN;
+    static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN, CHAINS = 2;
     typedef Image<F, ROWS, S::TURN> I;
-    static constexpr uint32_t DIGITS = CH * 1024, EXPS = DIGITS * S::TURN, SUMS = EXPS + 8 * S::TURN + 8 * (S::TURN & 1);
+    static constexpr uint32_t DIGITS = CHAINS * 1024, EXPS = DIGITS * S::TURN, SUMS = EXPS + 8 * S::TURN + 8 * (S::TURN & 1);
     static constexpr uint32_t X_BYTES = SUMS + 16 * S::NSUB * S::TURN, CLEAR = DIGITS, WAVE_BYTES = I::BYTES;
 
     template <class Load>
@@ -269,17 +270,13 @@ struct CodeTile {
             const uint32_t bad = e == 255 ? 0x7F7F7F7Fu : 0u;  // an infinity or NaN among them: e4m3's NaN
             e = e > 254 ? 254 : e;
             if (f % 4 == 0) to[EXPS + step * 8 + block] = (uint8_t)(e - 2);
-            // x = whole * 2^(e - 126 - 16 CH)
-            const float unit = __builtin_bit_cast(float, (253u + 16 * CH - e) << 23);
+            // x = whole * 2^(e - 158)
+            const float unit = __builtin_bit_cast(float, (285u - e) << 23);
             uint32_t whole[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) {
-                const float m = __builtin_fabsf(v[k]) * unit;
-                whole[k] = CH == 2 ? (uint32_t)m : (uint32_t)(m + 0.5f);
-                if (CH == 1) whole[k] = whole[k] < 65535u ? whole[k] : 65535u;
-            }
+            for (int k = 0; k < 8; ++k) whole[k] = (uint32_t)(__builtin_fabsf(v[k]) * unit);
             uint8_t *digits = to + step * DIGITS + block * 128 + half * 64 + f % 2 * 8;
-            uint32_t sign[2], plane[2][2 * CH];                // four elements a word; byte p of the whole numbers
+            uint32_t sign[2], plane[2][4];                     // four elements a word; byte p of the whole numbers
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 const uint32_t *n = whole + 4 * q;
@@ -290,16 +287,14 @@ struct CodeTile {
                 const uint32_t a = __builtin_amdgcn_perm(n[1], n[0], 0x05010400u), b = __builtin_amdgcn_perm(n[3], n[2], 0x05010400u);
                 plane[q][0] = __builtin_amdgcn_perm(b, a, 0x05040100u);
                 plane[q][1] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-                if constexpr (CH == 2) {
-                    const uint32_t c = __builtin_amdgcn_perm(n[1], n[0], 0x07030602u), d = __builtin_amdgcn_perm(n[3], n[2], 0x07030602u);
-                    plane[q][2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
-                    plane[q][3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
-                }
+                const uint32_t c = __builtin_amdgcn_perm(n[1], n[0], 0x07030602u), d = __builtin_amdgcn_perm(n[3], n[2], 0x07030602u);
+                plane[q][2] = __builtin_amdgcn_perm(d, c, 0x05040100u);
+                plane[q][3] = __builtin_amdgcn_perm(d, c, 0x07060302u);
             }
 #pragma unroll
-            for (int p = 0; p < 2 * CH; ++p) {                 // the highest byte first: digits 2 p and 2 p + 1
+            for (int p = 0; p < 4; ++p) {                      // the highest byte first: digits 2 p and 2 p + 1
                 uint8_t *d = digits + p / 2 * 1024 + p % 2 * 32;
-                const uint32_t w0 = plane[0][2 * CH - 1 - p], w1 = plane[1][2 * CH - 1 - p];
+                const uint32_t w0 = plane[0][3 - p], w1 = plane[1][3 - p];
                 *(u32x2 *)d = u32x2{((w0 >> 4) & LOW4) | sign[0], ((w1 >> 4) & LOW4) | sign[1]};
                 *(u32x2 *)(d + 16) = u32x2{(w0 & LOW4) | sign[0], (w1 & LOW4) | sign[1]};
             }
@@ -335,7 +330,7 @@ struct CodeTile {
     static __device__ __forceinline__ f32x4 sub_block(const i32x8 &lo, const i32x8 &hi, const uint8_t *x, uint32_t exps) {
         f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int c = 0; c < CH; ++c) {
+        for (uint32_t c = 0; c < CHAINS; ++c) {
             const uint8_t *at = x + c * 1024 + SB * 128;
             const u32x4 none = {0, 0, 0, 0};
             const i32x8 a = join(al16(at), S::PLANES ? none : al16(at + 64));

@@ -52,11 +52,6 @@ uint64_t launch_tiles(MatvecArgs a, hipStream_t st) {
     return 1;
 }
 
-// x is taken to 16 bits below an element, or the largest of 32, where the result is rounded to a 16-bit float anyway: what that
-// leaves out is at most 2^-17 of an element, beside half a step of the result, 2^-11 or 2^-8 of it.  q6_k 32000 x 4096 22.8
-// instead of 24.0 us.
-[[maybe_unused]] bool to_16_bits(uint32_t x_kind, uint32_t y_kind) { return x_kind != EK_F32 && y_kind != EK_F32; }
-
 // Waves that share the columns of R tiles: no more than `most`, or turns, or fit; all with as many turns or one less.
 template <class M>
 uint32_t dense_waves(uint32_t most, uint32_t turns, uint32_t tokens) {
@@ -128,7 +123,7 @@ uint64_t Launch<F>::matvec(MatvecArgs a, uint64_t tokens, hipStream_t st) {
             return launch_tiles<F, FloatTile<F, 3>>(a, st);
         }
     } else if (tokens == 1) {
-        return to_16_bits(a.x_kind, a.y_kind) ? launch_tiles<F, CodeTile<F, 1>>(a, st) : launch_tiles<F, CodeTile<F, 2>>(a, st);
+        return launch_tiles<F, CodeTile<F>>(a, st);
     }
     if (a.x_kind == EK_BF16) return launch_dense<F, X_BF16>(a, tokens, st);
     if (a.x_kind == EK_F16) return launch_dense<F, X_F16>(a, tokens, st);
@@ -192,8 +187,7 @@ void Launch<F>::up(MoeArgs a, hipStream_t st) {
             return;
         }
     } else if (a.tokens == 1) {
-        if (to_16_bits(a.x_kind, a.y_kind)) launch_up<F, CodeTile<F, 1>>(a, st);
-        else launch_up<F, CodeTile<F, 2>>(a, st);
+        launch_up<F, CodeTile<F>>(a, st);
         return;
     }
     if (a.x_kind == EK_BF16) launch_up_dense<F, X_BF16>(a, st);
@@ -203,18 +197,17 @@ void Launch<F>::up(MoeArgs a, hipStream_t st) {
 
 template <class F>
 void Launch<F>::down(MoeArgs a, hipStream_t st) {
-    const bool to_16 = to_16_bits(a.x_kind, a.y_kind);
     if constexpr (is_float_type<F>) {
         if (a.ff < 8) {
             moe_down_short<F><<<dim3((uint32_t)((a.hidden + MV_THREADS - 1) / MV_THREADS), a.tokens), MV_THREADS, 0, st>>>(a);
             return;
         }
     } else if (a.tokens == 1) {
-        if (to_16) launch_down_one<F, CodeTile<F, 1>>(a, st);
-        else launch_down_one<F, CodeTile<F, 2>>(a, st);
+        launch_down_one<F, CodeTile<F>>(a, st);
         return;
     }
-    if (to_16) launch_down_dense<F, X_F32_2>(a, st);
+    // h is taken to 2^-18 of each element where the result is rounded to a 16-bit float: beside half a step of it, 2^-11 or 2^-8
+    if (a.x_kind != EK_F32 && a.y_kind != EK_F32) launch_down_dense<F, X_F32_2>(a, st);
     else launch_down_dense<F, X_F32_3>(a, st);
 }
 

@@ -282,10 +282,10 @@ ggq_status ggq_dequantize_noalloc(uint32_t ggml_type, uint32_t out_type,
  * Strides are in elements, from one token's row to the next one's.
  *
  * ggq_matvec_device: y[t][r] = sum over c of W[r][c] * x[t][c], for t < tokens.  x is taken exactly by two tokens and
- *   more; for one token and packed codes to 2^-32 of the largest of 32 neighbours, or to 2^-17 of it where x and y are both
- *   F16 or BF16.  Products of that are exact, sums are held in 32 bits in an order that depends on the sizes alone, and one
- *   rounding to y_type ends each.  Made for the few tokens of decoding (up to 16 share one pass over W); any number is
- *   computed.  A token's result may differ in its last bits with the number of tokens of the call.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
+ *   more; by one token (the last of 17, 33, ... too) and packed codes to 2^-32 of the largest of 32 neighbours.  Products of that
+ *   are exact, sums are held in 32 bits in an order that depends on the sizes alone, and one rounding to y_type ends each.  Made
+ *   for the few tokens of decoding (up to 16 share one pass over W); any number is computed.  A token's result may differ in its
+ *   last bits with the number of tokens of the call.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
  *   there are two tokens or more (GGQ_INVALID).  cols must be whole blocks (GGQ_INDIVISIBLE) and below 2^26, rows and tokens below
  *   2^30 (GGQ_INVALID); cols == 0 gives zeros.
  *   Intermediate sums are those of whole-number codes times x: |x| stays below 2^100, and non-finite x makes the
@@ -306,8 +306,8 @@ ggq_status ggq_get_rows_device(uint32_t ggml_type, uint64_t rows, uint64_t cols,
  *   p = softmax(l) or sigmoid(l);  the top_k experts of the largest l, equal ones by the lowest index (a NaN counts as
  *   lowest);  w = p of those, divided by their sum if `normalize`, times `scale`;
  *   y = sum over the chosen e, in order, of w_e * down_e (act(gate_e x) * (up_e x)).
- * The products between are held in 32 bits; where x and y are both F16 or BF16, act(gate_e x) * (up_e x) goes into down to
- * 2^-17 of its largest of 32 neighbours.  Weights whose sum is 0 (a sigmoid of large negative logits) are NaN if `normalize`. */
+ * The products between are held in 32 bits and taken as a matvec takes its x; of several tokens whose x and y are both F16 or
+ * BF16, act(gate_e x) * (up_e x) goes into down to 2^-18 of itself.  Weights whose sum is 0 (a sigmoid of large negative logits) are NaN if `normalize`. */
 typedef struct ggq_moe {
     uint32_t router_type;           /* F32, F16 or BF16: [experts][hidden], row-major      */
     uint32_t up_type;               /* block type of gate and of up, [experts][ff][hidden] */

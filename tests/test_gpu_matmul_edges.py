@@ -27,3 +27,65 @@ def test_moe_rows_that_end_a_few_elements_into_a_turn(oracle, ty, tokens):
         m = Moe(oracle, 3, hidden, ff, ty, ty, seed=hidden + tokens)
         x, _ = activations(tokens, hidden, "f32", tokens)
         m.check(x, "f32", pad=1)
+
+
+# ---- one token: what its activations are taken to ----------------------------------------------------------------------------
+
+def one_token(ty, p, rows, cols, v, xk, yk):
+    """(y, x in 64 bits) of packed rows p times the row of values v."""
+    import torch
+    import gguf_amd as g
+    x = torch.from_numpy(np.asarray(v, dtype=np.float32)[None]).cuda().to(dtype(xk))
+    y = torch.empty(1, rows, dtype=dtype(yk), device="cuda")
+    g.matvec(ty, y, on_device(p), x)
+    torch.cuda.synchronize()
+    return y.float().cpu().numpy(), x.double().cpu().numpy()
+
+
+def small_codes(ty, p):
+    """Codes whose values are small beside the range that the type's codes have."""
+    import gguf_amd as g
+    b = p.reshape(-1, g.block_bytes(ty))
+    if ty in (8, 9, 15):                              # within +-10
+        lo = {8: 2, 9: 4, 15: 2}[ty]
+        q = b[:, lo:lo + g.block_elems(ty)].astype(np.int16) % 21 - 10
+        b[:, lo:lo + g.block_elems(ty)] = q.astype(np.int8).view(np.uint8)
+    elif ty in (20, 23):                              # the code book's -10 and 1
+        lo = {20: 2, 23: 8}[ty]
+        b[:, lo:] = 0x77 + (b[:, lo:] & 0x11)
+    else:                                             # q6_k: 32 to 39, values 0 to 7
+        b[:, :128] &= 0x77
+        b[:, 128:192] = 0xAA
+    return p
+
+
+@pytest.mark.parametrize("ty", [8, 9, 14, 15, 20, 23])
+@pytest.mark.parametrize("xk,yk", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16"), ("f16", "f32")])
+def test_one_token_small_codes(oracle, ty, xk, yk):
+    """The error goes by the weights' own size: no offset of the codes in the bound."""
+    rows, cols = 777, 2048
+    p = small_codes(ty, weights(ty, rows, cols, ty))
+    got, x = one_token(ty, p, rows, cols, np.random.default_rng(ty).standard_normal(cols), xk, yk)
+    w, _ = ref.decode(oracle, ty, p, rows, cols)
+    want, bound = ref.product(w, np.zeros_like(w), x)
+    assert ref.outside(got, want, bound, yk) == 0, np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("ty", [2])
+@pytest.mark.parametrize("xk,yk", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16")])
+def test_one_token_beside_an_outlier(oracle, ty, xk, yk):
+    """One of 32 neighbours is 2^10 times the others and meets a weight of 0: the others count in full.  Bound: the worst of the
+    roundings of f32 sums, 16 for a sub-block and its scale, 2 for each sub-block in the row's sum, 24 to join the row's parts,
+    of the sum of all magnitudes; and half of 2^-32 of the outlier for each element."""
+    import gguf_amd as g
+    rows, cols = 300, 256
+    p = weights(ty, rows, cols, ty + 5)
+    b = p.reshape(-1, g.block_bytes(ty))
+    b[:, 2] = 0 if ty == 8 else b[:, 2] & 0xF0 | 8
+    v = np.random.default_rng(ty).standard_normal(cols)
+    v[::32] = 1024.0
+    got, x = one_token(ty, p, rows, cols, v, xk, yk)
+    w, w0 = ref.decode(oracle, ty, p, rows, cols)
+    assert not w[:, ::32].any()
+    bound = (40 + 2 * cols // 32) * ref.U * (np.abs(x) @ (np.abs(w - w0) + np.abs(w0)).T) + 2.0 ** -33 * 1024 * np.abs(w).sum(axis=1)
+    assert ref.outside(got, x @ w.T, bound, yk) == 0, np.abs(got - x @ w.T).max()
