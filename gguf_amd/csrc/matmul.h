@@ -222,20 +222,24 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 // the scale that a lane has unpacked is applied where it is.  The lanes of A whose slice is not m / 4's read zeros.  Digits
 // carry their weight 16^-d in A's block scale, so a sub-block's sum is the sum of the four.
 //
+// Codes that are counted from -128 on: the constant is a third plane.  With 128 a (sum of x) as the offset instead, the f32 sums
+// carried it and lost it again: by codes that were small beside their range, next to an outlier, the result was 2^-13 off.  The
+// matrix unit has room for it (q8_0 11008 x 4096 12.5 instead of 12.3 us; codes by sign and magnitude 13.5).
+//
 // Codes need no conversion, and a sub-block's four digits one addition each: against codes in bf16 (x as three pieces,
 // v_mfma_f32_4x4x4, what 16-bit float weights take below) q6_k 4096 x 11008 took 11.2 instead of 12.6 us, q5_k 11008 x 4096 8.8
 // instead of 11.4.  Large matrices are bound by the bytes that the loads in flight bring (q4_k 28672 x 8192, f32: 26.8 us, 4.9
 // TB/s of 7.05), small ones by the way from the launch to the staged x (q4_0 256 x 2048: 4.2 us, an empty kernel 2.5).
 //
 // Staged x, per turn: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e - 2 as a byte, then
-// the sums of x, f32: [step][slice][sub-block].
+// the sums of x, f32, where the format has an offset: [step][slice][sub-block].
 template <class F>
 struct CodeTile {
     typedef Slice<F> S;
     static constexpr uint32_t ROWS = 16, ELEMS = 256 * S::TURN, CHAINS = 2;
     typedef Image<F, ROWS, S::TURN> I;
     static constexpr uint32_t DIGITS = CHAINS * 1024, EXPS = DIGITS * S::TURN, SUMS = EXPS + 8 * S::TURN + 8 * (S::TURN & 1);
-    static constexpr uint32_t X_BYTES = SUMS + 16 * S::NSUB * S::TURN, CLEAR = DIGITS, WAVE_BYTES = I::BYTES;
+    static constexpr uint32_t X_BYTES = SUMS + (S::OFFSET ? 16 * S::NSUB * S::TURN : 0), CLEAR = DIGITS, WAVE_BYTES = I::BYTES;
 
     template <class Load>
     static __device__ __forceinline__ void stage(uint8_t *lds, uint32_t turns, Load load) {
@@ -246,14 +250,16 @@ struct CodeTile {
             uint8_t *to = lds + turn * X_BYTES;
             float v[8];
             load(turn, f * 8, v);
-            float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-            sum += dpp<QUAD_XOR1>(sum);
-            float *sums = (float *)(to + SUMS) + step * 4 * S::NSUB;
-            if constexpr (S::PLANES) {                         // 16 elements: column `half` of sub-block block % 4
-                if (f % 2 == 0) sums[(block / 4 * 2 + half) * 4 + block % 4] = sum;
-            } else {
-                sum += dpp<QUAD_XOR2>(sum);
-                if (f % 4 == 0) sums[block] = sum;
+            if constexpr (S::OFFSET) {
+                float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+                sum += dpp<QUAD_XOR1>(sum);
+                float *sums = (float *)(to + SUMS) + step * 4 * S::NSUB;
+                if constexpr (S::PLANES) {                     // 16 elements: column `half` of sub-block block % 4
+                    if (f % 2 == 0) sums[(block / 4 * 2 + half) * 4 + block % 4] = sum;
+                } else {
+                    sum += dpp<QUAD_XOR2>(sum);
+                    if (f % 4 == 0) sums[block] = sum;
+                }
             }
             uint32_t top = 0;
 #pragma unroll
@@ -336,6 +342,10 @@ struct CodeTile {
             const i32x8 a = join(al16(at), S::PLANES ? none : al16(at + 64));
             d = multiply<SB>(a, exps - c * 0x10101010u, lo, S::template LOW_EXP<SB>, d);
             if constexpr (S::HIGH) d = multiply<SB>(a, exps - c * 0x10101010u, hi, S::template HIGH_EXP<SB>, d);
+            if constexpr (from_minus_128<F>) {                 // -8 times 16 for each code, before the next chain is added
+                constexpr int k = (int)0x88888888u;
+                d = multiply<SB>(a, exps - c * 0x10101010u, i32x8{k, k, k, k, k, k, k, k}, S::template HIGH_EXP<SB>, d);
+            }
         }
         return d;
     }
@@ -356,9 +366,11 @@ struct CodeTile {
         const uint32_t exps = (S::PLANES ? al4(x + EXPS + step * 8 + me.exps) : al2(x + EXPS + step * 8 + me.exps)) - me.weight;
         const uint8_t *digits = clear + ((uint32_t)(x + step * DIGITS + me.digits - clear) & me.own);
         const f32x4 d = sub_block<SB>(lo, hi, digits, exps);
-        const float sum = ((const float *)(x + SUMS))[(step * 4 + me.g) * S::NSUB + SB];
         acc.v[0] = __builtin_fmaf(s.a, (d[0] + d[1]) + (d[2] + d[3]), acc.v[0]);
-        acc.v[0] = __builtin_fmaf(-s.c, sum, acc.v[0]);
+        if constexpr (S::OFFSET) {
+            const float sum = ((const float *)(x + SUMS))[(step * 4 + me.g) * S::NSUB + SB];
+            acc.v[0] = __builtin_fmaf(-s.c, sum, acc.v[0]);
+        }
     }
     // one turn: `image` the wave's bytes, `x` the turn's staged x, `clear` the zeros, `left` bytes of the row from the turn on
     static __device__ __forceinline__ void add(const uint8_t *image, const Me &me, const uint8_t *clear, const uint8_t *x, uint32_t left,

@@ -71,7 +71,7 @@ def test_one_token_small_codes(oracle, ty, xk, yk):
     assert ref.outside(got, want, bound, yk) == 0, np.abs(got - want).max()
 
 
-@pytest.mark.parametrize("ty", [2])
+@pytest.mark.parametrize("ty", [2, 8, 9, 15])
 @pytest.mark.parametrize("xk,yk", [("f32", "f32"), ("f16", "f16"), ("bf16", "bf16")])
 def test_one_token_beside_an_outlier(oracle, ty, xk, yk):
     """One of 32 neighbours is 2^10 times the others and meets a weight of 0: the others count in full.  Bound: the worst of the
@@ -81,7 +81,10 @@ def test_one_token_beside_an_outlier(oracle, ty, xk, yk):
     rows, cols = 300, 256
     p = weights(ty, rows, cols, ty + 5)
     b = p.reshape(-1, g.block_bytes(ty))
-    b[:, 2] = 0 if ty == 8 else b[:, 2] & 0xF0 | 8
+    if ty == 2:
+        b[:, 2] = b[:, 2] & 0xF0 | 8
+    else:
+        b[:, {8: 2, 9: 4, 15: 2}[ty]::32][:, :g.block_elems(ty) // 32] = 0
     v = np.random.default_rng(ty).standard_normal(cols)
     v[::32] = 1024.0
     got, x = one_token(ty, p, rows, cols, v, xk, yk)
@@ -89,3 +92,14 @@ def test_one_token_beside_an_outlier(oracle, ty, xk, yk):
     assert not w[:, ::32].any()
     bound = (40 + 2 * cols // 32) * ref.U * (np.abs(x) @ (np.abs(w - w0) + np.abs(w0)).T) + 2.0 ** -33 * 1024 * np.abs(w).sum(axis=1)
     assert ref.outside(got, x @ w.T, bound, yk) == 0, np.abs(got - x @ w.T).max()
+
+
+@pytest.mark.parametrize("ty", [8, 9, 15])
+def test_one_token_codes_of_zero(oracle, ty):
+    """Weights that are all 0 under scales that are not: exactly 0."""
+    import gguf_amd as g
+    p = weights(ty, 40, 1024, ty)
+    lo = {8: 2, 9: 4, 15: 2}[ty]
+    p.reshape(-1, g.block_bytes(ty))[:, lo:lo + g.block_elems(ty)] = 0
+    got, _ = one_token(ty, p, 40, 1024, np.random.default_rng(1).standard_normal(1024), "f32", "f32")
+    assert not got.any()
