@@ -219,8 +219,9 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 // v_mfma_scale_f32_16x16x128: A is x, B the codes of 16 rows.  Lane (n, g), n = lane % 16, g = lane / 16, brings 32 codes of
 // row n, slice g.  Row m of A is digit m % 4 of the slices g = m / 4 and zero for the other slices, so that D's rows
 // 4 g .. 4 g + 3, which lane (n, g) receives, are the four digits' sums of the lane's own codes: slices are kept apart, and
-// the scale that a lane has unpacked is applied where it is.  The lanes of A whose slice is not m / 4's read zeros.  Digits
-// carry their weight 16^-d in A's block scale, so a sub-block's sum is the sum of the four.
+// the scale that a lane has unpacked is applied where it is.  The lanes of A whose slice is not m / 4's read zeros.  A's block
+// scale is e, whatever it is; the second chain's weight 2^-16 is in B's, and the digits' weights 16^-d are applied when a
+// sub-block's four sums are joined.
 //
 // Codes that are counted from -128 on: the constant is a third plane.  With 128 a (sum of x) as the offset instead, the f32 sums
 // carried it and lost it again: by codes that were small beside their range, next to an outlier, the result was 2^-13 off.  The
@@ -231,7 +232,7 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 // instead of 11.4.  Large matrices are bound by the bytes that the loads in flight bring (q4_k 28672 x 8192, f32: 26.8 us, 4.9
 // TB/s of 7.05), small ones by the way from the launch to the staged x (q4_0 256 x 2048: 4.2 us, an empty kernel 2.5).
 //
-// Staged x, per turn: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e - 2 as a byte, then
+// Staged x, per turn: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e as a byte, then
 // the sums of x, f32, where the format has an offset: [step][slice][sub-block].
 template <class F>
 struct CodeTile {
@@ -271,16 +272,15 @@ struct CodeTile {
             top = o1 > top ? o1 : top;
             const uint32_t o2 = dpp<QUAD_XOR2>(top);
             top = o2 > top ? o2 : top;
-            uint32_t e = top >> 23;                            // biased; smaller ones than 2^-95 are multiples of 2^-127
-            e = e < 32 ? 32 : e;
+            uint32_t e = top >> 23;                            // biased
+            e = e < 1 ? 1 : e;
             const uint32_t bad = e == 255 ? 0x7F7F7F7Fu : 0u;  // an infinity or NaN among them: e4m3's NaN
             e = e > 254 ? 254 : e;
-            if (f % 4 == 0) to[EXPS + step * 8 + block] = (uint8_t)(e - 2);
-            // x = whole * 2^(e - 158)
-            const float unit = __builtin_bit_cast(float, (285u - e) << 23);
+            if (f % 4 == 0) to[EXPS + step * 8 + block] = (uint8_t)e;
+            const int up = 158 - (int)e;                       // x = whole * 2^-up
             uint32_t whole[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) whole[k] = (uint32_t)(__builtin_fabsf(v[k]) * unit);
+            for (int k = 0; k < 8; ++k) whole[k] = (uint32_t)__builtin_amdgcn_ldexpf(__builtin_fabsf(v[k]), up);
             uint8_t *digits = to + step * DIGITS + block * 128 + half * 64 + f % 2 * 8;
             uint32_t sign[2], plane[2][4];                     // four elements a word; byte p of the whole numbers
 #pragma unroll
@@ -309,7 +309,6 @@ struct CodeTile {
     struct Me {
         uint32_t g, row;              // the lane's slice, its row's image
         uint32_t own, digits, exps;   // ~0 where the lane's part of A is not zero; its place in a step's digits; of its row's exponents
-        uint32_t weight;              // its digit's weight, in each byte
         // zeros: in shared memory, in front of the staged x
         __device__ __forceinline__ Me(uint32_t lane, const uint8_t *) {
             const uint32_t m = lane % 16, p = m % 4, gm = m / 4;
@@ -318,7 +317,6 @@ struct CodeTile {
             own = gm == g ? ~0u : 0u;
             digits = S::PLANES ? (g / 2 * 4) * 128 + g % 2 * 64 + p * 16 : g * 256 + p * 16;
             exps = S::PLANES ? gm / 2 * 4 : gm * 2;
-            weight = p * 0x04040404u;
         }
     };
     struct Sums { float v[1]; };
@@ -328,10 +326,10 @@ struct CodeTile {
     }
     template <int SB>
     static __device__ __forceinline__ f32x4 multiply(const i32x8 &x, uint32_t x_exp, const i32x8 &w, int w_exp, f32x4 d) {
-        // 8 of A's exponent stand in B's, which keeps A's in range for every x
-        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, d, 0, 0, SB, (int)x_exp, 0, w_exp + 127 + 8);
+        // a byte n is n 2^-9, and the first digit's unit 2^(e - 130): 6 in front of e - 127 and w_exp
+        return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, w, d, 0, 0, SB, (int)x_exp, 0, w_exp + 127 + 6);
     }
-    // `x`: the step's digits of the token, or the zeros; `weights`: the step's exponents less the digits' weights
+    // `x`: the step's digits of the token, or the zeros; `exps`: the step's exponents
     template <int SB>
     static __device__ __forceinline__ f32x4 sub_block(const i32x8 &lo, const i32x8 &hi, const uint8_t *x, uint32_t exps) {
         f32x4 d = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -340,14 +338,18 @@ struct CodeTile {
             const uint8_t *at = x + c * 1024 + SB * 128;
             const u32x4 none = {0, 0, 0, 0};
             const i32x8 a = join(al16(at), S::PLANES ? none : al16(at + 64));
-            d = multiply<SB>(a, exps - c * 0x10101010u, lo, S::template LOW_EXP<SB>, d);
-            if constexpr (S::HIGH) d = multiply<SB>(a, exps - c * 0x10101010u, hi, S::template HIGH_EXP<SB>, d);
+            d = multiply<SB>(a, exps, lo, S::template LOW_EXP<SB> - 16 * (int)c, d);
+            if constexpr (S::HIGH) d = multiply<SB>(a, exps, hi, S::template HIGH_EXP<SB> - 16 * (int)c, d);
             if constexpr (from_minus_128<F>) {                 // -8 times 16 for each code, before the next chain is added
                 constexpr int k = (int)0x88888888u;
-                d = multiply<SB>(a, exps - c * 0x10101010u, i32x8{k, k, k, k, k, k, k, k}, S::template HIGH_EXP<SB>, d);
+                d = multiply<SB>(a, exps, i32x8{k, k, k, k, k, k, k, k}, S::template HIGH_EXP<SB> - 16 * (int)c, d);
             }
         }
         return d;
+    }
+    // the four digits' sums, each 16 times the next one's weight
+    static __device__ __forceinline__ float joined(const f32x4 &d) {
+        return __builtin_fmaf(__builtin_fmaf(d[3], 0.0625f, d[2]), 0.00390625f, __builtin_fmaf(d[1], 0.0625f, d[0]));
     }
     template <int SB>
     static __device__ __forceinline__ void add_sub(const typename S::Raw &raw, const Me &me, const uint8_t *clear, const uint8_t *x, uint32_t step,
@@ -363,10 +365,10 @@ struct CodeTile {
             hi[i] = S::HIGH ? (int)h[i % WORDS] : 0;
         }
         const SubScale s = S::template scale<SB>(raw);
-        const uint32_t exps = (S::PLANES ? al4(x + EXPS + step * 8 + me.exps) : al2(x + EXPS + step * 8 + me.exps)) - me.weight;
+        const uint32_t exps = (S::PLANES ? al4(x + EXPS + step * 8 + me.exps) : al2(x + EXPS + step * 8 + me.exps));
         const uint8_t *digits = clear + ((uint32_t)(x + step * DIGITS + me.digits - clear) & me.own);
         const f32x4 d = sub_block<SB>(lo, hi, digits, exps);
-        acc.v[0] = __builtin_fmaf(s.a, (d[0] + d[1]) + (d[2] + d[3]), acc.v[0]);
+        acc.v[0] = __builtin_fmaf(s.a, joined(d), acc.v[0]);
         if constexpr (S::OFFSET) {
             const float sum = ((const float *)(x + SUMS))[(step * 4 + me.g) * S::NSUB + SB];
             acc.v[0] = __builtin_fmaf(-s.c, sum, acc.v[0]);

@@ -103,3 +103,25 @@ def test_one_token_codes_of_zero(oracle, ty):
     p.reshape(-1, g.block_bytes(ty))[:, lo:lo + g.block_elems(ty)] = 0
     got, _ = one_token(ty, p, 40, 1024, np.random.default_rng(1).standard_normal(1024), "f32", "f32")
     assert not got.any()
+
+
+@pytest.mark.parametrize("ty", [2, 3, 8, 10, 12, 14, 20, 23])
+@pytest.mark.parametrize("xk,yk,low,high", [("f32", "f32", -118, 60), ("f32", "f32", -118, -112), ("bf16", "bf16", -125, -119), ("bf16", "f32", -125, 60),
+                                            ("f16", "f16", -24, 10), ("f16", "f16", -24, -14), ("f32", "f32", 70, 98)])
+def test_one_token_of_every_size(oracle, ty, xk, yk, low, high):
+    """One block of 32 neighbours is small, the next large, and all of them may be small: down to where x's last bit is that of
+    the smallest f32, up to where codes times x stay in range.  Weights below 4, results that y's type holds."""
+    import gguf_amd as g
+    from gguf_amd import synth
+    rows, cols = 130, 1024
+    p = weights(ty, rows, cols, ty)
+    rng = np.random.default_rng(1000 + low + ty)
+    b = p.reshape(-1, g.block_bytes(ty))
+    for at in synth.HEADER_F16[ty]:
+        d = (2.0 ** (-12 if g.block_elems(ty) == 256 else -6) * (1 + rng.random(len(b)))).astype(np.float16)
+        b[:, at:at + 2] = d.view(np.uint8).reshape(-1, 2)
+    v = rng.standard_normal(cols) * 2.0 ** (np.repeat(rng.integers(low + 3, high - 1, cols // 32), 32))
+    got, x = one_token(ty, p, rows, cols, v, xk, yk)
+    assert np.isfinite(x).all()
+    want, bound = ref.product(*ref.decode(oracle, ty, p, rows, cols), x)
+    assert ref.outside(got, want, bound, yk) == 0, np.abs(got - want).max()
