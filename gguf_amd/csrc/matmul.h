@@ -211,9 +211,9 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 // ---- packed whole-number codes, one token: x in digits ------------------------------------------------------
 // The matrix unit multiplies e4m3 bytes with a block scale for each 32 of them.  Codes are such bytes already (slices.h),
 // and so are the digits of x: 32 neighbouring elements share an exponent e, the largest one's; each becomes a whole number
-// of 32 bits (truncated, 2^-32 of the largest element) and that eight hexadecimal digits, each a byte 0..15 with x's sign, in
-// two chains of four.  All products are exact, and a digit's sums over a sub-block are whole numbers below 2^13.  Sixteen bits,
-// one chain, would do for 16-bit results of ordinary x (q6_k 32000 x 4096, 22.8 instead of 24.0 us), but beside an outlier the
+// of 32 bits (rounded, to 2^-32 of the largest element) and that eight hexadecimal digits, each a byte 0..15 with x's sign, in
+// two chains of four.  All products are exact, and a chain's sums over a sub-block are whole numbers below 2^13 for each plane;
+// the two chains, 2^-16 apart, and the four digits are joined in f32.  Sixteen bits, one chain, would do for 16-bit results of ordinary x (q6_k 32000 x 4096, 22.8 instead of 24.0 us), but beside an outlier the
 // small elements would lose bits that the caller gave.
 //
 // v_mfma_scale_f32_16x16x128: A is x, B the codes of 16 rows.  Lane (n, g), n = lane % 16, g = lane / 16, brings 32 codes of
@@ -251,17 +251,6 @@ struct CodeTile {
             uint8_t *to = lds + turn * X_BYTES;
             float v[8];
             load(turn, f * 8, v);
-            if constexpr (S::OFFSET) {
-                float sum = ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
-                sum += dpp<QUAD_XOR1>(sum);
-                float *sums = (float *)(to + SUMS) + step * 4 * S::NSUB;
-                if constexpr (S::PLANES) {                     // 16 elements: column `half` of sub-block block % 4
-                    if (f % 2 == 0) sums[(block / 4 * 2 + half) * 4 + block % 4] = sum;
-                } else {
-                    sum += dpp<QUAD_XOR2>(sum);
-                    if (f % 4 == 0) sums[block] = sum;
-                }
-            }
             uint32_t top = 0;
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
@@ -277,10 +266,24 @@ struct CodeTile {
             const uint32_t bad = e == 255 ? 0x7F7F7F7Fu : 0u;  // an infinity or NaN among them: e4m3's NaN
             e = e > 254 ? 254 : e;
             if (f % 4 == 0) to[EXPS + step * 8 + block] = (uint8_t)e;
-            const int up = 158 - (int)e;                       // x = whole * 2^-up
+            const int up = 158 - (int)e;
             uint32_t whole[8];
 #pragma unroll
-            for (int k = 0; k < 8; ++k) whole[k] = (uint32_t)__builtin_amdgcn_ldexpf(__builtin_fabsf(v[k]), up);
+            for (int k = 0; k < 8; ++k) {
+                v[k] = __builtin_rintf(__builtin_amdgcn_ldexpf(v[k], up));          // what is taken of x, times 2^up
+                whole[k] = (uint32_t)__builtin_fabsf(v[k]);
+            }
+            if constexpr (S::OFFSET) {
+                float sum = __builtin_amdgcn_ldexpf(((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7])), -up);
+                sum += dpp<QUAD_XOR1>(sum);
+                float *sums = (float *)(to + SUMS) + step * 4 * S::NSUB;
+                if constexpr (S::PLANES) {                     // 16 elements: column `half` of sub-block block % 4
+                    if (f % 2 == 0) sums[(block / 4 * 2 + half) * 4 + block % 4] = sum;
+                } else {
+                    sum += dpp<QUAD_XOR2>(sum);
+                    if (f % 4 == 0) sums[block] = sum;
+                }
+            }
             uint8_t *digits = to + step * DIGITS + block * 128 + half * 64 + f % 2 * 8;
             uint32_t sign[2], plane[2][4];                     // four elements a word; byte p of the whole numbers
 #pragma unroll

@@ -76,7 +76,7 @@ def test_one_token_small_codes(oracle, ty, xk, yk):
 def test_one_token_beside_an_outlier(oracle, ty, xk, yk):
     """One of 32 neighbours is 2^10 times the others and meets a weight of 0: the others count in full.  Bound: the worst of the
     roundings of f32 sums, 16 for a sub-block and its scale, 2 for each sub-block in the row's sum, 24 to join the row's parts,
-    of the sum of all magnitudes; and half of 2^-32 of the outlier for each element."""
+    of the sum of all magnitudes; and 2^-32 of the outlier for each element, half a step of 32 bits below 2^11."""
     import gguf_amd as g
     rows, cols = 300, 256
     p = weights(ty, rows, cols, ty + 5)
@@ -90,7 +90,7 @@ def test_one_token_beside_an_outlier(oracle, ty, xk, yk):
     got, x = one_token(ty, p, rows, cols, v, xk, yk)
     w, w0 = ref.decode(oracle, ty, p, rows, cols)
     assert not w[:, ::32].any()
-    bound = (40 + 2 * cols // 32) * ref.U * (np.abs(x) @ (np.abs(w - w0) + np.abs(w0)).T) + 2.0 ** -33 * 1024 * np.abs(w).sum(axis=1)
+    bound = (40 + 2 * cols // 32) * ref.U * (np.abs(x) @ (np.abs(w - w0) + np.abs(w0)).T) + 2.0 ** -32 * 1024 * np.abs(w).sum(axis=1)
     assert ref.outside(got, x @ w.T, bound, yk) == 0, np.abs(got - x @ w.T).max()
 
 
@@ -125,3 +125,23 @@ def test_one_token_of_every_size(oracle, ty, xk, yk, low, high):
     assert np.isfinite(x).all()
     want, bound = ref.product(*ref.decode(oracle, ty, p, rows, cols), x)
     assert ref.outside(got, want, bound, yk) == 0, np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("ty", [8, 9, 15])
+def test_one_token_is_rounded_without_a_bias(oracle, ty):
+    """Elements 2^-24 of the largest among 32 keep eight bits behind the point.  Rounded to nearest, x of one sign and weights of
+    one sign are off by independent errors of at most half a step, 2^-8, which spread like 2^-8 / sqrt(3) sqrt(sum of w^2); six
+    times that is never met.  Cut off, they would all have one sign: half a step for each of them, 4.6 times the bound."""
+    import gguf_amd as g
+    rows, cols = 200, 256
+    p = weights(ty, rows, cols, ty)
+    b = p.reshape(-1, g.block_bytes(ty))
+    lo = {8: 2, 9: 4, 15: 2}[ty]
+    b[:, lo:lo + g.block_elems(ty)] = 10
+    b[:, lo:lo + g.block_elems(ty):32] = 0
+    v = 1.0 + np.random.default_rng(ty).random(cols)
+    v[::32] = 2.0 ** 24
+    got, x = one_token(ty, p, rows, cols, v, "f32", "f32")
+    w, _ = ref.decode(oracle, ty, p, rows, cols)
+    bound = 6 * 2.0 ** -8 / 3 ** 0.5 * np.sqrt((w ** 2).sum(axis=1)) + (40 + 2 * cols // 32) * ref.U * (x @ w.T)
+    assert ref.outside(got, x @ w.T, bound, "f32") == 0, (np.abs(got - x @ w.T) / bound).max()
