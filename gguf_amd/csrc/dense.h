@@ -3,8 +3,7 @@
 // With several tokens the matrix unit's rows are tokens: v_mfma_f32_16x16x32_bf16 multiplies 32 codes of 16 rows, one
 // sub-block, with 16 tokens (16x16x16 for sub-blocks of 16).  Codes are turned into bf16, which holds every code exactly (two at
 // a time by v_cvt_scalef32_pk_bf16_fp8 where they are below 16: an e4m3 byte of 0..15 times 2^9 is itself).  x goes in as bf16,
-// in pieces where its type is wider: three of f32, exactly, or two where the result is rounded to 16 bits anyway; f16 goes in as
-// it is, with codes as f16.  Lane (n, g), n = lane % 16, g = lane / 16, brings the codes k = 8 g .. 8 g + 7 (4 g .. 4 g + 3) of
+// in pieces where its type is wider: three of f32, exactly; f16 goes in as it is, with codes as f16.  Lane (n, g), n = lane % 16, g = lane / 16, brings the codes k = 8 g .. 8 g + 7 (4 g .. 4 g + 3) of
 // row n and receives the sums of tokens 4 g .. 4 g + 3, which it scales: a multiply-add for each eight codes and token.  The
 // offsets' part, sum over sub-blocks of c times the sum of x, is a product too: the sums come from a multiplication with ones,
 // and v_mfma_f32_16x16x4_f32 adds them up in f32.  The scales of 256 columns are unpacked once, each lane a quarter of its
@@ -326,7 +325,7 @@ typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 // How x goes into the matrix unit: its type, and the bf16 pieces that a value is cut into
-enum XForm : int { X_BF16, X_F16, X_F32_2, X_F32_3 };
+enum XForm : int { X_BF16, X_F16, X_F32 };
 
 // Up to 16 tokens times R tiles of 16 rows.  A wave takes whole turns, 256 columns of all its rows and tokens, and nobody else
 // needs that part of x: it lies in the wave's own shared memory, as it comes from global memory, beside the images of its
@@ -337,9 +336,9 @@ struct DenseTile {
     typedef Step<F> S;
     static constexpr uint32_t TILES = R, ROWS = 16, ELEMS = 256, TOKENS = 16;
     typedef Image<F, ROWS, 1> I;
-    static constexpr bool WIDE = X == X_F32_2 || X == X_F32_3;
+    static constexpr bool WIDE = X == X_F32;
     static constexpr bool H = X == X_F16 && !__is_same(F, WBF16);                           // f16 as it is
-    static constexpr int P = X == X_BF16 || H ? 1 : X == X_F32_3 ? 3 : 2;
+    static constexpr int P = X == X_BF16 || H ? 1 : WIDE ? 3 : 2;
     static constexpr uint32_t SUBS = 256 / S::SUB, EACH = SUBS / 4, N = S::SUB / 4;        // N: elements of a lane's fragment
     static constexpr uint32_t X_SIZE = WIDE ? 4 : 2, X_ROW = 256 * X_SIZE + 16;              // an odd number of 16-byte places
     static constexpr uint32_t X_LOADS = WIDE ? TOKENS : TOKENS / 2, X_EACH = 16 / X_SIZE;
@@ -354,23 +353,15 @@ struct DenseTile {
         return *(const float *)(space + tile * PART + (token * ROWS + row) * 4);
     }
     typedef float Values[N];
-    // N elements as pieces, in words of two: cut off behind eight bits each, which three pieces hold exactly (two, of f16); two
-    // of f32 are rounded, to 2^-18 of the element
+    // N elements as pieces, in words of two: cut off behind eight bits each, which three pieces hold exactly (two, of f16)
     static __device__ __forceinline__ void cut(Values &v, uint32_t (&out)[P][N / 2]) {
 #pragma unroll
         for (int p = 0; p < P; ++p)
 #pragma unroll
             for (uint32_t i = 0; i < N; i += 2) {
-                if constexpr (X == X_F32_2) {
-                    const uint32_t w = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{v[i], v[i + 1]}, bf16x2v));
-                    out[p][i / 2] = w;
-                    v[i] -= bf2f(w & 0xFFFFu);
-                    v[i + 1] -= __builtin_bit_cast(float, w & 0xFFFF0000u);
-                } else {
-                    out[p][i / 2] = upper_halves(v[i], v[i + 1]);
-                    v[i] = below_bf16(v[i]);
-                    v[i + 1] = below_bf16(v[i + 1]);
-                }
+                out[p][i / 2] = upper_halves(v[i], v[i + 1]);
+                v[i] = below_bf16(v[i]);
+                v[i + 1] = below_bf16(v[i + 1]);
             }
     }
     // the fragment of sub-block s: elements SUB s + N g ..

@@ -127,7 +127,7 @@ uint64_t Launch<F>::matvec(MatvecArgs a, uint64_t tokens, hipStream_t st) {
     }
     if (a.x_kind == EK_BF16) return launch_dense<F, X_BF16>(a, tokens, st);
     if (a.x_kind == EK_F16) return launch_dense<F, X_F16>(a, tokens, st);
-    return launch_dense<F, X_F32_3>(a, tokens, st);
+    return launch_dense<F, X_F32>(a, tokens, st);
 }
 
 template <class F, class O>
@@ -192,7 +192,7 @@ void Launch<F>::up(MoeArgs a, hipStream_t st) {
     }
     if (a.x_kind == EK_BF16) launch_up_dense<F, X_BF16>(a, st);
     else if (a.x_kind == EK_F16) launch_up_dense<F, X_F16>(a, st);
-    else launch_up_dense<F, X_F32_3>(a, st);
+    else launch_up_dense<F, X_F32>(a, st);
 }
 
 template <class F>
@@ -206,9 +206,7 @@ void Launch<F>::down(MoeArgs a, hipStream_t st) {
         launch_down_one<F, CodeTile<F>>(a, st);
         return;
     }
-    // h is taken to 2^-18 of each element where the result is rounded to a 16-bit float: beside half a step of it, 2^-11 or 2^-8
-    if (a.x_kind != EK_F32 && a.y_kind != EK_F32) launch_down_dense<F, X_F32_2>(a, st);
-    else launch_down_dense<F, X_F32_3>(a, st);
+    launch_down_dense<F, X_F32>(a, st);
 }
 
 template struct Launch<GGQ_FORMAT>;

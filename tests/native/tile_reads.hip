@@ -54,14 +54,14 @@ static void kind(const char *name, uint32_t step, uint32_t least, uint32_t most)
 template <class F>
 static void packed(const char *name) {
     typedef CodeTile<F> C;
-    typedef DenseTile<F, X_F32_3, 1> D;
+    typedef DenseTile<F, X_F32, 1> D;
     kind<F, typename C::I, C::ELEMS, false, C::ROWS>(name, F::N, F::N, 9 * 256);
     kind<F, typename D::I, D::ELEMS, true, D::ROWS>(name, F::N, F::N, 9 * 256);
 }
 template <class F>
 static void floats(const char *name) {
     typedef FloatTile<F, 3> C;
-    typedef DenseTile<F, X_F32_3, 1> D;
+    typedef DenseTile<F, X_F32, 1> D;
     kind<F, typename C::I, C::ELEMS, false, C::ROWS>(name, 1, 8, 4104);
     kind<F, typename D::I, D::ELEMS, true, D::ROWS>(name, 1, 8, 1300);
 }

@@ -145,3 +145,32 @@ def test_one_token_is_rounded_without_a_bias(oracle, ty):
     w, _ = ref.decode(oracle, ty, p, rows, cols)
     bound = 6 * 2.0 ** -8 / 3 ** 0.5 * np.sqrt((w ** 2).sum(axis=1)) + (40 + 2 * cols // 32) * ref.U * (x @ w.T)
     assert ref.outside(got, x @ w.T, bound, "f32") == 0, (np.abs(got - x @ w.T) / bound).max()
+
+
+# ---- several tokens ------------------------------------------------------------------------------------------------------------
+
+def test_moe_keeps_32_bits_between_its_products():
+    """Whole numbers in, so that gate and up are exact in any order, and a `down` that picks one element for each output: 16-bit
+    outputs are the f32 outputs rounded once."""
+    import torch
+    import gguf_amd as g
+    n = 256
+    rng = np.random.default_rng(3)
+
+    def q8_0(codes, d):
+        b = np.zeros((codes.size // 32, 34), dtype=np.uint8)
+        b[:, :2] = np.frombuffer(np.float16(d).tobytes(), dtype=np.uint8)
+        b[:, 2:] = codes.astype(np.int8).view(np.uint8).reshape(-1, 32)
+        return on_device(b.reshape(-1))
+
+    gate, up = (q8_0(rng.integers(-3, 4, (2, n, n)), d) for d in (2.0 ** -6, 2.0 ** -3))
+    down = q8_0(np.stack([np.eye(n), np.eye(n)]), 1.0)
+    layer = g.MoeLayer(torch.randn(2, n, device="cuda"), (8, gate), (8, up), (8, down), hidden=n, ff=n, top_k=1)
+    for xk in ("f16", "bf16"):
+        x = torch.from_numpy(rng.integers(-8, 9, (16, n)).astype(np.float32)).cuda().to(dtype(xk))
+        wide, y = torch.empty(16, n, device="cuda"), torch.empty(16, n, dtype=dtype(xk), device="cuda")
+        layer.run(wide, x)
+        layer.run(y, x)
+        torch.cuda.synchronize()
+        assert wide.unique().numel() > 2000
+        assert torch.equal(y, wide.to(dtype(xk)))
