@@ -3,7 +3,7 @@ table by their ids (`get_rows`), and a mixture-of-experts layer (`MoeLayer`).
 
 A packed matrix is a uint8 CUDA tensor as it lies in a GGUF file: `rows` rows of `cols` elements, cols contiguous, of any
 block type that `dequantize_slice` decodes (the reference decodes a tensor before it is used:
-ggml-quants/src/lib.rs:135-147).  As in `dequantize_slice` the destination comes first, the kernels run on torch's
+ggml-quants/src/lib.rs:135-147).  One of type F16 or BF16 may be a float16 or bfloat16 tensor instead.  As in `dequantize_slice` the destination comes first, the kernels run on torch's
 current stream of the tensors' device (or on `stream`, a raw handle), and nothing is synchronized.  No gradients are
 recorded: these are the products of serving.
 
@@ -20,6 +20,7 @@ from .quants import GGmlType, LengthMismatch, Indivisible, Unsupported, block_by
 
 _ELEM = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 _IDS = {torch.int32: 26, torch.int64: 27}
+_OWN = {1: torch.float16, 30: torch.bfloat16}      # element types that are block types too
 _BLOCK = {}          # type id -> (elements, bytes of a block, the id as a plain number)
 # A call takes about 5 us of the host's time, 3.9 of them for the launch; torch.cuda's own lookups would add 1.3.  Where this
 # torch has the functions behind them, those are asked.
@@ -72,7 +73,9 @@ def _device_of(first, *others):
     return dev
 
 
-def _packed_bytes(w):
+def _packed_bytes(ty, w):
+    if w.dtype != torch.uint8 and w.dtype != _OWN.get(ty):
+        raise TypeError(f"packed weights of type {ty} are uint8, not {w.dtype}")
     if not w.is_contiguous():
         raise ValueError("packed weights must be contiguous")
     return w.nbytes
@@ -103,7 +106,7 @@ def matvec(ty, dst, w, x, stream=None):
         raise LengthMismatch()
     if cols % be:
         raise Indivisible()
-    if _packed_bytes(w) != rows * (cols // be) * bb:
+    if _packed_bytes(ty, w) != rows * (cols // be) * bb:
         raise LengthMismatch()
     _call(_device_of(dst, w, x), stream, _matvec_device, ty, rows, cols, w.data_ptr(), _elem(x), x.data_ptr(), xs, n,
           _elem(dst), dst.data_ptr(), ys)
@@ -126,7 +129,7 @@ def get_rows(ty, dst, w, ids, stream=None):
     if cols % be:
         raise Indivisible()
     row = cols // be * bb
-    size = _packed_bytes(w)
+    size = _packed_bytes(ty, w)
     if row and size % row:
         raise LengthMismatch()
     _call(_device_of(dst, w, ids), stream, _get_rows_device, ty, size // row if row else 0, cols, w.data_ptr(), kind,
@@ -158,8 +161,8 @@ class MoeLayer:
         (ue, ub, _), (de, db, _) = _block(ut), _block(dt)
         if hidden % ue or ff % de:
             raise Indivisible()
-        for w, size in ((gw, experts * ff * (hidden // ue) * ub), (uw, experts * ff * (hidden // ue) * ub), (dw, experts * hidden * (ff // de) * db)):
-            if _packed_bytes(w) != size:
+        for ty, w, size in ((gt, gw, experts * ff * (hidden // ue) * ub), (ut, uw, experts * ff * (hidden // ue) * ub), (dt, dw, experts * hidden * (ff // de) * db)):
+            if _packed_bytes(int(ty), w) != size:
                 raise LengthMismatch()
         self._dev = _device_of(router, gw, uw, dw)
         self._keep = (router, gw, uw, dw)
