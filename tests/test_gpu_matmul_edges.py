@@ -147,6 +147,65 @@ def test_one_token_is_rounded_without_a_bias(oracle, ty):
     assert ref.outside(got, x @ w.T, bound, "f32") == 0, (np.abs(got - x @ w.T) / bound).max()
 
 
+PACKED = [2, 3, 6, 7, 8, 9, 10, 11, 12, 13, 14, 15, 20, 23]
+
+
+@pytest.mark.parametrize("ty", PACKED + [1, 30])
+@pytest.mark.parametrize("xk,yk", [("f32", "f32"), ("bf16", "bf16"), ("f16", "f16")])
+@pytest.mark.parametrize("bad", ["inf", "-inf", "nan"])
+def test_one_token_non_finite_x(oracle, ty, xk, yk, bad):
+    """Wherever it stands, in the first sub-block or another, in the first chunk of x or a later one."""
+    rows, cols = 37, 1536
+    p = weights(ty, rows, cols, ty)
+    for at in (0, 31, 700, 1535):
+        v = np.random.default_rng(at).standard_normal(cols)
+        v[at] = float(bad)
+        got, _ = one_token(ty, p, rows, cols, v, xk, yk)
+        assert not np.isfinite(got).any(), at
+
+
+@pytest.mark.parametrize("ty", PACKED + [1, 30])
+@pytest.mark.parametrize("tokens", [1, 2])
+def test_non_finite_scale_stays_in_its_row(oracle, ty, tokens):
+    import torch
+    import gguf_amd as g
+    from gguf_amd import synth
+    rows, cols, row = 37, 1536, 21
+    bb, be = g.block_bytes(ty), g.block_elems(ty)
+    for bits in (0x7C00, 0xFC00, 0x7E00) if ty != 30 else (0x7F80, 0xFF80, 0x7FC0):
+        p = weights(ty, rows, cols, ty)
+        at = row * (cols // be) * bb + 2 * bb + (synth.HEADER_F16[ty][0] if ty in PACKED else 0)
+        p[at:at + 2] = np.frombuffer(np.uint16(bits).tobytes(), dtype=np.uint8)
+        x, x64 = activations(tokens, cols, "f32", 3)
+        buf, y = output(tokens, rows, "f32", rows + 3)
+        g.matvec(ty, y, on_device(p), x)
+        torch.cuda.synchronize()
+        p[at:at + 2] = 0
+        want, bound = ref.product(*ref.decode(oracle, ty, p, rows, cols), x64)
+        got, others = y.cpu().numpy(), [r for r in range(rows) if r != row]
+        assert ref.outside(got[:, others], want[:, others], bound[:, others], "f32") == 0
+        assert not np.isfinite(got[:, row]).any()
+        assert untouched(buf, tokens, rows)
+
+
+@pytest.mark.parametrize("bad", ["nan", "inf", "-inf"])
+@pytest.mark.parametrize("ut,dt,xk", [(12, 14, "f32"), (2, 8, "bf16"), (20, 23, "f16"), (1, 30, "f32")])
+def test_moe_one_token_non_finite(oracle, bad, ut, dt, xk):
+    """The ids stay valid and different; the layer's next call is what it was."""
+    import torch
+    m = Moe(oracle, 9, 512, 256, ut, dt, seed=2, top_k=3)
+    x, _ = activations(1, 512, xk, 1)
+    hurt = x.clone()
+    hurt[0, 300] = float(bad)
+    y, ids = torch.empty(1, 512, device="cuda"), torch.full((1, 3), -7, dtype=torch.int32, device="cuda")
+    m.layer.run(y, hurt, ids=ids)
+    torch.cuda.synchronize()
+    got = ids.cpu().numpy()[0].tolist()
+    assert len(set(got)) == 3 and min(got) >= 0 and max(got) < 9
+    assert not np.isfinite(y.cpu().numpy()).any()
+    m.check(x, "f32")
+
+
 # ---- several tokens ------------------------------------------------------------------------------------------------------------
 
 def test_moe_keeps_32_bits_between_its_products():
@@ -174,3 +233,43 @@ def test_moe_keeps_32_bits_between_its_products():
         torch.cuda.synchronize()
         assert wide.unique().numel() > 2000
         assert torch.equal(y, wide.to(dtype(xk)))
+
+
+@pytest.mark.parametrize("ty", [1, 2, 12, 14, 30])
+@pytest.mark.parametrize("tokens", [2, 9])
+def test_several_tokens_of_every_size(oracle, ty, tokens):
+    """As for one token; of f32 x the bits below 2^-133 are left out."""
+    import torch
+    import gguf_amd as g
+    rows, cols = 70, 1024
+    p = weights(ty, rows, cols, ty)
+    for xk, low, high in (("f32", -118, 60), ("f32", -118, -112), ("f32", -126, -120), ("bf16", -125, -119), ("f16", -24, -14), ("f32", 70, 98)):
+        rng = np.random.default_rng(1000 + low + ty)
+        v = rng.standard_normal((tokens, cols)) * 2.0 ** np.repeat(rng.integers(low + 3, high - 1, (tokens, cols // 32)), 32, axis=1)
+        x = torch.from_numpy(v.astype(np.float32)).cuda().to(dtype(xk))
+        y = torch.empty(tokens, rows, device="cuda")
+        g.matvec(ty, y, on_device(p), x)
+        torch.cuda.synchronize()
+        w, w0 = ref.decode(oracle, ty, p, rows, cols)
+        want, bound = ref.product(w, w0, x.double().cpu().numpy())
+        # what is left out of an element meets its weight; a sub-block's offset meets the same sum of x
+        floor = 2.0 ** -133 * (np.abs(w)).sum(axis=1) if xk == "f32" else 0.0
+        assert ref.outside(y.cpu().numpy(), want, bound + floor, "f32") == 0, (xk, low)
+
+
+# ---- rows by id ----------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("ty,cols", [(2, 32), (14, 256), (1, 5)])
+def test_get_rows_of_more_ids_than_one_launch_takes(oracle, ty, cols):
+    import torch
+    import gguf_amd as g
+    rows, n = 50, 2 * 65535 + 37
+    p = weights(ty, rows, cols, ty)
+    ids = np.random.default_rng(ty).integers(-1, rows + 1, n)
+    buf, y = output(n, cols, "f32", cols + 1)
+    g.get_rows(ty, y, on_device(p), torch.from_numpy(ids).cuda())
+    torch.cuda.synchronize()
+    dec = oracle.dequantize(ty, p).reshape(rows, cols)
+    want = np.where(((ids >= 0) & (ids < rows))[:, None], dec[np.clip(ids, 0, rows - 1)], np.float32(0))
+    assert same_bits(y.contiguous().cpu().numpy(), want)
+    assert untouched(buf, n, cols)
