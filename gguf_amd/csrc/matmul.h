@@ -96,6 +96,9 @@ __device__ __forceinline__ void load8(const void *x, uint64_t at, uint64_t c, ui
     }
 }
 
+// Columns: the sixteen packed rows of a tile are within the offsets that Image::last can bound, whatever their type.
+constexpr uint64_t MAX_COLS = 1ull << 26;
+
 // A wave's packed bytes of one turn.  Lanes that multiply together hold different rows, so loads straight into their
 // registers would touch a line per lane: the memory pipeline takes about two cycles for each, which held the products at
 // 4.1 TB/s whatever the format's arithmetic.  Instead neighbouring lanes load neighbouring 16-byte pieces into registers,
@@ -109,6 +112,7 @@ struct Image {
     // an odd number of 16-byte places from row to row: the rows' parts of one column lie in different banks
     static constexpr uint32_t UNIT = PIECES * 16, ROW = 16 * (PER_ROW | 1);
     static constexpr uint32_t BYTES = ROW * ROWS;
+    static_assert((ROWS - 1) * (MAX_COLS / F::N * F::BYTES) + TURN_BYTES + 32 <= (1ull << 31), "offsets in a tile");
     // where this lane's pieces are
     struct Places {
         uint32_t src[LOADS], dst[LOADS];      // from the tile's first row on; in the image

@@ -55,8 +55,6 @@ bool elem_kind(uint32_t ty, uint32_t *kind, uint32_t *bytes) {
 
 // Sizes beyond these have no use and would let products of sizes wrap.
 constexpr uint64_t MAX_DIM = 1ull << 30;
-// Columns: eight packed rows of any type are within 32-bit offsets.
-constexpr uint64_t MAX_COLS = 1ull << 26;
 // Workgroups of one launch along y
 constexpr uint64_t MAX_GRID_Y = 65535;
 

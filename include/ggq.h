@@ -283,9 +283,10 @@ ggq_status ggq_dequantize_noalloc(uint32_t ggml_type, uint32_t out_type,
  *
  * ggq_matvec_device: y[t][r] = sum over c of W[r][c] * x[t][c], for t < tokens.  x is taken exactly by two tokens and
  *   more and by F16 / BF16 weights (less the bits of F32 x below 2^-133); by one token (the last of 17, 33, ... too) and packed
- *   codes to 2^-32 of the largest of 32 neighbours, to nearest.  Products of that are exact, sums are held in 32 bits in an order that depends on the sizes alone, and one rounding to y_type ends each.  Made
- *   for the few tokens of decoding (up to 16 share one pass over W); any number is computed.  A token's result may differ in its
- *   last bits with the number of tokens of the call.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
+ *   codes to 2^-32 of the largest of 32 neighbours, to nearest.  Products of that are exact, sums are held in 32 bits in an order
+ *   that depends on the sizes alone, and one rounding to y_type ends each.  Made for the few tokens of decoding (up to 16 share
+ *   one pass over W); any number is computed.  A token's result may differ in its last bits with the number of tokens of the
+ *   call.  x_stride may be 0 (one row for all tokens); y_stride >= rows where
  *   there are two tokens or more (GGQ_INVALID).  cols must be whole blocks (GGQ_INDIVISIBLE) and below 2^26, rows and tokens below
  *   2^30 (GGQ_INVALID); cols == 0 gives zeros.
  *   Intermediate sums are those of whole-number codes times x: |x| stays below 2^100, and non-finite x makes the

@@ -257,6 +257,40 @@ def test_several_tokens_of_every_size(oracle, ty, tokens):
         assert ref.outside(y.cpu().numpy(), want, bound + floor, "f32") == 0, (xk, low)
 
 
+@pytest.mark.parametrize("ty", [1, 8, 14])
+@pytest.mark.parametrize("tokens", [1, 2])
+def test_rows_near_the_longest(ty, tokens):
+    """Rows of nearly 2^26 elements, sixteen to a tile: nearly 2^31 bytes of 16-bit floats.  Whole numbers at a few places of each
+    row, zeros elsewhere: every sum is exact."""
+    import torch
+    import gguf_amd as g
+    be, bb = g.block_elems(ty), g.block_bytes(ty)
+    rows, cols = 17, (1 << 26) - (5 if ty == 1 else be)
+    w = torch.zeros(rows * (cols // be), bb, dtype=torch.uint8, device="cuda")
+    one = np.frombuffer(np.float16(1.0).tobytes(), dtype=np.uint8)
+    # block 0 of every type here: one code of the first element's is 1, its scale is 1
+    block = np.zeros(bb, dtype=np.uint8)
+    if ty == 1:
+        block[:] = one
+    elif ty == 8:
+        block[:2], block[2] = one, 1
+    else:                                              # q6_k: 32 is 0, 33 is 1; all scales are 1
+        block[128:192], block[192:208], block[208:], block[0] = 0xAA, 1, one, 1
+    blocks = cols // be
+    places = [0, blocks // 3, blocks - 1]
+    for r in range(rows):
+        for b in places[:1 + r % 3]:
+            w[r * blocks + b] = torch.from_numpy(block).cuda()
+    x = torch.zeros(tokens, cols, device="cuda")
+    for t in range(tokens):
+        for i, b in enumerate(places):
+            x[t, b * be] = 10.0 ** i * (t + 1)
+    y = torch.empty(tokens, rows, device="cuda")
+    g.matvec(ty, y, w.view(-1), x)
+    want = [[(t + 1) * float("111"[: 1 + r % 3]) for r in range(rows)] for t in range(tokens)]
+    assert y.cpu().tolist() == want
+
+
 # ---- rows by id ----------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("ty,cols", [(2, 32), (14, 256), (1, 5)])
