@@ -61,6 +61,7 @@ __global__ __launch_bounds__(MV_THREADS) void moe_logits(MoeArgs a) {
     double sum[T] = {};
     for (uint32_t c = threadIdx.x * 4; c < n; c += MV_THREADS * 16) {
         if constexpr (T == 1) {
+            // values as they are loaded: by way of the words, as below, a layer's call takes 0.3 to 0.5 us more (20.6 -> 20.9, 56.1 -> 56.6)
             float w[4][4], x[4][4];
 #pragma unroll
             for (uint32_t k = 0; k < 4; ++k) floats4(a.router, e * a.hidden, c + k * MV_THREADS * 4, n, a.router_kind, w[k]);
