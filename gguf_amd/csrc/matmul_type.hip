@@ -17,20 +17,30 @@ constexpr uint32_t X_LDS = 64 << 10;
 // ... of one workgroup for several tokens: what a CU has, less the kernel's own
 constexpr uint32_t DENSE_LDS = 152 << 10;
 
+// ... of one workgroup in all, so that two fit a CU.  Where there are more of them than CUs and shorter chunks are enough for that,
+// those are taken: q5_0 11008 x 4096 11.3 instead of 13.5 us, q2_k 28672 x 8192 25.0 instead of 31.1.  With one workgroup for a CU
+// they only cost: q5_0 8192 x 28672 45 instead of 38 us.
+constexpr uint32_t HALF_CU = 80 << 10;
+
 // The shape of a launch over `tiles` wave tiles, each of which takes `turns` turns: how many waves share a tile's turns,
 // the turns staged at a time (equal chunks, whole rounds of the waves), the shared memory.
 struct Shape {
     uint32_t ksplit = 1, groups;
+    bool two;             // more workgroups than CUs
     // `waves`: of a workgroup that may share a tile's turns; x_bytes: shared memory of a turn of x
     Shape(uint64_t tiles, uint32_t turns, uint32_t waves, uint32_t x_bytes) {
         // few rows: the columns are shared out, until there are 8 waves for each of 256 CUs (up to 32: q6_k 32000 x 4096 32.4
         // instead of 26.8 us, q4_k 28672 x 8192 36.5 instead of 26.8; up to 16: the same within 1 % for all that were tried)
         while (ksplit < waves && ksplit < turns && tiles * ksplit < 2048 && 2 * ksplit * x_bytes <= X_LDS) ksplit *= 2;
         groups = waves / ksplit;
+        two = tiles * ksplit > 256 * TILE_WAVES;
     }
     template <class M> uint32_t chunk(uint32_t turns) const {
-        const uint32_t rounds = (turns + ksplit - 1) / ksplit, most = std::max(1u, X_LDS / (M::X_BYTES * ksplit)), chunks = (rounds + most - 1) / most;
-        return (rounds + chunks - 1) / chunks * ksplit;
+        const uint32_t each = M::X_BYTES * ksplit, rounds = (turns + ksplit - 1) / ksplit, own = TILE_WAVES * M::WAVE_BYTES + M::CLEAR;
+        auto in_chunks = [&](uint32_t most) { const uint32_t chunks = (rounds + most - 1) / most; return (rounds + chunks - 1) / chunks; };
+        uint32_t take = in_chunks(std::max(1u, X_LDS / each));
+        if (two && own + take * each > HALF_CU && own + each <= HALF_CU) take = in_chunks((HALF_CU - own) / each);
+        return take * ksplit;
     }
     template <class M> uint32_t bytes(uint32_t turns) const {
         return TILE_WAVES * M::WAVE_BYTES + M::CLEAR + std::max<uint32_t>(std::min(chunk<M>(turns), turns) * M::X_BYTES, TILE_WAVES * M::ROWS * 4);
