@@ -198,7 +198,9 @@ class MoeLayer:
         if stream is None:
             space = torch.empty(size, dtype=torch.uint8, device=dst.device)
         else:
-            with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=dst.device)):
+            # torch takes the handle 0, the default stream's, for none at all and makes a stream of its own
+            owner = torch.cuda.ExternalStream(stream, device=dst.device) if stream else torch.cuda.default_stream(dst.device)
+            with torch.cuda.stream(owner):
                 space = torch.empty(size, dtype=torch.uint8, device=dst.device)
         _call(dev, stream, lib.ggq_moe_device, self._ref, _elem(x), x.data_ptr(), xs, n, _elem(dst), dst.data_ptr(), ys,
               ids.data_ptr() if ids is not None else None, weights.data_ptr() if weights is not None else None, space.data_ptr(), size)

@@ -291,6 +291,31 @@ def test_rows_near_the_longest(ty, tokens):
     assert y.cpu().tolist() == want
 
 
+def test_moe_workspace_belongs_to_the_stream_of_the_call(oracle, monkeypatch):
+    """... also where that is the default stream, whose handle is 0: memory of another stream could be handed out again while
+    the kernels still use it."""
+    import torch
+    m = Moe(oracle, 4, 256, 256, 2, 2, seed=1)
+    x, _ = activations(2, 256, "f32", 1)
+    y = torch.empty(2, 256, device="cuda")
+    side = torch.cuda.Stream()
+    owners, empty = [], torch.empty
+
+    def spy(*args, **kw):
+        owners.append(torch.cuda.current_stream().cuda_stream)
+        return empty(*args, **kw)
+
+    torch.cuda.synchronize()
+    monkeypatch.setattr(torch, "empty", spy)
+    for current in (torch.cuda.default_stream(), side):
+        with torch.cuda.stream(current):
+            for stream in (None, 0, torch.cuda.default_stream().cuda_stream, side.cuda_stream):
+                owners.clear()
+                m.layer.run(y, x, stream=stream)
+                torch.cuda.synchronize()
+                assert owners == [current.cuda_stream if stream is None else stream]
+
+
 # ---- rows by id ----------------------------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("ty,cols", [(2, 32), (14, 256), (1, 5)])
