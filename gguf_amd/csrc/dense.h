@@ -12,7 +12,7 @@
 // Bound by the vector instructions that unpack and scale (about 150 for 256 columns of 16 rows), and for few rows by the time
 // that a workgroup takes to begin and end.  Against all waves of a workgroup staging x for each other: q4_k 11008 x 4096 by 16
 // tokens (bf16) 11.4 against 20.5 us, q6_k 15.5 against 36.8.  Against one token's digits (matmul.h): q4_k 28672 x 8192 by one
-// token 42 against 27 us here, so one token is left to those.
+// token 33 (bf16) and 59 (f32) against 27 us, so one token is left to those.
 #pragma once
 #include "matmul.h"
 

@@ -231,10 +231,11 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 // carried it and lost it again: by codes that were small beside their range, next to an outlier, the result was 2^-13 off.  The
 // matrix unit has room for it (q8_0 11008 x 4096 12.5 instead of 12.3 us; codes by sign and magnitude 13.5).
 //
-// Codes need no conversion, and a sub-block's four digits one addition each: against codes in bf16 (x as three pieces,
-// v_mfma_f32_4x4x4, what 16-bit float weights take below) q6_k 4096 x 11008 took 11.2 instead of 12.6 us, q5_k 11008 x 4096 8.8
-// instead of 11.4.  Large matrices are bound by the bytes that the loads in flight bring (q4_k 28672 x 8192, f32: 26.8 us, 4.9
-// TB/s of 7.05), small ones by the way from the launch to the staged x (q4_0 256 x 2048: 4.2 us, an empty kernel 2.5).
+// Codes need no conversion, and a sub-block's four digits a multiply-add each: q6_k 4096 x 11008 takes 12.1 us, q5_k 11008 x 4096
+// 9.6; with codes in bf16 (x as three pieces, v_mfma_f32_4x4x4, what 16-bit float weights take below) 12.6 and 11.4.  Pieces of x
+// as e5m2, which would be exact too, are no way out: the unit keeps sums of such bytes only to some 2^-11 of the largest product.
+// Large matrices are bound by the bytes that the loads in flight bring (q4_k 28672 x 8192, f32: 26.5 us, 5.0 TB/s of 7.05, vector
+// units busy for 46 % of it), small ones by the way from the launch to the staged x (q4_0 256 x 2048: 4.2 us, an empty kernel 2.5).
 //
 // Staged x, per turn: [step][chain][block of 32][half][digit][16 bytes], then [step][block] e as a byte, then
 // the sums of x, f32, where the format has an offset: [step][slice][sub-block].

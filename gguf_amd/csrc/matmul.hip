@@ -227,7 +227,7 @@ ggq_status ggq_moe_device(const ggq_moe *m, uint32_t x_type, const void *d_x, ui
     else moe_logits<LOGIT_TOKENS><<<dim3(m->experts, ((uint32_t)tokens + LOGIT_TOKENS - 1) / LOGIT_TOKENS), MV_THREADS, 0, st>>>(a);
     // groups of pairs with the same expert: one for each pair, or one for each expert and one more for each slot_tokens pairs.
     // Shared memory is kept for as many tokens: where experts have four on average, or fewer, more than eight are rare (128
-    // experts, 8 chosen, 2048/768 by 16 tokens: 99.6 us, with room for 16 113).
+    // experts, 8 chosen, 2048/768 by 16 tokens: 102 us, with room for 16 110).
     const uint32_t pairs = (uint32_t)tokens * m->top_k, in_use = std::min(m->experts, pairs);
     a.slot_tokens = std::min((uint32_t)tokens, pairs > 4 * m->experts ? SLOT_TOKENS : SLOT_TOKENS / 2);
     a.slots = std::min(pairs, in_use + (pairs - in_use) / a.slot_tokens);

@@ -116,9 +116,10 @@ uint64_t launch_dense(MatvecArgs a, uint64_t tokens, hipStream_t st) {
 
 }  // namespace
 
-// One token is left to the digits, which need fewer instructions: q4_k 28672 x 8192 26.7 us (as several tokens 32.7), 11008 x 4096
-// 8.5 (9.6), q6_k 32000 x 4096 22.8 (29.4); few rows with long columns are as fast either way (8192 x 28672 29.7, 29.3) or
-// a little slower so (4096 x 11008 9.6, 8.5).  One launch over the first of the tokens.  Returns how many it takes.
+// One token is left to the digits, which need fewer instructions: q4_k 28672 x 8192 26.8 us (as several tokens 33.1 by bf16 x, 59 by
+// f32), 11008 x 4096 9.1 (9.6, 13.1), q6_k 32000 x 4096 24.5 (29.4, 44.5).  Few rows with long columns are slower so by 16-bit x
+// (q4_k 8192 x 28672 31.7, 30.8; 4096 x 11008 10.6, 8.4), but not for all types (q4_0 1024 x 8192 6.8, 7.9).  One launch over the
+// first of the tokens.  Returns how many it takes.
 template <class F>
 uint64_t Launch<F>::matvec(MatvecArgs a, uint64_t tokens, hipStream_t st) {
     if constexpr (is_float_type<F>) {

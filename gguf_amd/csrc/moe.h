@@ -6,9 +6,10 @@
 // Several: the logits; the choice and the table of slots (route.h); gate and up, slot by slot; down, slot by slot; the sum.
 // An expert's bytes are read once for each slot: for up to 16 of its tokens, or 8.
 //
-// Bound, for one token and large experts, by the bytes of the experts in use (8 experts, 2 chosen, 4096/11008: gate and up 101 MB
-// in 25 us, down 74 MB in 21); for small ones by the time that three launches take to begin and end (64, 8, 2048/1024: 20.6 us
-// for 29 MB); for several tokens by the instructions that unpack (128, 8, 2048/768 by 16 tokens: 98 us for 235 MB).
+// Bound, for one token and large experts, by the bytes of the experts in use and by x, which each workgroup turns into digits (8
+// experts, 2 chosen, 4096/11008: gate and up 101 MB in 27 us, down 74 MB in 24.7; 344 and 256 workgroups for 256 CUs); for small
+// ones by the time that three launches take to begin and end (64, 8, 2048/1024: 20.6 us for 29 MB); for several tokens by the
+// instructions that unpack (128, 8, 2048/768 by 16 tokens: 102 us for 235 MB, vector units busy for 51 and 65 % of gate / up and down).
 #pragma once
 #include "choice.h"
 #include "dense.h"

@@ -152,7 +152,7 @@ __device__ __forceinline__ void choose_maxima(const float *logits, uint32_t expe
 }
 // One workgroup: its waves take the tokens, then its threads the experts and the pairs.  The kernels of gate, up and down find
 // their slot in a table.  Where each of their workgroups looked for its own, down of 128 experts, 8 chosen, 2048/768 by 16 tokens
-// took 51 us instead of 39.
+// took 51 us instead of 39 (with three pieces of h, as now, 45).
 constexpr uint32_t ROUTE_WAVES = 16;
 __global__ __launch_bounds__(ROUTE_WAVES * 64) static void moe_route(MoeArgs a) {
     __shared__ int32_t ids[MOE_MAX_TOKENS * MOE_MAX_TOP_K];
