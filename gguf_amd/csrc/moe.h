@@ -16,12 +16,11 @@
 
 namespace ggq {
 
+// SiLU, or GELU's tanh form, (1 + tanh z) / 2 = 1 / (1 + exp(-2 z)): 1 + tanh z itself has no bits left for z below -9
 __device__ __forceinline__ float moe_act(float g, uint32_t gelu) {
-    if (!gelu) return g / (1.0f + expf(-g));
-    const float z = 0.7978845608028654f * (g + 0.044715f * g * g * g);
-    return 0.5f * g * (1.0f + tanhf(z));
+    const float z = gelu ? 1.5957691216057308f * (g + 0.044715f * g * g * g) : g;
+    return g / (1.0f + expf(-z));
 }
-
 
 // ---- gate and up ----------------------------------------------------------------------------------------
 // One token.  As matvec_tiles; half of a workgroup's waves take gate's rows, the others the same rows of up.  Each workgroup finds

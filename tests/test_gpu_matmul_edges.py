@@ -291,6 +291,46 @@ def test_rows_near_the_longest(ty, tokens):
     assert y.cpu().tolist() == want
 
 
+@pytest.mark.parametrize("activation", ["silu", "gelu"])
+@pytest.mark.parametrize("tokens", [1, 3])
+def test_moe_activation_over_its_range(activation, tokens):
+    """Gate values from -24 to 24 in steps of 1/16 and more, exact in any order, by an `up` of ones and a `down` that picks one element: the
+    activation itself, in its own size.  32-bit roundings, half a unit each: z takes 5, each of which exp turns into 2 |z| of its
+    result (SiLU: |z|, and none), exp, the sum, the quotient and two products below 8."""
+    import torch
+    import gguf_amd as g
+    n = 512
+
+    def q8_0(codes, d):
+        b = np.zeros((codes.size // 32, 34), dtype=np.uint8)
+        b[:, :2] = np.frombuffer(np.float16(d).tobytes(), dtype=np.uint8)
+        b[:, 2:] = codes.astype(np.int8).view(np.uint8).reshape(-1, 32)
+        return on_device(b.reshape(-1))
+
+    # x = (t + 1, 1, 0, ..): gate = (t + 1) code 2^-4 in column 0, up = 1 in column 1
+    codes = np.zeros((1, n, n))
+    codes[0, :, 0] = np.arange(n) % 256 - 128
+    ones = np.zeros((1, n, n))
+    ones[0, :, 1] = 1
+    layer = g.MoeLayer(torch.ones(1, n, device="cuda"), (8, q8_0(codes, 2.0 ** -4)), (8, q8_0(ones, 1.0)), (8, q8_0(np.eye(n)[None], 1.0)), hidden=n, ff=n,
+                       top_k=1, activation=activation)
+    x = torch.zeros(tokens, n, device="cuda")
+    x[:, 0] = torch.arange(1, tokens + 1) if tokens > 1 else 2.0
+    x[:, 1] = 1.0
+    y = torch.empty(tokens, n, device="cuda")
+    layer.run(y, x)
+    torch.cuda.synchronize()
+    v = (x[:, :1].double().cpu().numpy()) * codes[0, :, 0][None] * 2.0 ** -4
+    z = v if activation == "silu" else 2.0 * np.sqrt(2.0 / np.pi) * (v + 0.044715 * v ** 3)
+    with np.errstate(over="ignore"):
+        want = v / (1.0 + np.exp(-z))
+    tol = (8 + 10 * np.abs(z)) * ref.U * np.abs(want) + 2.0 ** -126
+    if tokens == 1:
+        # an element of h is taken to 2^-32 of the largest of 32 neighbours
+        tol = tol + 2.0 ** -32 * np.repeat(np.abs(want).reshape(tokens, -1, 32).max(axis=2), 32, axis=1)
+    assert (np.abs(y.cpu().numpy() - want) <= tol).all(), np.abs(y.cpu().numpy() - want).max()
+
+
 def test_moe_workspace_belongs_to_the_stream_of_the_call(oracle, monkeypatch):
     """... also where that is the default stream, whose handle is 0: memory of another stream could be handed out again while
     the kernels still use it."""
