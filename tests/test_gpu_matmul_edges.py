@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import matmul_ref as ref
-from test_gpu_matmul import Moe, activations, dtype, on_device, output, run_matvec, untouched, weights
+from test_gpu_matmul import SENTINEL, Moe, activations, dtype, on_device, output, run_matvec, untouched, weights
 from util import same_bits
 
 pytestmark = pytest.mark.gpu
@@ -354,6 +354,38 @@ def test_moe_workspace_belongs_to_the_stream_of_the_call(oracle, monkeypatch):
                 m.layer.run(y, x, stream=stream)
                 torch.cuda.synchronize()
                 assert owners == [current.cuda_stream if stream is None else stream]
+
+
+@pytest.mark.parametrize("experts,top_k", [(512, 32), (40, 32)])
+def test_moe_most_pairs(oracle, experts, top_k):
+    """64 tokens of 32 experts each."""
+    m = Moe(oracle, experts, 64, 32, 7, 20, seed=experts, top_k=top_k)
+    x, _ = activations(64, 64, "f32", 5)
+    m.check(x, "f32", pad=3)
+
+
+@pytest.mark.parametrize("ty", [1, 2, 12, 14])
+@pytest.mark.parametrize("tokens", [1, 2])
+@pytest.mark.parametrize("xk", ["f32", "f16", "bf16"])
+def test_x_and_y_begin_anywhere(oracle, ty, tokens, xk):
+    """x and y at any multiple of their element size."""
+    import torch
+    import gguf_amd as g
+    rows, cols = 37, 768
+    p = weights(ty, rows, cols, ty)
+    w, w0 = ref.decode(oracle, ty, p, rows, cols)
+    m = Moe(oracle, 5, 256, 256, 2, ty if ty != 1 else 12, seed=ty)
+    for off in (1, 3, 6):
+        v, x64 = activations(1, tokens * cols + off, xk, off)
+        x = v[0, off:].view(tokens, cols)
+        out = torch.full((tokens * rows + off + 1,), SENTINEL, dtype=dtype(xk), device="cuda")
+        y = out[off:-1].view(tokens, rows)
+        g.matvec(ty, y, on_device(p), x)
+        torch.cuda.synchronize()
+        want, bound = ref.product(w, w0, x64[0, off:].reshape(tokens, cols))
+        assert ref.outside(y.float().cpu().numpy(), want, bound, xk) == 0
+        assert bool((out[:off] == SENTINEL).all()) and float(out[-1]) == SENTINEL
+        m.check(v[0, off:off + tokens * 256].view(tokens, 256), xk)
 
 
 # ---- rows by id ----------------------------------------------------------------------------------------------------------------
