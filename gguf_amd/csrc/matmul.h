@@ -217,8 +217,8 @@ __host__ __device__ __forceinline__ RowTile<T> full_tile_at(T row, T total) {
 // and so are the digits of x: 32 neighbouring elements share an exponent e, the largest one's; each becomes a whole number
 // of 32 bits (rounded, to 2^-32 of the largest element) and that eight hexadecimal digits, each a byte 0..15 with x's sign, in
 // two chains of four.  All products are exact, and a chain's sums over a sub-block are whole numbers below 2^13 for each plane;
-// the two chains, 2^-16 apart, and the four digits are joined in f32.  Sixteen bits, one chain, would do for 16-bit results of ordinary x (q6_k 32000 x 4096, 22.8 instead of 24.0 us), but beside an outlier the
-// small elements would lose bits that the caller gave.
+// the two chains, 2^-16 apart, and the four digits are joined in f32.  Sixteen bits, one chain, would do for 16-bit results of
+// ordinary x (q6_k 32000 x 4096 22.8 instead of 24.0 us), but beside an outlier small elements would lose bits that the caller gave.
 //
 // v_mfma_scale_f32_16x16x128: A is x, B the codes of 16 rows.  Lane (n, g), n = lane % 16, g = lane / 16, brings 32 codes of
 // row n, slice g.  Row m of A is digit m % 4 of the slices g = m / 4 and zero for the other slices, so that D's rows
