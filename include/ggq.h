@@ -307,7 +307,8 @@ ggq_status ggq_get_rows_device(uint32_t ggml_type, uint64_t rows, uint64_t cols,
  *   p = softmax(l) or sigmoid(l);  the top_k experts of the largest l, equal ones by the lowest index (a NaN counts as
  *   lowest);  w = p of those, divided by their sum if `normalize`, times `scale`;
  *   y = sum over the chosen e, in order, of w_e * down_e (act(gate_e x) * (up_e x)).
- * The products between are held in 32 bits and taken as a matvec takes F32 x.  Weights whose sum is 0 (a sigmoid of large negative logits) are NaN if `normalize`. */
+ * x goes into gate and up as into ggq_matvec_device; what comes out of them is held in 32 bits and goes into down as F32 x does.
+ * Weights whose sum is 0 (a sigmoid of large negative logits) are NaN if `normalize`. */
 typedef struct ggq_moe {
     uint32_t router_type;           /* F32, F16 or BF16: [experts][hidden], row-major      */
     uint32_t up_type;               /* block type of gate and of up, [experts][ff][hidden] */
