@@ -4,10 +4,10 @@
 // sub-block, with 16 tokens (16x16x16 for sub-blocks of 16).  Codes are turned into bf16, which holds every code exactly (two at
 // a time by v_cvt_scalef32_pk_bf16_fp8 where they are below 16: an e4m3 byte of 0..15 times 2^9 is itself).  x goes in as bf16,
 // in pieces where its type is wider: three of f32, exactly; f16 goes in as it is, with codes as f16.  Lane (n, g), n = lane % 16,
-// g = lane / 16, brings the codes k = 8 g .. 8 g + 7 (4 g .. 4 g + 3) of row n and receives the sums of tokens 4 g .. 4 g + 3, which it scales: a multiply-add for each eight codes and token.  The
-// offsets' part, sum over sub-blocks of c times the sum of x, is a product too: the sums come from a multiplication with ones,
-// and v_mfma_f32_16x16x4_f32 adds them up in f32.  The scales of 256 columns are unpacked once, each lane a quarter of its
-// row's, and handed round through shared memory.
+// g = lane / 16, brings the codes k = 8 g .. 8 g + 7 (4 g .. 4 g + 3) of row n and receives the sums of tokens 4 g .. 4 g + 3,
+// which it scales: a multiply-add for each eight codes and token.  The offsets' part, sum over sub-blocks of c times the sum of x,
+// is a product too: the sums come from a multiplication with ones, and v_mfma_f32_16x16x4_f32 adds them up in f32.  The scales of
+// 256 columns are unpacked once, each lane a quarter of its row's, and handed round through shared memory.
 //
 // Bound by the vector instructions that unpack and scale (about 150 for 256 columns of 16 rows), and for few rows by the time
 // that a workgroup takes to begin and end.  Against all waves of a workgroup staging x for each other: q4_k 11008 x 4096 by 16
